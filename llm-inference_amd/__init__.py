@@ -31,6 +31,8 @@ __all__ = [
     "qk_norm_rope_attention_forward", "dump_open",
     "dump_close", "dump_enabled", "attention_forward_noalloc", "EXPORTED_SYMBOLS",
     "qk_norm_rope_attention_one_pass", "attention_one_pass_bytes", "attention_one_pass_supported",
+    "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_YARN", "rope_frequencies", "qk_norm_rope_paged",
+    "attention_paged_forward", "attention_paged_workspace_floats", "logits_penalty_forward",
 ]
 
 # Every symbol include/llm_amd/*.h declares.
@@ -48,6 +50,8 @@ EXPORTED_SYMBOLS = [
     "synth_fill", "generate_greedy", "attention_forward_noalloc",
     "qk_norm_rope_attention_forward", "qk_norm_rope_attention_one_pass",
     "attention_one_pass_bytes", "attention_one_pass_supported",
+    "rope_frequencies", "qk_norm_rope_paged", "attention_paged_forward",
+    "attention_paged_workspace_floats", "logits_penalty_forward",
 ]
 
 
@@ -62,6 +66,16 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
 _sz = ctypes.c_size_t
+_i64 = ctypes.c_int64
+
+
+class PagedBatch(ctypes.Structure):
+    """include/llm_amd/paged.h PagedBatch."""
+    _fields_ = [("key_cache", _vp), ("value_cache", _vp), ("page_stride", _i64), ("slot_stride", _i64),
+                ("head_stride", _i64), ("page_table", _vp), ("q_start", _vp), ("kv_len", _vp),
+                ("n_seqs", _i), ("n_pages", _i), ("page_size", _i), ("table_pages", _i),
+                ("n_kv_heads", _i), ("head_dim", _i)]
+
 
 _SIGS = {
     "embedding_forward": (None, [_vp, _vp, _vp, _i, _vp]),
@@ -88,6 +102,11 @@ _SIGS = {
     "attention_one_pass_bytes": (_sz, [_i, _i, _i]),
     "attention_one_pass_supported": (_i, [_i, _i, _i, _i]),
     "sample_forward": (None, [_vp, _vp, _i, _f, _f, _vp]),
+    "rope_frequencies": (_f, [_vp, _i, ctypes.c_double, _i, ctypes.c_double, _i]),
+    "qk_norm_rope_paged": (None, [_vp] * 8 + [_i, _i, _i, _i, _f, _f] + [_i64] * 4 + [_vp]),
+    "attention_paged_forward": (None, [_vp] * 4 + [_i] * 5 + [_f, _i64, _i64, _vp]),
+    "attention_paged_workspace_floats": (_sz, [_i] * 7),
+    "logits_penalty_forward": (None, [_vp] * 12 + [_i] * 5 + [_i64, _i64, _vp]),
     "dump_open": (None, [ctypes.c_char_p]),
     "dump_close": (None, []),
     "dump_enabled": (_i, []),
@@ -409,3 +428,164 @@ def swiglu_forward(act, gate, up, n, stream=None):
         return
     _call(lib().swiglu_forward, _bf16(act, "act"), _bf16(gate, "gate"), _bf16(up, "up"), n,
           _stream(stream))
+
+
+# ---- serving operators over a paged KV cache (include/llm_amd/paged.h). They take tensors alone and
+# read every size and stride from them ----
+
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
+
+
+def rope_frequencies(rotary_dim, theta, kind=ROPE_PLAIN, factor=1.0, trained=0):
+    """(inv_freq, rope_scale): radians per position of the rotary_dim / 2 rotated pairs, a float64 CPU
+    tensor, and the factor of cos and sin, for positions stretched by `kind`."""
+    import torch
+    inv_freq = torch.zeros(max(rotary_dim // 2, 0), dtype=torch.float64)
+    scale = lib().rope_frequencies(inv_freq.data_ptr() or None, rotary_dim, theta, kind, factor, trained)
+    check()
+    return inv_freq, scale
+
+
+def _on_device(name, t, dtypes):
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise LlmError(f"{name} must be a tensor on the GPU")
+    if t.device.index != torch.cuda.current_device():
+        raise LlmError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if t.dtype not in dtypes:
+        raise LlmError(f"{name} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
+
+
+def _dense(name, t, dtype, shape):
+    """Address of a contiguous tensor of this type and shape; None stays None."""
+    if t is None:
+        return None
+    _on_device(name, t, (dtype,))
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise LlmError(f"{name} must be contiguous of shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _bits16():
+    import torch
+    return torch.bfloat16, torch.int16, torch.uint16
+
+
+def _head_rows(name, t, shape):
+    """(address, elements between rows) of rows of whole heads, contiguous within a row."""
+    _on_device(name, t, _bits16())
+    if tuple(t.shape) != tuple(shape):
+        raise LlmError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    n, heads, dim = t.shape
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != dim):
+        raise LlmError(f"the rows of {name} must be contiguous")
+    return t.data_ptr(), t.stride(0) if n > 1 else heads * dim
+
+
+def _paged_batch(key_cache, value_cache, page_table, q_start, kv_len):
+    import torch
+    for name, t in (("key_cache", key_cache), ("value_cache", value_cache)):
+        _on_device(name, t, _bits16())
+        if t.dim() != 4 or t.stride(3) != 1:
+            raise LlmError(f"{name} must have shape [pages, slots, kv heads, head_dim], the last contiguous")
+    if key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
+        raise LlmError("key_cache and value_cache must have the same shape and strides")
+    if page_table.dim() != 2:
+        raise LlmError(f"page_table must have shape [sequences, pages], got {tuple(page_table.shape)}")
+    pages, slots, kv_heads, dim = key_cache.shape
+    seqs = page_table.shape[0]
+    strides = [s if n > 1 else 0 for n, s in zip(key_cache.shape, key_cache.stride())]
+    return PagedBatch(key_cache.data_ptr(), value_cache.data_ptr(), *strides[:3],
+                      _dense("page_table", page_table, torch.int32, page_table.shape),
+                      _dense("q_start", q_start, torch.int32, (seqs + 1,)),
+                      _dense("kv_len", kv_len, torch.int32, (seqs,)),
+                      seqs, pages, slots, page_table.shape[1], kv_heads, dim)
+
+
+def qk_norm_rope_paged(q_out, q, k, v, q_norm_w, k_norm_w, inv_freq, key_cache, value_cache, page_table,
+                       q_start, kv_len, eps, rope_scale=1.0, interleaved=False, stream=None):
+    """Norm and rotation of q [tokens, heads, head_dim] into q_out and of k into key_cache, v into
+    value_cache [pages, slots, kv heads, head_dim], at the places that page_table [sequences, pages], q_start
+    [sequences + 1] and kv_len [sequences] give. inv_freq: float64 [rotary_dim / 2] on the GPU. Norm weights
+    None: no norm. Rows of q, k, v and q_out may lie apart (slices of one projection's rows)."""
+    import torch
+    batch = _paged_batch(key_cache, value_cache, page_table, q_start, kv_len)
+    if q.dim() != 3:
+        raise LlmError(f"q must have shape [tokens, heads, head_dim], got {tuple(q.shape)}")
+    n, heads, dim = q.shape[0], q.shape[1], batch.head_dim
+    rows = [_head_rows("q_out", q_out, (n, heads, dim)), _head_rows("q", q, (n, heads, dim)),
+            _head_rows("k", k, (n, batch.n_kv_heads, dim)), _head_rows("v", v, (n, batch.n_kv_heads, dim))]
+    for name, w in (("q_norm_w", q_norm_w), ("k_norm_w", k_norm_w)):
+        if w is not None:
+            _on_device(name, w, _bits16())
+            _dense(name, w, w.dtype, (dim,))
+    _on_device("inv_freq", inv_freq, (torch.float64,))
+    _dense("inv_freq", inv_freq, torch.float64, (inv_freq.numel(),))
+    _call(lib().qk_norm_rope_paged, *(r[0] for r in rows), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(inv_freq),
+          ctypes.byref(batch), n, heads, 2 * inv_freq.numel(), int(interleaved), eps, rope_scale,
+          *(r[1] for r in rows), _stream(stream))
+
+
+def attention_paged_workspace_floats(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len):
+    floats = lib().attention_paged_workspace_floats(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim,
+                                                    max_q_len, max_kv_len)
+    check()
+    return floats
+
+
+def attention_paged_forward(out, q, key_cache, value_cache, page_table, q_start, kv_len, ws, scale,
+                            max_q_len, max_kv_len, window=0, stream=None):
+    """Attention of q [tokens, heads, head_dim] over the pages of its rows' sequences, into out. ws: a
+    float32 tensor of at least attention_paged_workspace_floats(...) floats for these sizes (None where that
+    is 0), kept between calls that do not overlap."""
+    import torch
+    batch = _paged_batch(key_cache, value_cache, page_table, q_start, kv_len)
+    if q.dim() != 3:
+        raise LlmError(f"q must have shape [tokens, heads, head_dim], got {tuple(q.shape)}")
+    n, heads, dim = q.shape[0], q.shape[1], batch.head_dim
+    out_at, out_stride = _head_rows("out", out, (n, heads, dim))
+    q_at, q_stride = _head_rows("q", q, (n, heads, dim))
+    if n and heads % max(batch.n_kv_heads, 1) == 0:
+        need = attention_paged_workspace_floats(n, batch.n_seqs, heads, batch.n_kv_heads, dim, max_q_len,
+                                                max_kv_len)
+        have = 0 if ws is None else ws.numel()
+        if have < need:
+            raise LlmError(f"ws holds {have} floats, attention needs {need}")
+    if ws is not None:
+        _dense("ws", ws, torch.float32, ws.shape)
+    _call(lib().attention_paged_forward, out_at, q_at, ctypes.byref(batch), _ptr(ws), n, heads, max_q_len,
+          max_kv_len, window, scale, out_stride, q_stride, _stream(stream))
+
+
+def logits_penalty_forward(out, logits, tokens=None, prompt_len=None, token_len=None, repetition=None,
+                           frequency=None, presence=None, bias_tokens=None, bias=None, bias_len=None,
+                           allowed=None, stream=None):
+    """Penalties over each row's tokens [rows, capacity], biases [rows, capacity] and the mask of allowed
+    tokens [rows, words] (int32 words, bit t % 32 of word t / 32) on logits [rows, vocab], into out (which
+    may be logits)."""
+    import torch
+    for name, t in (("out", out), ("logits", logits)):
+        _on_device(name, t, _bits16())
+        if t.dim() != 2 or t.shape != logits.shape or (t.shape[1] > 1 and t.stride(1) != 1):
+            raise LlmError(f"{name} must have shape [rows, vocab], the same for both, with contiguous rows")
+    rows, vocab = logits.shape
+    strides = [t.stride(0) if rows > 1 else max(vocab, 1) for t in (out, logits)]
+    if allowed is not None:
+        _on_device("allowed", allowed, (torch.int32, torch.uint32))
+    wide = {}
+    for name, t in (("tokens", tokens), ("bias_tokens", bias_tokens), ("allowed", allowed)):
+        if t is not None and t.dim() != 2:
+            raise LlmError(f"{name} must have two dimensions, got {tuple(t.shape)}")
+        wide[name] = 0 if t is None else t.shape[1]
+    _call(lib().logits_penalty_forward, out.data_ptr() or None, logits.data_ptr() or None,
+          _dense("tokens", tokens, torch.int32, (rows, wide["tokens"])),
+          _dense("prompt_len", prompt_len, torch.int32, (rows,)),
+          _dense("token_len", token_len, torch.int32, (rows,)),
+          _dense("repetition", repetition, torch.float32, (rows,)),
+          _dense("frequency", frequency, torch.float32, (rows,)),
+          _dense("presence", presence, torch.float32, (rows,)),
+          _dense("bias_tokens", bias_tokens, torch.int32, (rows, wide["bias_tokens"])),
+          _dense("bias", bias, torch.float32, (rows, wide["bias_tokens"])),
+          _dense("bias_len", bias_len, torch.int32, (rows,)),
+          allowed if allowed is None else _dense("allowed", allowed, allowed.dtype, (rows, wide["allowed"])),
+          rows, vocab, wide["tokens"], wide["bias_tokens"], wide["allowed"], *strides, _stream(stream))

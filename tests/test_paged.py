@@ -1,0 +1,696 @@
+"""Operators over a paged KV cache (include/llm_amd/paged.h) against their definitions in 64 bits: the
+QK-norm + RoPE that writes pages, the attention over pages, both together with the logits' penalties as a
+serving loop runs them, in captured graphs too; and what they refuse."""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+HALF_STEP = 2.0 ** -8   # of bf16, relative to the value
+F32 = 2.0 ** -24        # half a step of fp32
+
+
+# ---------------------------------------------------------------- batches
+
+class Batch:
+    """Sequences (new rows, cached tokens with them) over a shuffled pool. Slots that hold no token of
+    a sequence hold NaN and infinities."""
+
+    def __init__(self, seqs, kv_heads, dim, page, seed, lead=0, trail=0, extra_pages=3, layout="pages"):
+        import torch
+        self.seqs, self.kv_heads, self.dim, self.page = seqs, kv_heads, dim, page
+        self.rng = np.random.default_rng(seed)
+        g = self.g = torch.Generator().manual_seed(seed)
+        need = [max(0, -(-n // page)) for _, n in seqs]
+        self.pages = sum(need) + extra_pages
+        self.table_pages = max(need + [1]) + 1
+        order = torch.randperm(self.pages, generator=g)
+        table = torch.full((len(seqs), self.table_pages), -1, dtype=torch.int32)
+        at = 0
+        for s, n in enumerate(need):
+            table[s, :n] = order[at:at + n].int()
+            at += n
+        self.table = table
+        starts = [lead]
+        for new, _ in seqs:
+            starts.append(starts[-1] + new)
+        self.starts, self.tokens = starts, starts[-1] + trail
+        self.q_start = torch.tensor(starts, dtype=torch.int32)
+        self.kv_len = torch.tensor([n for _, n in seqs], dtype=torch.int32)
+        bad = torch.tensor([math.nan, math.inf, -math.inf])
+        self.k, self.v = (bad[torch.randint(0, 3, (self.pages, page, kv_heads, dim), generator=g)].bfloat16()
+                          for _ in range(2))
+        for s, (_, n) in enumerate(seqs):
+            for p in range(max(0, n)):
+                slot = self.slot(s, p)
+                if slot:
+                    self.k[slot], self.v[slot] = self.normal(kv_heads, dim), self.normal(kv_heads, dim)
+        self.layout = layout
+
+    def normal(self, *shape, std=1.0):
+        import torch
+        return (torch.randn(*shape, generator=self.g) * std).bfloat16()
+
+    def slot(self, s, p):
+        if p < 0 or p // self.page >= self.table.shape[1]:
+            return None
+        page = int(self.table[s, p // self.page])
+        return (page, p % self.page) if 0 <= page < self.pages else None
+
+    def rows(self):
+        """(row, sequence, position) of every row of a sequence."""
+        for s, (new, n) in enumerate(self.seqs):
+            for i in range(new):
+                yield self.starts[s] + i, s, n - new + i
+
+    def pools(self):
+        """The caches on the GPU, dense or as views of one pool that holds both (by page, by kv head)."""
+        import torch
+        if self.layout == "pages":
+            return self.k.cuda(), self.v.cuda()
+        both = torch.empty(self.pages, 2, self.kv_heads, self.page, self.dim, dtype=torch.bfloat16, device="cuda")
+        k, v = both[:, 0].transpose(1, 2), both[:, 1].transpose(1, 2)
+        k.copy_(self.k)
+        v.copy_(self.v)
+        return k, v
+
+    def where(self):
+        return self.table.cuda(), self.q_start.cuda(), self.kv_len.cuda()
+
+
+def bits(t):
+    import torch
+    return t.contiguous().view(torch.int16).cpu()
+
+
+def workspace(gpu, b, heads, max_q, max_kv):
+    import torch
+    n = gpu.attention_paged_workspace_floats(b.tokens, len(b.seqs), heads, b.kv_heads, b.dim, max_q, max_kv)
+    return torch.full((max(n, 1),), math.nan, device="cuda")
+
+
+# ---------------------------------------------------------------- QK-norm + RoPE into pages
+
+def rotated(x, weight, pos, inv_freq, scale, interleaved, eps):
+    """(value, a bound on its fp32 arithmetic's error) of one row's heads [heads, dim] in 64 bits."""
+    x = x.double().numpy()
+    dim = x.shape[-1]
+    err = 8 * F32
+    if weight is not None:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * weight.double().numpy()
+        err += (dim / 2 + 8) * F32  # the sum of squares under the root, then root, quotient and products
+    n = 2 * len(inv_freq)
+    i = np.arange(n // 2)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + n // 2)
+    angle = pos * inv_freq
+    c, s = np.cos(angle) * scale, np.sin(angle) * scale
+    y, size = x.copy(), np.abs(x)
+    y[:, a], y[:, b] = x[:, a] * c - x[:, b] * s, x[:, b] * c + x[:, a] * s
+    size[:, a] = size[:, b] = (size[:, a] + size[:, b]) * abs(scale)
+    return y, err * size
+
+
+def close(got, want, err):
+    """got is bf16 of a value within err of want."""
+    got = got.double().numpy()
+    off = np.abs(got - want) - (HALF_STEP * (np.abs(want) + err) + err)
+    assert (off <= 0).all(), f"{(off > 0).sum()} of {off.size} off by up to {off.max():.3g} more than allowed"
+
+
+APPEND = [
+    # heads, kv heads, dim, rotary, interleaved, norm, page, sequences (new, cached), layout
+    (16, 8, 128, 128, False, True, 16, [(1, 261)], "pages"),
+    (32, 8, 128, 128, False, True, 16, [(1, 1), (1, 16), (1, 17), (1, 300)], "pages"),
+    (5, 1, 128, 128, True, True, 7, [(19, 40), (0, 9), (1, 3)], "heads"),
+    (6, 2, 64, 32, True, False, 1, [(33, 33)], "pages"),
+    (3, 3, 64, 64, False, True, 32, [(70, 131), (2, 65)], "heads"),
+    (4, 4, 256, 256, False, True, 16, [(9, 9), (17, 100)], "pages"),
+    (8, 2, 256, 16, True, True, 128, [(130, 130)], "heads"),
+    (9, 3, 128, 48, False, False, 24, [(3, 25), (25, 25)], "pages"),
+    # sequences longer in new rows than in cached tokens: the first rows' positions are negative
+    (2, 1, 64, 64, False, True, 16, [(5, 2), (3, 0), (2, 2)], "pages"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(APPEND)))
+@pytest.mark.parametrize("fused", [False, True])
+def test_append_against_the_definition(gpu, case, fused):
+    import torch
+    heads, kv_heads, dim, rotary, interleaved, norm, page, seqs, layout = APPEND[case]
+    b = Batch(seqs, kv_heads, dim, page, 100 + case, lead=2, trail=3, layout=layout)
+    # one page of the first sequence is not there
+    gone = case % 2 == 1 and seqs[0][1] > page
+    if gone:
+        b.table[0, 0] = b.pages if case % 4 == 1 else -7
+    rows = b.normal(b.tokens, heads + 2 * kv_heads, dim)
+    q, k, v = rows[:, :heads], rows[:, heads:heads + kv_heads], rows[:, heads + kv_heads:]
+    qn, kn = (b.normal(dim), b.normal(dim)) if norm else (None, None)
+    kind = [gpu.ROPE_PLAIN, gpu.ROPE_LINEAR, gpu.ROPE_YARN][case % 3]
+    inv_freq, scale = gpu.rope_frequencies(rotary, 1e4 if case % 2 else 1e6, kind, 4.0 if kind else 1.0, 4096)
+    kc, vc = b.pools()
+    dev = [t.cuda() for t in (q, k, v)]
+    if fused:
+        whole = rows.cuda()
+        dev = [whole[:, :heads], whole[:, heads:heads + kv_heads], whole[:, heads + kv_heads:]]
+    q_out = torch.full((b.tokens, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    gpu.qk_norm_rope_paged(q_out, *dev, qn.cuda() if norm else None, kn.cuda() if norm else None,
+                           inv_freq.cuda(), kc, vc, *b.where(), 1e-6, scale, interleaved=interleaved)
+    got_q, got_k, got_v = q_out.cpu(), kc.cpu(), vc.cpu()
+    written = torch.zeros(b.pages, page, dtype=torch.bool)
+    mine = torch.zeros(b.tokens, dtype=torch.bool)
+    for t, s, p in b.rows():
+        mine[t] = True
+        close(got_q[t], *rotated(q[t], qn, p, inv_freq.numpy(), scale, interleaved, 1e-6))
+        slot = b.slot(s, p)
+        if slot:
+            written[slot] = True
+            close(got_k[slot], *rotated(k[t], kn, p, inv_freq.numpy(), scale, interleaved, 1e-6))
+            assert torch.equal(bits(got_v[slot]), bits(v[t]))
+    assert (got_q[~mine] == 7).all()
+    for got, before in ((got_k, b.k), (got_v, b.v)):
+        assert torch.equal(bits(got[~written]), bits(before[~written]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_append_far_positions_and_in_place(gpu, interleaved):
+    """A long context's last rows (positions around 2^20): the angle's 64 bits; q_out may be q."""
+    import torch
+    heads, dim, page, far = 4, 128, 64, (1 << 20) + 5
+    b = Batch([(3, 3)], 2, dim, page, 5)
+    b.seqs = [(3, far)]
+    b.kv_len = torch.tensor([far], dtype=torch.int32)
+    table = torch.full((1, far // page + 1), -1, dtype=torch.int32)
+    table[0, -1] = 2
+    table[0, -2] = 1
+    b.table, b.table_pages = table, table.shape[1]
+    q, k, v = b.normal(3, heads, dim), b.normal(3, 2, dim), b.normal(3, 2, dim)
+    inv_freq, scale = gpu.rope_frequencies(dim, 1e6)
+    kc, vc = b.pools()
+    q_dev = q.cuda()
+    gpu.qk_norm_rope_paged(q_dev, q_dev, k.cuda(), v.cuda(), None, None, inv_freq.cuda(), kc, vc, *b.where(),
+                           1e-6, interleaved=interleaved)
+    for t, s, p in b.rows():
+        close(q_dev[t].cpu(), *rotated(q[t], None, p, inv_freq.numpy(), 1.0, interleaved, 0))
+        slot = b.slot(s, p)
+        close(kc.cpu()[slot], *rotated(k[t], None, p, inv_freq.numpy(), 1.0, interleaved, 0))
+        assert torch.equal(bits(vc.cpu()[slot]), bits(v[t]))
+
+
+def test_rope_frequencies(pkg):
+    """Closed forms: the powers; divided pairs; YaRN's ends and its ramp, which is straight in the pair."""
+    j = np.arange(64)
+    base = 1e6 ** (-2.0 * j / 128)
+    got, scale = pkg.rope_frequencies(128, 1e6)
+    assert scale == 1.0 and np.allclose(got.numpy(), base, rtol=1e-14, atol=0)
+    got, scale = pkg.rope_frequencies(128, 1e6, pkg.ROPE_LINEAR, 8.0)
+    assert scale == 1.0 and np.allclose(got.numpy(), base / 8, rtol=1e-14, atol=0)
+    got, scale = pkg.rope_frequencies(128, 1e6, pkg.ROPE_YARN, 4.0, 32768)
+    assert scale == pytest.approx(0.1 * math.log(4) + 1, rel=1e-6)
+    turns = 32768 * base / (2 * math.pi)
+    share = (base - got.numpy()) / (base - base / 4)  # 0: left as it is, 1: divided
+    assert np.allclose(share[turns > 32 * 1.3], 0, atol=1e-12) and np.allclose(share[turns < 0.7], 1, atol=1e-12)
+    inner = (share > 1e-9) & (share < 1 - 1e-9)
+    assert inner.sum() > 8 and np.allclose(np.diff(share[inner]), np.diff(share[inner])[0], atol=1e-9)
+    for args in [(0, 1e4), (7, 1e4), (64, 1.0), (64, math.nan), (64, 1e4, 3), (64, 1e4, 1, 0.5),
+                 (64, 1e4, 2, math.inf, 4096), (64, 1e4, 2, 2.0, 0)]:
+        with pytest.raises(pkg.LlmError, match="rope_frequencies"):
+            pkg.rope_frequencies(*args)
+
+
+# ---------------------------------------------------------------- attention over pages
+
+def attended(b, q, scale, window):
+    """(value, a bound on the error before the last rounding) in 64 bits, row by row and key by key that
+    the row sees; rows of no sequence None. The bound: every weight is off by its rounding to bf16 and
+    by twice its score's error (the dot's fp32 sums, then the largest score's), the sums in fp32."""
+    k, v = b.k.double().numpy(), b.v.double().numpy()
+    q = q.double().numpy()
+    heads, dim = q.shape[1:]
+    out, err = np.zeros(q.shape), np.zeros(q.shape)
+    for t, s, p in b.rows():
+        first = max(0, p - window + 1) if window else 0
+        slots = [b.slot(s, i) for i in range(first, p + 1)]
+        slots = [x for x in slots if x]
+        if not slots:
+            continue
+        pages, at = np.array(slots).T
+        for h in range(heads):
+            kk, vv = (x[pages, at, h // (heads // b.kv_heads)] for x in (k, v))
+            with np.errstate(all="ignore"):
+                score = kk @ q[t, h] * scale
+                keep = score != -np.inf
+                if not keep.any():
+                    continue
+                score, kk, vv = score[keep], kk[keep], vv[keep]
+                w = np.exp(score - score.max())
+                w /= w.sum()
+                out[t, h] = w @ vv
+                off = 2 * (dim * F32 * (np.abs(kk) @ np.abs(q[t, h])).max() * scale + 8 * F32 * np.abs(score).max())
+                err[t, h] = (HALF_STEP + off + (len(w) + 64) * F32) * (w @ np.abs(vv))
+    return out, err
+
+
+def attend(gpu, b, q, scale, window=0, max_q=None, max_kv=None, pools=None, ws=None, out=None):
+    import torch
+    heads = q.shape[1]
+    max_q = max_q or max([new for new, _ in b.seqs] + [1])
+    max_kv = max_kv or max([n for _, n in b.seqs] + [1])
+    kc, vc = pools or b.pools()
+    ws = workspace(gpu, b, heads, max_q, max_kv) if ws is None else ws
+    out = torch.full((b.tokens, heads, b.dim), 7.0, dtype=torch.bfloat16, device="cuda") if out is None else out
+    gpu.attention_paged_forward(out, q.cuda(), kc, vc, *b.where(), ws, scale, max_q, max_kv, window=window)
+    return out
+
+
+def check_attend(b, out, q, scale, window):
+    import torch
+    got = out.cpu()
+    want, err = attended(b, q, scale, window)
+    mine = [t for t, _, _ in b.rows()]
+    fine = np.isfinite(want[mine])
+    assert np.array_equal(fine, np.isfinite(got[mine].double().numpy())), "finite elsewhere than the definition"
+    close(got[mine][torch.from_numpy(fine)], want[mine][fine], err[mine][fine])
+    other = np.setdiff1d(np.arange(b.tokens), mine)
+    assert (got[other] == 7).all(), "rows of no sequence were written"
+
+
+ATTEND = [
+    # heads, kv heads, dim, page, window, sequences (new, cached), layout
+    (16, 8, 128, 16, 0, [(1, 261)], "pages"),
+    (16, 8, 128, 16, 0, [(1, 1)], "pages"),
+    (32, 8, 128, 16, 0, [(1, 1), (1, 31), (1, 32), (1, 33), (1, 64), (1, 65), (1, 700), (1, 129)], "pages"),
+    (4, 4, 128, 1, 0, [(1, 77), (1, 5)], "heads"),
+    (7, 1, 128, 24, 0, [(1, 500), (3, 130), (4, 4)], "pages"),
+    (40, 1, 64, 16, 0, [(1, 300), (2, 90)], "heads"),
+    (6, 2, 64, 7, 50, [(1, 200), (13, 149), (1, 20)], "pages"),
+    (8, 2, 256, 16, 0, [(1, 90), (1, 257), (5, 40)], "pages"),
+    (2, 2, 256, 128, 33, [(70, 200)], "heads"),
+    (8, 2, 128, 64, 0, [(200, 333)], "pages"),
+    (4, 4, 64, 32, 0, [(129, 129), (1, 400), (64, 64), (65, 300)], "heads"),
+    (24, 4, 64, 16, 100, [(150, 400), (131, 131)], "pages"),
+    (12, 3, 128, 16, 1, [(40, 80), (1, 9)], "pages"),
+    (16, 8, 128, 32, 0, [(127, 300), (1, 17), (0, 50), (1, 900), (30, 30)], "heads"),
+    (6, 1, 256, 20, 0, [(90, 311)], "pages"),
+    # nothing cached, nothing new, more new rows than cached tokens: rows that see nothing
+    (4, 2, 128, 16, 0, [(1, 0), (0, 0), (5, 2), (1, 1), (2, -3)], "pages"),
+    (4, 2, 64, 16, 4, [(40, 7), (70, 40)], "pages"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", range(len(ATTEND)))
+def test_attention_against_the_definition(gpu, case):
+    heads, kv_heads, dim, page, window, seqs, layout = ATTEND[case]
+    b = Batch(seqs, kv_heads, dim, page, 200 + case, lead=1, trail=2, layout=layout)
+    q = b.normal(b.tokens, heads, dim, std=1.5)
+    scale = 1 / math.sqrt(dim)
+    check_attend(b, attend(gpu, b, q, scale, window), q, scale, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_q,max_kv", [(1, 1), (1, 4000), (400, 1), (5000, 100000), (33, 70000)])
+@pytest.mark.parametrize("case", [2, 4, 9, 13])
+def test_attention_whatever_the_expected_lengths(gpu, case, max_q, max_kv):
+    """The expected lengths split the work and nothing else: shorter and longer ones than the batch has."""
+    heads, kv_heads, dim, page, window, seqs, layout = ATTEND[case]
+    b = Batch(seqs, kv_heads, dim, page, 300 + case, lead=1, trail=2, layout=layout)
+    q = b.normal(b.tokens, heads, dim, std=1.5)
+    scale = 1 / math.sqrt(dim)
+    check_attend(b, attend(gpu, b, q, scale, window, max_q, max_kv), q, scale, window)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,dim,heads", [([(1, 9000)], 128, 4), ([(1, 70000), (1, 3)], 64, 2),
+                                            ([(3, 5000), (1, 2500), (1, 1)], 256, 2), ([(150, 6000)], 128, 2)])
+def test_attention_long_histories(gpu, seqs, dim, heads):
+    """Split over the keys: a peak of the scores late, early and in the middle of the history."""
+    import torch
+    b = Batch(seqs, 1, dim, 64, 7)
+    q = b.normal(b.tokens, heads, dim)
+    for p, size in ((3, 6.0), (seqs[0][1] // 2, 9.0), (seqs[0][1] - 1, 12.0)):
+        b.k[b.slot(0, p)] = (q[0, 0].float() * size / 4).bfloat16()
+    scale = 1 / math.sqrt(dim)
+    out = attend(gpu, b, q, scale)
+    check_attend(b, out, q, scale, 0)
+    again = attend(gpu, b, q, scale)
+    assert torch.equal(bits(out), bits(again))  # the joins have one order
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,window,dim", [([(40, 100), (1, 100), (1, 65)], 0, 128),
+                                             ([(40, 100), (1, 100), (1, 65)], 21, 64),
+                                             ([(200, 230)], 0, 128), ([(200, 230)], 30, 256)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_attention_bad_values_stay_with_the_rows_that_see_them(gpu, seqs, window, dim, bad, which):
+    """A NaN or an infinity in a key or value: rows in front of its position and past its window are what
+    they are without it; pages that are not there are not seen."""
+    heads, kv_heads = 4, 2
+    b = Batch(seqs, kv_heads, dim, 16, 11)
+    q = b.normal(b.tokens, heads, dim)
+    last = seqs[0][1] - 1
+    for p, h, d in ((last, 0, 3), (last - 20, 1, dim - 1), (last - 7, 0, dim // 2)):
+        getattr(b, which)[b.slot(0, p) + (h, d)] = bad
+    b.table[0, 1] = -1
+    if len(seqs) > 1:
+        b.table[1, 2] = b.pages + 5
+    scale = 1 / math.sqrt(dim)
+    check_attend(b, attend(gpu, b, q, scale, window), q, scale, window)
+
+
+@pytest.mark.gpu
+def test_attention_scores_of_minus_infinity(gpu):
+    """A score of -inf weighs nothing; a row of none but those gives zeros, as one that sees nothing."""
+    b = Batch([(1, 40), (70, 90), (1, 30)], 2, 64, 16, 13)
+    q = b.normal(b.tokens, 4, 64)
+    q[:, :, 5] = 1.0
+    for s, p in [(0, 3), (0, 39), (1, 20), (1, 60), (1, 89)] + [(2, p) for p in range(30)]:
+        b.k[b.slot(s, p)] = 0
+        b.k[b.slot(s, p) + (slice(None), 5)] = -math.inf
+    out = attend(gpu, b, q, 0.125)
+    check_attend(b, out, q, 0.125, 0)
+    assert (out[-1] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [1e-30, 1.0, 3e4])
+def test_attention_extreme_scores(gpu, size):
+    """Scores far apart (one key takes it all), tiny, and a large scale."""
+    import torch
+    b = Batch([(1, 200), (70, 70)], 2, 128, 16, 17)
+    q = (b.normal(b.tokens, 4, 128).float() * size).bfloat16()
+    if size > 1:  # one key ahead of the others by more than any rounding of the scores
+        for s, n in ((0, 200), (1, 70)):
+            for p in range(n):
+                b.k[b.slot(s, p)] = (torch.ones(2, 128) * (1.0 if p == 0 else -1.0)).bfloat16()
+        q = q.abs()
+    for scale in (1 / math.sqrt(128), 4.0):
+        if size == 1.0 and scale == 4.0:
+            continue  # sums of many near-equal large scores: the bound is of no use
+        check_attend(b, attend(gpu, b, q, scale), q, scale, 0)
+
+
+@pytest.mark.gpu
+def test_attention_pools_past_32_bits(gpu):
+    """Pages past 2^31 elements and 2^32 bytes of the pool, written and read."""
+    import torch
+    kv_heads, dim, page = 8, 128, 64
+    b = Batch([(1, 200), (90, 120)], kv_heads, dim, page, 19)
+    pages = (1 << 31) // (page * kv_heads * dim) + 40
+    far = torch.arange(b.pages, dtype=torch.int32) + (pages - b.pages)
+    kc, vc = (torch.empty(pages, page, kv_heads, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    kc[far[0]:], vc[far[0]:] = b.k.cuda(), b.v.cuda()
+    q, k, v = b.normal(b.tokens, 16, dim), b.normal(b.tokens, kv_heads, dim), b.normal(b.tokens, kv_heads, dim)
+    inv_freq, scale = gpu.rope_frequencies(dim, 1e6)
+    table = torch.where(b.table >= 0, b.table + int(far[0]), b.table).cuda()
+    q_out = torch.empty_like(q, device="cuda")
+    gpu.qk_norm_rope_paged(q_out, q.cuda(), k.cuda(), v.cuda(), None, None, inv_freq.cuda(), kc, vc, table,
+                           b.q_start.cuda(), b.kv_len.cuda(), 1e-6)
+    b.k, b.v = kc[far[0]:].cpu(), vc[far[0]:].cpu()
+    for t, s, p in b.rows():
+        close(b.k[b.slot(s, p)], *rotated(k[t], None, p, inv_freq.numpy(), 1.0, False, 0))
+        assert torch.equal(bits(b.v[b.slot(s, p)]), bits(v[t]))
+    out = torch.full((b.tokens, 16, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    ws = workspace(gpu, b, 16, 90, 200)
+    gpu.attention_paged_forward(out, q_out, kc, vc, table, b.q_start.cuda(), b.kv_len.cuda(), ws, 0.09, 90, 200)
+    check_attend(b, out, q_out.cpu(), 0.09, 0)
+
+
+@pytest.mark.gpu
+def test_attention_strided_rows(gpu):
+    """q from one projection's rows, out into a wider buffer's rows, whose rest stays."""
+    import torch
+    b = Batch([(3, 50), (40, 70)], 2, 64, 16, 23, trail=1)
+    q = b.normal(b.tokens, 4, 64)
+    rows = torch.zeros(b.tokens, 8, 64, dtype=torch.bfloat16, device="cuda")
+    rows[:, :4] = q.cuda()
+    wide = torch.full((b.tokens, 6, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    kc, vc = b.pools()
+    gpu.attention_paged_forward(wide[:, :4], rows[:, :4], kc, vc, *b.where(), workspace(gpu, b, 4, 40, 70), 0.125, 40, 70)
+    check_attend(b, wide[:, :4].contiguous(), q, 0.125, 0)
+    assert (wide[:, 4:] == 7).all()
+
+
+# ---------------------------------------------------------------- together
+
+@pytest.mark.gpu
+def test_serving_loop_with_captured_steps(gpu):
+    """Two prompts (one in two chunks), then tokens: rows into pages, attention over them, penalties and
+    the pick. The whole against 64 bits; the token steps once eagerly and once as one captured graph that
+    is replayed as lengths grow, with other work between, equal to the eager ones bit for bit."""
+    import torch
+    heads, kv_heads, dim, page, vocab, steps = 8, 2, 128, 16, 1003, 5
+    rng = torch.Generator().manual_seed(3)
+
+    def normal(*shape, std=1.0):
+        return (torch.randn(*shape, generator=rng) * std).bfloat16()
+
+    prompts, pages = [70, 21], 14
+    table = torch.randperm(pages, generator=rng).int().view(2, 7)
+    inv_freq, scale_r = gpu.rope_frequencies(dim, 1e6, gpu.ROPE_YARN, 4.0, 64)
+    qn, kn = normal(dim, std=0.1) + 1, normal(dim, std=0.1) + 1
+    head = normal(vocab, heads * dim, std=0.05).cuda()
+    total = [p + steps for p in prompts]
+    rows = [[normal(n, h, dim) for n in total] for h in (heads, kv_heads, kv_heads)]
+
+    def run(captured):
+        kc, vc = (torch.zeros(pages, page, kv_heads, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        history = torch.zeros(2, 16, dtype=torch.int32, device="cuda")
+        lens = torch.zeros(2, dtype=torch.int32, device="cuda")
+        prompt_len = torch.ones(2, dtype=torch.int32, device="cuda")
+        rep, freq = torch.full((2,), 1.3, device="cuda"), torch.full((2,), 0.4, device="cuda")
+        d = [qn.cuda(), kn.cuda(), inv_freq.cuda()]
+        outs, picks, all_logits, turned = [], [], [], []
+
+        def layer(q, k, v, where, out, ws, max_q):
+            gpu.qk_norm_rope_paged(q, q, k, v, *d, kc, vc, *where, 1e-6, scale_r)
+            gpu.attention_paged_forward(out, q, kc, vc, *where, ws, 0.09, max_q, 112)
+
+        # chunks: 40 + 0 rows, then 30 + 21
+        for spans in [((0, 40), (0, 0)), ((40, 70), (0, 21))]:
+            q, k, v = (torch.cat([rows[i][s][a:e] for s, (a, e) in enumerate(spans)]).cuda() for i in range(3))
+            n = [e - a for a, e in spans]
+            where = (table.cuda(), torch.tensor([0, n[0], n[0] + n[1]], dtype=torch.int32).cuda(),
+                     torch.tensor([e for _, e in spans], dtype=torch.int32).cuda())
+            ws = torch.empty(max(1, gpu.attention_paged_workspace_floats(sum(n), 2, heads, kv_heads, dim, 40, 112)), device="cuda")
+            out = torch.empty_like(q)
+            layer(q, k, v, where, out, ws, 40)
+            outs.append(out.cpu())
+            turned.append(q.cpu())
+        # token steps: fixed buffers
+        q, k, v = (torch.empty(2, h, dim, dtype=torch.bfloat16, device="cuda") for h in (heads, kv_heads, kv_heads))
+        where = (table.cuda(), torch.arange(3, dtype=torch.int32).cuda(), torch.tensor(prompts, dtype=torch.int32).cuda())
+        ws = torch.empty(max(1, gpu.attention_paged_workspace_floats(2, 2, heads, kv_heads, dim, 1, 112)), device="cuda")
+        out = torch.empty_like(q)
+        logits, raw = (torch.empty(2, vocab, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        pick = torch.zeros(2, dtype=torch.int32, device="cuda")
+
+        def step():
+            layer(q, k, v, where, out, ws, 1)
+            for s in range(2):
+                gpu.gemv_forward(raw[s], head, out[s], vocab, heads * dim)
+            gpu.logits_penalty_forward(logits, raw, history, prompt_len, lens, rep, freq)
+            for s in range(2):
+                gpu.argmax_forward(pick[s:s + 1], logits[s], vocab)
+
+        graph = None
+        for i in range(steps):
+            for buffer, source in ((q, rows[0]), (k, rows[1]), (v, rows[2])):
+                buffer.copy_(torch.stack([source[s][prompts[s] + i] for s in range(2)]))
+            where[2].add_(1)
+            if captured and graph is None:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    step()
+            if graph:
+                graph.replay()
+            else:
+                step()
+            torch.cuda.synchronize()
+            outs.append(out.cpu())
+            turned.append(q.cpu())
+            all_logits.append((raw.cpu(), logits.cpu()))
+            picks.append(pick.cpu())
+            history[:, i] = pick
+            lens.add_(1)
+        return outs, turned, picks, all_logits, kc.cpu(), vc.cpu()
+
+    eager, again = run(False), run(True)
+    for x, y in zip(eager, again):
+        for a, c in zip(*((z,) if torch.is_tensor(z) else (z,) for z in (x, y))):
+            pairs = zip(a, c) if isinstance(a, (list, tuple)) else [(a, c)]
+            for m, n in pairs:
+                m, n = (m, n) if isinstance(m, tuple) else ((m,), (n,))
+                assert all(torch.equal(u.view(torch.int16) if u.dtype == torch.bfloat16 else u,
+                                       w.view(torch.int16) if w.dtype == torch.bfloat16 else w) for u, w in zip(m, n))
+    outs, turned, picks, all_logits, kc, vc = eager
+
+    # the attention of every row against 64 bits, over the caches that the loop wrote
+    b = Batch([(total[s], total[s]) for s in range(2)], kv_heads, dim, page, 1)
+    b.table, b.table_pages, b.pages, b.k, b.v = table, 7, pages, kc, vc
+
+    def in_order(x):  # rows of the chunks and steps by sequence and position
+        return torch.cat([x[0], x[1][:30]] + [o[:1] for o in x[2:]] + [x[1][30:]] + [o[1:] for o in x[2:]])
+
+    q = in_order(turned)
+    for t, s, p in b.rows():
+        close(q[t], *rotated(rows[0][s][p], qn, p, inv_freq.numpy(), scale_r, False, 1e-6))
+        close(kc[b.slot(s, p)], *rotated(rows[1][s][p], kn, p, inv_freq.numpy(), scale_r, False, 1e-6))
+    close(in_order(outs), *attended(b, q, 0.09, 0))
+
+    # the picks: penalties by their definition on the loop's own logits, the lowest index of the largest
+    for i, (raw, logits) in enumerate(all_logits):
+        for s in range(2):
+            x = raw[s].double()
+            before = [int(picks[j][s]) for j in range(i)]
+            for t in set(before):
+                x[t] = x[t] / float(np.float32(1.3)) if x[t] > 0 else x[t] * float(np.float32(1.3))
+                n = before[1:].count(t)
+                x[t] -= float(np.float32(0.4)) * n
+            close(logits[s], x.numpy(), 8 * F32 * (np.abs(x.numpy()) + 4))
+            assert int(picks[i][s]) == int(torch.nonzero(logits[s] == logits[s].max())[0])
+
+
+@pytest.mark.gpu
+def test_two_captured_graphs_and_streams(gpu):
+    """Two graphs with a workspace each, replayed at once on two streams, with eager work on a third; every
+    replay equal to the eager result."""
+    import torch
+    made = []
+    for seed, seqs, heads in ((1, [(1, 3000), (1, 40)], 8), (2, [(1, 700), (60, 900)], 4)):
+        b = Batch(seqs, 2, 128, 16, seed)
+        q = b.normal(b.tokens, heads, 128).cuda()
+        max_q, max_kv = max(n for n, _ in seqs), max(n for _, n in seqs)
+        ws, out, pools, where = workspace(gpu, b, heads, max_q, max_kv), torch.zeros_like(q), b.pools(), b.where()
+        args = (q, *pools, *where, ws, 0.09, max_q, max_kv)
+        gpu.attention_paged_forward(out, *args)
+        want = out.clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            gpu.attention_paged_forward(out, *args)
+        made.append((graph, out, want, args))
+    streams = [torch.cuda.Stream() for _ in made]
+    for _ in range(4):
+        torch.cuda.synchronize()
+        for (graph, out, _, _), stream in zip(made, streams):
+            with torch.cuda.stream(stream):
+                out.zero_()
+                graph.replay()
+        torch.randn(1000, 1000, device="cuda").sum()
+        torch.cuda.synchronize()
+        for _, out, want, args in made:
+            assert torch.equal(bits(out), bits(want))
+            out.fill_(3)
+            gpu.attention_paged_forward(out, *args, stream=streams[0])
+            torch.cuda.synchronize()
+            assert torch.equal(bits(out), bits(want))
+
+
+# ---------------------------------------------------------------- refusals
+
+def record(pkg, **change):
+    base = dict(key_cache=0x1000, value_cache=0x1000, page_stride=2048, slot_stride=128, head_stride=64,
+                page_table=0x1000, q_start=0x1000, kv_len=0x1000, n_seqs=2, n_pages=4, page_size=16,
+                table_pages=3, n_kv_heads=2, head_dim=64)
+    base.update(change)
+    return pkg.PagedBatch(**base)
+
+
+BATCHES = [
+    (dict(head_dim=96), "head_dim 96"), (dict(n_kv_heads=0), "n_kv_heads 0"), (dict(n_kv_heads=3), "multiple of n_kv_heads 3"),
+    (dict(n_seqs=0), "n_seqs 0"), (dict(n_pages=-1), "n_pages -1"), (dict(page_size=0), "page_size 0"),
+    (dict(table_pages=0), "table_pages 0"), (dict(key_cache=None), "null"), (dict(kv_len=None), "null"),
+    (dict(value_cache=0x1002), "16-byte aligned"), (dict(slot_stride=100), "multiples of 8"),
+    (dict(page_size=(1 << 20) + 1), "over 1048576"),
+]
+
+
+def refused(pkg, fn, *args):
+    L = pkg.lib()
+    L.llm_clear_error()
+    getattr(L, fn)(*args)
+    message = L.llm_last_error()
+    L.llm_clear_error()
+    return message.decode() if message else ""
+
+
+@pytest.mark.parametrize("change,message", BATCHES)
+def test_batches_that_are_refused(pkg, change, message):
+    b = ctypes.byref(record(pkg, **change))
+    p = 0x1000
+    assert message in refused(pkg, "qk_norm_rope_paged", p, p, p, p, None, None, p, b, 4, 4, 64, 0, 1e-6, 1.0,
+                              256, 256, 128, 128, None)
+    assert message in refused(pkg, "attention_paged_forward", p, p, b, p, 4, 4, 1, 100, 0, 0.1, 256, 256, None)
+
+
+@pytest.mark.parametrize("at,value,message", [
+    (0, None, "q_out is null"), (2, 0x1008, "k must be 16-byte aligned"), (4, 0x1002, "norm weights"),
+    (6, None, "inv_freq"), (6, 0x1004, "inv_freq"), (7, None, "no batch"), (8, -1, "n_tokens -1"),
+    (9, 0, "n_heads 0"), (10, 24, "rotary_dim 24"), (10, 0, "rotary_dim 0"), (10, 80, "rotary_dim 80"),
+    (14, 248, "rows of q_out"), (15, 260, "rows of q "), (16, 64, "rows of k"), (17, 0, "rows of v")])
+def test_append_refusals(pkg, at, value, message):
+    p, b = 0x1000, record(pkg)
+    args = [p, p, p, p, None, None, p, ctypes.byref(b), 4, 4, 64, 0, 1e-6, 1.0, 256, 256, 128, 128, None]
+    args[at] = value
+    assert message in refused(pkg, "qk_norm_rope_paged", *args)
+
+
+@pytest.mark.parametrize("at,value,message", [
+    (0, None, "out is null"), (1, 0x1004, "q must be 16-byte aligned"), (2, None, "no batch"), (3, 0x1004, "ws must be"),
+    (4, 1 << 25, "n_tokens"), (5, 5, "multiple of n_kv_heads"), (6, 0, "max_q_len 0"), (7, -4, "max_kv_len -4"),
+    (8, -1, "window -1"), (9, 0.0, "scale 0"), (9, -1.0, "scale -1"), (9, math.nan, "scale nan"), (9, math.inf, "scale inf"),
+    (10, 128, "rows of out"), (11, 257, "rows of q")])
+def test_attention_refusals(pkg, at, value, message):
+    p, b = 0x1000, record(pkg)
+    args = [p, p, ctypes.byref(b), p, 4, 4, 1, 100, 0, 0.1, 256, 256, None]
+    args[at] = value
+    assert message in refused(pkg, "attention_paged_forward", *args)
+
+
+def test_no_rows_is_no_launch(pkg):
+    p, b = 0x1000, record(pkg)
+    assert refused(pkg, "qk_norm_rope_paged", p, p, p, p, None, None, p, ctypes.byref(b), 0, 4, 64, 0, 1e-6, 1.0,
+                   256, 256, 128, 128, None) == ""
+    assert refused(pkg, "attention_paged_forward", p, p, ctypes.byref(b), p, 0, 4, 1, 100, 0, 0.1, 256, 256, None) == ""
+
+
+@pytest.mark.gpu
+def test_wrapper_refusals(gpu):
+    import torch
+    b = Batch([(2, 20), (1, 5)], 2, 64, 16, 1)
+    kc, vc = b.pools()
+    q, k, v = (b.normal(3, h, 64).cuda() for h in (4, 2, 2))
+    where, f = b.where(), gpu.rope_frequencies(64, 1e4)[0].cuda()
+    good = dict(q_out=torch.empty_like(q), q=q, k=k, v=v, q_norm_w=None, k_norm_w=None, inv_freq=f, key_cache=kc,
+                value_cache=vc, page_table=where[0], q_start=where[1], kv_len=where[2], eps=1e-6)
+    gpu.qk_norm_rope_paged(**good)
+    for change, message in [
+            (dict(q=q.cpu()), "q must be a tensor on the GPU"), (dict(k=k.float()), "k must be torch.bfloat16"),
+            (dict(v=v[:2]), "v must have shape"), (dict(q_out=q.transpose(0, 1).contiguous().transpose(0, 1)), "q_out must be contiguous"),
+            (dict(key_cache=kc[:2]), "same shape and strides"), (dict(page_table=where[0].long()), "page_table must be torch.int32"),
+            (dict(q_start=where[1][:2]), "q_start must be contiguous of shape"), (dict(kv_len=where[2][:1]), "kv_len must be"),
+            (dict(inv_freq=f.float()), "inv_freq must be torch.float64"), (dict(inv_freq=f[:3].contiguous()), "rotary_dim 6"),
+            (dict(q_norm_w=torch.ones(32, device="cuda", dtype=torch.bfloat16)), "q_norm_w must be")]:
+        with pytest.raises(gpu.LlmError, match=message):
+            gpu.qk_norm_rope_paged(**dict(good, **change))
+    need = gpu.attention_paged_workspace_floats(3, 2, 4, 2, 64, 2, 100000)
+    good = dict(out=torch.empty_like(q), q=q, key_cache=kc, value_cache=vc, page_table=where[0], q_start=where[1],
+                kv_len=where[2], ws=torch.empty(max(need, 1), device="cuda"), scale=0.1, max_q_len=2, max_kv_len=100000)
+    gpu.attention_paged_forward(**good)
+    for change, message in [
+            (dict(out=q.float()), "out must be torch.bfloat16"), (dict(q=q[:, :3]), "out must have shape|n_heads 3"),
+            (dict(ws=good["ws"].half()), "ws must be torch.float32"), (dict(scale=0.0), "scale"), (dict(window=-1), "window"),
+            (dict(max_kv_len=0), "max_kv_len")]:
+        with pytest.raises(gpu.LlmError, match=message):
+            gpu.attention_paged_forward(**dict(good, **change))
+    if need:
+        with pytest.raises(gpu.LlmError, match=f"ws holds {need - 1} floats"):
+            gpu.attention_paged_forward(**dict(good, ws=good["ws"][:need - 1]))
+        with pytest.raises(gpu.LlmError, match="ws holds 0 floats"):
+            gpu.attention_paged_forward(**dict(good, ws=None))
+    torch.cuda.synchronize()
