@@ -1,125 +1,12 @@
-// Operators over a paged KV cache: QK-norm + RoPE that writes new keys and values into pages, and the
-// attention of new tokens over pages (include/llm_amd/paged.h).
+// QK-norm + RoPE that writes new keys and values into pages (include/llm_amd/paged.h).
 #include <math.h>
 #include <string.h>
 
-#include <algorithm>
-
-#include "common.h"
-#include "llm_amd/paged.h"
+#include "paged_batch.h"
 
 using namespace llm;
 
 namespace {
-
-bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
-
-// ------------------------------------------------------------------------------------------
-// the batch on the device
-// ------------------------------------------------------------------------------------------
-
-// n / d for 0 <= n < 2^31 by a multiplication: with 2^(l-1) < d <= 2^l and m = floor(2^(31+l) / d) + 1,
-// m d exceeds 2^(31+l) by at most d <= 2^l, so floor(n m / 2^(31+l)) = floor(n / d) for n < 2^31.
-struct Divisor {
-    uint32_t m;
-    int l;
-    explicit Divisor(uint32_t d = 1) : m(0), l(0) {
-        while ((1ull << l) < d) l++;
-        m = (uint32_t)((1ull << (31 + l)) / d + 1);
-    }
-};
-__device__ __forceinline__ int divide(int n, uint32_t m, int l) {
-    return l == 0 ? n : (int)(__umulhi((uint32_t)n, m) >> (l - 1));
-}
-
-// What the kernels read of a PagedBatch.
-struct Batch {
-    bf16 *kc, *vc;
-    int64_t page_stride, slot_stride, head_stride;
-    const int *table, *q_start, *kv_len;
-    int n_seqs, n_pages, page_size, table_pages, n_tokens;
-    Divisor page;
-};
-
-// The sequence whose rows hold row t, or -1: the number of sequences that end at or before t, found by
-// all 64 lanes at once (64 probes per round), then checked against that sequence's first row. Whatever
-// q_start holds, the result is in [-1, n_seqs).
-__device__ __forceinline__ int sequence_of(const Batch &b, int t) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, hi = b.n_seqs;
-    while (lo < hi) {
-        const int step = (hi - lo + 63) / 64;
-        const int64_t at = lo + (int64_t)(lane + 1) * step - 1;  // the last of the lane's share
-        const bool ends = at < hi && gptr(b.q_start)[at + 1] <= t;
-        const int n = __popcll(__ballot(ends));
-        hi = min(hi, lo + n * step + step - 1);
-        lo += n * step;
-    }
-    if (lo >= b.n_seqs || gptr(b.q_start)[lo] > t || gptr(b.q_start)[lo + 1] <= t) return -1;
-    return lo;
-}
-
-// Lengths outside [-2^30, 2^30] are cut to it, so that positions do not overflow.
-__device__ __forceinline__ int kv_length(const Batch &b, int s) {
-    return max(-(1 << 30), min(1 << 30, gptr(b.kv_len)[s]));
-}
-
-// Element offset of position p of sequence s in the caches (head 0), or -1 where it is not there.
-__device__ __forceinline__ int64_t place(const Batch &b, int s, int p) {
-    if (p < 0) return -1;
-    const int i = divide(p, b.page.m, b.page.l);
-    if (i >= b.table_pages) return -1;
-    const int page = gptr(b.table)[(int64_t)s * b.table_pages + i];
-    if ((unsigned)page >= (unsigned)b.n_pages) return -1;
-    return page * b.page_stride + (p - i * b.page_size) * b.slot_stride;
-}
-
-bool take_batch(const char *name, const PagedBatch *p, int n_tokens, int n_heads, Batch *b) {
-    if (!p) return llm_fail("%s: no batch", name);
-    if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
-        return llm_fail("%s: head_dim %d is not 64, 128 or 256", name, p->head_dim);
-    if (p->n_kv_heads <= 0 || n_heads <= 0 || n_heads % p->n_kv_heads != 0)
-        return llm_fail("%s: n_heads %d is not a positive multiple of n_kv_heads %d", name, n_heads,
-                        p->n_kv_heads);
-    if (n_heads > 65535) return llm_fail("%s: n_heads %d is over 65535", name, n_heads);
-    if (p->n_seqs <= 0 || p->n_pages <= 0 || p->page_size <= 0 || p->table_pages <= 0)
-        return llm_fail("%s: n_seqs %d, n_pages %d, page_size %d and table_pages %d must be positive", name,
-                        p->n_seqs, p->n_pages, p->page_size, p->table_pages);
-    if (p->page_size > 1 << 20) return llm_fail("%s: page_size %d is over 1048576", name, p->page_size);
-    if (n_tokens < 0 || n_tokens > 1 << 24)
-        return llm_fail("%s: n_tokens %d is not in 0..16777216", name, n_tokens);
-    if (!p->key_cache || !p->value_cache || !p->page_table || !p->q_start || !p->kv_len)
-        return llm_fail("%s: the batch has a null pointer", name);
-    if (!aligned16(p->key_cache) || !aligned16(p->value_cache))
-        return llm_fail("%s: the caches must be 16-byte aligned", name);
-    if (p->page_stride % 8 || p->slot_stride % 8 || p->head_stride % 8)
-        return llm_fail("%s: cache strides %lld, %lld, %lld are not multiples of 8", name,
-                        (long long)p->page_stride, (long long)p->slot_stride, (long long)p->head_stride);
-    b->kc = p->key_cache;
-    b->vc = p->value_cache;
-    b->page_stride = p->page_stride;
-    b->slot_stride = p->slot_stride;
-    b->head_stride = p->head_stride;
-    b->table = p->page_table;
-    b->q_start = p->q_start;
-    b->kv_len = p->kv_len;
-    b->n_seqs = p->n_seqs;
-    b->n_pages = p->n_pages;
-    b->page_size = p->page_size;
-    b->table_pages = p->table_pages;
-    b->n_tokens = n_tokens;
-    b->page = Divisor((uint32_t)p->page_size);
-    return true;
-}
-
-bool check_rows(const char *name, const char *what, const void *p, int64_t stride, int64_t width) {
-    if (!p) return llm_fail("%s: %s is null", name, what);
-    if (!aligned16(p)) return llm_fail("%s: %s must be 16-byte aligned", name, what);
-    if (stride < width || stride % 8)
-        return llm_fail("%s: the rows of %s are %lld elements apart, not a multiple of 8 of at least %lld",
-                        name, what, (long long)stride, (long long)width);
-    return true;
-}
 
 // ------------------------------------------------------------------------------------------
 // QK-norm + RoPE into pages
@@ -321,115 +208,5 @@ extern "C" void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, co
         append_kernel<128><<<(unsigned)blocks, 256, 0, stream>>>(a);
     else
         append_kernel<256><<<(unsigned)blocks, 256, 0, stream>>>(a);
-    LAUNCH_OK();
-}
-
-// ------------------------------------------------------------------------------------------
-// attention over pages
-// ------------------------------------------------------------------------------------------
-
-namespace {
-
-struct AttendArgs {
-    Batch b;
-    bf16 *out;
-    const bf16 *q;
-    int64_t out_stride, q_stride;
-    int n_heads, n_kv_heads, window;
-    float scale;
-};
-
-// One wave per row and head, one key at a time with a running maximum and sum.
-template <int D>
-__global__ __launch_bounds__(256) void attend_rows_kernel(AttendArgs a) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x & 63;
-    const int64_t wave = (int64_t)blockIdx.x * 4 + wave_id();
-    const int t = (int)(wave / a.n_heads), h = (int)(wave - (int64_t)t * a.n_heads);
-    if (t >= a.b.n_tokens) return;
-    const int s = sequence_of(a.b, t);
-    if (s < 0) return;
-    const int pos = kv_length(a.b, s) - gptr(a.b.q_start)[s + 1] + t;
-    const int kv = h / (a.n_heads / a.n_kv_heads);
-    float q[E], acc[E], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        q[e] = bf2f(gptr(a.q)[t * a.q_stride + h * D + lane + 64 * e]);
-        acc[e] = 0.0f;
-    }
-    for (int p = a.window > 0 ? max(0, pos - a.window + 1) : 0; p <= pos; p++) {
-        const int64_t at = place(a.b, s, p);
-        if (at < 0) continue;
-        const bf16 *k = a.b.kc + at + kv * a.b.head_stride, *v = a.b.vc + at + kv * a.b.head_stride;
-        float dot = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) dot = fmaf(q[e], bf2f(gptr(k)[lane + 64 * e]), dot);
-        const float x = wave_sum(dot) * a.scale;
-        if (x == -INFINITY) continue;
-        const float next = fmaxf(top, x);
-        const float keep = exp_f32(top - next), weight = exp_f32(x - next);
-        top = next;
-        sum = sum * keep + weight;
-#pragma unroll
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + weight * bf2f(gptr(v)[lane + 64 * e]);
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        gptr(a.out)[t * a.out_stride + h * D + lane + 64 * e] =
-            (bf16)f2bf(top == -INFINITY ? 0.0f : acc[e] / sum);
-}
-
-}  // namespace
-
-extern "C" size_t attention_paged_workspace_floats(int n_tokens, int n_seqs, int n_heads,
-                                                   int n_kv_heads, int head_dim, int max_q_len,
-                                                   int max_kv_len) {
-    (void)n_tokens, (void)n_seqs, (void)n_heads, (void)n_kv_heads, (void)head_dim, (void)max_q_len;
-    (void)max_kv_len;
-    return 0;
-}
-
-extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBatch *batch, float *ws,
-                                        int n_tokens, int n_heads, int max_q_len, int max_kv_len,
-                                        int window, float scale, int64_t out_stride,
-                                        int64_t q_stride, hipStream_t stream) {
-    static const char name[] = "attention_paged";
-    AttendArgs a;
-    if (!take_batch(name, batch, n_tokens, n_heads, &a.b)) return;
-    if (n_tokens == 0) return;
-    if (max_q_len <= 0 || max_kv_len <= 0) {
-        llm_fail("%s: max_q_len %d and max_kv_len %d must be positive", name, max_q_len, max_kv_len);
-        return;
-    }
-    if (window < 0) {
-        llm_fail("%s: window %d is negative", name, window);
-        return;
-    }
-    if (!(scale > 0.0f) || !isfinite(scale)) {
-        llm_fail("%s: scale %g is not positive and finite", name, (double)scale);
-        return;
-    }
-    const int64_t width = (int64_t)n_heads * batch->head_dim;
-    if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width))
-        return;
-    if (!aligned16(ws)) {
-        llm_fail("%s: ws must be 16-byte aligned", name);
-        return;
-    }
-    a.out = out;
-    a.q = q;
-    a.out_stride = out_stride;
-    a.q_stride = q_stride;
-    a.n_heads = n_heads;
-    a.n_kv_heads = batch->n_kv_heads;
-    a.window = window;
-    a.scale = scale;
-    const int64_t blocks = ((int64_t)n_tokens * n_heads + 3) / 4;
-    if (batch->head_dim == 64)
-        attend_rows_kernel<64><<<(unsigned)blocks, 256, 0, stream>>>(a);
-    else if (batch->head_dim == 128)
-        attend_rows_kernel<128><<<(unsigned)blocks, 256, 0, stream>>>(a);
-    else
-        attend_rows_kernel<256><<<(unsigned)blocks, 256, 0, stream>>>(a);
     LAUNCH_OK();
 }

@@ -1,0 +1,816 @@
+// Attention of new tokens over a paged KV cache (include/llm_amd/paged.h).
+//
+// A sequence's new rows times the query heads of one kv head are the columns of the matrix products:
+// scores S^T = K Q^T (keys x columns) and outputs O^T += V^T P^T (head_dim x columns), both on
+// 32x32x16 MFMAs with the columns spread over the lanes, so that the softmax runs down a lane's registers
+// and P^T goes from the first product's accumulators into the second's operand without crossing lanes: of
+// 16 keys, lane half h holds 4h..4h+3 and 8+4h..8+4h+3, and the second product sums over any order of keys.
+#include <math.h>
+
+#include "paged_batch.h"
+
+using namespace llm;
+
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+#define LLM_LDS __attribute__((address_space(3)))
+typedef LLM_LDS char lds_char;
+
+constexpr float LOWEST = -3.402823466e+38f;
+
+struct AttendArgs {
+    Batch b;
+    bf16 *out;
+    const bf16 *q;
+    int64_t out_stride, q_stride;
+    float *part, *stats;  // of this kernel's units: [unit][split][row][head_dim], [unit][split][row][2]
+    int n_heads, n_kv_heads, group, window;
+    int n_split, chunk;   // keys per split, a multiple of 128
+    int by_sequence;      // few: tile i is sequence i, of at most 32 rows; many: sequences of more
+    float scale_log2;     // scale * log2(e)
+};
+
+// ------------------------------------------------------------------------------------------
+// which rows and keys
+// ------------------------------------------------------------------------------------------
+
+// T rows (new tokens x query heads of a kv head) of one sequence.
+struct Tile {
+    int s, first, rows;      // sequence, first row among the sequence's, rows of this tile
+    int q0;                  // the sequence's first token
+    int before;              // position of its first token
+    int begin, end, active;  // keys of any row (begin a multiple of 64), splits that have some
+};
+
+__device__ __forceinline__ int token_at(const Batch &b, int i) {
+    return max(0, min(b.n_tokens, gptr(b.q_start)[i]));
+}
+
+// Tile i of a launch, false where there is none. Sequence s has the tiles from floor(rows before it / T) + s
+// on: at least as many as its own rows fill.
+template <int T>
+__device__ __forceinline__ bool find_tile(const AttendArgs &a, int i, bool by_sequence, Tile &t) {
+    int j = 0;
+    if (by_sequence) {
+        t.s = i;
+    } else {
+        const auto start = [&](int s) { return (int)((int64_t)token_at(a.b, s) * a.group / T) + s; };
+        t.s = count_leading(a.b.n_seqs - 1, [&](int m) { return start(m + 1) <= i; });
+        j = i - start(t.s);
+    }
+    t.q0 = token_at(a.b, t.s);
+    const int n = token_at(a.b, t.s + 1) - t.q0;
+    if (j < 0 || (int64_t)j * T >= (int64_t)n * a.group) return false;
+    t.first = j * T;
+    t.rows = min(T, n * a.group - t.first);
+    t.before = kv_length(a.b, t.s) - n;
+    const int lo = t.before + t.first / a.group, hi = t.before + (t.first + t.rows - 1) / a.group;
+    const int64_t room = (int64_t)a.b.table_pages * a.b.page_size;
+    t.end = (int)min((int64_t)(hi + 1), room);
+    t.begin = a.window > 0 ? max(0, lo - a.window + 1) & ~63 : 0;
+    t.active = t.end > t.begin ? min(a.n_split, (t.end - t.begin + a.chunk - 1) / a.chunk) : 1;
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------
+// pages into LDS
+// ------------------------------------------------------------------------------------------
+
+// Rows of keys or values lie in LDS as they are, 16-byte chunk c of row r at chunk c ^ swizzle(r): the 16 rows
+// that a product's operand reads at one chunk, and the four rows of 64 bytes that a transposing read takes,
+// then lie in different banks. Linear in the bits of r.
+template <int D>
+__device__ __forceinline__ constexpr int swizzle(int r) {
+    return D == 64 ? ((r >> 1 & 1) << 2 | (r >> 2 & 3)) : ((r & 3) << 2 | (r >> 2 & 3));
+}
+
+// 64 lanes' 16 bytes from base + offset into LDS at `to` on, without passing registers. The wave waits for
+// it with wait_loads: the compiler does not know of it.
+__device__ __forceinline__ void load_to_lds(unsigned to, const void *base, unsigned offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+                 : "memory");
+}
+__device__ __forceinline__ void load_to_lds(unsigned to, const void *at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
+}
+// All but the last N vector memory operations of the wave are done.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// A wave's ROWS consecutive positions at a time, of every STEP, out of the pages into LDS. Positions that are
+// not there read the pool's first rows (the scores' mask leaves them out).
+// WHOLE: the 16 positions from a multiple of 16 on lie in one page, so a page is looked up once for them, 64
+// lookups at a time, one per lane; otherwise every position's place is looked up, 128 at a time, into LDS.
+template <int D, int ROWS, int STEP, bool WHOLE>
+struct Pages {
+    static constexpr int PER = 512 / D;        // rows per load
+    static constexpr int LOADS = ROWS / PER;   // of keys, and as many of values
+    static constexpr int GROUPS = ROWS < 16 ? 1 : ROWS / 16;
+    static constexpr int AHEAD = WHOLE ? 64 / GROUPS : 128 / ROWS;  // steps looked up at a time
+    const Batch &b;
+    int s, first;        // sequence, the first step's first position
+    int64_t head;        // element offset of the kv head
+    int entry;           // WHOLE: the lane's page
+    LLM_LDS int64_t *places;  // 128 of them
+    unsigned row_bytes, chunk_bytes;  // the lane's row and chunk within a load
+
+    __device__ __forceinline__ Pages(const Batch &b_, int s_, int kv, int first_, int row0, LLM_LDS int64_t *places_)
+        : b(b_), s(s_), first(first_), head(kv * b_.head_stride), entry(-1), places(places_) {
+        const int lane = threadIdx.x & 63, r = lane / (D / 8);
+        row_bytes = r * (unsigned)b.slot_stride * 2;
+        chunk_bytes = (lane % (D / 8) ^ swizzle<D>(r + row0)) * 16;  // row0, of the buffer: a multiple of PER
+    }
+
+    // Looks up steps step .. step + AHEAD - 1, when step is a multiple of AHEAD.
+    __device__ __forceinline__ void look_up(int step) {
+        if (step % AHEAD != 0) return;
+        const int lane = threadIdx.x & 63;
+        if constexpr (WHOLE) {
+            const int p = first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16;
+            const int i = divide(p, b.page.m, b.page.l);
+            entry = i < b.table_pages ? gptr(b.table)[(int64_t)s * b.table_pages + i] : -1;
+            if ((unsigned)entry >= (unsigned)b.n_pages) entry = -1;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const int n = lane + 64 * k;
+                places[n] = place(b, s, first + (step + n / ROWS) * STEP + n % ROWS);
+            }
+            wait_lds();
+        }
+    }
+
+    // Bit r: the step's position r is there.
+    __device__ __forceinline__ uint32_t there(int step) const {
+        if constexpr (WHOLE) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++)
+                if (__builtin_amdgcn_readlane(entry, step % AHEAD * GROUPS + g) >= 0)
+                    bits |= (ROWS < 16 ? (1u << ROWS) - 1 : 0xffffu) << (16 * g);
+            return bits;
+        } else {
+            const int lane = threadIdx.x & 63;
+            return (uint32_t)__ballot(lane < ROWS && places[step % AHEAD * ROWS + (lane & (ROWS - 1))] >= 0);
+        }
+    }
+
+    // Requests the step's rows of one cache into LDS at `to`.
+    __device__ __forceinline__ void request(const bf16 *cache, int step, unsigned to) const {
+        if constexpr (WHOLE) {
+#pragma unroll
+            for (int g = 0; g < GROUPS; g++) {
+                const int page = __builtin_amdgcn_readlane(entry, step % AHEAD * GROUPS + g);
+                const int p = first + step * STEP + g * 16;
+                const int slot = p - divide(p, b.page.m, b.page.l) * b.page_size;
+                const char *base = (const char *)(cache + head + (int64_t)max(page, 0) * b.page_stride +
+                                                  (page < 0 ? 0 : slot) * b.slot_stride);
+#pragma unroll
+                for (int i = 0; i < LOADS / GROUPS; i++)
+                    load_to_lds(to + (g * (LOADS / GROUPS) + i) * 1024, base + i * PER * b.slot_stride * 2,
+                                row_bytes + (chunk_bytes ^ (swizzle<D>(i * PER) * 16)));
+            }
+        } else {
+            const int r = (threadIdx.x & 63) / (D / 8);
+#pragma unroll
+            for (int i = 0; i < LOADS; i++) {
+                const int64_t at = places[step % AHEAD * ROWS + i * PER + r];
+                load_to_lds(to + i * 1024, (const char *)(cache + head + (at < 0 ? 0 : at)) +
+                                               (chunk_bytes ^ (swizzle<D>(i * PER) * 16)));
+            }
+        }
+    }
+};
+
+// The wave's own rows of values in LDS (as LOADS loads of its lanes left them) with zeros in place of NaN
+// and infinities; whether there were any. A weight of 0 times such a value would not be 0.
+template <int LOADS>
+__device__ __forceinline__ bool zero_bad_values(lds_char *rows) {
+    const int lane = threadIdx.x & 63;
+    const auto bad = [](uint32_t w) {
+        return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
+    };
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        const u32x4 x = *(LLM_LDS u32x4 *)(rows + i * 1024 + lane * 16);
+        any |= bad(x.x) | bad(x.y) | bad(x.z) | bad(x.w);
+    }
+    if (!__any(any != 0)) return false;
+#pragma unroll 1
+    for (int i = 0; i < LOADS; i++) {
+        LLM_LDS u32x4 *at = (LLM_LDS u32x4 *)(rows + i * 1024 + lane * 16);
+        const u32x4 x = *at;
+        *at = u32x4{x.x & ~bad(x.x), x.y & ~bad(x.y), x.z & ~bad(x.z), x.w & ~bad(x.w)};
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------------------------------
+// a wave's 32 columns
+// ------------------------------------------------------------------------------------------
+
+template <int D>
+struct Columns {
+    f32x16 o[D / 32];      // O^T: rows 32 dt + (r & 3) + 8 (r / 4) + 4 h in register r of lane half h
+    u32x4 q[D / 16];       // Q^T: elements 16 ks + 8 h .. + 7
+    float top, sum;        // the running maximum (times scale_log2) and this half's part of the sum
+    int position, column;  // of the lane's row (-1: no row), its index in the wave
+
+    __device__ __forceinline__ void start(const AttendArgs &a, const Tile &t, int kv, int first) {
+        const int lane = threadIdx.x & 63, h = lane >> 5;
+        column = lane & 31;
+        const int row = t.first + first + column;
+        const bool there = first + column < t.rows;
+        const int token = row / a.group;
+        position = there ? t.before + token : -1;
+        const bf16 *src = a.q + (t.q0 + token) * a.q_stride + (kv * a.group + row - token * a.group) * D + 8 * h;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) q[k] = there ? ld16(src + 16 * k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+        top = LOWEST;
+        sum = 0.0f;
+    }
+
+    // Bit k: the lane's row sees position at + k, k < 32.
+    __device__ __forceinline__ uint32_t sees(int at, int window) const {
+        const int last = position - at;  // the last bit
+        uint32_t bits = last < 0 ? 0 : last >= 31 ? ~0u : (2u << last) - 1;
+        if (window > 0) {
+            const int first = last - window + 1;
+            if (first > 31)
+                bits = 0;
+            else if (first > 0)
+                bits &= ~0u << first;
+        }
+        return bits;
+    }
+
+    // Scores of 32 keys in LDS.
+    __device__ __forceinline__ f32x16 scores(const lds_char *keys) const {
+        const int lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+        const lds_char *row = keys + r * (2 * D);
+        const int c0 = (h ^ swizzle<D>(r)) * 16;
+        f32x16 s;
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+            const u32x4 x = *(const LLM_LDS u32x4 *)(row + (c0 ^ (k * 32)));
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x),
+                                                        __builtin_bit_cast(bf16x8_t, q[k]), s, 0, 0, 0);
+        }
+        return s;
+    }
+
+    // Scores to weights 2^(s c - top), with the maximum moved where it has grown by more than 2^8 for any
+    // column: below that the weights stay in range and a larger maximum changes no relative rounding.
+    template <int KT>
+    __device__ __forceinline__ void weigh(f32x16 (&s)[KT], float c) {
+        float m = s[0][0];
+#pragma unroll
+        for (int k = 0; k < KT; k++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) m = fmaxf(m, s[k][r]);
+        float x, y;
+        swap_pair<32>(m, x, y);
+        m = fmaxf(x, y) * c;
+        if (__any(m > top + 8.0f)) {
+            const float next = fmaxf(top, m);
+            const float keep = __builtin_amdgcn_exp2f(top - next);
+            top = next;
+            sum *= keep;
+#pragma unroll
+            for (int d = 0; d < D / 32; d++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) o[d][r] *= keep;
+        }
+        float part[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KT; k++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                s[k][r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, -top));
+                part[r & 3] += s[k][r];
+            }
+        sum += (part[0] + part[1]) + (part[2] + part[3]);
+    }
+
+    // O^T += V^T P^T over 32 keys: the weights rounded to bf16, with EXACT their remainders too.
+    template <bool EXACT>
+    __device__ __forceinline__ void add(const lds_char *values, const f32x16 &p) {
+        const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
+        const int row = 4 * h + (i >> 2);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            u32x4 hi, lo;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float x = p[8 * t + 2 * j], y = p[8 * t + 2 * j + 1];
+                const uint32_t w = pack2(x, y);
+                hi[j] = w;
+                if constexpr (EXACT) lo[j] = pack2(x - lo_f(w), y - hi_f(w));
+            }
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) {
+                const int c = d * 4 + (lane >> 4 & 1) * 2 + ((i & 3) >> 1);
+                s16x4 v[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int r = 16 * t + 8 * u + row;
+                    v[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (LLM_LDS s16x4 *)(values + r * (2 * D) + (c ^ swizzle<D>(r)) * 16 + (i & 1) * 8));
+                }
+                const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
+                const bf16x8_t vt = __builtin_bit_cast(bf16x8_t, (u32x4{v0.x, v0.y, v1.x, v1.y}));
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, hi), o[d], 0, 0, 0);
+                if constexpr (EXACT)
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, lo), o[d], 0, 0, 0);
+            }
+        }
+    }
+
+    // The share of the NaN and infinities that zero_bad_values took out, where a row sees them: 32 keys
+    // from position `at` on, read from the cache again, one by one. p: their weights; sees: the lane's
+    // bits; space: 16 x 32 floats of the wave's own LDS.
+    __device__ __forceinline__ void add_bad(const AttendArgs &a, int s, int kv, int at, uint32_t sees, const f32x16 &p,
+                                            LLM_LDS float *space) {
+        const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            wait_lds();
+#pragma unroll
+            for (int j = 0; j < 8; j++) space[((j & 3) + 8 * (j >> 2) + 4 * h) * 32 + column] = p[8 * t + j];
+            wait_lds();
+#pragma unroll 1
+            for (int k = 0; k < 16; k++) {
+                const int64_t where = place(a.b, s, at + 16 * t + k);
+                if (where < 0) continue;
+                const float w = space[k * 32 + column];
+                const bool seen = sees >> (16 * t + k) & 1;
+                const bf16 *v = a.b.vc + where + kv * a.b.head_stride + 4 * h;
+#pragma unroll
+                for (int d = 0; d < D / 32; d++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const u32x2 x = *gptr((const u32x2 *)(v + 32 * d + 8 * r));
+                        const float e[4] = {lo_f(x.x), hi_f(x.x), lo_f(x.y), hi_f(x.y)};
+#pragma unroll
+                        for (int n = 0; n < 4; n++)
+                            if (seen && !(fabsf(e[n]) < INFINITY)) o[d][4 * r + n] = fmaf(w, e[n], o[d][4 * r + n]);
+                    }
+            }
+        }
+    }
+};
+
+// Leaves a score of what a row does not see at -inf. bits: the lane's (Columns::sees and what is there).
+__device__ __forceinline__ void hide(f32x16 &s, uint32_t bits) {
+    const uint32_t mine = bits >> ((threadIdx.x & 32) / 8);
+#pragma unroll
+    for (int r = 0; r < 16; r++)
+        if (!(mine >> ((r & 3) + 8 * (r >> 2)) & 1)) s[r] = -INFINITY;
+}
+
+// Four consecutive elements of an output row.
+__device__ __forceinline__ void store4(bf16 *to, float a, float b, float c, float d) {
+    *gptr((u32x2 *)to) = u32x2{pack2(a, b), pack2(c, d)};
+}
+
+// ------------------------------------------------------------------------------------------
+// few rows: at most 32 per sequence and kv head
+// ------------------------------------------------------------------------------------------
+
+// One token, or a few, over a long history: bound by the bytes of the keys and values. A workgroup takes a
+// split's keys, each of its four waves a quarter of them with the same 32 columns and buffers of its own, so
+// nothing waits between waves until their outputs are joined. A wave keeps 32 keys' rows and 32 values' rows in
+// LDS: the next keys are requested once the scores are formed and the next values once they are summed.
+template <int D, bool WHOLE>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(AttendArgs a) {
+    constexpr int ROWS = 32, BYTES = ROWS * 2 * D;
+    typedef Pages<D, ROWS, ROWS, WHOLE> P;
+    constexpr int LOADS = P::LOADS;
+    __shared__ __align__(1024) char lds[4][2 * BYTES];
+    __shared__ float space[4][512];
+    __shared__ int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
+    __shared__ float tops[4][32], sums[4][32];
+    const int tile = blockIdx.x / a.n_kv_heads, kv = blockIdx.x - tile * a.n_kv_heads;
+    const int w = wave_id(), lane = threadIdx.x & 63;
+    Tile t;
+    if (!find_tile<32>(a, tile, a.by_sequence, t)) return;
+    if (a.by_sequence && (int64_t)(token_at(a.b, t.s + 1) - t.q0) * a.group > 32) return;
+    const int z = blockIdx.y;
+    if (z >= t.active) return;
+    const int begin = t.begin + z * a.chunk;
+    const int end = z == a.n_split - 1 ? t.end : min(t.end, begin + a.chunk);
+    const int steps = end > begin ? (end - begin + ROWS - 1) / ROWS : 0;
+    const int s0 = (int)((int64_t)steps * w / 4), n = (int)((int64_t)steps * (w + 1) / 4) - s0;
+
+    Columns<D> c;
+    c.start(a, t, kv, 0);
+    const int lowest = t.before + t.first / a.group, highest = t.before + (t.first + t.rows - 1) / a.group;
+    P pages(a.b, t.s, kv, begin + s0 * ROWS, 0, (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
+    lds_char *keys = (lds_char *)lds[w], *values = keys + BYTES;
+    const unsigned key_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)keys), value_at = key_at + BYTES;
+    uint32_t there = 0;
+    if (n > 0) {
+        pages.look_up(0);
+        there = pages.there(0);
+        pages.request(a.b.kc, 0, key_at);
+        pages.request(a.b.vc, 0, value_at);
+    }
+    for (int i = 0; i < n; i++) {
+        const int at = begin + (s0 + i) * ROWS;
+        const bool more = i + 1 < n;
+        wait_loads<LOADS>();
+        f32x16 s[1] = {c.scores(keys)};
+        const bool edge = at + ROWS - 1 > lowest || (a.window > 0 && at <= highest - a.window) || there != ~0u;
+        uint32_t bits = ~0u;
+        if (edge) {
+            bits = c.sees(at, a.window) & there;
+            hide(s[0], bits);
+        }
+        wait_lds();
+        if (more) {
+            pages.look_up(i + 1);
+            there = pages.there(i + 1);
+            pages.request(a.b.kc, i + 1, key_at);
+        }
+        c.weigh(s, a.scale_log2);
+        if (more)
+            wait_loads<LOADS>();
+        else
+            wait_loads<0>();
+        const bool bad = edge && zero_bad_values<LOADS>(values);
+        c.template add<true>(values, s[0]);
+        if (bad) c.add_bad(a, t.s, kv, at, bits, s[0], (LLM_LDS float *)space[w]);
+        wait_lds();
+        if (more) pages.request(a.b.vc, i + 1, value_at);
+    }
+
+    // join the waves: each one's output, maximum and sum through LDS
+    float x, y;
+    swap_pair<32>(c.sum, x, y);
+    __syncthreads();
+    if (lane < 32) {
+        tops[w][lane] = c.top;
+        sums[w][lane] = x + y;
+    }
+    constexpr int CHUNKS = D / 4;  // of four elements, chunk k of a column at k ^ (column & 15)
+    LLM_LDS f32x4 *joined = (LLM_LDS f32x4 *)lds;
+    if (c.column < t.rows) {
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int k = 8 * d + 2 * r + (lane >> 5);
+                joined[(w * 32 + c.column) * CHUNKS + (k ^ (c.column & 15))] =
+                    f32x4{c.o[d][4 * r], c.o[d][4 * r + 1], c.o[d][4 * r + 2], c.o[d][4 * r + 3]};
+            }
+    }
+    __syncthreads();
+    const int64_t unit = ((int64_t)blockIdx.x * a.n_split + z) * 32;
+    for (int i = threadIdx.x; i < t.rows * CHUNKS; i += 256) {
+        const int row = i / CHUNKS, k = i % CHUNKS;
+        float top = tops[0][row];
+#pragma unroll
+        for (int v = 1; v < 4; v++) top = fmaxf(top, tops[v][row]);
+        float sum = 0.0f;
+        f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const float f = __builtin_amdgcn_exp2f(tops[v][row] - top);
+            sum = fmaf(f, sums[v][row], sum);
+            const f32x4 e = joined[(v * 32 + row) * CHUNKS + (k ^ (row & 15))];
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] = fmaf(f, e[j], o[j]);
+        }
+        if (t.active > 1) {
+            *gptr((f32x4 *)(a.part + (unit + row) * D + 4 * k)) = o;
+            if (k == 0) {
+                gptr(a.stats)[(unit + row) * 2] = top;
+                gptr(a.stats)[(unit + row) * 2 + 1] = sum;
+            }
+        } else {
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const int r = t.first + row, token = r / a.group;
+            store4(a.out + (t.q0 + token) * a.out_stride + (kv * a.group + r - token * a.group) * D + 4 * k, o[0] * f,
+                   o[1] * f, o[2] * f, o[3] * f);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// many rows
+// ------------------------------------------------------------------------------------------
+
+constexpr int MANY = 128;  // rows of a workgroup
+
+// A chunk of new tokens: bound by the matrix products. The four waves of a workgroup take 32 columns each and
+// share the keys and values in LDS, two buffers of NK rows: while one is used the other is filled, a quarter by
+// each wave, with one barrier per NK keys.
+template <int D, bool WHOLE>
+__global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
+    constexpr int NK = D == 256 ? 32 : 64, KT = NK / 32, BYTES = NK * 2 * D;
+    typedef Pages<D, NK / 4, NK, WHOLE> P;
+    constexpr int LOADS = P::LOADS;
+    __shared__ __align__(1024) char lds[2][2 * BYTES];  // keys, values
+    __shared__ float space[4][512];
+    __shared__ int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
+    __shared__ __align__(16) uint32_t state[2][4];  // of each wave's rows: which are there, and bit 31: bad values among them
+    const int w = wave_id(), lane = threadIdx.x & 63;
+    const int units = gridDim.x / a.n_kv_heads;
+    const int tile = units - 1 - blockIdx.x / a.n_kv_heads, kv = blockIdx.x % a.n_kv_heads;
+    Tile t;
+    if (!find_tile<MANY>(a, tile, false, t)) return;
+    if (a.by_sequence && (int64_t)(token_at(a.b, t.s + 1) - t.q0) * a.group <= 32) return;
+    const int z = blockIdx.y;
+    if (z >= t.active) return;
+    const int begin = t.begin + z * a.chunk;
+    const int end = z == a.n_split - 1 ? t.end : min(t.end, begin + a.chunk);
+    const int n = end > begin ? (end - begin + NK - 1) / NK : 0;
+
+    Columns<D> c;
+    c.start(a, t, kv, 32 * w);
+    const auto position_of = [&](int row) { return t.before + (t.first + row) / a.group; };
+    const bool any_rows = 32 * w < t.rows;
+    const int lowest = position_of(0), highest = position_of(t.rows - 1);  // of the workgroup
+    const int low = position_of(32 * w), high = position_of(min(t.rows, 32 * w + 32) - 1);  // of the wave
+    P pages(a.b, t.s, kv, begin + w * (NK / 4), w * (NK / 4), (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
+    const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char *)lds) + w * (BYTES / 4);
+    if (n > 0) {
+        pages.look_up(0);
+        pages.request(a.b.kc, 0, mine);
+        pages.request(a.b.vc, 0, mine + BYTES);
+    }
+    constexpr uint32_t ALL = NK / 4 == 16 ? 0xffffu : (1u << (NK / 4)) - 1;
+    for (int i = 0; i < n; i++) {
+        const int at = begin + i * NK, buffer = i & 1;
+        const uint32_t there = pages.there(i);
+        wait_loads<0>();
+        bool bad = false;
+        if (at + NK - 1 > lowest || (a.window > 0 && at <= highest - a.window) || there != ALL)
+            bad = zero_bad_values<LOADS>((lds_char *)lds[buffer] + BYTES + w * (BYTES / 4));
+        if (lane == 0) state[buffer][w] = there | (bad ? 1u << 31 : 0u);
+        __syncthreads();
+        if (i + 1 < n) {
+            pages.look_up(i + 1);
+            pages.request(a.b.kc, i + 1, mine + (buffer ^ 1) * 2 * BYTES);
+            pages.request(a.b.vc, i + 1, mine + (buffer ^ 1) * 2 * BYTES + BYTES);
+        }
+        if (!any_rows || at > high || (a.window > 0 && at + NK - 1 <= low - a.window)) continue;
+        const u32x4 st = *(LLM_LDS u32x4 *)(lds_char *)state[buffer];
+        uint32_t st_of[4], whole = ~0u, bad_any = 0;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            st_of[v] = __builtin_amdgcn_readfirstlane(st[v]);
+            whole &= st_of[v];
+            bad_any |= st_of[v] >> 31;
+        }
+        const lds_char *keys = (lds_char *)lds[buffer], *values = keys + BYTES;
+        f32x16 s[KT];
+#pragma unroll
+        for (int k = 0; k < KT; k++) s[k] = c.scores(keys + k * 32 * 2 * D);
+        const bool edge = at + NK - 1 > low || (a.window > 0 && at <= high - a.window) || (whole & ALL) != ALL;
+        uint32_t bits[KT];
+#pragma unroll
+        for (int k = 0; k < KT; k++) bits[k] = ~0u;
+        if (edge) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                uint32_t there32 = 0;
+                constexpr int WAVES = 32 / (NK / 4);  // waves whose rows make 32
+#pragma unroll
+                for (int v = 0; v < WAVES; v++) there32 |= (st_of[k * WAVES + v] & ALL) << (v * (NK / 4));
+                bits[k] = c.sees(at + 32 * k, a.window) & there32;
+                hide(s[k], bits[k]);
+            }
+        }
+        c.weigh(s, a.scale_log2);
+#pragma unroll
+        for (int k = 0; k < KT; k++) c.template add<false>(values + k * 32 * 2 * D, s[k]);
+        if (bad_any)
+#pragma unroll
+            for (int k = 0; k < KT; k++)
+                c.add_bad(a, t.s, kv, at + 32 * k, bits[k], s[k], (LLM_LDS float *)space[w]);
+    }
+
+    if (!any_rows || c.column >= t.rows - 32 * w) return;
+    float x, y;
+    swap_pair<32>(c.sum, x, y);
+    const float sum = x + y;
+    const int h = lane >> 5, row = 32 * w + c.column;
+    if (t.active > 1) {
+        const int64_t unit = ((int64_t)(tile * a.n_kv_heads + kv) * a.n_split + z) * MANY + row;
+        if (h == 0) {
+            gptr(a.stats)[unit * 2] = c.top;
+            gptr(a.stats)[unit * 2 + 1] = sum;
+        }
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                *gptr((f32x4 *)(a.part + unit * D + 32 * d + 8 * r + 4 * h)) =
+                    f32x4{c.o[d][4 * r], c.o[d][4 * r + 1], c.o[d][4 * r + 2], c.o[d][4 * r + 3]};
+        return;
+    }
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int r0 = t.first + row, token = r0 / a.group;
+    bf16 *to = a.out + (t.q0 + token) * a.out_stride + (kv * a.group + r0 - token * a.group) * D + 4 * h;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            store4(to + 32 * d + 8 * r, c.o[d][4 * r] * f, c.o[d][4 * r + 1] * f, c.o[d][4 * r + 2] * f,
+                   c.o[d][4 * r + 3] * f);
+}
+
+// ------------------------------------------------------------------------------------------
+// the splits' join
+// ------------------------------------------------------------------------------------------
+
+// Four elements of a row per thread, the splits in order.
+template <int D, int T>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+    constexpr int CHUNKS = D / 4;
+    const int tile = blockIdx.x / a.n_kv_heads, kv = blockIdx.x - tile * a.n_kv_heads;
+    Tile t;
+    if (!find_tile<T>(a, tile, T == 32 && a.by_sequence, t)) return;
+    const bool few = (int64_t)(token_at(a.b, t.s + 1) - t.q0) * a.group <= 32;
+    if (t.active <= 1 || (a.by_sequence && few != (T == 32))) return;
+    for (int i = blockIdx.y * 256 + threadIdx.x; i < t.rows * CHUNKS; i += 256 * gridDim.y) {
+        const int row = i / CHUNKS, k = i % CHUNKS;
+        const int64_t unit = (int64_t)blockIdx.x * a.n_split * T + row;
+        float top = LOWEST, sum = 0.0f;
+        f32x4 o = {0, 0, 0, 0};
+        for (int z = 0; z < t.active; z++) {
+            const int64_t at = unit + (int64_t)z * T;
+            const float m = gptr(a.stats)[at * 2], n = gptr(a.stats)[at * 2 + 1];
+            const f32x4 e = *gptr((const f32x4 *)(a.part + at * D + 4 * k));
+            const float next = fmaxf(top, m);
+            const float f = __builtin_amdgcn_exp2f(top - next), g = __builtin_amdgcn_exp2f(m - next);
+            top = next;
+            sum = sum * f + n * g;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] = o[j] * f + e[j] * g;
+        }
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int r = t.first + row, token = r / a.group;
+        store4(a.out + (t.q0 + token) * a.out_stride + (kv * a.group + r - token * a.group) * D + 4 * k, o[0] * f,
+               o[1] * f, o[2] * f, o[3] * f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// the host
+// ------------------------------------------------------------------------------------------
+
+constexpr int CUS = 256;
+
+// How the work is split, from the host's sizes alone. A sequence's rows (new tokens x group) go to
+// attend_few_kernel up to 32 and to attend_many_kernel above, or all to one of them where the expected lengths
+// leave the other nothing.
+struct Plan {
+    bool few, many;
+    int few_tiles, many_tiles, few_split, few_chunk, many_split, many_chunk;
+    size_t few_rows, many_rows, floats;  // rows of partial outputs
+
+    Plan(int n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len,
+         int window) {
+        const int64_t group = n_heads / n_kv_heads, rows = n_tokens * group;
+        const int64_t longest = std::min<int64_t>(max_q_len, n_tokens) * group;
+        few = longest <= 32 || n_seqs > 1;
+        many = longest > 32;
+        few_tiles = many ? n_seqs : (int)(rows / 32 + n_seqs);
+        many_tiles = (int)(rows / MANY + n_seqs);
+        const auto split = [&](int64_t units, int least, int64_t span, int &n, int &chunk) {
+            const int64_t all = max_kv_len, ragged = (all + 2047) / 2048;
+            n = (int)std::max<int64_t>(1, std::min((all + least - 1) / least,
+                                                   std::max((2 * CUS + units - 1) / units, units < 16 * CUS ? ragged : 1)));
+            n = (int)std::min<int64_t>(n, (span + least - 1) / least);
+            chunk = (int)((span + n - 1) / n + 127) / 128 * 128;
+        };
+        const auto span = [&](int64_t tokens) {
+            return window > 0 ? std::min<int64_t>(max_kv_len, (int64_t)window + tokens + 63) : (int64_t)max_kv_len;
+        };
+        split((int64_t)n_seqs * n_kv_heads, 256, span(32), few_split, few_chunk);
+        split(((rows + MANY - 1) / MANY) * n_kv_heads, 512, span(MANY), many_split, many_chunk);
+        few_rows = few && few_split > 1 ? (size_t)few_tiles * n_kv_heads * few_split * 32 : 0;
+        many_rows = many && many_split > 1 ? (size_t)many_tiles * n_kv_heads * many_split * MANY : 0;
+        floats = (few_rows + many_rows) * (head_dim + 2);
+    }
+};
+
+bool check_sizes(const char *name, int n_tokens, int n_heads, int max_q_len, int max_kv_len) {
+    if (max_q_len <= 0 || max_kv_len <= 0)
+        return llm_fail("%s: max_q_len %d and max_kv_len %d must be positive", name, max_q_len, max_kv_len);
+    if (max_kv_len > 1 << 30) return llm_fail("%s: max_kv_len %d is over 1073741824", name, max_kv_len);
+    if ((int64_t)n_tokens * n_heads > INT32_MAX / 2)
+        return llm_fail("%s: %d rows of %d heads are too many", name, n_tokens, n_heads);
+    return true;
+}
+
+template <int D, bool WHOLE>
+void launch_attention(AttendArgs a, const Plan &p, float *ws, hipStream_t stream) {
+    AttendArgs few = a, many = a;
+    few.part = ws;
+    few.stats = ws + p.few_rows * D;
+    many.part = few.stats + p.few_rows * 2;
+    many.stats = many.part + p.many_rows * D;
+    few.n_split = p.few_split;
+    few.chunk = p.few_chunk;
+    many.n_split = p.many_split;
+    many.chunk = p.many_chunk;
+    few.by_sequence = p.many;
+    many.by_sequence = p.few;
+    const int h = a.n_kv_heads;
+    if (p.many) {
+        attend_many_kernel<D, WHOLE><<<dim3(p.many_tiles * h, p.many_split), 256, 0, stream>>>(many);
+        if (!LAUNCH_OK()) return;
+    }
+    if (p.few) {
+        attend_few_kernel<D, WHOLE><<<dim3(p.few_tiles * h, p.few_split), 256, 0, stream>>>(few);
+        if (!LAUNCH_OK()) return;
+    }
+    if (p.many && p.many_split > 1) {
+        attend_join_kernel<D, MANY><<<dim3(p.many_tiles * h, D / 32), 256, 0, stream>>>(many);
+        if (!LAUNCH_OK()) return;
+    }
+    if (p.few && p.few_split > 1) {
+        attend_join_kernel<D, 32><<<dim3(p.few_tiles * h, 1), 256, 0, stream>>>(few);
+        LAUNCH_OK();
+    }
+}
+
+}  // namespace
+
+extern "C" size_t attention_paged_workspace_floats(int n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim,
+                                                   int max_q_len, int max_kv_len) {
+    static const char name[] = "attention_paged_workspace_floats";
+    if (n_tokens < 0 || n_tokens > 1 << 24 || n_seqs <= 0 || n_seqs > 1 << 20 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads ||
+        (head_dim != 64 && head_dim != 128 && head_dim != 256)) {
+        llm_fail("%s: no attention of %d rows in %d sequences, %d heads on %d of %d", name, n_tokens, n_seqs, n_heads,
+                 n_kv_heads, head_dim);
+        return 0;
+    }
+    if (!check_sizes(name, n_tokens, n_heads, max_q_len, max_kv_len)) return 0;
+    if (n_tokens == 0) return 0;
+    return Plan(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len, 0).floats;
+}
+
+extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBatch *batch, float *ws, int n_tokens,
+                                        int n_heads, int max_q_len, int max_kv_len, int window, float scale,
+                                        int64_t out_stride, int64_t q_stride, hipStream_t stream) {
+    static const char name[] = "attention_paged";
+    AttendArgs a;
+    if (!take_batch(name, batch, n_tokens, n_heads, &a.b)) return;
+    if (!check_sizes(name, n_tokens, n_heads, max_q_len, max_kv_len)) return;
+    if (n_tokens == 0) return;
+    if (window < 0) {
+        llm_fail("%s: window %d is negative", name, window);
+        return;
+    }
+    if (!(scale > 0.0f) || !isfinite(scale)) {
+        llm_fail("%s: scale %g is not positive and finite", name, (double)scale);
+        return;
+    }
+    const int D = batch->head_dim;
+    const int64_t width = (int64_t)n_heads * D;
+    if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width)) return;
+    const Plan plan(n_tokens, batch->n_seqs, n_heads, batch->n_kv_heads, D, max_q_len, max_kv_len, window);
+    if (!aligned16(ws) || (plan.floats && !ws)) {
+        llm_fail("%s: ws must be a 16-byte aligned device address", name);
+        return;
+    }
+    a.out = out;
+    a.q = q;
+    a.out_stride = out_stride;
+    a.q_stride = q_stride;
+    a.n_heads = n_heads;
+    a.n_kv_heads = batch->n_kv_heads;
+    a.group = n_heads / batch->n_kv_heads;
+    a.window = window;
+    a.scale_log2 = scale * 1.44269504f;
+    const bool whole = batch->page_size % 16 == 0;
+#define ATTEND(D_)                                      \
+    if (D == D_) {                                      \
+        if (whole)                                      \
+            launch_attention<D_, true>(a, plan, ws, stream);  \
+        else                                            \
+            launch_attention<D_, false>(a, plan, ws, stream); \
+    }
+    ATTEND(64) ATTEND(128) ATTEND(256)
+#undef ATTEND
+}
