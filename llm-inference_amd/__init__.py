@@ -508,6 +508,9 @@ def qk_norm_rope_paged(q_out, q, k, v, q_norm_w, k_norm_w, inv_freq, key_cache, 
     value_cache [pages, slots, kv heads, head_dim], at the places that page_table [sequences, pages], q_start
     [sequences + 1] and kv_len [sequences] give. inv_freq: float64 [rotary_dim / 2] on the GPU. Norm weights
     None: no norm. Rows of q, k, v and q_out may lie apart (slices of one projection's rows)."""
+    if _native and _native.qk_norm_rope_paged(q_out, q, k, v, q_norm_w, k_norm_w, inv_freq, key_cache, value_cache,
+                                              page_table, q_start, kv_len, eps, rope_scale, interleaved, stream):
+        return
     import torch
     batch = _paged_batch(key_cache, value_cache, page_table, q_start, kv_len)
     if q.dim() != 3:
@@ -538,6 +541,9 @@ def attention_paged_forward(out, q, key_cache, value_cache, page_table, q_start,
     """Attention of q [tokens, heads, head_dim] over the pages of its rows' sequences, into out. ws: a
     float32 tensor of at least attention_paged_workspace_floats(...) floats for these sizes (None where that
     is 0), kept between calls that do not overlap."""
+    if _native and _native.attention_paged_forward(out, q, key_cache, value_cache, page_table, q_start, kv_len, ws,
+                                                   scale, max_q_len, max_kv_len, window, stream):
+        return
     import torch
     batch = _paged_batch(key_cache, value_cache, page_table, q_start, kv_len)
     if q.dim() != 3:
@@ -563,6 +569,9 @@ def logits_penalty_forward(out, logits, tokens=None, prompt_len=None, token_len=
     """Penalties over each row's tokens [rows, capacity], biases [rows, capacity] and the mask of allowed
     tokens [rows, words] (int32 words, bit t % 32 of word t / 32) on logits [rows, vocab], into out (which
     may be logits)."""
+    if _native and _native.logits_penalty_forward(out, logits, tokens, prompt_len, token_len, repetition, frequency,
+                                                  presence, bias_tokens, bias, bias_len, allowed, stream):
+        return
     import torch
     for name, t in (("out", out), ("logits", logits)):
         _on_device(name, t, _bits16())

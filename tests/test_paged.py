@@ -694,3 +694,42 @@ def test_wrapper_refusals(gpu):
         with pytest.raises(gpu.LlmError, match="ws holds 0 floats"):
             gpu.attention_paged_forward(**dict(good, ws=None))
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+def test_native_and_general_way_are_one(gpu, monkeypatch):
+    """The native launchers and the general ctypes way: the same results from the same arguments, and the
+    same refusals."""
+    import torch
+    b = Batch([(3, 50), (40, 70), (1, 9000)], 2, 64, 16, 29, layout="heads")
+    rows = b.normal(b.tokens, 8, 64).cuda()
+    norm, f = b.normal(64).cuda(), gpu.rope_frequencies(32, 1e4)[0].cuda()
+    x = torch.randn(3, 1001, device="cuda").bfloat16()
+    ids, n = torch.randint(0, 1001, (3, 40), device="cuda", dtype=torch.int32), torch.tensor([40, 3, 0], device="cuda", dtype=torch.int32)
+    results = []
+    for general in (False, True):
+        with monkeypatch.context() as m:
+            if general:
+                m.setattr(gpu, "_native", None)
+            kc, vc = b.pools()
+            q_out = torch.zeros(b.tokens, 4, 64, device="cuda", dtype=torch.int16)
+            out, z = torch.zeros_like(q_out, dtype=torch.bfloat16), torch.zeros_like(x)
+            ws = workspace(gpu, b, 4, 40, 9000)
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            gpu.qk_norm_rope_paged(q_out, rows[:, :4], rows[:, 4:6], rows[:, 6:], norm, norm, f, kc, vc, *b.where(), 1e-5,
+                                   1.5, True, side)
+            gpu.attention_paged_forward(out, q_out, kc, vc, *b.where(), ws, 0.25, 40, 9000, window=60, stream=side.cuda_stream)
+            gpu.logits_penalty_forward(z, x, ids, n, n, bias_tokens=ids, bias=ids.float(), stream=side)
+            torch.cuda.synchronize()
+            refusals = []
+            for call in (lambda: gpu.attention_paged_forward(out, q_out, kc, vc, *b.where(), ws, 1, 40, 9000, -1),
+                         lambda: gpu.attention_paged_forward(out, q_out, kc, vc, *b.where(), None, 0.1, 40, 9000),
+                         lambda: gpu.qk_norm_rope_paged(q_out, rows[:, :4], rows[:, 4:6], rows[:, 6:], None, None, f[:4], kc, vc, *b.where(), 1e-5),
+                         lambda: gpu.logits_penalty_forward(z, x[:, :1000], ids, n, n)):
+                with pytest.raises(gpu.LlmError) as e:
+                    call()
+                refusals.append(str(e.value))
+            results.append(([bits(t) for t in (q_out, out, z, kc, vc)], refusals))
+    assert results[0][1] == results[1][1]
+    assert all(torch.equal(a, c) for a, c in zip(results[0][0], results[1][0]))
