@@ -46,6 +46,7 @@ struct Tile {
     int q0;                  // the sequence's first token
     int before;              // position of its first token
     int begin, end, active;  // keys of any row (begin a multiple of 64), splits that have some
+    int from, to, least, most;  // positions from..to are seen by every row, least..most by any
 };
 
 __device__ __forceinline__ int token_at(const Batch &b, int i) {
@@ -71,9 +72,13 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int i, bool by_se
     t.rows = min(T, n * a.group - t.first);
     t.before = kv_length(a.b, t.s) - n;
     const int lo = t.before + t.first / a.group, hi = t.before + (t.first + t.rows - 1) / a.group;
+    t.to = lo;
+    t.most = hi;
+    t.from = a.window > 0 ? max(0, hi - a.window + 1) : 0;
+    t.least = a.window > 0 ? max(0, lo - a.window + 1) : 0;
     const int64_t room = (int64_t)a.b.table_pages * a.b.page_size;
     t.end = (int)min((int64_t)(hi + 1), room);
-    t.begin = a.window > 0 ? max(0, lo - a.window + 1) & ~63 : 0;
+    t.begin = t.least & ~63;
     t.active = t.end > t.begin ? min(a.n_split, (t.end - t.begin + a.chunk - 1) / a.chunk) : 1;
     return true;
 }
@@ -99,6 +104,11 @@ __device__ __forceinline__ void load_to_lds(unsigned to, const void *base, unsig
 __device__ __forceinline__ void load_to_lds(unsigned to, const void *at) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
 }
+// A wave-uniform value in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+    const int lo = __builtin_amdgcn_readfirstlane((int)x), hi = __builtin_amdgcn_readfirstlane((int)(x >> 32));
+    return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
+}
 // All but the last N vector memory operations of the wave are done.
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -108,42 +118,43 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 
 // A wave's ROWS consecutive positions at a time, of every STEP, out of the pages into LDS. Positions that are
 // not there read the pool's first rows (the scores' mask leaves them out).
-// WHOLE: the 16 positions from a multiple of 16 on lie in one page, so a page is looked up once for them, 64
-// lookups at a time, one per lane; otherwise every position's place is looked up, 128 at a time, into LDS.
+// WHOLE: the 16 positions from a multiple of 16 on lie in one page, so a place is looked up once for them, 64
+// at a time, one per lane; otherwise every position's place is looked up, 128 at a time, into LDS.
 template <int D, int ROWS, int STEP, bool WHOLE>
 struct Pages {
     static constexpr int PER = 512 / D;        // rows per load
     static constexpr int LOADS = ROWS / PER;   // of keys, and as many of values
-    static constexpr int GROUPS = ROWS < 16 ? 1 : ROWS / 16;
+    static constexpr int GROUPS = ROWS < 16 ? 1 : ROWS / 16, GROUP_LOADS = LOADS / GROUPS;
     static constexpr int AHEAD = WHOLE ? 64 / GROUPS : 128 / ROWS;  // steps looked up at a time
-    const Batch &b;
-    int s, first;        // sequence, the first step's first position
-    int64_t head;        // element offset of the kv head
-    int entry;           // WHOLE: the lane's page
-    LLM_LDS int64_t *places;  // 128 of them
-    unsigned row_bytes, chunk_bytes;  // the lane's row and chunk within a load
+    int first;                // the first step's first position
+    int64_t mine;             // WHOLE: the lane's place, in bytes, with the kv head; -1 where it is not there
+    LLM_LDS int64_t *places;  // otherwise: 128 of them
+    int64_t head;             // bytes to the kv head
+    unsigned offset[GROUP_LOADS];  // the lane's bytes within load i: WHOLE with its row, otherwise its chunk alone
 
-    __device__ __forceinline__ Pages(const Batch &b_, int s_, int kv, int first_, int row0, LLM_LDS int64_t *places_)
-        : b(b_), s(s_), first(first_), head(kv * b_.head_stride), entry(-1), places(places_) {
+    // row0: where in the buffer the wave's rows begin, a multiple of PER
+    __device__ __forceinline__ Pages(const Batch &b, int kv, int first_, int row0, LLM_LDS int64_t *places_)
+        : first(first_), mine(-1), places(places_), head(uniform(kv * b.head_stride * 2)) {
         const int lane = threadIdx.x & 63, r = lane / (D / 8);
-        row_bytes = r * (unsigned)b.slot_stride * 2;
-        chunk_bytes = (lane % (D / 8) ^ swizzle<D>(r + row0)) * 16;  // row0, of the buffer: a multiple of PER
+#pragma unroll
+        for (int i = 0; i < GROUP_LOADS; i++)
+            offset[i] = (lane % (D / 8) ^ swizzle<D>(row0 + i * PER + r)) * 16 +
+                        (WHOLE ? (unsigned)(i * PER + r) * (unsigned)b.slot_stride * 2 : 0);
     }
 
     // Looks up steps step .. step + AHEAD - 1, when step is a multiple of AHEAD.
-    __device__ __forceinline__ void look_up(int step) {
+    __device__ __forceinline__ void look_up(const Batch &b, int s, int step) {
         if (step % AHEAD != 0) return;
         const int lane = threadIdx.x & 63;
         if constexpr (WHOLE) {
-            const int p = first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16;
-            const int i = divide(p, b.page.m, b.page.l);
-            entry = i < b.table_pages ? gptr(b.table)[(int64_t)s * b.table_pages + i] : -1;
-            if ((unsigned)entry >= (unsigned)b.n_pages) entry = -1;
+            const int64_t at = place(b, s, first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16);
+            mine = at < 0 ? -1 : at * 2 + head;
         } else {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
                 const int n = lane + 64 * k;
-                places[n] = place(b, s, first + (step + n / ROWS) * STEP + n % ROWS);
+                const int64_t at = place(b, s, first + (step + n / ROWS) * STEP + n % ROWS);
+                places[n] = at < 0 ? -1 : at * 2 + head;
             }
             wait_lds();
         }
@@ -155,7 +166,7 @@ struct Pages {
             uint32_t bits = 0;
 #pragma unroll
             for (int g = 0; g < GROUPS; g++)
-                if (__builtin_amdgcn_readlane(entry, step % AHEAD * GROUPS + g) >= 0)
+                if (__builtin_amdgcn_readlane((int)(mine >> 32), step % AHEAD * GROUPS + g) >= 0)
                     bits |= (ROWS < 16 ? (1u << ROWS) - 1 : 0xffffu) << (16 * g);
             return bits;
         } else {
@@ -169,50 +180,53 @@ struct Pages {
         if constexpr (WHOLE) {
 #pragma unroll
             for (int g = 0; g < GROUPS; g++) {
-                const int page = __builtin_amdgcn_readlane(entry, step % AHEAD * GROUPS + g);
-                const int p = first + step * STEP + g * 16;
-                const int slot = p - divide(p, b.page.m, b.page.l) * b.page_size;
-                const char *base = (const char *)(cache + head + (int64_t)max(page, 0) * b.page_stride +
-                                                  (page < 0 ? 0 : slot) * b.slot_stride);
+                const int lane = step % AHEAD * GROUPS + g;
+                const int hi = __builtin_amdgcn_readlane((int)(mine >> 32), lane);
+                const unsigned lo = __builtin_amdgcn_readlane((int)mine, lane);
+                const char *base = (const char *)uniform((int64_t)cache + (hi < 0 ? head : (int64_t)hi << 32 | lo));
 #pragma unroll
-                for (int i = 0; i < LOADS / GROUPS; i++)
-                    load_to_lds(to + (g * (LOADS / GROUPS) + i) * 1024, base + i * PER * b.slot_stride * 2,
-                                row_bytes + (chunk_bytes ^ (swizzle<D>(i * PER) * 16)));
+                for (int i = 0; i < GROUP_LOADS; i++)
+                    load_to_lds(to + (g * GROUP_LOADS + i) * 1024, base, offset[i]);
             }
         } else {
             const int r = (threadIdx.x & 63) / (D / 8);
 #pragma unroll
             for (int i = 0; i < LOADS; i++) {
                 const int64_t at = places[step % AHEAD * ROWS + i * PER + r];
-                load_to_lds(to + i * 1024, (const char *)(cache + head + (at < 0 ? 0 : at)) +
-                                               (chunk_bytes ^ (swizzle<D>(i * PER) * 16)));
+                load_to_lds(to + i * 1024, (const char *)cache + (at < 0 ? head : at) + offset[i % GROUP_LOADS]);
             }
         }
     }
 };
 
-// The wave's own rows of values in LDS (as LOADS loads of its lanes left them) with zeros in place of NaN
-// and infinities; whether there were any. A weight of 0 times such a value would not be 0.
-template <int LOADS>
-__device__ __forceinline__ bool zero_bad_values(lds_char *rows) {
+// The wave's own rows of values in LDS, as LOADS loads of its lanes left them, from position `at` on: those that
+// no row of the tile sees become zeros, since 0 times a NaN or an infinity would not be 0. Of those that some
+// rows see and others do not, NaN and infinities become zeros; whether there were any (add_bad then gives
+// them back to the rows that see them). seen: positions from..to are seen by every row, least..most by any.
+template <int D, int LOADS>
+__device__ __forceinline__ bool clear_unseen(lds_char *rows, int at, uint32_t there, int from, int to, int least,
+                                             int most) {
     const int lane = threadIdx.x & 63;
-    const auto bad = [](uint32_t w) {
-        return ((w & 0x7f80u) == 0x7f80u ? 0xffffu : 0u) | ((w & 0x7f800000u) == 0x7f800000u ? 0xffff0000u : 0u);
-    };
-    uint32_t any = 0;
-#pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-        const u32x4 x = *(LLM_LDS u32x4 *)(rows + i * 1024 + lane * 16);
-        any |= bad(x.x) | bad(x.y) | bad(x.z) | bad(x.w);
-    }
-    if (!__any(any != 0)) return false;
+    bool found = false;
 #pragma unroll 1
     for (int i = 0; i < LOADS; i++) {
-        LLM_LDS u32x4 *at = (LLM_LDS u32x4 *)(rows + i * 1024 + lane * 16);
-        const u32x4 x = *at;
-        *at = u32x4{x.x & ~bad(x.x), x.y & ~bad(x.y), x.z & ~bad(x.z), x.w & ~bad(x.w)};
+        const int r = i * (512 / D) + lane / (D / 8), p = at + r;
+        LLM_LDS u32x4 *x = (LLM_LDS u32x4 *)(rows + i * 1024 + lane * 16);
+        if (!(there >> r & 1) || p < least || p > most) {
+            *x = u32x4{0, 0, 0, 0};
+        } else if (p < from || p > to) {
+            u32x4 v = *x;
+            bool bad = false;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if ((v[j] & 0x7f80u) == 0x7f80u) v[j] &= 0xffff0000u, bad = true;
+                if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] &= 0xffffu, bad = true;
+            }
+            if (bad) *x = v;
+            found |= bad;
+        }
     }
-    return true;
+    return __any(found);
 }
 
 // ------------------------------------------------------------------------------------------
@@ -342,36 +356,31 @@ struct Columns {
         }
     }
 
-    // The share of the NaN and infinities that zero_bad_values took out, where a row sees them: 32 keys
-    // from position `at` on, read from the cache again, one by one. p: their weights; sees: the lane's
-    // bits; space: 16 x 32 floats of the wave's own LDS.
-    __device__ __forceinline__ void add_bad(const AttendArgs &a, int s, int kv, int at, uint32_t sees, const f32x16 &p,
-                                            LLM_LDS float *space) {
-        const int h = (threadIdx.x & 63) >> 5;
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            wait_lds();
-#pragma unroll
-            for (int j = 0; j < 8; j++) space[((j & 3) + 8 * (j >> 2) + 4 * h) * 32 + column] = p[8 * t + j];
-            wait_lds();
+    // What clear_unseen took out, for the rows that see it: the keys first .. last, one by one, each weight from
+    // its own score.
+    __device__ __forceinline__ void add_bad(const AttendArgs &a, const Tile &t, int kv, int first, int last, int base) {
+        const int h = (threadIdx.x & 63) >> 5, row = min(base + column, t.rows - 1) + t.first, token = row / a.group;
+        const bf16 *query = a.q + (t.q0 + token) * a.q_stride + (kv * a.group + row - token * a.group) * D;
 #pragma unroll 1
-            for (int k = 0; k < 16; k++) {
-                const int64_t where = place(a.b, s, at + 16 * t + k);
-                if (where < 0) continue;
-                const float w = space[k * 32 + column];
-                const bool seen = sees >> (16 * t + k) & 1;
-                const bf16 *v = a.b.vc + where + kv * a.b.head_stride + 4 * h;
+        for (int p = first; p <= last; p++) {
+            const int64_t where = place(a.b, t.s, p);
+            if (where < 0) continue;
+            const bf16 *k = a.b.kc + where + kv * a.b.head_stride, *v = a.b.vc + where + kv * a.b.head_stride;
+            float dot = 0.0f;
+#pragma unroll 1
+            for (int d = 0; d < D; d += 8) dot = dot8(ld16(query + d), ld16(k + d), dot);
+            const float weight = __builtin_amdgcn_exp2f(fmaf(dot, a.scale_log2, -top));
+            const bool seen = p <= position && (a.window <= 0 || p > position - a.window);
 #pragma unroll
-                for (int d = 0; d < D / 32; d++)
+            for (int d = 0; d < D / 32; d++)
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const u32x2 x = *gptr((const u32x2 *)(v + 32 * d + 8 * r));
-                        const float e[4] = {lo_f(x.x), hi_f(x.x), lo_f(x.y), hi_f(x.y)};
+                for (int r = 0; r < 4; r++) {
+                    const u32x2 x = *gptr((const u32x2 *)(v + 32 * d + 8 * r + 4 * h));
+                    const float e[4] = {lo_f(x.x), hi_f(x.x), lo_f(x.y), hi_f(x.y)};
 #pragma unroll
-                        for (int n = 0; n < 4; n++)
-                            if (seen && !(fabsf(e[n]) < INFINITY)) o[d][4 * r + n] = fmaf(w, e[n], o[d][4 * r + n]);
-                    }
-            }
+                    for (int n = 0; n < 4; n++)
+                        o[d][4 * r + n] = fmaf(weight, seen && !(fabsf(e[n]) < INFINITY) ? e[n] : 0.0f, o[d][4 * r + n]);
+                }
         }
     }
 };
@@ -403,7 +412,6 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
     typedef Pages<D, ROWS, ROWS, WHOLE> P;
     constexpr int LOADS = P::LOADS;
     __shared__ __align__(1024) char lds[4][2 * BYTES];
-    __shared__ float space[4][512];
     __shared__ int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
     __shared__ float tops[4][32], sums[4][32];
     const int tile = blockIdx.x / a.n_kv_heads, kv = blockIdx.x - tile * a.n_kv_heads;
@@ -420,31 +428,28 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 
     Columns<D> c;
     c.start(a, t, kv, 0);
-    const int lowest = t.before + t.first / a.group, highest = t.before + (t.first + t.rows - 1) / a.group;
-    P pages(a.b, t.s, kv, begin + s0 * ROWS, 0, (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
+    P pages(a.b, kv, begin + s0 * ROWS, 0, (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
     lds_char *keys = (lds_char *)lds[w], *values = keys + BYTES;
     const unsigned key_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)keys), value_at = key_at + BYTES;
     uint32_t there = 0;
     if (n > 0) {
-        pages.look_up(0);
+        pages.look_up(a.b, t.s, 0);
         there = pages.there(0);
         pages.request(a.b.kc, 0, key_at);
         pages.request(a.b.vc, 0, value_at);
     }
+    bool bad = false;
     for (int i = 0; i < n; i++) {
         const int at = begin + (s0 + i) * ROWS;
         const bool more = i + 1 < n;
+        const bool edge = at < t.from || at + ROWS - 1 > t.to || there != ~0u;
+        const uint32_t here = there;
         wait_loads<LOADS>();
         f32x16 s[1] = {c.scores(keys)};
-        const bool edge = at + ROWS - 1 > lowest || (a.window > 0 && at <= highest - a.window) || there != ~0u;
-        uint32_t bits = ~0u;
-        if (edge) {
-            bits = c.sees(at, a.window) & there;
-            hide(s[0], bits);
-        }
+        if (edge) hide(s[0], c.sees(at, a.window) & here);
         wait_lds();
         if (more) {
-            pages.look_up(i + 1);
+            pages.look_up(a.b, t.s, i + 1);
             there = pages.there(i + 1);
             pages.request(a.b.kc, i + 1, key_at);
         }
@@ -453,11 +458,15 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
             wait_loads<LOADS>();
         else
             wait_loads<0>();
-        const bool bad = edge && zero_bad_values<LOADS>(values);
+        if (edge) bad |= clear_unseen<D, LOADS>(values, at, here, t.from, t.to, t.least, t.most);
         c.template add<true>(values, s[0]);
-        if (bad) c.add_bad(a, t.s, kv, at, bits, s[0], (LLM_LDS float *)space[w]);
         wait_lds();
         if (more) pages.request(a.b.vc, i + 1, value_at);
+    }
+    if (bad) {
+        const int first = begin + s0 * ROWS, last = min(first + n * ROWS, t.end) - 1;
+        c.add_bad(a, t, kv, max(first, t.least), min(last, t.from - 1), 0);
+        c.add_bad(a, t, kv, max(max(first, t.least), max(t.from, t.to + 1)), min(last, t.most), 0);
     }
 
     // join the waves: each one's output, maximum and sum through LDS
@@ -527,9 +536,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     typedef Pages<D, NK / 4, NK, WHOLE> P;
     constexpr int LOADS = P::LOADS;
     __shared__ __align__(1024) char lds[2][2 * BYTES];  // keys, values
-    __shared__ float space[4][512];
     __shared__ int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
-    __shared__ __align__(16) uint32_t state[2][4];  // of each wave's rows: which are there, and bit 31: bad values among them
+    __shared__ __align__(16) uint32_t present[2][4];  // of each wave's rows: which are there
+    __shared__ int any_bad[4];
     const int w = wave_id(), lane = threadIdx.x & 63;
     const int units = gridDim.x / a.n_kv_heads;
     const int tile = units - 1 - blockIdx.x / a.n_kv_heads, kv = blockIdx.x % a.n_kv_heads;
@@ -546,65 +555,57 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     c.start(a, t, kv, 32 * w);
     const auto position_of = [&](int row) { return t.before + (t.first + row) / a.group; };
     const bool any_rows = 32 * w < t.rows;
-    const int lowest = position_of(0), highest = position_of(t.rows - 1);  // of the workgroup
     const int low = position_of(32 * w), high = position_of(min(t.rows, 32 * w + 32) - 1);  // of the wave
-    P pages(a.b, t.s, kv, begin + w * (NK / 4), w * (NK / 4), (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
+    P pages(a.b, kv, begin + w * (NK / 4), w * (NK / 4), (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
     const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char *)lds) + w * (BYTES / 4);
     if (n > 0) {
-        pages.look_up(0);
+        pages.look_up(a.b, t.s, 0);
         pages.request(a.b.kc, 0, mine);
         pages.request(a.b.vc, 0, mine + BYTES);
     }
     constexpr uint32_t ALL = NK / 4 == 16 ? 0xffffu : (1u << (NK / 4)) - 1;
+    bool bad = false;
     for (int i = 0; i < n; i++) {
         const int at = begin + i * NK, buffer = i & 1;
         const uint32_t there = pages.there(i);
         wait_loads<0>();
-        bool bad = false;
-        if (at + NK - 1 > lowest || (a.window > 0 && at <= highest - a.window) || there != ALL)
-            bad = zero_bad_values<LOADS>((lds_char *)lds[buffer] + BYTES + w * (BYTES / 4));
-        if (lane == 0) state[buffer][w] = there | (bad ? 1u << 31 : 0u);
+        if (at < t.from || at + NK - 1 > t.to || there != ALL)
+            bad |= clear_unseen<D, LOADS>((lds_char *)lds[buffer] + BYTES + w * (BYTES / 4), at + w * (NK / 4), there,
+                                          t.from, t.to, t.least, t.most);
+        if (lane == 0) present[buffer][w] = there;
         __syncthreads();
         if (i + 1 < n) {
-            pages.look_up(i + 1);
+            pages.look_up(a.b, t.s, i + 1);
             pages.request(a.b.kc, i + 1, mine + (buffer ^ 1) * 2 * BYTES);
             pages.request(a.b.vc, i + 1, mine + (buffer ^ 1) * 2 * BYTES + BYTES);
         }
         if (!any_rows || at > high || (a.window > 0 && at + NK - 1 <= low - a.window)) continue;
-        const u32x4 st = *(LLM_LDS u32x4 *)(lds_char *)state[buffer];
-        uint32_t st_of[4], whole = ~0u, bad_any = 0;
-#pragma unroll
-        for (int v = 0; v < 4; v++) {
-            st_of[v] = __builtin_amdgcn_readfirstlane(st[v]);
-            whole &= st_of[v];
-            bad_any |= st_of[v] >> 31;
-        }
+        const u32x4 got = *(LLM_LDS u32x4 *)(lds_char *)present[buffer];
         const lds_char *keys = (lds_char *)lds[buffer], *values = keys + BYTES;
         f32x16 s[KT];
 #pragma unroll
         for (int k = 0; k < KT; k++) s[k] = c.scores(keys + k * 32 * 2 * D);
-        const bool edge = at + NK - 1 > low || (a.window > 0 && at <= high - a.window) || (whole & ALL) != ALL;
-        uint32_t bits[KT];
-#pragma unroll
-        for (int k = 0; k < KT; k++) bits[k] = ~0u;
-        if (edge) {
+        const uint32_t all = __builtin_amdgcn_readfirstlane(got[0] & got[1] & got[2] & got[3]);
+        if (at + NK - 1 > low || (a.window > 0 && at <= high - a.window) || all != ALL) {
 #pragma unroll
             for (int k = 0; k < KT; k++) {
-                uint32_t there32 = 0;
                 constexpr int WAVES = 32 / (NK / 4);  // waves whose rows make 32
+                uint32_t here = 0;
 #pragma unroll
-                for (int v = 0; v < WAVES; v++) there32 |= (st_of[k * WAVES + v] & ALL) << (v * (NK / 4));
-                bits[k] = c.sees(at + 32 * k, a.window) & there32;
-                hide(s[k], bits[k]);
+                for (int v = 0; v < WAVES; v++) here |= got[k * WAVES + v] << (v * (NK / 4));
+                hide(s[k], c.sees(at + 32 * k, a.window) & here);
             }
         }
         c.weigh(s, a.scale_log2);
 #pragma unroll
         for (int k = 0; k < KT; k++) c.template add<false>(values + k * 32 * 2 * D, s[k]);
-        if (bad_any)
-#pragma unroll
-            for (int k = 0; k < KT; k++)
-                c.add_bad(a, t.s, kv, at + 32 * k, bits[k], s[k], (LLM_LDS float *)space[w]);
+    }
+    if (lane == 0) any_bad[w] = bad;
+    __syncthreads();
+    if (any_bad[0] | any_bad[1] | any_bad[2] | any_bad[3]) {
+        const int last = min(begin + n * NK, t.end) - 1;
+        c.add_bad(a, t, kv, max(begin, t.least), min(last, t.from - 1), 32 * w);
+        c.add_bad(a, t, kv, max(max(begin, t.least), max(t.from, t.to + 1)), min(last, t.most), 32 * w);
     }
 
     if (!any_rows || c.column >= t.rows - 32 * w) return;
@@ -695,18 +696,17 @@ struct Plan {
         many = longest > 32;
         few_tiles = many ? n_seqs : (int)(rows / 32 + n_seqs);
         many_tiles = (int)(rows / MANY + n_seqs);
-        const auto split = [&](int64_t units, int least, int64_t span, int &n, int &chunk) {
-            const int64_t all = max_kv_len, ragged = (all + 2047) / 2048;
-            n = (int)std::max<int64_t>(1, std::min((all + least - 1) / least,
-                                                   std::max((2 * CUS + units - 1) / units, units < 16 * CUS ? ragged : 1)));
+        const auto split = [&](int64_t units, int least, int64_t even, int64_t span, int &n, int &chunk) {
+            const int64_t all = max_kv_len;
+            n = (int)std::max<int64_t>(1, std::min((all + least - 1) / least, std::max((2 * CUS + units - 1) / units, even)));
             n = (int)std::min<int64_t>(n, (span + least - 1) / least);
             chunk = (int)((span + n - 1) / n + 127) / 128 * 128;
         };
         const auto span = [&](int64_t tokens) {
             return window > 0 ? std::min<int64_t>(max_kv_len, (int64_t)window + tokens + 63) : (int64_t)max_kv_len;
         };
-        split((int64_t)n_seqs * n_kv_heads, 256, span(32), few_split, few_chunk);
-        split(((rows + MANY - 1) / MANY) * n_kv_heads, 512, span(MANY), many_split, many_chunk);
+        split((int64_t)n_seqs * n_kv_heads, 256, (int64_t)n_seqs * n_kv_heads < 16 * CUS ? (max_kv_len + 2047) / 2048 : 1, span(32), few_split, few_chunk);
+        split(((rows + MANY - 1) / MANY) * n_kv_heads, 512, 1, span(MANY), many_split, many_chunk);
         few_rows = few && few_split > 1 ? (size_t)few_tiles * n_kv_heads * few_split * 32 : 0;
         many_rows = many && many_split > 1 ? (size_t)many_tiles * n_kv_heads * many_split * MANY : 0;
         floats = (few_rows + many_rows) * (head_dim + 2);
