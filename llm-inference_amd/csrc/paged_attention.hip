@@ -32,7 +32,7 @@ struct AttendArgs {
     float *part, *stats;  // of this kernel's units: [unit][split][row][head_dim], [unit][split][row][2]
     int n_heads, n_kv_heads, group, window;
     int n_split, chunk;   // keys per split, a multiple of 128
-    int by_sequence;      // few: tile i is sequence i, of at most 32 rows; many: sequences of more
+    int which;            // the sequences whose rows these are
     float scale_log2;     // scale * log2(e)
 };
 
@@ -53,21 +53,43 @@ __device__ __forceinline__ int token_at(const Batch &b, int i) {
     return max(0, min(b.n_tokens, gptr(b.q_start)[i]));
 }
 
-// Tile i of a launch, false where there is none. Sequence s has the tiles from floor(rows before it / T) + s
-// on: at least as many as its own rows fill.
+// Which sequences a kernel takes.
+enum { ALL_ROWS, FEW_ROWS, MANY_ROWS };  // any number of rows; at most FEW; more than FEW
+constexpr int FEW = 32;                  // rows of a tile of attend_few
+constexpr int MANY = 128;                // rows of a tile of attend_many
+
+// Tile i, counted over the sequences that `which` takes, false past the last one. A sequence's tiles come
+// last rows first: those see the most keys.
 template <int T>
-__device__ __forceinline__ bool find_tile(const AttendArgs &a, int i, bool by_sequence, Tile &t) {
-    int j = 0;
-    if (by_sequence) {
-        t.s = i;
-    } else {
-        const auto start = [&](int s) { return (int)((int64_t)token_at(a.b, s) * a.group / T) + s; };
-        t.s = count_leading(a.b.n_seqs - 1, [&](int m) { return start(m + 1) <= i; });
-        j = i - start(t.s);
+__device__ __forceinline__ bool find_tile(const AttendArgs &a, int which, int i, Tile &t) {
+    const int lane = threadIdx.x & 63;
+    int j = -1;
+    for (int s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
+        const int s = s0 + lane;
+        int n = 0;
+        if (s < a.b.n_seqs) {
+            const int first = token_at(a.b, s);
+            const int64_t rows = (int64_t)max(0, token_at(a.b, s + 1) - first) * a.group;
+            if (which == ALL_ROWS || (rows <= FEW) == (which == FEW_ROWS)) n = (int)((rows + T - 1) / T);
+        }
+        int upto = n;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int before = __shfl_up(upto, d);
+            if (lane >= d) upto += before;
+        }
+        const uint64_t past = __ballot(upto > i);
+        if (past) {
+            const int at = __builtin_ctzll(past);
+            t.s = s0 + at;
+            j = __builtin_amdgcn_readlane(upto, at) - 1 - i;
+            break;
+        }
+        i -= __builtin_amdgcn_readlane(upto, 63);
     }
+    if (j < 0) return false;
     t.q0 = token_at(a.b, t.s);
     const int n = token_at(a.b, t.s + 1) - t.q0;
-    if (j < 0 || (int64_t)j * T >= (int64_t)n * a.group) return false;
     t.first = j * T;
     t.rows = min(T, n * a.group - t.first);
     t.before = kv_length(a.b, t.s) - n;
@@ -398,6 +420,16 @@ __device__ __forceinline__ void store4(bf16 *to, float a, float b, float c, floa
     *gptr((u32x2 *)to) = u32x2{pack2(a, b), pack2(c, d)};
 }
 
+// A workgroup's LDS: 512 D bytes of keys and values and little else.
+template <int D, bool WHOLE>
+struct Space {
+    __align__(1024) char rows[512 * D];
+    int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
+    float tops[4][32], sums[4][32];        // few: of each wave's columns
+    __align__(16) uint32_t present[2][4];  // many: which of each wave's rows are there
+    int bad[4];
+};
+
 // ------------------------------------------------------------------------------------------
 // few rows: at most 32 per sequence and kv head
 // ------------------------------------------------------------------------------------------
@@ -407,20 +439,14 @@ __device__ __forceinline__ void store4(bf16 *to, float a, float b, float c, floa
 // nothing waits between waves until their outputs are joined. A wave keeps 32 keys' rows and 32 values' rows in
 // LDS: the next keys are requested once the scores are formed and the next values once they are summed.
 template <int D, bool WHOLE>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(AttendArgs a) {
+__device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int ROWS = 32, BYTES = ROWS * 2 * D;
     typedef Pages<D, ROWS, ROWS, WHOLE> P;
     constexpr int LOADS = P::LOADS;
-    __shared__ __align__(1024) char lds[4][2 * BYTES];
-    __shared__ int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
-    __shared__ float tops[4][32], sums[4][32];
-    const int tile = blockIdx.x / a.n_kv_heads, kv = blockIdx.x - tile * a.n_kv_heads;
+    const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
     const int w = wave_id(), lane = threadIdx.x & 63;
     Tile t;
-    if (!find_tile<32>(a, tile, a.by_sequence, t)) return;
-    if (a.by_sequence && (int64_t)(token_at(a.b, t.s + 1) - t.q0) * a.group > 32) return;
-    const int z = blockIdx.y;
-    if (z >= t.active) return;
+    if (!find_tile<FEW>(a, a.which, tile, t) || z >= t.active) return;
     const int begin = t.begin + z * a.chunk;
     const int end = z == a.n_split - 1 ? t.end : min(t.end, begin + a.chunk);
     const int steps = end > begin ? (end - begin + ROWS - 1) / ROWS : 0;
@@ -428,8 +454,8 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 
     Columns<D> c;
     c.start(a, t, kv, 0);
-    P pages(a.b, kv, begin + s0 * ROWS, 0, (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
-    lds_char *keys = (lds_char *)lds[w], *values = keys + BYTES;
+    P pages(a.b, kv, begin + s0 * ROWS, 0, (LLM_LDS int64_t *)space.places[WHOLE ? 0 : w]);
+    lds_char *keys = (lds_char *)space.rows + w * 2 * BYTES, *values = keys + BYTES;
     const unsigned key_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)keys), value_at = key_at + BYTES;
     uint32_t there = 0;
     if (n > 0) {
@@ -474,11 +500,11 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
     swap_pair<32>(c.sum, x, y);
     __syncthreads();
     if (lane < 32) {
-        tops[w][lane] = c.top;
-        sums[w][lane] = x + y;
+        space.tops[w][lane] = c.top;
+        space.sums[w][lane] = x + y;
     }
     constexpr int CHUNKS = D / 4;  // of four elements, chunk k of a column at k ^ (column & 15)
-    LLM_LDS f32x4 *joined = (LLM_LDS f32x4 *)lds;
+    LLM_LDS f32x4 *joined = (LLM_LDS f32x4 *)(lds_char *)space.rows;
     if (c.column < t.rows) {
 #pragma unroll
         for (int d = 0; d < D / 32; d++)
@@ -490,27 +516,27 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
             }
     }
     __syncthreads();
-    const int64_t unit = ((int64_t)blockIdx.x * a.n_split + z) * 32;
+    const int64_t at = ((int64_t)unit * a.n_split + z) * FEW;
     for (int i = threadIdx.x; i < t.rows * CHUNKS; i += 256) {
         const int row = i / CHUNKS, k = i % CHUNKS;
-        float top = tops[0][row];
+        float top = space.tops[0][row];
 #pragma unroll
-        for (int v = 1; v < 4; v++) top = fmaxf(top, tops[v][row]);
+        for (int v = 1; v < 4; v++) top = fmaxf(top, space.tops[v][row]);
         float sum = 0.0f;
         f32x4 o = {0, 0, 0, 0};
 #pragma unroll
         for (int v = 0; v < 4; v++) {
-            const float f = __builtin_amdgcn_exp2f(tops[v][row] - top);
-            sum = fmaf(f, sums[v][row], sum);
+            const float f = __builtin_amdgcn_exp2f(space.tops[v][row] - top);
+            sum = fmaf(f, space.sums[v][row], sum);
             const f32x4 e = joined[(v * 32 + row) * CHUNKS + (k ^ (row & 15))];
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] = fmaf(f, e[j], o[j]);
         }
         if (t.active > 1) {
-            *gptr((f32x4 *)(a.part + (unit + row) * D + 4 * k)) = o;
+            *gptr((f32x4 *)(a.part + (at + row) * D + 4 * k)) = o;
             if (k == 0) {
-                gptr(a.stats)[(unit + row) * 2] = top;
-                gptr(a.stats)[(unit + row) * 2 + 1] = sum;
+                gptr(a.stats)[(at + row) * 2] = top;
+                gptr(a.stats)[(at + row) * 2 + 1] = sum;
             }
         } else {
             const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -525,28 +551,18 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_few_kernel(Atten
 // many rows
 // ------------------------------------------------------------------------------------------
 
-constexpr int MANY = 128;  // rows of a workgroup
-
 // A chunk of new tokens: bound by the matrix products. The four waves of a workgroup take 32 columns each and
 // share the keys and values in LDS, two buffers of NK rows: while one is used the other is filled, a quarter by
 // each wave, with one barrier per NK keys.
 template <int D, bool WHOLE>
-__global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
-    constexpr int NK = D == 256 ? 32 : 64, KT = NK / 32, BYTES = NK * 2 * D;
+__device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
+    constexpr int NK = 64, KT = NK / 32, BYTES = NK * 2 * D;
     typedef Pages<D, NK / 4, NK, WHOLE> P;
     constexpr int LOADS = P::LOADS;
-    __shared__ __align__(1024) char lds[2][2 * BYTES];  // keys, values
-    __shared__ int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
-    __shared__ __align__(16) uint32_t present[2][4];  // of each wave's rows: which are there
-    __shared__ int any_bad[4];
     const int w = wave_id(), lane = threadIdx.x & 63;
-    const int units = gridDim.x / a.n_kv_heads;
-    const int tile = units - 1 - blockIdx.x / a.n_kv_heads, kv = blockIdx.x % a.n_kv_heads;
+    const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
     Tile t;
-    if (!find_tile<MANY>(a, tile, false, t)) return;
-    if (a.by_sequence && (int64_t)(token_at(a.b, t.s + 1) - t.q0) * a.group <= 32) return;
-    const int z = blockIdx.y;
-    if (z >= t.active) return;
+    if (!find_tile<MANY>(a, a.which, tile, t) || z >= t.active) return;
     const int begin = t.begin + z * a.chunk;
     const int end = z == a.n_split - 1 ? t.end : min(t.end, begin + a.chunk);
     const int n = end > begin ? (end - begin + NK - 1) / NK : 0;
@@ -556,8 +572,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     const auto position_of = [&](int row) { return t.before + (t.first + row) / a.group; };
     const bool any_rows = 32 * w < t.rows;
     const int low = position_of(32 * w), high = position_of(min(t.rows, 32 * w + 32) - 1);  // of the wave
-    P pages(a.b, kv, begin + w * (NK / 4), w * (NK / 4), (LLM_LDS int64_t *)places[WHOLE ? 0 : w]);
-    const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char *)lds) + w * (BYTES / 4);
+    P pages(a.b, kv, begin + w * (NK / 4), w * (NK / 4), (LLM_LDS int64_t *)space.places[WHOLE ? 0 : w]);
+    const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char *)space.rows) + w * (BYTES / 4);
     if (n > 0) {
         pages.look_up(a.b, t.s, 0);
         pages.request(a.b.kc, 0, mine);
@@ -570,9 +586,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
         const uint32_t there = pages.there(i);
         wait_loads<0>();
         if (at < t.from || at + NK - 1 > t.to || there != ALL)
-            bad |= clear_unseen<D, LOADS>((lds_char *)lds[buffer] + BYTES + w * (BYTES / 4), at + w * (NK / 4), there,
+            bad |= clear_unseen<D, LOADS>((lds_char *)space.rows + buffer * 2 * BYTES + BYTES + w * (BYTES / 4), at + w * (NK / 4), there,
                                           t.from, t.to, t.least, t.most);
-        if (lane == 0) present[buffer][w] = there;
+        if (lane == 0) space.present[buffer][w] = there;
         __syncthreads();
         if (i + 1 < n) {
             pages.look_up(a.b, t.s, i + 1);
@@ -580,8 +596,8 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
             pages.request(a.b.vc, i + 1, mine + (buffer ^ 1) * 2 * BYTES + BYTES);
         }
         if (!any_rows || at > high || (a.window > 0 && at + NK - 1 <= low - a.window)) continue;
-        const u32x4 got = *(LLM_LDS u32x4 *)(lds_char *)present[buffer];
-        const lds_char *keys = (lds_char *)lds[buffer], *values = keys + BYTES;
+        const u32x4 got = *(LLM_LDS u32x4 *)(lds_char *)space.present[buffer];
+        const lds_char *keys = (lds_char *)space.rows + buffer * 2 * BYTES, *values = keys + BYTES;
         f32x16 s[KT];
 #pragma unroll
         for (int k = 0; k < KT; k++) s[k] = c.scores(keys + k * 32 * 2 * D);
@@ -600,9 +616,9 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
 #pragma unroll
         for (int k = 0; k < KT; k++) c.template add<false>(values + k * 32 * 2 * D, s[k]);
     }
-    if (lane == 0) any_bad[w] = bad;
+    if (lane == 0) space.bad[w] = bad;
     __syncthreads();
-    if (any_bad[0] | any_bad[1] | any_bad[2] | any_bad[3]) {
+    if (space.bad[0] | space.bad[1] | space.bad[2] | space.bad[3]) {
         const int last = min(begin + n * NK, t.end) - 1;
         c.add_bad(a, t, kv, max(begin, t.least), min(last, t.from - 1), 32 * w);
         c.add_bad(a, t, kv, max(max(begin, t.least), max(t.from, t.to + 1)), min(last, t.most), 32 * w);
@@ -614,16 +630,16 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
     const float sum = x + y;
     const int h = lane >> 5, row = 32 * w + c.column;
     if (t.active > 1) {
-        const int64_t unit = ((int64_t)(tile * a.n_kv_heads + kv) * a.n_split + z) * MANY + row;
+        const int64_t at = ((int64_t)unit * a.n_split + z) * MANY + row;
         if (h == 0) {
-            gptr(a.stats)[unit * 2] = c.top;
-            gptr(a.stats)[unit * 2 + 1] = sum;
+            gptr(a.stats)[at * 2] = c.top;
+            gptr(a.stats)[at * 2 + 1] = sum;
         }
 #pragma unroll
         for (int d = 0; d < D / 32; d++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                *gptr((f32x4 *)(a.part + unit * D + 32 * d + 8 * r + 4 * h)) =
+                *gptr((f32x4 *)(a.part + at * D + 32 * d + 8 * r + 4 * h)) =
                     f32x4{c.o[d][4 * r], c.o[d][4 * r + 1], c.o[d][4 * r + 2], c.o[d][4 * r + 3]};
         return;
     }
@@ -639,38 +655,121 @@ __global__ __launch_bounds__(256, 2) void attend_many_kernel(AttendArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------
+// the launch
+// ------------------------------------------------------------------------------------------
+
+struct LaunchArgs {
+    AttendArgs few, many;
+    int few_units, many_units, few_groups, many_groups;  // tiles x kv heads, and those x splits
+};
+
+// Workgroups of both kinds in turn while there are both: the ones read, the others multiply.
+template <int D, bool WHOLE>
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArgs l) {
+    __shared__ Space<D, WHOLE> space;
+    const int both = min(l.few_groups, l.many_groups);
+    int i = blockIdx.x;
+    bool many;
+    if (i < 2 * both) {
+        many = !(i & 1);
+        i >>= 1;
+    } else {
+        many = l.many_groups > both;
+        i -= both;
+    }
+    if (many)
+        attend_many<D, WHOLE>(l.many, i % l.many_units, i / l.many_units, space);
+    else
+        attend_few<D, WHOLE>(l.few, i % l.few_units, i / l.few_units, space);
+}
+
+// ------------------------------------------------------------------------------------------
 // the splits' join
 // ------------------------------------------------------------------------------------------
 
-// Four elements of a row per thread, the splits in order.
+// A wave joins 256 / D rows, four elements of a row per lane, up to 8 splits' parts requested at a time and
+// added in order. Few rows of many splits: the four waves of a workgroup take a quarter of the splits each and
+// are joined in order through LDS; many rows of few splits: each wave takes rows of its own.
 template <int D, int T>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
-    constexpr int CHUNKS = D / 4;
-    const int tile = blockIdx.x / a.n_kv_heads, kv = blockIdx.x - tile * a.n_kv_heads;
+__device__ __forceinline__ void join_tile(const AttendArgs &a, int unit, int part, int parts, f32x4 (&outs)[4][64],
+                                          float (&tops)[4][64], float (&sums)[4][64]) {
+    constexpr int CHUNKS = D / 4, ROWS = 64 / CHUNKS, U = 8;
+    constexpr bool SHARED = T == FEW;
+    const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
+    const int w = wave_id(), lane = threadIdx.x & 63, k = lane % CHUNKS;
     Tile t;
-    if (!find_tile<T>(a, tile, T == 32 && a.by_sequence, t)) return;
-    const bool few = (int64_t)(token_at(a.b, t.s + 1) - t.q0) * a.group <= 32;
-    if (t.active <= 1 || (a.by_sequence && few != (T == 32))) return;
-    for (int i = blockIdx.y * 256 + threadIdx.x; i < t.rows * CHUNKS; i += 256 * gridDim.y) {
-        const int row = i / CHUNKS, k = i % CHUNKS;
-        const int64_t unit = (int64_t)blockIdx.x * a.n_split * T + row;
+    if (!find_tile<T>(a, a.which, tile, t) || t.active <= 1) return;
+    const int z0 = SHARED ? t.active * w / 4 : 0, z1 = SHARED ? t.active * (w + 1) / 4 : t.active;
+    for (int r0 = part * ROWS * (SHARED ? 1 : 4); r0 < t.rows; r0 += parts * ROWS * (SHARED ? 1 : 4)) {
+        const int row = r0 + (SHARED ? 0 : w * ROWS) + lane / CHUNKS;
+        const int64_t at = (int64_t)unit * a.n_split * T + min(row, t.rows - 1);
         float top = LOWEST, sum = 0.0f;
         f32x4 o = {0, 0, 0, 0};
-        for (int z = 0; z < t.active; z++) {
-            const int64_t at = unit + (int64_t)z * T;
-            const float m = gptr(a.stats)[at * 2], n = gptr(a.stats)[at * 2 + 1];
-            const f32x4 e = *gptr((const f32x4 *)(a.part + at * D + 4 * k));
-            const float next = fmaxf(top, m);
-            const float f = __builtin_amdgcn_exp2f(top - next), g = __builtin_amdgcn_exp2f(m - next);
-            top = next;
-            sum = sum * f + n * g;
+        for (int z = z0; z < z1; z += U) {
+            float m[U], n[U];
+            f32x4 e[U];
 #pragma unroll
-            for (int j = 0; j < 4; j++) o[j] = o[j] * f + e[j] * g;
+            for (int u = 0; u < U; u++) {
+                const int64_t from = at + (int64_t)min(z + u, z1 - 1) * T;
+                const u32x2 s = *gptr((const u32x2 *)(a.stats + from * 2));
+                m[u] = z + u < z1 ? __uint_as_float(s.x) : LOWEST;
+                n[u] = z + u < z1 ? __uint_as_float(s.y) : 0.0f;
+                e[u] = *gptr((const f32x4 *)(a.part + from * D + 4 * k));
+            }
+            float next = top;
+#pragma unroll
+            for (int u = 0; u < U; u++) next = fmaxf(next, m[u]);
+            const float f = __builtin_amdgcn_exp2f(top - next);
+            top = next;
+            sum *= f;
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[j] *= f;
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                if (z + u >= z1) break;
+                const float g = __builtin_amdgcn_exp2f(m[u] - next);
+                sum = fmaf(n[u], g, sum);
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = fmaf(e[u][j], g, o[j]);
+            }
         }
+        if constexpr (SHARED) {
+            __syncthreads();  // the last rows' parts have been read
+            outs[w][lane] = o;
+            tops[w][lane] = top;
+            sums[w][lane] = sum;
+            __syncthreads();
+            if (w != 0) continue;
+            for (int v = 1; v < 4; v++) top = fmaxf(top, tops[v][lane]);
+            sum = 0.0f;
+            o = f32x4{0, 0, 0, 0};
+            for (int v = 0; v < 4; v++) {
+                const float g = __builtin_amdgcn_exp2f(tops[v][lane] - top);
+                sum = fmaf(sums[v][lane], g, sum);
+                const f32x4 e = outs[v][lane];
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = fmaf(e[j], g, o[j]);
+            }
+        }
+        if (row >= t.rows) continue;
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int r = t.first + row, token = r / a.group;
         store4(a.out + (t.q0 + token) * a.out_stride + (kv * a.group + r - token * a.group) * D + 4 * k, o[0] * f,
                o[1] * f, o[2] * f, o[3] * f);
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(256) void attend_join_kernel(LaunchArgs l, int few_parts, int many_parts) {
+    __shared__ f32x4 outs[4][64];
+    __shared__ float tops[4][64], sums[4][64];
+    const int few = l.few.n_split > 1 ? l.few_units * few_parts : 0;
+    int i = blockIdx.x;
+    if (i < few) {
+        join_tile<D, FEW>(l.few, i / few_parts, i % few_parts, few_parts, outs, tops, sums);
+    } else {
+        i -= few;
+        join_tile<D, MANY>(l.many, i / many_parts, i % many_parts, many_parts, outs, tops, sums);
     }
 }
 
@@ -680,22 +779,24 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
 
 constexpr int CUS = 256;
 
-// How the work is split, from the host's sizes alone. A sequence's rows (new tokens x group) go to
-// attend_few_kernel up to 32 and to attend_many_kernel above, or all to one of them where the expected lengths
-// leave the other nothing.
+// How the work is split, from the host's sizes alone. A sequence's rows (new tokens x group) go to attend_few
+// up to FEW and to attend_many above, or all to one of them where the expected lengths leave the other nothing.
 struct Plan {
     bool few, many;
-    int few_tiles, many_tiles, few_split, few_chunk, many_split, many_chunk;
+    int few_units, many_units, few_split, few_chunk, many_split, many_chunk;
     size_t few_rows, many_rows, floats;  // rows of partial outputs
 
     Plan(int n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len,
          int window) {
         const int64_t group = n_heads / n_kv_heads, rows = n_tokens * group;
         const int64_t longest = std::min<int64_t>(max_q_len, n_tokens) * group;
-        few = longest <= 32 || n_seqs > 1;
-        many = longest > 32;
-        few_tiles = many ? n_seqs : (int)(rows / 32 + n_seqs);
-        many_tiles = (int)(rows / MANY + n_seqs);
+        few = longest <= FEW || n_seqs > 1;
+        many = longest > FEW;
+        // at most one tile of a sequence is not full; one of many rows has over FEW of them
+        const int64_t few_tiles = many ? n_seqs : rows / FEW + std::min<int64_t>(n_seqs, rows);
+        const int64_t many_tiles = rows / MANY + (few ? std::min<int64_t>(n_seqs, rows / (FEW + 1)) : n_seqs);
+        few_units = few ? (int)(few_tiles * n_kv_heads) : 0;
+        many_units = many ? (int)(many_tiles * n_kv_heads) : 0;
         const auto split = [&](int64_t units, int least, int64_t even, int64_t span, int &n, int &chunk) {
             const int64_t all = max_kv_len;
             n = (int)std::max<int64_t>(1, std::min((all + least - 1) / least, std::max((2 * CUS + units - 1) / units, even)));
@@ -707,8 +808,8 @@ struct Plan {
         };
         split((int64_t)n_seqs * n_kv_heads, 256, (int64_t)n_seqs * n_kv_heads < 16 * CUS ? (max_kv_len + 2047) / 2048 : 1, span(32), few_split, few_chunk);
         split(((rows + MANY - 1) / MANY) * n_kv_heads, 512, 1, span(MANY), many_split, many_chunk);
-        few_rows = few && few_split > 1 ? (size_t)few_tiles * n_kv_heads * few_split * 32 : 0;
-        many_rows = many && many_split > 1 ? (size_t)many_tiles * n_kv_heads * many_split * MANY : 0;
+        few_rows = few_split > 1 ? (size_t)few_units * few_split * FEW : 0;
+        many_rows = many_split > 1 ? (size_t)many_units * many_split * MANY : 0;
         floats = (few_rows + many_rows) * (head_dim + 2);
     }
 };
@@ -723,33 +824,31 @@ bool check_sizes(const char *name, int n_tokens, int n_heads, int max_q_len, int
 }
 
 template <int D, bool WHOLE>
-void launch_attention(AttendArgs a, const Plan &p, float *ws, hipStream_t stream) {
-    AttendArgs few = a, many = a;
-    few.part = ws;
-    few.stats = ws + p.few_rows * D;
-    many.part = few.stats + p.few_rows * 2;
-    many.stats = many.part + p.many_rows * D;
-    few.n_split = p.few_split;
-    few.chunk = p.few_chunk;
-    many.n_split = p.many_split;
-    many.chunk = p.many_chunk;
-    few.by_sequence = p.many;
-    many.by_sequence = p.few;
-    const int h = a.n_kv_heads;
-    if (p.many) {
-        attend_many_kernel<D, WHOLE><<<dim3(p.many_tiles * h, p.many_split), 256, 0, stream>>>(many);
-        if (!LAUNCH_OK()) return;
-    }
-    if (p.few) {
-        attend_few_kernel<D, WHOLE><<<dim3(p.few_tiles * h, p.few_split), 256, 0, stream>>>(few);
-        if (!LAUNCH_OK()) return;
-    }
-    if (p.many && p.many_split > 1) {
-        attend_join_kernel<D, MANY><<<dim3(p.many_tiles * h, D / 32), 256, 0, stream>>>(many);
-        if (!LAUNCH_OK()) return;
-    }
-    if (p.few && p.few_split > 1) {
-        attend_join_kernel<D, 32><<<dim3(p.few_tiles * h, 1), 256, 0, stream>>>(few);
+void launch_attention(const AttendArgs &a, const Plan &p, float *ws, int max_q_len, hipStream_t stream) {
+    LaunchArgs l;
+    l.few = l.many = a;
+    l.few.part = ws;
+    l.few.stats = ws + p.few_rows * D;
+    l.many.part = l.few.stats + p.few_rows * 2;
+    l.many.stats = l.many.part + p.many_rows * D;
+    l.few.n_split = p.few_split;
+    l.few.chunk = p.few_chunk;
+    l.many.n_split = p.many_split;
+    l.many.chunk = p.many_chunk;
+    l.few.which = p.many ? FEW_ROWS : ALL_ROWS;
+    l.many.which = p.few ? MANY_ROWS : ALL_ROWS;
+    l.few_units = p.few_units;
+    l.many_units = p.many_units;
+    l.few_groups = p.few_units * p.few_split;
+    l.many_groups = p.many_units * p.many_split;
+    attend_kernel<D, WHOLE><<<l.few_groups + l.many_groups, 256, 0, stream>>>(l);
+    if (!LAUNCH_OK()) return;
+    constexpr int ROWS = 256 / D;  // of a wave of the join
+    const int expected = (int)std::min<int64_t>(FEW, (int64_t)max_q_len * a.group);
+    const int few_parts = (expected + ROWS - 1) / ROWS, many_parts = MANY / (4 * ROWS);
+    const int joins = (p.few_split > 1 ? p.few_units * few_parts : 0) + (p.many_split > 1 ? p.many_units * many_parts : 0);
+    if (joins > 0) {
+        attend_join_kernel<D><<<joins, 256, 0, stream>>>(l, few_parts, many_parts);
         LAUNCH_OK();
     }
 }
@@ -790,6 +889,11 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
     const int64_t width = (int64_t)n_heads * D;
     if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width)) return;
     const Plan plan(n_tokens, batch->n_seqs, n_heads, batch->n_kv_heads, D, max_q_len, max_kv_len, window);
+    if ((int64_t)plan.few_units * plan.few_split + (int64_t)plan.many_units * plan.many_split > INT32_MAX / 64) {
+        llm_fail("%s: %d rows in %d sequences of up to %d tokens are too many for one launch", name, n_tokens,
+                 batch->n_seqs, max_kv_len);
+        return;
+    }
     if (!aligned16(ws) || (plan.floats && !ws)) {
         llm_fail("%s: ws must be a 16-byte aligned device address", name);
         return;
@@ -807,9 +911,9 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
 #define ATTEND(D_)                                      \
     if (D == D_) {                                      \
         if (whole)                                      \
-            launch_attention<D_, true>(a, plan, ws, stream);  \
+            launch_attention<D_, true>(a, plan, ws, max_q_len, stream);  \
         else                                            \
-            launch_attention<D_, false>(a, plan, ws, stream); \
+            launch_attention<D_, false>(a, plan, ws, max_q_len, stream); \
     }
     ATTEND(64) ATTEND(128) ATTEND(256)
 #undef ATTEND
