@@ -311,10 +311,11 @@ struct Columns {
         return s;
     }
 
-    // Scores to weights 2^(s c - top), with the maximum moved where it has grown by more than 2^8 for any
-    // column: below that the weights stay in range and a larger maximum changes no relative rounding.
+    // Scores to weights 2^(s c - top) in two steps. The maximum moves where a column's has grown by more than a
+    // factor of 2^8 (for all 32 columns then): below that the weights stay in range, and a larger maximum would
+    // change no relative rounding.
     template <int KT>
-    __device__ __forceinline__ void weigh(f32x16 (&s)[KT], float c) {
+    __device__ __forceinline__ float peak(const f32x16 (&s)[KT], float c) const {
         float m = s[0][0];
 #pragma unroll
         for (int k = 0; k < KT; k++)
@@ -322,18 +323,22 @@ struct Columns {
             for (int r = 0; r < 16; r++) m = fmaxf(m, s[k][r]);
         float x, y;
         swap_pair<32>(m, x, y);
-        m = fmaxf(x, y) * c;
-        if (__any(m > top + 8.0f)) {
-            const float next = fmaxf(top, m);
-            const float keep = __builtin_amdgcn_exp2f(top - next);
-            top = next;
-            sum *= keep;
+        return fmaxf(x, y) * c;
+    }
+    __device__ __forceinline__ void raise(float m) {
+        if (!__any(m > top + 8.0f)) return;
+        const float next = fmaxf(top, m);
+        const float keep = __builtin_amdgcn_exp2f(top - next);
+        top = next;
+        sum *= keep;
 #pragma unroll
-            for (int d = 0; d < D / 32; d++)
+        for (int d = 0; d < D / 32; d++)
 #pragma unroll
-                for (int r = 0; r < 16; r++) o[d][r] *= keep;
-        }
-        float part[4] = {0, 0, 0, 0};
+            for (int r = 0; r < 16; r++) o[d][r] *= keep;
+    }
+    template <int KT>
+    __device__ __forceinline__ void weigh(f32x16 (&s)[KT], float c) {
+        float part[4] = {sum, 0, 0, 0};
 #pragma unroll
         for (int k = 0; k < KT; k++)
 #pragma unroll
@@ -341,7 +346,7 @@ struct Columns {
                 s[k][r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, -top));
                 part[r & 3] += s[k][r];
             }
-        sum += (part[0] + part[1]) + (part[2] + part[3]);
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
     }
 
     // O^T += V^T P^T over 32 keys: the weights rounded to bf16, with EXACT their remainders too.
@@ -424,7 +429,7 @@ __device__ __forceinline__ void store4(bf16 *to, float a, float b, float c, floa
 template <int D, bool WHOLE>
 struct Space {
     __align__(1024) char rows[512 * D];
-    int64_t places[WHOLE ? 1 : 4][WHOLE ? 1 : 128];
+    int64_t places[WHOLE ? 1 : 8][WHOLE ? 1 : 128];  // of each wave; many: for keys, then for values
     float tops[4][32], sums[4][32];        // few: of each wave's columns
     __align__(16) uint32_t present[2][4];  // many: which of each wave's rows are there
     int bad[4];
@@ -479,6 +484,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
             there = pages.there(i + 1);
             pages.request(a.b.kc, i + 1, key_at);
         }
+        c.raise(c.peak(s, a.scale_log2));
         c.weigh(s, a.scale_log2);
         if (more)
             wait_loads<LOADS>();
@@ -572,35 +578,47 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
     const auto position_of = [&](int row) { return t.before + (t.first + row) / a.group; };
     const bool any_rows = 32 * w < t.rows;
     const int low = position_of(32 * w), high = position_of(min(t.rows, 32 * w + 32) - 1);  // of the wave
-    P pages(a.b, kv, begin + w * (NK / 4), w * (NK / 4), (LLM_LDS int64_t *)space.places[WHOLE ? 0 : w]);
+    const int first = begin + w * (NK / 4);
+    P kp(a.b, kv, first, w * (NK / 4), (LLM_LDS int64_t *)space.places[WHOLE ? 0 : w]);
+    P vp(a.b, kv, first, w * (NK / 4), (LLM_LDS int64_t *)space.places[WHOLE ? 0 : 4 + w]);
     const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char *)space.rows) + w * (BYTES / 4);
-    if (n > 0) {
-        pages.look_up(a.b, t.s, 0);
-        pages.request(a.b.kc, 0, mine);
-        pages.request(a.b.vc, 0, mine + BYTES);
-    }
     constexpr uint32_t ALL = NK / 4 == 16 ? 0xffffu : (1u << (NK / 4)) - 1;
+    lds_char *keys = (lds_char *)space.rows, *values = keys + 2 * BYTES;  // two buffers each
+    f32x16 s[KT], next[KT];
     bool bad = false;
+    if (n > 0) {
+        kp.look_up(a.b, t.s, 0);
+        kp.request(a.b.kc, 0, mine);
+        vp.look_up(a.b, t.s, 0);
+        vp.request(a.b.vc, 0, mine + 2 * BYTES);
+        wait_loads<LOADS>();  // the keys
+        __syncthreads();
+        if (n > 1) {
+            kp.look_up(a.b, t.s, 1);
+            kp.request(a.b.kc, 1, mine + BYTES);
+        }
+#pragma unroll
+        for (int k = 0; k < KT; k++) s[k] = c.scores(keys + k * 32 * 2 * D);
+    }
     for (int i = 0; i < n; i++) {
         const int at = begin + i * NK, buffer = i & 1;
-        const uint32_t there = pages.there(i);
+        const uint32_t there = vp.there(i);
         wait_loads<0>();
         if (at < t.from || at + NK - 1 > t.to || there != ALL)
-            bad |= clear_unseen<D, LOADS>((lds_char *)space.rows + buffer * 2 * BYTES + BYTES + w * (BYTES / 4), at + w * (NK / 4), there,
-                                          t.from, t.to, t.least, t.most);
+            bad |= clear_unseen<D, LOADS>(values + buffer * BYTES + w * (BYTES / 4), at + w * (NK / 4), there, t.from, t.to,
+                                          t.least, t.most);
         if (lane == 0) space.present[buffer][w] = there;
         __syncthreads();
         if (i + 1 < n) {
-            pages.look_up(a.b, t.s, i + 1);
-            pages.request(a.b.kc, i + 1, mine + (buffer ^ 1) * 2 * BYTES);
-            pages.request(a.b.vc, i + 1, mine + (buffer ^ 1) * 2 * BYTES + BYTES);
+            vp.look_up(a.b, t.s, i + 1);
+            vp.request(a.b.vc, i + 1, mine + (2 + (buffer ^ 1)) * BYTES);
         }
-        if (!any_rows || at > high || (a.window > 0 && at + NK - 1 <= low - a.window)) continue;
+        if (i + 2 < n) {
+            kp.look_up(a.b, t.s, i + 2);
+            kp.request(a.b.kc, i + 2, mine + buffer * BYTES);
+        }
+        if (!any_rows) continue;
         const u32x4 got = *(LLM_LDS u32x4 *)(lds_char *)space.present[buffer];
-        const lds_char *keys = (lds_char *)space.rows + buffer * 2 * BYTES, *values = keys + BYTES;
-        f32x16 s[KT];
-#pragma unroll
-        for (int k = 0; k < KT; k++) s[k] = c.scores(keys + k * 32 * 2 * D);
         const uint32_t all = __builtin_amdgcn_readfirstlane(got[0] & got[1] & got[2] & got[3]);
         if (at + NK - 1 > low || (a.window > 0 && at <= high - a.window) || all != ALL) {
 #pragma unroll
@@ -612,9 +630,17 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
                 hide(s[k], c.sees(at + 32 * k, a.window) & here);
             }
         }
+        // the next scores' products run beside this softmax (past the last keys, on what the buffer holds)
+        const lds_char *ahead = keys + (buffer ^ 1) * BYTES;
+        next[0] = c.scores(ahead);
+        const float peak = c.peak(s, a.scale_log2);
+        c.raise(peak);
+        next[1] = c.scores(ahead + 32 * 2 * D);
         c.weigh(s, a.scale_log2);
 #pragma unroll
-        for (int k = 0; k < KT; k++) c.template add<false>(values + k * 32 * 2 * D, s[k]);
+        for (int k = 0; k < KT; k++) c.template add<false>(values + buffer * BYTES + k * 32 * 2 * D, s[k]);
+#pragma unroll
+        for (int k = 0; k < KT; k++) s[k] = next[k];
     }
     if (lane == 0) space.bad[w] = bad;
     __syncthreads();
@@ -786,6 +812,31 @@ struct Plan {
     int few_units, many_units, few_split, few_chunk, many_split, many_chunk;
     size_t few_rows, many_rows, floats;  // rows of partial outputs
 
+    // A join costs 2 to 3 us, what a workgroup takes for about 640 keys alone (one token, 32 heads on 8, 511 / 1023
+    // / 8191 / 40959 positions: unsplit 9.6 / 14.6 / 88.6 / 446.8 us, 128 keys or 256 workgroups 9.8 / 10.2 / 14.5 /
+    // 34.6, 512 workgroups 9.8 / 10.2 / 15.2 / 36.8). Sequences of unequal length gain from twice the workgroups
+    // (4 sequences up to 8000: 22.2 / 21.0), and from pieces of 2048 keys where there are enough (64 up to 8447:
+    // 239.9 / 219.9).
+    static int64_t few_splits(int64_t units, int n_seqs, int64_t span) {
+        if (span <= 640) return 1;
+        const int64_t target = n_seqs > 1 ? 2 * CUS : CUS;
+        return std::max<int64_t>(1, std::min((span + 127) / 128, std::max(target / units, (span + 2047) / 2048)));
+    }
+
+    // The least of an estimate in ns: a workgroup's keys, alone on a CU or two to one, the parts' bytes written and
+    // read, and the join's launch.
+    static int64_t many_splits(int64_t units, int head_dim, int64_t span) {
+        int64_t best = 1;
+        double least = 0;
+        for (int64_t n = 1; n <= std::min<int64_t>(64, (span + 127) / 128); n++) {
+            const double groups = (double)units * n, keys = (double)((span + n - 1) / n);
+            const double key = (groups <= CUS ? 24.0 : 35.0 * std::max(1.0, groups / (2 * CUS))) * (head_dim + 64) / 192;
+            const double cost = keys * key + (n > 1 ? 4000 + groups * MANY * (head_dim + 2) * 8 / 4000 : 0);
+            if (n == 1 || cost < least) best = n, least = cost;
+        }
+        return best;
+    }
+
     Plan(int n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len, int max_kv_len,
          int window) {
         const int64_t group = n_heads / n_kv_heads, rows = n_tokens * group;
@@ -797,17 +848,19 @@ struct Plan {
         const int64_t many_tiles = rows / MANY + (few ? std::min<int64_t>(n_seqs, rows / (FEW + 1)) : n_seqs);
         few_units = few ? (int)(few_tiles * n_kv_heads) : 0;
         many_units = many ? (int)(many_tiles * n_kv_heads) : 0;
-        const auto split = [&](int64_t units, int least, int64_t even, int64_t span, int &n, int &chunk) {
-            const int64_t all = max_kv_len;
-            n = (int)std::max<int64_t>(1, std::min((all + least - 1) / least, std::max((2 * CUS + units - 1) / units, even)));
-            n = (int)std::min<int64_t>(n, (span + least - 1) / least);
-            chunk = (int)((span + n - 1) / n + 127) / 128 * 128;
+        // a window shortens what the rows see; the workspace is asked for without it, so never more splits than then
+        const auto cut = [&](int64_t tokens, auto splits, int &n, int &chunk) {
+            n = INT32_MAX;
+            for (const int64_t span : {(int64_t)max_kv_len, std::min<int64_t>(max_kv_len, window + tokens + 63)}) {
+                const int64_t want = std::min<int64_t>(n, splits(span));
+                chunk = (int)((span + want - 1) / want + 127) / 128 * 128;
+                n = (int)((span + chunk - 1) / chunk);
+                if (window == 0) break;
+            }
         };
-        const auto span = [&](int64_t tokens) {
-            return window > 0 ? std::min<int64_t>(max_kv_len, (int64_t)window + tokens + 63) : (int64_t)max_kv_len;
-        };
-        split((int64_t)n_seqs * n_kv_heads, 256, (int64_t)n_seqs * n_kv_heads < 16 * CUS ? (max_kv_len + 2047) / 2048 : 1, span(32), few_split, few_chunk);
-        split(((rows + MANY - 1) / MANY) * n_kv_heads, 512, 1, span(MANY), many_split, many_chunk);
+        cut(FEW, [&](int64_t span) { return few_splits((int64_t)n_seqs * n_kv_heads, n_seqs, span); }, few_split, few_chunk);
+        cut(MANY, [&](int64_t span) { return many_splits((rows + MANY - 1) / MANY * n_kv_heads, head_dim, span); },
+            many_split, many_chunk);
         few_rows = few_split > 1 ? (size_t)few_units * few_split * FEW : 0;
         many_rows = many_split > 1 ? (size_t)many_units * many_split * MANY : 0;
         floats = (few_rows + many_rows) * (head_dim + 2);
