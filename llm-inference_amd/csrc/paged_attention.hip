@@ -7,6 +7,8 @@
 // 16 keys, lane half h holds 4h..4h+3 and 8+4h..8+4h+3, and the second product sums over any order of keys.
 #include <math.h>
 
+#include <type_traits>
+
 #include "paged_batch.h"
 
 using namespace llm;
@@ -35,6 +37,20 @@ struct AttendArgs {
     int which;            // the sequences whose rows these are
     float scale_log2;     // scale * log2(e)
 };
+
+// The same arguments read from the kernel's argument memory where they are used: what only rare steps need
+// does not hold scalar registers through the loops.
+struct LaunchArgs {
+    AttendArgs few, many;
+    int few_units, many_units, few_groups, many_groups;  // tiles x kv heads, and those x splits
+};
+#define LLM_CONST __attribute__((address_space(4)))
+__device__ __forceinline__ const LLM_CONST AttendArgs *again(bool many) {
+    const LLM_CONST LaunchArgs *l = (const LLM_CONST LaunchArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+    const LLM_CONST AttendArgs *a = many ? &l->many : &l->few;
+    asm volatile("" : "+s"(a));
+    return a;
+}
 
 // ------------------------------------------------------------------------------------------
 // which rows and keys
@@ -165,9 +181,10 @@ struct Pages {
     }
 
     // Looks up steps step .. step + AHEAD - 1, when step is a multiple of AHEAD.
-    __device__ __forceinline__ void look_up(const Batch &b, int s, int step) {
+    __device__ __forceinline__ void look_up(bool many, int s, int step) {
         if (step % AHEAD != 0) return;
         const int lane = threadIdx.x & 63;
+        const auto &b = again(many)->b;
         if constexpr (WHOLE) {
             const int64_t at = place(b, s, first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16);
             mine = at < 0 ? -1 : at * 2 + head;
@@ -336,34 +353,40 @@ struct Columns {
 #pragma unroll
             for (int r = 0; r < 16; r++) o[d][r] *= keep;
     }
-    template <int KT>
-    __device__ __forceinline__ void weigh(f32x16 (&s)[KT], float c) {
-        float part[4] = {sum, 0, 0, 0};
+    // Weights 2^(s c - top) of 32 keys as the second product's operands of 16 keys each, rounded to bf16 (half
+    // a step each, at random; their sum adds the rounded ones), with EXACT what the rounding left as well.
+    template <bool EXACT>
+    __device__ __forceinline__ void weigh(f32x16 &s, float c, u32x4 (&hi)[2], u32x4 (&lo)[2]) {
+        float part = 0.0f;
+        const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
-        for (int k = 0; k < KT; k++)
+        for (int t = 0; t < 2; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                s[k][r] = __builtin_amdgcn_exp2f(fmaf(s[k][r], c, -top));
-                part[r & 3] += s[k][r];
+            for (int j = 0; j < 4; j++) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[8 * t + 2 * j], c, -top));
+                const float y = __builtin_amdgcn_exp2f(fmaf(s[8 * t + 2 * j + 1], c, -top));
+                const uint32_t w = pack2(x, y);
+                hi[t][j] = w;
+                if constexpr (EXACT) {
+                    lo[t][j] = pack2(x - lo_f(w), y - hi_f(w));
+                    sum += x;
+                    part += y;
+                } else if (t == 0) {
+                    sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), ones, sum, false);
+                } else {
+                    part = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, w), ones, part, false);
+                }
             }
-        sum = (part[0] + part[1]) + (part[2] + part[3]);
+        sum += part;
     }
 
-    // O^T += V^T P^T over 32 keys: the weights rounded to bf16, with EXACT their remainders too.
+    // O^T += V^T P^T over 32 keys.
     template <bool EXACT>
-    __device__ __forceinline__ void add(const lds_char *values, const f32x16 &p) {
+    __device__ __forceinline__ void add(const lds_char *values, const u32x4 (&hi)[2], const u32x4 (&lo)[2]) {
         const int lane = threadIdx.x & 63, i = lane & 15, h = lane >> 5;
         const int row = 4 * h + (i >> 2);
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
-            u32x4 hi, lo;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float x = p[8 * t + 2 * j], y = p[8 * t + 2 * j + 1];
-                const uint32_t w = pack2(x, y);
-                hi[j] = w;
-                if constexpr (EXACT) lo[j] = pack2(x - lo_f(w), y - hi_f(w));
-            }
+        for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int d = 0; d < D / 32; d++) {
                 const int c = d * 4 + (lane >> 4 & 1) * 2 + ((i & 3) >> 1);
@@ -376,16 +399,16 @@ struct Columns {
                 }
                 const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
                 const bf16x8_t vt = __builtin_bit_cast(bf16x8_t, (u32x4{v0.x, v0.y, v1.x, v1.y}));
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, hi), o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, hi[t]), o[d], 0, 0, 0);
                 if constexpr (EXACT)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, lo), o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, lo[t]), o[d], 0, 0, 0);
             }
-        }
     }
 
     // What clear_unseen took out, for the rows that see it: the keys first .. last, one by one, each weight from
     // its own score.
-    __device__ __forceinline__ void add_bad(const AttendArgs &a, const Tile &t, int kv, int first, int last, int base) {
+    __device__ __forceinline__ void add_bad(bool many, const Tile &t, int kv, int first, int last, int base) {
+        const auto &a = *again(many);
         const int h = (threadIdx.x & 63) >> 5, row = min(base + column, t.rows - 1) + t.first, token = row / a.group;
         const bf16 *query = a.q + (t.q0 + token) * a.q_stride + (kv * a.group + row - token * a.group) * D;
 #pragma unroll 1
@@ -464,7 +487,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
     const unsigned key_at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)keys), value_at = key_at + BYTES;
     uint32_t there = 0;
     if (n > 0) {
-        pages.look_up(a.b, t.s, 0);
+        pages.look_up(false, t.s, 0);
         there = pages.there(0);
         pages.request(a.b.kc, 0, key_at);
         pages.request(a.b.vc, 0, value_at);
@@ -480,25 +503,26 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
         if (edge) hide(s[0], c.sees(at, a.window) & here);
         wait_lds();
         if (more) {
-            pages.look_up(a.b, t.s, i + 1);
+            pages.look_up(false, t.s, i + 1);
             there = pages.there(i + 1);
             pages.request(a.b.kc, i + 1, key_at);
         }
         c.raise(c.peak(s, a.scale_log2));
-        c.weigh(s, a.scale_log2);
+        u32x4 hi[2], lo[2];
+        c.template weigh<true>(s[0], a.scale_log2, hi, lo);
         if (more)
             wait_loads<LOADS>();
         else
             wait_loads<0>();
         if (edge) bad |= clear_unseen<D, LOADS>(values, at, here, t.from, t.to, t.least, t.most);
-        c.template add<true>(values, s[0]);
+        c.template add<true>(values, hi, lo);
         wait_lds();
         if (more) pages.request(a.b.vc, i + 1, value_at);
     }
     if (bad) {
         const int first = begin + s0 * ROWS, last = min(first + n * ROWS, t.end) - 1;
-        c.add_bad(a, t, kv, max(first, t.least), min(last, t.from - 1), 0);
-        c.add_bad(a, t, kv, max(max(first, t.least), max(t.from, t.to + 1)), min(last, t.most), 0);
+        c.add_bad(false, t, kv, max(first, t.least), min(last, t.from - 1), 0);
+        c.add_bad(false, t, kv, max(max(first, t.least), max(t.from, t.to + 1)), min(last, t.most), 0);
     }
 
     // join the waves: each one's output, maximum and sum through LDS
@@ -578,76 +602,109 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
     const auto position_of = [&](int row) { return t.before + (t.first + row) / a.group; };
     const bool any_rows = 32 * w < t.rows;
     const int low = position_of(32 * w), high = position_of(min(t.rows, 32 * w + 32) - 1);  // of the wave
-    const int first = begin + w * (NK / 4);
+    const int first = begin + w * (NK / 4), window = a.window;
+    const float scale = a.scale_log2;
+    const bf16 *kc = a.b.kc, *vc = a.b.vc;
     P kp(a.b, kv, first, w * (NK / 4), (LLM_LDS int64_t *)space.places[WHOLE ? 0 : w]);
     P vp(a.b, kv, first, w * (NK / 4), (LLM_LDS int64_t *)space.places[WHOLE ? 0 : 4 + w]);
     const unsigned mine = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_char *)space.rows) + w * (BYTES / 4);
-    constexpr uint32_t ALL = NK / 4 == 16 ? 0xffffu : (1u << (NK / 4)) - 1;
+    constexpr int QUARTER = NK / 4;  // the rows that a wave brings
     lds_char *keys = (lds_char *)space.rows, *values = keys + 2 * BYTES;  // two buffers each
-    f32x16 s[KT], next[KT];
+    f32x16 scores[2][KT];
     bool bad = false;
+    int groups = 0;  // WHOLE: which quarters of the lane's step are there
+    // Which of the step's rows are there, by quarters.
+    const auto look_up_values = [&](int i) {
+        vp.look_up(true, t.s, i);
+        if constexpr (WHOLE) {
+            if (i % P::AHEAD == 0) {
+                const auto &b = again(true)->b;
+                groups = 0;
+#pragma unroll
+                for (int v = 0; v < 4; v++)
+                    if (place(b, t.s, begin + (i + lane) * NK + v * QUARTER) >= 0) groups |= 1 << v;
+            }
+        }
+    };
     if (n > 0) {
-        kp.look_up(a.b, t.s, 0);
-        kp.request(a.b.kc, 0, mine);
-        vp.look_up(a.b, t.s, 0);
-        vp.request(a.b.vc, 0, mine + 2 * BYTES);
+        kp.look_up(true, t.s, 0);
+        kp.request(kc, 0, mine);
+        look_up_values(0);
+        vp.request(vc, 0, mine + 2 * BYTES);
         wait_loads<LOADS>();  // the keys
         __syncthreads();
         if (n > 1) {
-            kp.look_up(a.b, t.s, 1);
-            kp.request(a.b.kc, 1, mine + BYTES);
+            kp.look_up(true, t.s, 1);
+            kp.request(kc, 1, mine + BYTES);
         }
 #pragma unroll
-        for (int k = 0; k < KT; k++) s[k] = c.scores(keys + k * 32 * 2 * D);
+        for (int k = 0; k < KT; k++) scores[0][k] = c.scores(keys + k * 32 * 2 * D);
     }
-    for (int i = 0; i < n; i++) {
-        const int at = begin + i * NK, buffer = i & 1;
-        const uint32_t there = vp.there(i);
+    const auto step = [&](auto which, int i) {
+        constexpr int B = decltype(which)::value;
+        f32x16(&s)[KT] = scores[B], (&next)[KT] = scores[B ^ 1];
+        const int at = begin + i * NK;
+        int there = 0;  // WHOLE: the step's quarters
+        uint32_t own;
+        if constexpr (WHOLE) {
+            there = __builtin_amdgcn_readlane(groups, i % P::AHEAD);
+            own = there >> w & 1 ? (1u << QUARTER) - 1 : 0;
+        } else {
+            own = vp.there(i);
+        }
         wait_loads<0>();
-        if (at < t.from || at + NK - 1 > t.to || there != ALL)
-            bad |= clear_unseen<D, LOADS>(values + buffer * BYTES + w * (BYTES / 4), at + w * (NK / 4), there, t.from, t.to,
-                                          t.least, t.most);
-        if (lane == 0) space.present[buffer][w] = there;
+        if (at < t.from || at + NK - 1 > t.to || own != (1u << QUARTER) - 1)
+            bad |= clear_unseen<D, LOADS>(values + B * BYTES + w * (BYTES / 4), at + w * QUARTER, own, t.from, t.to, t.least,
+                                          t.most);
+        if constexpr (!WHOLE)
+            if (lane == 0) space.present[B][w] = own;
         __syncthreads();
         if (i + 1 < n) {
-            vp.look_up(a.b, t.s, i + 1);
-            vp.request(a.b.vc, i + 1, mine + (2 + (buffer ^ 1)) * BYTES);
+            look_up_values(i + 1);
+            vp.request(vc, i + 1, mine + (2 + (B ^ 1)) * BYTES);
         }
         if (i + 2 < n) {
-            kp.look_up(a.b, t.s, i + 2);
-            kp.request(a.b.kc, i + 2, mine + buffer * BYTES);
+            kp.look_up(true, t.s, i + 2);
+            kp.request(kc, i + 2, mine + B * BYTES);
         }
-        if (!any_rows) continue;
-        const u32x4 got = *(LLM_LDS u32x4 *)(lds_char *)space.present[buffer];
-        const uint32_t all = __builtin_amdgcn_readfirstlane(got[0] & got[1] & got[2] & got[3]);
-        if (at + NK - 1 > low || (a.window > 0 && at <= high - a.window) || all != ALL) {
+        if (!any_rows) return;
+        uint32_t here[KT];
+        bool all = true;
 #pragma unroll
-            for (int k = 0; k < KT; k++) {
-                constexpr int WAVES = 32 / (NK / 4);  // waves whose rows make 32
-                uint32_t here = 0;
-#pragma unroll
-                for (int v = 0; v < WAVES; v++) here |= got[k * WAVES + v] << (v * (NK / 4));
-                hide(s[k], c.sees(at + 32 * k, a.window) & here);
+        for (int k = 0; k < KT; k++) {
+            if constexpr (WHOLE) {
+                here[k] = (there >> (2 * k) & 1 ? 0xffffu : 0) | (there >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
+            } else {
+                here[k] = __builtin_amdgcn_readfirstlane(space.present[B][2 * k] | space.present[B][2 * k + 1] << 16);
             }
+            all = all && here[k] == ~0u;
+        }
+        if (at + NK - 1 > low || (window > 0 && at <= high - window) || !all) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) hide(s[k], c.sees(at + 32 * k, window) & here[k]);
         }
         // the next scores' products run beside this softmax (past the last keys, on what the buffer holds)
-        const lds_char *ahead = keys + (buffer ^ 1) * BYTES;
+        const lds_char *ahead = keys + (B ^ 1) * BYTES;
         next[0] = c.scores(ahead);
-        const float peak = c.peak(s, a.scale_log2);
+        const float peak = c.peak(s, scale);
         c.raise(peak);
         next[1] = c.scores(ahead + 32 * 2 * D);
-        c.weigh(s, a.scale_log2);
+        u32x4 hi[KT][2], lo[2];
 #pragma unroll
-        for (int k = 0; k < KT; k++) c.template add<false>(values + buffer * BYTES + k * 32 * 2 * D, s[k]);
+        for (int k = 0; k < KT; k++) c.template weigh<false>(s[k], scale, hi[k], lo);
 #pragma unroll
-        for (int k = 0; k < KT; k++) s[k] = next[k];
+        for (int k = 0; k < KT; k++) c.template add<false>(values + B * BYTES + k * 32 * 2 * D, hi[k], lo);
+    };
+    for (int i = 0; i < n; i += 2) {
+        step(std::integral_constant<int, 0>(), i);
+        if (i + 1 < n) step(std::integral_constant<int, 1>(), i + 1);
     }
     if (lane == 0) space.bad[w] = bad;
     __syncthreads();
     if (space.bad[0] | space.bad[1] | space.bad[2] | space.bad[3]) {
         const int last = min(begin + n * NK, t.end) - 1;
-        c.add_bad(a, t, kv, max(begin, t.least), min(last, t.from - 1), 32 * w);
-        c.add_bad(a, t, kv, max(max(begin, t.least), max(t.from, t.to + 1)), min(last, t.most), 32 * w);
+        c.add_bad(true, t, kv, max(begin, t.least), min(last, t.from - 1), 32 * w);
+        c.add_bad(true, t, kv, max(max(begin, t.least), max(t.from, t.to + 1)), min(last, t.most), 32 * w);
     }
 
     if (!any_rows || c.column >= t.rows - 32 * w) return;
@@ -683,11 +740,6 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
 // ------------------------------------------------------------------------------------------
 // the launch
 // ------------------------------------------------------------------------------------------
-
-struct LaunchArgs {
-    AttendArgs few, many;
-    int few_units, many_units, few_groups, many_groups;  // tiles x kv heads, and those x splits
-};
 
 // Workgroups of both kinds in turn while there are both: the ones read, the others multiply.
 template <int D, bool WHOLE>

@@ -68,7 +68,8 @@ __device__ __forceinline__ int kv_length(const Batch &b, int s) {
 }
 
 // Element offset of position p of sequence s in the caches (head 0), or -1 where it is not there.
-__device__ __forceinline__ int64_t place(const Batch &b, int s, int p) {
+template <class B>
+__device__ __forceinline__ int64_t place(B &b, int s, int p) {
     if (p < 0) return -1;
     const int i = divide(p, b.page.m, b.page.l);
     if (i >= b.table_pages) return -1;
