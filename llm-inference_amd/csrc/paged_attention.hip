@@ -25,6 +25,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef LLM_LDS char lds_char;
 
 constexpr float LOWEST = -3.402823466e+38f;
+constexpr int CUS = 256;
 
 struct AttendArgs {
     Batch b;
@@ -43,6 +44,7 @@ struct AttendArgs {
 struct LaunchArgs {
     AttendArgs few, many;
     int few_units, many_units, few_groups, many_groups;  // tiles x kv heads, and those x splits
+    int mirrored;
 };
 #define LLM_CONST __attribute__((address_space(4)))
 __device__ __forceinline__ const LLM_CONST AttendArgs *again(bool many) {
@@ -165,14 +167,15 @@ struct Pages {
     static constexpr int GROUPS = ROWS < 16 ? 1 : ROWS / 16, GROUP_LOADS = LOADS / GROUPS;
     static constexpr int AHEAD = WHOLE ? 64 / GROUPS : 128 / ROWS;  // steps looked up at a time
     int first;                // the first step's first position
-    int64_t mine;             // WHOLE: the lane's place, in bytes, with the kv head; -1 where it is not there
+    int64_t mine;             // WHOLE: the lane's place, in bytes, with the kv head
+    int present;              // WHOLE: whether it is there
     LLM_LDS int64_t *places;  // otherwise: 128 of them
     int64_t head;             // bytes to the kv head
     unsigned offset[GROUP_LOADS];  // the lane's bytes within load i: WHOLE with its row, otherwise its chunk alone
 
     // row0: where in the buffer the wave's rows begin, a multiple of PER
     __device__ __forceinline__ Pages(const Batch &b, int kv, int first_, int row0, LLM_LDS int64_t *places_)
-        : first(first_), mine(-1), places(places_), head(uniform(kv * b.head_stride * 2)) {
+        : first(first_), mine(0), present(0), places(places_), head(uniform(kv * b.head_stride * 2)) {
         const int lane = threadIdx.x & 63, r = lane / (D / 8);
 #pragma unroll
         for (int i = 0; i < GROUP_LOADS; i++)
@@ -187,7 +190,8 @@ struct Pages {
         const auto &b = again(many)->b;
         if constexpr (WHOLE) {
             const int64_t at = place(b, s, first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16);
-            mine = at < 0 ? -1 : at * 2 + head;
+            present = at >= 0;
+            mine = (at < 0 ? 0 : at * 2) + head;
         } else {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -205,7 +209,7 @@ struct Pages {
             uint32_t bits = 0;
 #pragma unroll
             for (int g = 0; g < GROUPS; g++)
-                if (__builtin_amdgcn_readlane((int)(mine >> 32), step % AHEAD * GROUPS + g) >= 0)
+                if (__builtin_amdgcn_readlane(present, step % AHEAD * GROUPS + g))
                     bits |= (ROWS < 16 ? (1u << ROWS) - 1 : 0xffffu) << (16 * g);
             return bits;
         } else {
@@ -214,26 +218,30 @@ struct Pages {
         }
     }
 
-    // Requests the step's rows of one cache into LDS at `to`.
-    __device__ __forceinline__ void request(const bf16 *cache, int step, unsigned to) const {
+    // WHOLE: where 16 of the step's positions begin in a cache.
+    __device__ __forceinline__ const char *base(const bf16 *cache, int step, int group = 0) const {
+        if constexpr (!WHOLE) return (const char *)cache;
+        const int lane = step % AHEAD * GROUPS + group;
+        const int hi = __builtin_amdgcn_readlane((int)(mine >> 32), lane);
+        const unsigned lo = __builtin_amdgcn_readlane((int)mine, lane);
+        return (const char *)cache + (int64_t)((uint64_t)(unsigned)hi << 32 | lo);
+    }
+    // Load i of the step's rows into LDS at `to` (where load 0 goes); from: base() of the load's group.
+    __device__ __forceinline__ void load(const char *from, int step, int i, unsigned to) const {
         if constexpr (WHOLE) {
-#pragma unroll
-            for (int g = 0; g < GROUPS; g++) {
-                const int lane = step % AHEAD * GROUPS + g;
-                const int hi = __builtin_amdgcn_readlane((int)(mine >> 32), lane);
-                const unsigned lo = __builtin_amdgcn_readlane((int)mine, lane);
-                const char *base = (const char *)uniform((int64_t)cache + (hi < 0 ? head : (int64_t)hi << 32 | lo));
-#pragma unroll
-                for (int i = 0; i < GROUP_LOADS; i++)
-                    load_to_lds(to + (g * GROUP_LOADS + i) * 1024, base, offset[i]);
-            }
+            load_to_lds(to + i * 1024, from, offset[i % GROUP_LOADS]);
         } else {
-            const int r = (threadIdx.x & 63) / (D / 8);
+            const int64_t at = places[step % AHEAD * ROWS + i * PER + (threadIdx.x & 63) / (D / 8)];
+            load_to_lds(to + i * 1024, from + (at < 0 ? head : at) + offset[i % GROUP_LOADS]);
+        }
+    }
+    // All loads of the step's rows of one cache.
+    __device__ __forceinline__ void request(const bf16 *cache, int step, unsigned to) const {
 #pragma unroll
-            for (int i = 0; i < LOADS; i++) {
-                const int64_t at = places[step % AHEAD * ROWS + i * PER + r];
-                load_to_lds(to + i * 1024, (const char *)cache + (at < 0 ? head : at) + offset[i % GROUP_LOADS]);
-            }
+        for (int g = 0; g < GROUPS; g++) {
+            const char *from = base(cache, step, g);
+#pragma unroll
+            for (int i = g * GROUP_LOADS; i < (g + 1) * GROUP_LOADS; i++) load(from, step, i, to);
         }
     }
 };
@@ -403,6 +411,92 @@ struct Columns {
                 if constexpr (EXACT)
                     o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vt, __builtin_bit_cast(bf16x8_t, lo[t]), o[d], 0, 0, 0);
             }
+    }
+
+    // One step of 64 keys, the matrix products with everything else between them: the next keys' scores into
+    // `next` beside the first 32 weights and the loads of later keys and values (bring), then O^T += V^T P^T beside
+    // the other 32 weights and the maximum of `next`, which is the result. The matrix unit takes an instruction
+    // every 32 cycles, and the other units' fit in between where they are spread evenly and do not wait for
+    // each other: a weight's fma, exponential and rounding stand in three places. The fences keep the order written.
+    template <class Bring>
+    __device__ __forceinline__ float step(const lds_char *keys, const lds_char *values, const f32x16 (&s)[2],
+                                          f32x16 (&next)[2], float c, Bring bring) {
+        constexpr int QK = D / 8, PV = D / 8, RING = 4;  // products of each kind; operands in flight
+        const int lane = threadIdx.x & 63, r = lane & 31, i = lane & 15, h = lane >> 5;
+        const lds_char *key_row = keys + r * (2 * D);
+        const int c0 = (h ^ swizzle<D>(r)) * 16, value_row = 4 * h + (i >> 2);
+        const auto key = [&](int j) {
+            return __builtin_bit_cast(bf16x8_t, *(const LLM_LDS u32x4 *)(key_row + (j & 1) * 64 * D + (c0 ^ (j / 2 * 32))));
+        };
+        const auto value = [&](int j) {
+            const int d = j % (D / 32), t = j / (D / 32), chunk = d * 4 + (lane >> 4 & 1) * 2 + ((i & 3) >> 1);
+            u32x4 v;
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int row = 16 * t + 8 * u + value_row;
+                const u32x2 x = __builtin_bit_cast(
+                    u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((LLM_LDS s16x4 *)(
+                               values + row * (2 * D) + (chunk ^ swizzle<D>(row)) * 16 + (i & 1) * 8)));
+                v[2 * u] = x.x;
+                v[2 * u + 1] = x.y;
+            }
+            return __builtin_bit_cast(bf16x8_t, v);
+        };
+        const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
+        u32x4 p[4];                   // weights of 16 keys each
+        float odd = 0.0f, w[4];       // the last weights
+        float arg = fmaf(s[0][0], c, -top);
+        const auto pair = [&](int e) {  // weights e and e + 1 of 64: rounded, and added
+            const uint32_t both = pack2(w[e & 3], w[(e & 3) + 1]);
+            p[e / 16 * 2 + e % 16 / 8][e % 8 / 2] = both;
+            float &to = e & 2 ? odd : sum;
+            to = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, both), ones, to, false);
+        };
+        const auto weigh_one = [&](int e) {  // weight e of 32; the pair before it where it begins a new one
+            w[e & 3] = __builtin_amdgcn_exp2f(arg);
+            if (e < 31) arg = fmaf(s[(e + 1) / 16][(e + 1) % 16], c, -top);
+            if (e >= 2 && !(e & 1)) pair(e - 2);
+        };
+        bf16x8_t ring[RING];
+#pragma unroll
+        for (int j = 0; j < RING - 1; j++) ring[j] = key(j);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < QK; j++) {
+            ring[(j + RING - 1) % RING] = j + RING - 1 < QK ? key(j + RING - 1) : value(j + RING - 1 - QK);
+            f32x16 from = next[j & 1];
+            if (j < 2)
+#pragma unroll
+                for (int e = 0; e < 16; e++) from[e] = 0.0f;
+            next[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[j % RING], __builtin_bit_cast(bf16x8_t, q[j / 2]),
+                                                                  from, 0, 0, 0);
+#pragma unroll
+            for (int e = 16 * j / QK; e < 16 * (j + 1) / QK; e++) weigh_one(e);
+            if (j & 1) bring(j / 2);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float peak = LOWEST;
+#pragma unroll
+        for (int j = 0; j < PV; j++) {
+            if (j + RING - 1 < PV) ring[(QK + j + RING - 1) % RING] = value(j + RING - 1);
+            f32x16 &to = o[j % (D / 32)];
+            to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[(QK + j) % RING], __builtin_bit_cast(bf16x8_t, p[j / (D / 32)]),
+                                                         to, 0, 0, 0);
+            if (j < PV / 2) {
+#pragma unroll
+                for (int e = 32 * j / PV; e < 32 * (j + 1) / PV; e++) weigh_one(16 + e);
+            } else {
+                if (j == PV / 2) pair(30);
+#pragma unroll
+                for (int e = 64 * j / PV - 32; e < 64 * (j + 1) / PV - 32; e++) peak = fmaxf(peak, next[e / 16][e % 16]);
+                asm volatile("" : "+v"(peak));
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sum += odd;
+        float x, y;
+        swap_pair<32>(peak, x, y);
+        return fmaxf(x, y) * c;
     }
 
     // What clear_unseen took out, for the rows that see it: the keys first .. last, one by one, each weight from
@@ -599,9 +693,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
 
     Columns<D> c;
     c.start(a, t, kv, 32 * w);
-    const auto position_of = [&](int row) { return t.before + (t.first + row) / a.group; };
     const bool any_rows = 32 * w < t.rows;
-    const int low = position_of(32 * w), high = position_of(min(t.rows, 32 * w + 32) - 1);  // of the wave
     const int first = begin + w * (NK / 4), window = a.window;
     const float scale = a.scale_log2;
     const bf16 *kc = a.b.kc, *vc = a.b.vc;
@@ -611,9 +703,12 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
     constexpr int QUARTER = NK / 4;  // the rows that a wave brings
     lds_char *keys = (lds_char *)space.rows, *values = keys + 2 * BYTES;  // two buffers each
     f32x16 scores[2][KT];
+    float peak = LOWEST;  // of the step's scores, as long as none is hidden
     bool bad = false;
-    int groups = 0;  // WHOLE: which quarters of the lane's step are there
-    // Which of the step's rows are there, by quarters.
+    // Every row of the workgroup sees all of the steps plain0 .. plain1 - 1 as far as it is there.
+    const int plain0 = max(0, t.from - begin + NK - 1) / NK, plain1 = (t.to + 1 - begin) / NK;
+    int groups = 0;      // WHOLE: which quarters of the lane's step are there
+    bool whole = false;  // WHOLE: all of the steps looked up that are plain
     const auto look_up_values = [&](int i) {
         vp.look_up(true, t.s, i);
         if constexpr (WHOLE) {
@@ -623,6 +718,7 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
 #pragma unroll
                 for (int v = 0; v < 4; v++)
                     if (place(b, t.s, begin + (i + lane) * NK + v * QUARTER) >= 0) groups |= 1 << v;
+                whole = !__any(groups != 15 && i + lane >= plain0 && i + lane < plain1);
             }
         }
     };
@@ -639,66 +735,66 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
         }
 #pragma unroll
         for (int k = 0; k < KT; k++) scores[0][k] = c.scores(keys + k * 32 * 2 * D);
+        peak = c.peak(scores[0], scale);
     }
     const auto step = [&](auto which, int i) {
         constexpr int B = decltype(which)::value;
         f32x16(&s)[KT] = scores[B], (&next)[KT] = scores[B ^ 1];
         const int at = begin + i * NK;
+        const bool plain = whole && i >= plain0 && i < plain1;
         int there = 0;  // WHOLE: the step's quarters
-        uint32_t own;
-        if constexpr (WHOLE) {
-            there = __builtin_amdgcn_readlane(groups, i % P::AHEAD);
-            own = there >> w & 1 ? (1u << QUARTER) - 1 : 0;
-        } else {
-            own = vp.there(i);
-        }
         wait_loads<0>();
-        if (at < t.from || at + NK - 1 > t.to || own != (1u << QUARTER) - 1)
+        if (!plain) {
+            uint32_t own;
+            if constexpr (WHOLE) {
+                there = __builtin_amdgcn_readlane(groups, i % P::AHEAD);
+                own = there >> w & 1 ? (1u << QUARTER) - 1 : 0;
+            } else {
+                own = vp.there(i);
+                if (lane == 0) space.present[B][w] = own;
+            }
             bad |= clear_unseen<D, LOADS>(values + B * BYTES + w * (BYTES / 4), at + w * QUARTER, own, t.from, t.to, t.least,
                                           t.most);
-        if constexpr (!WHOLE)
-            if (lane == 0) space.present[B][w] = own;
+        }
         __syncthreads();
-        if (i + 1 < n) {
-            look_up_values(i + 1);
-            vp.request(vc, i + 1, mine + (2 + (B ^ 1)) * BYTES);
-        }
-        if (i + 2 < n) {
-            kp.look_up(true, t.s, i + 2);
-            kp.request(kc, i + 2, mine + B * BYTES);
-        }
-        if (!any_rows) return;
-        uint32_t here[KT];
-        bool all = true;
+        // later steps' keys and values; past the last one its own again
+        const int next_values = min(i + 1, n - 1), next_keys = min(i + 2, n - 1);
+        if ((i + 1) % P::AHEAD == 0 && i + 1 < n) look_up_values(i + 1);
+        if ((i + 2) % P::AHEAD == 0 && i + 2 < n) kp.look_up(true, t.s, i + 2);
+        const char *key_base = kp.base(kc, next_keys), *value_base = vp.base(vc, next_values);
+        const auto bring = [&](int l) {
+            if (l < LOADS)
+                kp.load(key_base, next_keys, l, mine + B * BYTES);
+            else
+                vp.load(value_base, next_values, l - LOADS, mine + (2 + (B ^ 1)) * BYTES);
+        };
+        if (!any_rows) {
 #pragma unroll
-        for (int k = 0; k < KT; k++) {
-            if constexpr (WHOLE) {
-                here[k] = (there >> (2 * k) & 1 ? 0xffffu : 0) | (there >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
-            } else {
-                here[k] = __builtin_amdgcn_readfirstlane(space.present[B][2 * k] | space.present[B][2 * k + 1] << 16);
+            for (int l = 0; l < 2 * LOADS; l++) bring(l);
+            return;
+        }
+        if (!plain) {
+#pragma unroll
+            for (int k = 0; k < KT; k++) {
+                uint32_t here;
+                if constexpr (WHOLE)
+                    here = (there >> (2 * k) & 1 ? 0xffffu : 0) | (there >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
+                else
+                    here = space.present[B][2 * k] | space.present[B][2 * k + 1] << 16;
+                hide(s[k], c.sees(at + 32 * k, window) & here);
             }
-            all = all && here[k] == ~0u;
+            peak = c.peak(s, scale);
         }
-        if (at + NK - 1 > low || (window > 0 && at <= high - window) || !all) {
-#pragma unroll
-            for (int k = 0; k < KT; k++) hide(s[k], c.sees(at + 32 * k, window) & here[k]);
-        }
+        c.raise(peak);
         // the next scores' products run beside this softmax (past the last keys, on what the buffer holds)
         const lds_char *ahead = keys + (B ^ 1) * BYTES;
-        next[0] = c.scores(ahead);
-        const float peak = c.peak(s, scale);
-        c.raise(peak);
-        next[1] = c.scores(ahead + 32 * 2 * D);
-        u32x4 hi[KT][2], lo[2];
-#pragma unroll
-        for (int k = 0; k < KT; k++) c.template weigh<false>(s[k], scale, hi[k], lo);
-#pragma unroll
-        for (int k = 0; k < KT; k++) c.template add<false>(values + B * BYTES + k * 32 * 2 * D, hi[k], lo);
+        peak = c.step(ahead, values + B * BYTES, s, next, scale, bring);
     };
     for (int i = 0; i < n; i += 2) {
         step(std::integral_constant<int, 0>(), i);
         if (i + 1 < n) step(std::integral_constant<int, 1>(), i + 1);
     }
+    wait_loads<0>();
     if (lane == 0) space.bad[w] = bad;
     __syncthreads();
     if (space.bad[0] | space.bad[1] | space.bad[2] | space.bad[3]) {
@@ -755,8 +851,13 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArg
         many = l.many_groups > both;
         i -= both;
     }
-    if (many)
-        attend_many<D, WHOLE>(l.many, i % l.many_units, i / l.many_units, space);
+    if (many) {
+        // where the device holds all of these workgroups at once, two to a CU, the second of a CU is as much
+        // shorter as its first is longer
+        int unit = i % l.many_units;
+        if (l.mirrored && unit >= CUS) unit = l.many_units - 1 - (unit - CUS);
+        attend_many<D, WHOLE>(l.many, unit, i / l.many_units, space);
+    }
     else
         attend_few<D, WHOLE>(l.few, i % l.few_units, i / l.few_units, space);
 }
@@ -855,8 +956,6 @@ __global__ __launch_bounds__(256) void attend_join_kernel(LaunchArgs l, int few_
 // the host
 // ------------------------------------------------------------------------------------------
 
-constexpr int CUS = 256;
-
 // How the work is split, from the host's sizes alone. A sequence's rows (new tokens x group) go to attend_few
 // up to FEW and to attend_many above, or all to one of them where the expected lengths leave the other nothing.
 struct Plan {
@@ -946,6 +1045,7 @@ void launch_attention(const AttendArgs &a, const Plan &p, float *ws, int max_q_l
     l.many_units = p.many_units;
     l.few_groups = p.few_units * p.few_split;
     l.many_groups = p.many_units * p.many_split;
+    l.mirrored = !p.few && p.many_split == 1 && p.many_units > CUS && p.many_units <= 2 * CUS;
     attend_kernel<D, WHOLE><<<l.few_groups + l.many_groups, 256, 0, stream>>>(l);
     if (!LAUNCH_OK()) return;
     constexpr int ROWS = 256 / D;  // of a wave of the join

@@ -103,6 +103,8 @@ bool take_batch(const char *name, const PagedBatch *p, int n_tokens, int n_heads
     if (p->page_stride % 8 || p->slot_stride % 8 || p->head_stride % 8)
         return llm_fail("%s: cache strides %lld, %lld, %lld are not multiples of 8", name,
                         (long long)p->page_stride, (long long)p->slot_stride, (long long)p->head_stride);
+    if (p->page_size > 1 && p->slot_stride < p->head_dim)
+        return llm_fail("%s: slots %lld elements apart overlap (head_dim %d)", name, (long long)p->slot_stride, p->head_dim);
     b->kc = p->key_cache;
     b->vc = p->value_cache;
     b->page_stride = p->page_stride;
