@@ -21,54 +21,66 @@ struct PenaltyArgs {
     int64_t out_stride, x_stride;
 };
 
+constexpr int T = 512;                     // threads of a workgroup
 constexpr uint32_t IN_PROMPT = 1u << 31;  // above the count of a token's answers
 
-// What a token's logit becomes. met: its prompt bit and its count of answers.
-struct Row {
-    bool repeats;
-    float repetition, frequency, presence;
-    __device__ __forceinline__ float operator()(float x, uint32_t met, float bias, bool biased, bool allowed) const {
-        const uint32_t count = met & ~IN_PROMPT;
-        if (met && repeats) x = x > 0.0f ? x / repetition : x * repetition;
-        if (count) x = x - frequency * (float)count - presence;
-        if (biased) x += bias;
-        return allowed ? x : -INFINITY;
+// The values of a row, four per thread at a time where the row is 16-byte aligned: the first U times T fours
+// are requested (as far as the row's `room` goes) before the row's length is known.
+constexpr int U = 4;
+struct Values {
+    const int *p;
+    int room;
+    bool wide;
+    u32x4 first[U];
+    __device__ __forceinline__ Values(const int *p_, int room_) : p(p_), room(room_), wide(((uintptr_t)p_ & 15) == 0) {
+        if (!wide || room < 4) return;
+#pragma unroll
+        for (int u = 0; u < U; u++) first[u] = *gptr((const u32x4 *)p + min((int)threadIdx.x + u * T, room / 4 - 1));
+    }
+    // f(i, value i) for the first n values, n <= room.
+    template <class F>
+    __device__ __forceinline__ void each(int n, F f) {
+        int done = 0;
+        if (wide && n >= 4) {
+            const int quads = n / 4;
+            const u32x4 *q = (const u32x4 *)p;
+            for (int i = threadIdx.x; i < quads; i += U * T) {
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (i + u * T < quads) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) f(4 * (i + u * T) + e, (int)first[u][e]);
+                        if (i + (u + U) * T < quads) first[u] = *gptr(q + i + (u + U) * T);
+                    }
+            }
+            done = 4 * quads;
+        }
+        for (int i = done + threadIdx.x; i < n; i += T) f(i, gptr(p)[i]);
     }
 };
 
-// Calls f(i, v) for the n values at p, four at a time from the first 16-byte boundary on, several requested
-// ahead.
-template <int T, class F>
-__device__ __forceinline__ void each(const int *p, int n, F f) {
-    const int lead = min(n, (int)((16 - ((uintptr_t)p & 15)) & 15) / 4), quads = (n - lead) / 4;
-    if ((int)threadIdx.x < lead) f(threadIdx.x, gptr(p)[threadIdx.x]);
-    const u32x4 *q = (const u32x4 *)(p + lead);
-    constexpr int U = 4;
-    for (int i = threadIdx.x; i < quads; i += U * T) {
-        u32x4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; u++) v[u] = *gptr(q + min(i + u * T, quads - 1));
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (i + u * T < quads)
-#pragma unroll
-                for (int e = 0; e < 4; e++) f(lead + 4 * (i + u * T) + e, (int)v[u][e]);
-    }
-    const int done = lead + 4 * quads;
-    if ((int)threadIdx.x < n - done) f(done + threadIdx.x, gptr(p)[done + threadIdx.x]);
-}
-
 // One workgroup per slice of a row's vocabulary. The row's history is read once by every slice (from L2 after
 // the first); the slice's tokens are counted in LDS, by whole numbers, so that the order of the additions does
-// not matter, and a bias is the last entry's because the largest index of a token's entries is kept. Then
-// eight logits per thread at a time, 16 bytes where the rows' alignment allows it. Bound by the logits' bytes
-// where there are many rows; one row by the launch and two round trips to memory.
-template <int T>
+// not matter. Then eight logits per thread at a time, 16 bytes where the rows' alignment allows it. Bound by the
+// logits' bytes in flight where there are many rows, so LDS per token is kept small and slices large; one row by
+// the launch and two round trips to memory.
+// NARROW: counts of 16 bits instead of 32, for histories that cannot count further.
+// DENSE: a word per token for its bias, for any number of biases: entry i leaves -(i + 1) there if that is the
+// least, so the last entry of a token stays, and then puts its value there. As floats those numbers are NaN,
+// which no value put there is, so no other entry can take a value for its number. Otherwise, for up to T biases,
+// a bit per token, and the values in the order of their tokens: a token's place is the number of bits before
+// its own.
+template <bool NARROW, bool DENSE>
 __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
     extern __shared__ uint32_t lds[];
+    constexpr int PER = NARROW ? 2 : 1;  // tokens per word of the counts
+    constexpr int WORD = DENSE ? 1 : 32;  // tokens per word of the biases
+    constexpr int LISTED = DENSE ? 1 : T;
+    __shared__ __align__(16) int entries[LISTED], ids[LISTED];
+    __shared__ int listed, before[LISTED], totals[T / 64];
+    __shared__ float sorted[LISTED];
     const int r = blockIdx.y, t0 = blockIdx.x * a.slice, n = min(a.slice, a.vocab - t0);
-    uint32_t *met = lds;                                          // per token of the slice
-    int *entry = (int *)(lds + (a.tokens ? a.slice : 0));         // 1 + the index of the token's last bias
+    uint32_t *met = lds, *biased = lds + (a.tokens ? a.slice / PER : 0);
     const bf16 *from = a.x + r * a.x_stride + t0;
     bf16 *to = a.out + r * a.out_stride + t0;
     // eight logits from a multiple of 8 on; the first ones are requested before the history is read
@@ -85,39 +97,89 @@ __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
         return x;
     };
     const uint32_t *allowed = a.allowed ? a.allowed + (int64_t)r * a.allowed_stride + t0 / 32 : nullptr;
+    Values tokens(a.tokens + (int64_t)r * a.token_stride, a.tokens ? a.token_stride : 0);
     u32x4 x = {0, 0, 0, 0};
     uint32_t word = ~0u;
     if (8 * (int)threadIdx.x < n) {
         x = request(8 * threadIdx.x);
         if (allowed) word = gptr(allowed)[threadIdx.x / 4];
     }
+    int bias_token = -1;  // this thread's entry, where there are no more than threads
+    float value = 0.0f;
+    if (!DENSE && a.bias_tokens && (int)threadIdx.x < a.bias_stride) {
+        bias_token = gptr(a.bias_tokens)[(int64_t)r * a.bias_stride + threadIdx.x];
+        value = gptr(a.bias)[(int64_t)r * a.bias_stride + threadIdx.x];
+    }
     const int history = a.tokens ? max(0, min(a.token_stride, gptr(a.token_len)[r])) : 0;
     const int prompt = a.tokens && a.prompt_len ? gptr(a.prompt_len)[r] : 0;
     const int biases = !a.bias_tokens ? 0
                        : a.bias_len   ? max(0, min(a.bias_stride, gptr(a.bias_len)[r]))
                                       : a.bias_stride;
-    const Row row = {a.repetition != nullptr, a.repetition ? gptr(a.repetition)[r] : 1.0f,
-                     a.frequency ? gptr(a.frequency)[r] : 0.0f, a.presence ? gptr(a.presence)[r] : 0.0f};
-    const int clear = (a.tokens ? a.slice : 0) + (a.bias_tokens ? a.slice : 0);
+    const float repetition = a.repetition ? gptr(a.repetition)[r] : 1.0f, inverse = 1.0f / repetition;
+    const float frequency = a.frequency ? gptr(a.frequency)[r] : 0.0f;
+    const float presence = a.presence ? gptr(a.presence)[r] : 0.0f;
+    const int *bias_tokens = a.bias_tokens + (int64_t)r * a.bias_stride;
+    const float *bias = a.bias + (int64_t)r * a.bias_stride;
+    const auto in_slice = [&](int token) { return (unsigned)token - (unsigned)t0 < (unsigned)n; };
+    const int clear = (a.tokens ? a.slice / PER : 0) + (a.bias_tokens ? a.slice / WORD : 0);
     for (int i = 4 * threadIdx.x; i < clear; i += 4 * T) *(u32x4 *)(lds + i) = u32x4{0, 0, 0, 0};
+    if (threadIdx.x == 0) listed = 0;
+    if (!DENSE) ids[threadIdx.x] = -1;
     __syncthreads();
     if (history)
-        each<T>(a.tokens + (int64_t)r * a.token_stride, history, [&](int i, int token) {
+        tokens.each(history, [&](int i, int token) {
             const unsigned t = (unsigned)token - (unsigned)t0;
             if (t < (unsigned)n) {
+                const int shift = NARROW ? t % 2 * 16 : 0;
                 if (i < prompt)
-                    atomicOr(&met[t], IN_PROMPT);
+                    atomicOr(&met[t / PER], (NARROW ? 0x8000u : IN_PROMPT) << shift);
                 else
-                    atomicAdd(&met[t], 1u);
+                    atomicAdd(&met[t / PER], 1u << shift);
             }
         });
-    if (biases)
-        each<T>(a.bias_tokens + (int64_t)r * a.bias_stride, biases, [&](int i, int token) {
-            const unsigned t = (unsigned)token - (unsigned)t0;
-            if (t < (unsigned)n) atomicMax(&entry[t], i + 1);
-        });
+    if (DENSE && biases) {
+        for (int i = threadIdx.x; i < biases; i += T)
+            if (in_slice(gptr(bias_tokens)[i])) atomicMin((int *)&biased[gptr(bias_tokens)[i] - t0], -(i + 1));
+        __syncthreads();
+        for (int i = threadIdx.x; i < biases; i += T) {
+            if (!in_slice(gptr(bias_tokens)[i])) continue;
+            uint32_t *at = &biased[gptr(bias_tokens)[i] - t0];
+            if ((int)*at != -(i + 1)) continue;
+            const float v = gptr(bias)[i];
+            *at = v == v ? __float_as_uint(v) : 0x7fc00000u;
+        }
+    } else if (biases) {
+        const int t = bias_token - t0, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+        bool mine = (int)threadIdx.x < biases && in_slice(bias_token);
+        if (mine) {
+            atomicOr(&biased[t / 32], 1u << (t % 32));
+            const int at = atomicAdd(&listed, 1);
+            entries[at] = threadIdx.x;
+            ids[at] = t;
+        }
+        __syncthreads();
+        for (int k = 0; k < listed; k += 4) {  // is there a later one of the same token?
+            const u32x4 id = *(const u32x4 *)&ids[k], entry = *(const u32x4 *)&entries[k];
+#pragma unroll
+            for (int e = 0; e < 4; e++) mine = mine && ((int)id[e] != t || (int)entry[e] <= (int)threadIdx.x);
+        }
+        const int bits = (int)threadIdx.x < a.slice / 32 ? __popc(biased[threadIdx.x]) : 0;
+        int upto = bits;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int other = __shfl_up(upto, d);
+            if (lane >= d) upto += other;
+        }
+        if (lane == 63) totals[w] = upto;
+        __syncthreads();
+        int first = upto - bits;
+#pragma unroll
+        for (int v = 0; v < T / 64; v++) first += v < w ? totals[v] : 0;
+        before[threadIdx.x] = first;
+        __syncthreads();
+        if (mine) sorted[before[t / 32] + __popc(biased[t / 32] & ((1u << (t % 32)) - 1))] = value;
+    }
     __syncthreads();
-    const float *bias = a.bias_tokens ? a.bias + (int64_t)r * a.bias_stride : nullptr;
     for (int i = 8 * threadIdx.x; i < n; i += 8 * T) {
         u32x4 more = {0, 0, 0, 0};
         uint32_t next = ~0u;
@@ -129,10 +191,28 @@ __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const uint32_t m = history ? met[i + e] : 0;
-            const int k = biases ? entry[i + e] : 0;
-            y[e] = row(elem(x, e), m, k ? gptr(bias)[k - 1] : 0.0f, k != 0, bits >> e & 1);
+            uint32_t m = history ? met[(i + e) / PER] : 0;
+            if constexpr (NARROW) m = e & 1 ? m >> 16 : m & 0xffff;
+            const uint32_t count = m & (NARROW ? 0x7fff : ~IN_PROMPT);
+            const float z = elem(x, e), factor = z > 0.0f ? inverse : repetition;
+            const float less = fmaf(frequency, (float)count, presence);
+            y[e] = z * (m ? factor : 1.0f) - (count ? less : 0.0f);
         }
+        if (DENSE && biases) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (biased[i + e]) y[e] += __uint_as_float(biased[i + e]);
+        } else if (biases) {
+            const uint32_t all = biased[i / 32];
+            if (all >> (i % 32) & 0xff) {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (all >> (i % 32 + e) & 1)
+                        y[e] += sorted[before[i / 32] + __popc(all & ((1u << (i % 32 + e)) - 1))];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = bits >> e & 1 ? y[e] : -INFINITY;
         if (wide && i + 8 <= n) {
             st16(to + i, u32x4{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7])});
         } else {
@@ -192,18 +272,22 @@ extern "C" void logits_penalty_forward(bf16 *out, const bf16 *logits, const int 
                  (vocab + 31) / 32, vocab);
         return;
     }
-    // a slice as large as the device is still filled with, so that histories are read less often (whole
-    // 512s of tokens: a bias entry and a count are 8 bytes of LDS each)
-    int slice = 8192;
-    while (slice > 1024 && (int64_t)rows * ((vocab + slice - 1) / slice) < 512) slice /= 2;
+    // as large a slice as leaves workgroups enough: histories are read by fewer
+    const bool narrow = token_stride < 1 << 15, dense = bias_tokens && bias_stride > T;
+    int slice = narrow && !dense ? 16384 : 4096;
+    while (slice > 2048 && (int64_t)rows * ((vocab + slice - 1) / slice) < 512) slice /= 2;
     PenaltyArgs a = {out, logits, tokens, prompt_len, token_len, repetition, frequency, presence,
                      bias_tokens, bias, bias_len, allowed, vocab, token_stride, bias_stride,
                      allowed_stride, slice, out_stride, logits_stride};
     const dim3 grid((vocab + slice - 1) / slice, rows);
-    const unsigned lds = slice * ((tokens ? 4 : 0) + (bias_tokens ? 4 : 0));
-    if (slice > 2048)
-        penalty_kernel<512><<<grid, 512, lds, stream>>>(a);
+    const unsigned lds = (tokens ? slice * (narrow ? 2 : 4) : 0) + (bias_tokens ? dense ? slice * 4 : slice / 8 : 0);
+    if (narrow && !dense)
+        penalty_kernel<true, false><<<grid, T, lds, stream>>>(a);
+    else if (narrow)
+        penalty_kernel<true, true><<<grid, T, lds, stream>>>(a);
+    else if (!dense)
+        penalty_kernel<false, false><<<grid, T, lds, stream>>>(a);
     else
-        penalty_kernel<256><<<grid, 256, lds, stream>>>(a);
+        penalty_kernel<false, true><<<grid, T, lds, stream>>>(a);
     LAUNCH_OK();
 }

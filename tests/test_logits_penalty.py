@@ -121,6 +121,21 @@ def test_a_long_history_of_few_tokens(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("history,biases", [(100, 512), (100, 513), (33000, 512), (40000, 2000), (32767, 1), (32768, 1)])
+@pytest.mark.parametrize("vocab", [40, 5000, 70001])
+def test_many_biases_and_long_histories(gpu, history, biases, vocab):
+    """Both sides of the sizes from which counts and biases take more room; every bias in one place; one token
+    counted 32767 times and more."""
+    import torch
+    rng = np.random.default_rng(7)
+    logits = torch.randn(3, vocab, device="cuda").bfloat16()
+    c = make(rng, 3, vocab, history, biases, True, True)
+    c["bias_tokens"][1] = rng.integers(0, 30, biases)
+    c["tokens"][2], c["token_len"][2], c["prompt_len"][2], c["frequency"][2] = 7, history, 0, 1e-3
+    check(run(gpu, logits, c), logits, c)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("off", ["repetition", "frequency", "presence", "prompt_len"])
 def test_each_part_can_be_off(gpu, off):
     import torch
