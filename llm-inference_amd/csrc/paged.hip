@@ -36,6 +36,19 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const int t = (int)(wave / a.waves_per_token);
     if (t >= a.b.n_tokens) return;
     const int part = (int)(wave - (int64_t)t * a.waves_per_token);
+    const int L = lane % LH, hg = lane / LH;
+    const int groups = a.q_groups + 2 * a.kv_groups, last = min(groups, (part + 1) * a.share);
+    // the lane's 16 bytes of its head of group g (of q, then k, then v)
+    const auto request = [&](int g) {
+        const bool is_q = g < a.q_groups, is_v = g >= a.q_groups + a.kv_groups;
+        const int h = (is_q ? g : is_v ? g - a.q_groups - a.kv_groups : g - a.q_groups) * HPW + hg;
+        const bf16 *src = is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride : a.k + t * a.k_stride;
+        u32x4 x = {0, 0, 0, 0};
+        if (h < (is_q ? a.n_heads : a.n_kv_heads)) x = ld16_nt(src + h * D + 8 * L);
+        return x;
+    };
+    u32x4 ahead = request(part * a.share);
+    const u32x4 wq = a.qn ? ld16(a.qn + 8 * L) : u32x4{0, 0, 0, 0}, wk = a.kn ? ld16(a.kn + 8 * L) : u32x4{0, 0, 0, 0};
     const int s = sequence_of(a.b, t);
     if (s < 0) return;
     const int pos = kv_length(a.b, s) - gptr(a.b.q_start)[s + 1] + t;
@@ -50,7 +63,6 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         sincos_d(r, &sn, &cs);
         turn[w][j] = make_float2((float)cs * a.scale, (float)sn * a.scale);
     }
-    const int L = lane % LH, hg = lane / LH;
     const bool turned = 8 * L < a.rotary;
     const bool second = !a.interleaved && 8 * L >= half;
     float c[8], sn[8];
@@ -63,17 +75,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         sn[e] = (a.interleaved ? !(e & 1) : !second) ? -cs.y : cs.y;
     }
     const int partner = second ? lane - half / 8 : lane + half / 8;
-    const int groups = a.q_groups + 2 * a.kv_groups;
-    for (int g = part * a.share; g < min(groups, (part + 1) * a.share); g++) {
+    for (int g = part * a.share; g < last; g++) {
         const bool is_q = g < a.q_groups, is_v = g >= a.q_groups + a.kv_groups;
         const int h = (is_q ? g : is_v ? g - a.q_groups - a.kv_groups : g - a.q_groups) * HPW + hg;
-        const bool there = h < (is_q ? a.n_heads : a.n_kv_heads);
-        if (!is_q && at < 0) continue;
-        const bf16 *src = is_q   ? a.q + t * a.q_stride
-                          : is_v ? a.v + t * a.v_stride
-                                 : a.k + t * a.k_stride;
-        u32x4 x = {0, 0, 0, 0};
-        if (there) x = ld16(src + h * D + 8 * L);
+        const bool there = h < (is_q ? a.n_heads : a.n_kv_heads) && (is_q || at >= 0);
+        const u32x4 x = ahead;
+        if (g + 1 < last) ahead = request(g + 1);
         if (is_v) {
             if (there) st16(a.b.vc + at + h * a.b.head_stride + 8 * L, x);
             continue;
@@ -81,12 +88,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) y[e] = elem(x, e);
-        const bf16 *weight = is_q ? a.qn : a.kn;
-        if (weight) {
-            const u32x4 wt = ld16(weight + 8 * L);
+        if (is_q ? a.qn != nullptr : a.kn != nullptr) {
             const float inv = 1.0f / sqrtf(group_sum<LH>(dot8(x, x, 0.0f)) / (float)D + a.eps);
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = y[e] * inv * elem(wt, e);
+            for (int e = 0; e < 8; e++) y[e] = y[e] * inv * elem(is_q ? wq : wk, e);
         }
         float o[8];
 #pragma unroll
@@ -195,8 +200,12 @@ extern "C" void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, co
     const int hpw = 512 / D;
     a.q_groups = (n_heads + hpw - 1) / hpw;
     a.kv_groups = (batch->n_kv_heads + hpw - 1) / hpw;
-    a.share = 1;
-    a.waves_per_token = a.q_groups + 2 * a.kv_groups;
+    const int groups = a.q_groups + 2 * a.kv_groups;
+    // about 6144 waves (24 to a CU), as far as the rows go: with fewer a wave's loads wait too long for each
+    // other, with more the angles are computed too often (3402 rows of 48 heads of 128: one group of heads per
+    // wave 36.8 us, 3 23.8, 6 20.6, 12 23.9; 411 rows: one 6.8, two 6.9, six 9.5)
+    a.share = (int)std::min<int64_t>(groups, std::max<int64_t>(1, (int64_t)n_tokens * groups / 6144));
+    a.waves_per_token = (groups + a.share - 1) / a.share;
     const int64_t blocks = ((int64_t)n_tokens * a.waves_per_token + 3) / 4;
     if (blocks > INT32_MAX) {
         llm_fail("%s: %d rows of %d heads are too many for one launch", name, n_tokens, n_heads);
