@@ -81,15 +81,14 @@ constexpr int MANY = 128;                // rows of a tile of attend_many
 template <int T>
 __device__ __forceinline__ bool find_tile(const AttendArgs &a, int which, int i, Tile &t) {
     const int lane = threadIdx.x & 63;
-    int j = -1;
+    int j = -1, tokens = 0;
     for (int s0 = 0; s0 < a.b.n_seqs; s0 += 64) {
-        const int s = s0 + lane;
+        const int s = min(s0 + lane, a.b.n_seqs - 1);  // what the lanes read goes out together
+        const int first = token_at(a.b, s), count = max(0, token_at(a.b, s + 1) - first), length = kv_length(a.b, s);
+        const int64_t rows = (int64_t)count * a.group;
         int n = 0;
-        if (s < a.b.n_seqs) {
-            const int first = token_at(a.b, s);
-            const int64_t rows = (int64_t)max(0, token_at(a.b, s + 1) - first) * a.group;
-            if (which == ALL_ROWS || (rows <= FEW) == (which == FEW_ROWS)) n = (int)((rows + T - 1) / T);
-        }
+        if (s0 + lane < a.b.n_seqs && (which == ALL_ROWS || (rows <= FEW) == (which == FEW_ROWS)))
+            n = (int)((rows + T - 1) / T);
         int upto = n;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -100,17 +99,17 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int which, int i,
         if (past) {
             const int at = __builtin_ctzll(past);
             t.s = s0 + at;
+            t.q0 = __builtin_amdgcn_readlane(first, at);
+            tokens = __builtin_amdgcn_readlane(count, at);
+            t.before = __builtin_amdgcn_readlane(length, at) - tokens;
             j = __builtin_amdgcn_readlane(upto, at) - 1 - i;
             break;
         }
         i -= __builtin_amdgcn_readlane(upto, 63);
     }
     if (j < 0) return false;
-    t.q0 = token_at(a.b, t.s);
-    const int n = token_at(a.b, t.s + 1) - t.q0;
     t.first = j * T;
-    t.rows = min(T, n * a.group - t.first);
-    t.before = kv_length(a.b, t.s) - n;
+    t.rows = min(T, tokens * a.group - t.first);
     const int lo = t.before + t.first / a.group, hi = t.before + (t.first + t.rows - 1) / a.group;
     t.to = lo;
     t.most = hi;
@@ -837,19 +836,21 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
 // the launch
 // ------------------------------------------------------------------------------------------
 
-// Workgroups of both kinds in turn while there are both: the ones read, the others multiply.
+// Workgroups of both kinds in turn while there are both, eight at a time (consecutive ones go to different
+// XCDs): the ones read, the others multiply.
 template <int D, bool WHOLE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArgs l) {
     __shared__ Space<D, WHOLE> space;
-    const int both = min(l.few_groups, l.many_groups);
+    const int both = min(l.few_groups, l.many_groups) & ~7;
     int i = blockIdx.x;
     bool many;
     if (i < 2 * both) {
-        many = !(i & 1);
-        i >>= 1;
+        many = !(i & 8);
+        i = (i >> 4) * 8 + (i & 7);
     } else {
-        many = l.many_groups > both;
-        i -= both;
+        i -= 2 * both;  // the rest of the one kind, and up to seven of the other
+        many = i < l.many_groups - both;
+        i += both - (many ? 0 : l.many_groups - both);
     }
     if (many) {
         // where the device holds all of these workgroups at once, two to a CU, the second of a CU is as much
