@@ -182,15 +182,17 @@ struct Pages {
                         (WHOLE ? (unsigned)(i * PER + r) * (unsigned)b.slot_stride * 2 : 0);
     }
 
+    __device__ __forceinline__ void set(int64_t at) {
+        present = at >= 0;
+        mine = (at < 0 ? 0 : at * 2) + head;
+    }
     // Looks up steps step .. step + AHEAD - 1, when step is a multiple of AHEAD.
     __device__ __forceinline__ void look_up(bool many, int s, int step) {
         if (step % AHEAD != 0) return;
         const int lane = threadIdx.x & 63;
         const auto &b = again(many)->b;
         if constexpr (WHOLE) {
-            const int64_t at = place(b, s, first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16);
-            present = at >= 0;
-            mine = (at < 0 ? 0 : at * 2) + head;
+            set(place(b, s, first + (step + lane / GROUPS) * STEP + lane % GROUPS * 16));
         } else {
 #pragma unroll
             for (int k = 0; k < 2; k++) {
@@ -709,22 +711,32 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
     int groups = 0;      // WHOLE: which quarters of the lane's step are there
     bool whole = false;  // WHOLE: all of the steps looked up that are plain
     const auto look_up_values = [&](int i) {
-        vp.look_up(true, t.s, i);
         if constexpr (WHOLE) {
-            if (i % P::AHEAD == 0) {
-                const auto &b = again(true)->b;
-                groups = 0;
+            if (i % P::AHEAD != 0) return;
+            const auto &b = again(true)->b;
+            int64_t at[4];
+            groups = 0;
 #pragma unroll
-                for (int v = 0; v < 4; v++)
-                    if (place(b, t.s, begin + (i + lane) * NK + v * QUARTER) >= 0) groups |= 1 << v;
-                whole = !__any(groups != 15 && i + lane >= plain0 && i + lane < plain1);
+            for (int v = 0; v < 4; v++) at[v] = place(b, t.s, begin + (i + lane) * NK + v * QUARTER);
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                if (at[v] >= 0) groups |= 1 << v;
+                if (v == w) vp.set(at[v]);
             }
+            whole = !__any(groups != 15 && i + lane >= plain0 && i + lane < plain1);
+        } else {
+            vp.look_up(true, t.s, i);
         }
     };
     if (n > 0) {
-        kp.look_up(true, t.s, 0);
-        kp.request(kc, 0, mine);
         look_up_values(0);
+        if constexpr (WHOLE) {
+            kp.mine = vp.mine;
+            kp.present = vp.present;
+        } else {
+            kp.look_up(true, t.s, 0);
+        }
+        kp.request(kc, 0, mine);
         vp.request(vc, 0, mine + 2 * BYTES);
         wait_loads<LOADS>();  // the keys
         __syncthreads();
@@ -836,31 +848,23 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
 // the launch
 // ------------------------------------------------------------------------------------------
 
-// Workgroups of both kinds in turn while there are both, eight at a time (consecutive ones go to different
-// XCDs): the ones read, the others multiply.
+// Workgroups of many rows first: they take longest, and those of few rows, where there are any, fill up beside
+// them (a chunk of 511 after 4095 and another beside 20 single tokens, 16 heads on 8: many first 55 us, in
+// turns 71, few first 69; two windowed chunks and no few rows, whose empty workgroups then come last: 34 / 45 / 34).
 template <int D, bool WHOLE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArgs l) {
     __shared__ Space<D, WHOLE> space;
-    const int both = min(l.few_groups, l.many_groups) & ~7;
-    int i = blockIdx.x;
-    bool many;
-    if (i < 2 * both) {
-        many = !(i & 8);
-        i = (i >> 4) * 8 + (i & 7);
-    } else {
-        i -= 2 * both;  // the rest of the one kind, and up to seven of the other
-        many = i < l.many_groups - both;
-        i += both - (many ? 0 : l.many_groups - both);
-    }
+    const bool many = (int)blockIdx.x < l.many_groups;
+    const int i = blockIdx.x - (many ? 0 : l.many_groups);
     if (many) {
         // where the device holds all of these workgroups at once, two to a CU, the second of a CU is as much
         // shorter as its first is longer
         int unit = i % l.many_units;
         if (l.mirrored && unit >= CUS) unit = l.many_units - 1 - (unit - CUS);
         attend_many<D, WHOLE>(l.many, unit, i / l.many_units, space);
-    }
-    else
+    } else {
         attend_few<D, WHOLE>(l.few, i % l.few_units, i / l.few_units, space);
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -965,25 +969,28 @@ struct Plan {
     size_t few_rows, many_rows, floats;  // rows of partial outputs
 
     // A join costs 2 to 3 us, what a workgroup takes for about 640 keys alone (one token, 32 heads on 8, 511 / 1023
-    // / 8191 / 40959 positions: unsplit 9.6 / 14.6 / 88.6 / 446.8 us, 128 keys or 256 workgroups 9.8 / 10.2 / 14.5 /
-    // 34.6, 512 workgroups 9.8 / 10.2 / 15.2 / 36.8). Sequences of unequal length gain from twice the workgroups
-    // (4 sequences up to 8000: 22.2 / 21.0), and from pieces of 2048 keys where there are enough (64 up to 8447:
-    // 239.9 / 219.9).
+    // / 8191 / 40959 positions: unsplit 8.6 / 12.3 / 64.6 / 425 us, 128 keys or 256 workgroups 9.5 / 10.0 / 16.1 /
+    // 39.7, 512 workgroups 9.6 / 10.1 / 17.8 / 41.3). Sequences of unequal length gain from twice the workgroups
+    // (4 sequences up to 8000 20.4 / 20.4), and from pieces of 1024 keys, or 2048 where there are enough of those
+    // (16 up to 8000, pieces of 2048 / 1024: 67.5 / 60.5; 64 up to 8447, whole / 2048 / 1024: 234 / 216 / 219).
     static int64_t few_splits(int64_t units, int n_seqs, int64_t span) {
         if (span <= 640) return 1;
-        const int64_t target = n_seqs > 1 ? 2 * CUS : CUS;
-        return std::max<int64_t>(1, std::min((span + 127) / 128, std::max(target / units, (span + 2047) / 2048)));
+        const int64_t target = n_seqs > 1 ? 2 * CUS : CUS, piece = units <= CUS ? 1024 : 2048;
+        return std::max<int64_t>(
+            1, std::min((span + 127) / 128, std::max(target / units, n_seqs > 1 ? (span + piece - 1) / piece : 1)));
     }
 
     // The least of an estimate in ns: a workgroup's keys, alone on a CU or two to one, the parts' bytes written and
-    // read, and the join's launch.
-    static int64_t many_splits(int64_t units, int head_dim, int64_t span) {
+    // read, and the join's launch. Beside workgroups of few rows at most `most`.
+    static int64_t many_splits(int64_t units, int head_dim, int64_t span, int64_t most) {
         int64_t best = 1;
         double least = 0;
-        for (int64_t n = 1; n <= std::min<int64_t>(64, (span + 127) / 128); n++) {
+        for (int64_t n = 1; n <= std::min<int64_t>(most, (span + 127) / 128); n++) {
             const double groups = (double)units * n, keys = (double)((span + n - 1) / n);
-            const double key = (groups <= CUS ? 24.0 : 35.0 * std::max(1.0, groups / (2 * CUS))) * (head_dim + 64) / 192;
-            const double cost = keys * key + (n > 1 ? 4000 + groups * MANY * (head_dim + 2) * 8 / 4000 : 0);
+            const double key = head_dim == 256 ? 47.0 * std::max(1.0, groups / CUS)
+                                               : (groups <= CUS ? 24.0 : 35.0 * std::max(1.0, groups / (2 * CUS))) *
+                                                     (head_dim + 64) / 192;
+            const double cost = keys * key + (n > 1 ? 4000 + groups * 128 * (head_dim + 2) * 8 / 4000 : 0);
             if (n == 1 || cost < least) best = n, least = cost;
         }
         return best;
@@ -1010,8 +1017,12 @@ struct Plan {
                 if (window == 0) break;
             }
         };
+        // Workgroups of few rows need places of their own beside those of many: the mixed step above, 88 tiles x kv
+        // heads in 1 / 2 / 3 / 4 / 6 splits 115 / 84 / 70 / 76 / 84 us; 64 single tokens of up to 8000 beside one
+        // chunk, 128 in 1 / 2 / 3 / 4 276 / 267 / 288 / 310.
+        const int64_t units = (rows + MANY - 1) / MANY * n_kv_heads, most = few ? std::max<int64_t>(1, 288 / units) : 64;
         cut(FEW, [&](int64_t span) { return few_splits((int64_t)n_seqs * n_kv_heads, n_seqs, span); }, few_split, few_chunk);
-        cut(MANY, [&](int64_t span) { return many_splits((rows + MANY - 1) / MANY * n_kv_heads, head_dim, span); },
+        cut(MANY, [&](int64_t span) { return many_splits(units, head_dim, span, most); },
             many_split, many_chunk);
         few_rows = few_split > 1 ? (size_t)few_units * few_split * FEW : 0;
         many_rows = many_split > 1 ? (size_t)many_units * many_split * MANY : 0;

@@ -67,15 +67,14 @@ __device__ __forceinline__ int kv_length(const Batch &b, int s) {
     return max(-(1 << 30), min(1 << 30, gptr(b.kv_len)[s]));
 }
 
-// Element offset of position p of sequence s in the caches (head 0), or -1 where it is not there.
+// Element offset of position p of sequence s in the caches (head 0), or -1 where it is not there. Without
+// branches, so that several lookups' loads go out together.
 template <class B>
 __device__ __forceinline__ int64_t place(B &b, int s, int p) {
-    if (p < 0) return -1;
-    const int i = divide(p, b.page.m, b.page.l);
-    if (i >= b.table_pages) return -1;
-    const int page = gptr(b.table)[(int64_t)s * b.table_pages + i];
-    if ((unsigned)page >= (unsigned)b.n_pages) return -1;
-    return page * b.page_stride + (p - i * b.page_size) * b.slot_stride;
+    const int i = divide(max(p, 0), b.page.m, b.page.l);
+    const int page = gptr(b.table)[(int64_t)s * b.table_pages + min(i, b.table_pages - 1)];
+    const bool there = p >= 0 && i < b.table_pages && (unsigned)page < (unsigned)b.n_pages;
+    return there ? page * b.page_stride + (p - i * b.page_size) * b.slot_stride : -1;
 }
 
 bool take_batch(const char *name, const PagedBatch *p, int n_tokens, int n_heads, Batch *b) {
