@@ -23,10 +23,10 @@ extern "C" {
 /* A batch of sequences over a pool of pages. A host struct; every pointer is device memory and is read
  * when the launched kernels run, so a captured graph follows the lengths and the table as they change.
  *
- * Sequence s has the new tokens of rows q_start[s] .. q_start[s + 1] - 1 (q_start does not decrease; rows
- * before q_start[0] and from q_start[n_seqs] on belong to no sequence and are left as they are), and
- * kv_len[s] tokens in the cache once the new ones are in: its i-th new row has the position
- * kv_len[s] - (q_start[s + 1] - q_start[s]) + i. Position p lies in page page_table[s, p / page_size] of the
+ * Sequence s has the new tokens of rows q_start[s] .. q_start[s + 1] - 1 (from 0 to the call's n_tokens, not
+ * decreasing; rows before q_start[0] and from q_start[n_seqs] on belong to no sequence and are left as they
+ * are), and kv_len[s] tokens in the cache once the new ones are in (more than 2^30 count as 2^30): its i-th
+ * new row has the position kv_len[s] - (q_start[s + 1] - q_start[s]) + i. Position p lies in page page_table[s, p / page_size] of the
  * pool, at slot p % page_size; element d of its kv head h is at
  * page * page_stride + slot * slot_stride + h * head_stride + d of the key and of the value cache.
  * Positions past the table's row, and those whose page is outside [0, n_pages), are not there: they are
@@ -34,8 +34,8 @@ extern "C" {
 typedef struct {
     bf16 *key_cache;        /* 16-byte aligned */
     bf16 *value_cache;
-    int64_t page_stride;    /* elements, multiples of 8 */
-    int64_t slot_stride;
+    int64_t page_stride;    /* elements, multiples of 8, not negative */
+    int64_t slot_stride;    /* at least head_dim, at most 2^26 */
     int64_t head_stride;
     const int *page_table;  /* [n_seqs, table_pages] */
     const int *q_start;     /* [n_seqs + 1] */
@@ -81,7 +81,8 @@ void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, const bf16 *v
  * not reach it. Query head h reads kv head h / (n_heads / n_kv_heads). Rows of q and out are q_stride and
  * out_stride elements apart; out must not overlap anything. scale > 0.
  * max_q_len and max_kv_len say how many new rows and how many cached tokens a sequence is expected to have at
- * most: the split of the work goes by them. A longer sequence gives the same results, more slowly.
+ * most: the split of the work goes by them. Longer sequences are computed all the
+ * same, more slowly. How the work is split changes the order of the sums and with it the last bits.
  * ws: attention_paged_workspace_floats() floats, 16-byte aligned, needing no preparation; calls that share
  * it must not overlap (NULL where the count is 0). */
 void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBatch *batch, float *ws,

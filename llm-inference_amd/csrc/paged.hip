@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     const u32x4 wq = a.qn ? ld16(a.qn + 8 * L) : u32x4{0, 0, 0, 0}, wk = a.kn ? ld16(a.kn + 8 * L) : u32x4{0, 0, 0, 0};
     const int s = sequence_of(a.b, t);
     if (s < 0) return;
-    const int pos = kv_length(a.b, s) - gptr(a.b.q_start)[s + 1] + t;
+    const int pos = kv_length(a.b, s) - min(a.b.n_tokens, gptr(a.b.q_start)[s + 1]) + t;
     const int64_t at = place(a.b, s, pos);
     const int half = a.rotary / 2;
     for (int j = lane; j < half; j += 64) {
@@ -112,8 +112,12 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
 
 extern "C" float rope_frequencies(double *inv_freq, int rotary_dim, double theta, int kind,
                                   double factor, int trained) {
-    if (!inv_freq || rotary_dim <= 0 || rotary_dim % 2) {
+    if (rotary_dim <= 0 || rotary_dim % 2) {
         llm_fail("rope_frequencies: rotary_dim %d is not a positive even number", rotary_dim);
+        return 0.0f;
+    }
+    if (!inv_freq) {
+        llm_fail("rope_frequencies: inv_freq is null");
         return 0.0f;
     }
     if (!(theta > 1.0) || !isfinite(theta)) {

@@ -965,7 +965,8 @@ __global__ __launch_bounds__(256) void attend_join_kernel(LaunchArgs l, int few_
 // up to FEW and to attend_many above, or all to one of them where the expected lengths leave the other nothing.
 struct Plan {
     bool few, many;
-    int few_units, many_units, few_split, few_chunk, many_split, many_chunk;
+    int64_t few_units, many_units;  // tiles x kv heads, at most
+    int few_split, few_chunk, many_split, many_chunk;
     size_t few_rows, many_rows, floats;  // rows of partial outputs
 
     // A join costs 2 to 3 us, what a workgroup takes for about 640 keys alone (one token, 32 heads on 8, 511 / 1023
@@ -1005,8 +1006,8 @@ struct Plan {
         // at most one tile of a sequence is not full; one of many rows has over FEW of them
         const int64_t few_tiles = many ? n_seqs : rows / FEW + std::min<int64_t>(n_seqs, rows);
         const int64_t many_tiles = rows / MANY + (few ? std::min<int64_t>(n_seqs, rows / (FEW + 1)) : n_seqs);
-        few_units = few ? (int)(few_tiles * n_kv_heads) : 0;
-        many_units = many ? (int)(many_tiles * n_kv_heads) : 0;
+        few_units = few ? few_tiles * n_kv_heads : 0;
+        many_units = many ? many_tiles * n_kv_heads : 0;
         // a window shortens what the rows see; the workspace is asked for without it, so never more splits than then
         const auto cut = [&](int64_t tokens, auto splits, int &n, int &chunk) {
             n = INT32_MAX;
@@ -1053,17 +1054,17 @@ void launch_attention(const AttendArgs &a, const Plan &p, float *ws, int max_q_l
     l.many.chunk = p.many_chunk;
     l.few.which = p.many ? FEW_ROWS : ALL_ROWS;
     l.many.which = p.few ? MANY_ROWS : ALL_ROWS;
-    l.few_units = p.few_units;
-    l.many_units = p.many_units;
-    l.few_groups = p.few_units * p.few_split;
-    l.many_groups = p.many_units * p.many_split;
+    l.few_units = (int)p.few_units;
+    l.many_units = (int)p.many_units;
+    l.few_groups = l.few_units * p.few_split;
+    l.many_groups = l.many_units * p.many_split;
     l.mirrored = !p.few && p.many_split == 1 && p.many_units > CUS && p.many_units <= 2 * CUS;
     attend_kernel<D, WHOLE><<<l.few_groups + l.many_groups, 256, 0, stream>>>(l);
     if (!LAUNCH_OK()) return;
     constexpr int ROWS = 256 / D;  // of a wave of the join
     const int expected = (int)std::min<int64_t>(FEW, (int64_t)max_q_len * a.group);
     const int few_parts = (expected + ROWS - 1) / ROWS, many_parts = MANY / (4 * ROWS);
-    const int joins = (p.few_split > 1 ? p.few_units * few_parts : 0) + (p.many_split > 1 ? p.many_units * many_parts : 0);
+    const int joins = (p.few_split > 1 ? l.few_units * few_parts : 0) + (p.many_split > 1 ? l.many_units * many_parts : 0);
     if (joins > 0) {
         attend_join_kernel<D><<<joins, 256, 0, stream>>>(l, few_parts, many_parts);
         LAUNCH_OK();
@@ -1106,7 +1107,7 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
     const int64_t width = (int64_t)n_heads * D;
     if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width)) return;
     const Plan plan(n_tokens, batch->n_seqs, n_heads, batch->n_kv_heads, D, max_q_len, max_kv_len, window);
-    if ((int64_t)plan.few_units * plan.few_split + (int64_t)plan.many_units * plan.many_split > INT32_MAX / 64) {
+    if (plan.few_units * plan.few_split + plan.many_units * plan.many_split > INT32_MAX / 64) {
         llm_fail("%s: %d rows in %d sequences of up to %d tokens are too many for one launch", name, n_tokens,
                  batch->n_seqs, max_kv_len);
         return;

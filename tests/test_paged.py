@@ -394,6 +394,57 @@ def test_attention_extreme_scores(gpu, size):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("count,max_q", [(130, 1), (130, 40), (5000, 1)])
+def test_many_sequences(gpu, count, max_q):
+    """More sequences than lanes, most of them short, some without rows, some with many."""
+    rng = np.random.default_rng(count)
+    seqs = [(int(n), int(n + k)) for n, k in zip(rng.integers(0, 2 if count > 1000 else 3, count), rng.integers(0, 6, count))]
+    if max_q > 1:
+        seqs[70], seqs[129], seqs[0] = (40, 90), (33, 33), (0, 0)
+    b = Batch(seqs, 1, 64, 4, 31, lead=3, trail=1)
+    rows = b.normal(b.tokens, 4, 64)
+    q_out, (kc, vc) = rows[:, :2].contiguous().cuda(), b.pools()
+    inv_freq, scale = gpu.rope_frequencies(64, 1e4)
+    gpu.qk_norm_rope_paged(q_out, q_out, rows[:, 2:3].cuda(), rows[:, 3:].cuda(), None, None, inv_freq.cuda(), kc, vc,
+                           *b.where(), 1e-6, scale)
+    b.k, b.v, q = kc.cpu(), vc.cpu(), q_out.cpu()
+    for t, s, p in b.rows():
+        close(q[t], *rotated(rows[t, :2], None, p, inv_freq.numpy(), 1.0, False, 0))
+        close(b.k[b.slot(s, p)], *rotated(rows[t, 2:3], None, p, inv_freq.numpy(), 1.0, False, 0))
+        assert np.array_equal(bits(b.v[b.slot(s, p)]), bits(rows[t, 3:]))
+    check_attend(b, attend(gpu, b, q, 0.2, 0, max_q, 90, pools=(kc, vc)), q, 0.2, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page", [(128, 16), (64, 5)])
+def test_lengths_past_the_table(gpu, dim, page):
+    """Tokens past the end of the table's row, by a little or as far as numbers go, are neither written nor seen;
+    lengths below nothing see nothing."""
+    import torch
+    b = Batch([(2, 60), (1, 33), (70, 100), (1, 5), (3, 40)], 2, dim, page, 37)
+    keep = 40 // page
+    b.table = b.table[:, :keep].contiguous()
+    b.seqs[1], b.seqs[3] = (1, 1 << 30), (1, -(1 << 30))
+    b.kv_len = torch.tensor([60, 2 ** 31 - 1, 100, -2 ** 31, 40], dtype=torch.int32)
+    q, k, v = b.normal(b.tokens, 4, dim), b.normal(b.tokens, 2, dim), b.normal(b.tokens, 2, dim)
+    kc, vc = b.pools()
+    gpu.qk_norm_rope_paged(torch.empty_like(q, device="cuda"), q.cuda(), k.cuda(), v.cuda(), None, None,
+                           gpu.rope_frequencies(dim, 1e4)[0].cuda(), kc, vc, *b.where(), 1e-6)
+    written = torch.zeros(b.pages, page, dtype=torch.bool)
+    for t, s, p in b.rows():
+        if b.slot(s, p):
+            written[b.slot(s, p)] = True
+    assert written.any()
+    got_k, got_v = kc.cpu(), vc.cpu()
+    assert torch.equal(bits(got_k[~written]), bits(b.k[~written])) and torch.equal(bits(got_v[~written]), bits(b.v[~written]))
+    # what every row sees lies in the table's keep * page positions, whatever its own
+    b.k, b.v = got_k, got_v
+    far = Batch.rows
+    b.rows = lambda: ((t, s, min(p, keep * page - 1)) for t, s, p in far(b))
+    check_attend(b, attend(gpu, b, q, 0.1, 0, 70, 100, pools=(kc, vc)), q, 0.1, 0)
+
+
+@pytest.mark.gpu
 def test_attention_pools_past_32_bits(gpu):
     """Pages past 2^31 elements and 2^32 bytes of the pool, written and read."""
     import torch
@@ -606,7 +657,9 @@ BATCHES = [
     (dict(n_seqs=0), "n_seqs 0"), (dict(n_pages=-1), "n_pages -1"), (dict(page_size=0), "page_size 0"),
     (dict(table_pages=0), "table_pages 0"), (dict(key_cache=None), "null"), (dict(kv_len=None), "null"),
     (dict(value_cache=0x1002), "16-byte aligned"), (dict(slot_stride=100), "multiples of 8"),
-    (dict(page_size=(1 << 20) + 1), "over 1048576"),
+    (dict(page_size=(1 << 20) + 1), "over 1048576"), (dict(n_seqs=(1 << 20) + 1), "n_seqs 1048577"),
+    (dict(page_stride=-2048), "may be negative"), (dict(slot_stride=(1 << 26) + 8), "over 2^26"),
+    (dict(slot_stride=56), "overlap"),
 ]
 
 
