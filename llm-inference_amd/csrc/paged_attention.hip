@@ -1001,8 +1001,12 @@ struct Plan {
          int window) {
         const int64_t group = n_heads / n_kv_heads, rows = n_tokens * group;
         const int64_t longest = std::min<int64_t>(max_q_len, n_tokens) * group;
-        few = longest <= FEW || n_seqs > 1;
         many = longest > FEW;
+        // with sequences of at most FEW / group tokens of few rows and the others of at most max_q_len, this many
+        // at least have many rows: where that is all of them, all go to attend_many (and one that is short
+        // after all is only slower there)
+        const int64_t tokens = FEW / group, rest = n_tokens - n_seqs * tokens;
+        few = !many || (n_seqs > 1 && rest <= (int64_t)(n_seqs - 1) * (max_q_len - tokens));
         // at most one tile of a sequence is not full; one of many rows has over FEW of them
         const int64_t few_tiles = many ? n_seqs : rows / FEW + std::min<int64_t>(n_seqs, rows);
         const int64_t many_tiles = rows / MANY + (few ? std::min<int64_t>(n_seqs, rows / (FEW + 1)) : n_seqs);
@@ -1062,8 +1066,9 @@ void launch_attention(const AttendArgs &a, const Plan &p, float *ws, int max_q_l
     attend_kernel<D, WHOLE><<<l.few_groups + l.many_groups, 256, 0, stream>>>(l);
     if (!LAUNCH_OK()) return;
     constexpr int ROWS = 256 / D;  // of a wave of the join
-    const int expected = (int)std::min<int64_t>(FEW, (int64_t)max_q_len * a.group);
-    const int few_parts = (expected + ROWS - 1) / ROWS, many_parts = MANY / (4 * ROWS);
+    // workgroups per tile: those of few rows mostly hold one token's
+    const int expected = (int)std::min<int64_t>(FEW, p.many ? a.group : (int64_t)max_q_len * a.group);
+    const int few_parts = (expected + ROWS - 1) / ROWS, many_parts = MANY / (8 * ROWS);
     const int joins = (p.few_split > 1 ? l.few_units * few_parts : 0) + (p.many_split > 1 ? l.many_units * many_parts : 0);
     if (joins > 0) {
         attend_join_kernel<D><<<joins, 256, 0, stream>>>(l, few_parts, many_parts);
