@@ -340,6 +340,18 @@ def test_attention_long_histories(gpu, seqs, dim, heads):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,page", [(64, 32), (128, 16), (128, 5), (256, 16)])
+@pytest.mark.parametrize("window", [0, 2500])
+def test_attention_split_chunks_beside_single_tokens(gpu, dim, page, window):
+    """Chunks whose keys are split over workgroups and joined, single tokens beside them, a page gone."""
+    b = Batch([(150, 6000), (1, 5000), (40, 3000), (0, 100), (1, 2), (33, 40)], 1, dim, page, 41, lead=1, trail=1)
+    b.table[0, 2000 // page], b.table[1, 4000 // page] = -1, b.pages
+    q = b.normal(b.tokens, 2, dim, std=1.5)
+    scale = 1 / math.sqrt(dim)
+    check_attend(b, attend(gpu, b, q, scale, window), q, scale, window)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs,window,dim", [([(40, 100), (1, 100), (1, 65)], 0, 128),
                                              ([(40, 100), (1, 100), (1, 65)], 21, 64),
                                              ([(200, 230)], 0, 128), ([(200, 230)], 30, 256)])
