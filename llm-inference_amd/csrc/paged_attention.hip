@@ -414,20 +414,23 @@ struct Columns {
             }
     }
 
-    // One step of 64 keys, the matrix products with everything else between them: the next keys' scores into
-    // `next` beside the first 32 weights and the loads of later keys and values (bring), then O^T += V^T P^T beside
-    // the other 32 weights and the maximum of `next`, which is the result. The matrix unit takes an instruction
-    // every 32 cycles, and the other units' fit in between where they are spread evenly and do not wait for
-    // each other: a weight's fma, exponential and rounding stand in three places. The fences keep the order written.
-    template <class Bring>
-    __device__ __forceinline__ float step(const lds_char *keys, const lds_char *values, const f32x16 (&s)[2],
-                                          f32x16 (&next)[2], float c, Bring bring) {
-        constexpr int QK = D / 8, PV = D / 8, RING = 4;  // products of each kind; operands in flight
+    // One step of 32 KT keys, the matrix products with everything else between them: the next keys' scores into
+    // `next` beside the first 32 weights per two lanes and the loads of later keys and values (bring), then
+    // O^T += V^T P^T beside the other weights and the maximum of `next`, which is the result. The matrix unit takes
+    // an instruction every 32 cycles, and the other units' fit in between where they are spread evenly and do not
+    // wait for each other: a weight's fma, exponential and rounding stand in three places. The fences keep the
+    // order written.
+    template <int KT, class Bring>
+    __device__ __forceinline__ float step(const lds_char *keys, const lds_char *values, const f32x16 (&s)[KT],
+                                          f32x16 (&next)[KT], float c, Bring bring) {
+        constexpr int QK = KT * D / 16, PV = KT * D / 16, RING = 4;  // products of each kind; operands in flight
+        constexpr int ALL = 16 * KT;                                 // weights of a lane
         const int lane = threadIdx.x & 63, r = lane & 31, i = lane & 15, h = lane >> 5;
         const lds_char *key_row = keys + r * (2 * D);
         const int c0 = (h ^ swizzle<D>(r)) * 16, value_row = 4 * h + (i >> 2);
         const auto key = [&](int j) {
-            return __builtin_bit_cast(bf16x8_t, *(const LLM_LDS u32x4 *)(key_row + (j & 1) * 64 * D + (c0 ^ (j / 2 * 32))));
+            return __builtin_bit_cast(
+                bf16x8_t, *(const LLM_LDS u32x4 *)(key_row + (j % KT) * 64 * D + (c0 ^ (j / KT * 32))));
         };
         const auto value = [&](int j) {
             const int d = j % (D / 32), t = j / (D / 32), chunk = d * 4 + (lane >> 4 & 1) * 2 + ((i & 3) >> 1);
@@ -444,18 +447,18 @@ struct Columns {
             return __builtin_bit_cast(bf16x8_t, v);
         };
         const bf16x2_t ones = {(__bf16)1.0f, (__bf16)1.0f};
-        u32x4 p[4];                   // weights of 16 keys each
+        u32x4 p[2 * KT];              // weights of 16 keys each
         float odd = 0.0f, w[4];       // the last weights
         float arg = fmaf(s[0][0], c, -top);
-        const auto pair = [&](int e) {  // weights e and e + 1 of 64: rounded, and added
+        const auto pair = [&](int e) {  // weights e and e + 1: rounded, and added
             const uint32_t both = pack2(w[e & 3], w[(e & 3) + 1]);
             p[e / 16 * 2 + e % 16 / 8][e % 8 / 2] = both;
             float &to = e & 2 ? odd : sum;
             to = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, both), ones, to, false);
         };
-        const auto weigh_one = [&](int e) {  // weight e of 32; the pair before it where it begins a new one
+        const auto weigh_one = [&](int e) {  // weight e; the pair before it where it begins a new one
             w[e & 3] = __builtin_amdgcn_exp2f(arg);
-            if (e < 31) arg = fmaf(s[(e + 1) / 16][(e + 1) % 16], c, -top);
+            if (e + 1 < ALL) arg = fmaf(s[(e + 1) / 16][(e + 1) % 16], c, -top);
             if (e >= 2 && !(e & 1)) pair(e - 2);
         };
         bf16x8_t ring[RING];
@@ -465,31 +468,34 @@ struct Columns {
 #pragma unroll
         for (int j = 0; j < QK; j++) {
             ring[(j + RING - 1) % RING] = j + RING - 1 < QK ? key(j + RING - 1) : value(j + RING - 1 - QK);
-            f32x16 from = next[j & 1];
-            if (j < 2)
+            f32x16 from = next[j % KT];
+            if (j < KT)
 #pragma unroll
                 for (int e = 0; e < 16; e++) from[e] = 0.0f;
-            next[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[j % RING], __builtin_bit_cast(bf16x8_t, q[j / 2]),
-                                                                  from, 0, 0, 0);
+            next[j % KT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[j % RING], __builtin_bit_cast(bf16x8_t, q[j / KT]),
+                                                                   from, 0, 0, 0);
 #pragma unroll
             for (int e = 16 * j / QK; e < 16 * (j + 1) / QK; e++) weigh_one(e);
-            if (j & 1) bring(j / 2);
+            if (j & 1) bring(j / 2);  // QK / 2 of them
             __builtin_amdgcn_sched_barrier(0);
         }
+        if (KT == 1) pair(14);
         float peak = LOWEST;
+        constexpr int FIRST = KT == 1 ? 0 : PV / 2;  // products beside the last weights; then the maximum
 #pragma unroll
         for (int j = 0; j < PV; j++) {
             if (j + RING - 1 < PV) ring[(QK + j + RING - 1) % RING] = value(j + RING - 1);
             f32x16 &to = o[j % (D / 32)];
             to = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ring[(QK + j) % RING], __builtin_bit_cast(bf16x8_t, p[j / (D / 32)]),
                                                          to, 0, 0, 0);
-            if (j < PV / 2) {
+            if (j < FIRST) {
 #pragma unroll
                 for (int e = 32 * j / PV; e < 32 * (j + 1) / PV; e++) weigh_one(16 + e);
             } else {
-                if (j == PV / 2) pair(30);
+                if (KT == 2 && j == FIRST) pair(30);
 #pragma unroll
-                for (int e = 64 * j / PV - 32; e < 64 * (j + 1) / PV - 32; e++) peak = fmaxf(peak, next[e / 16][e % 16]);
+                for (int e = ALL * (j - FIRST) / (PV - FIRST); e < ALL * (j + 1 - FIRST) / (PV - FIRST); e++)
+                    peak = fmaxf(peak, next[e / 16][e % 16]);
                 asm volatile("" : "+v"(peak));
             }
             __builtin_amdgcn_sched_barrier(0);
@@ -681,9 +687,10 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
 // each wave, with one barrier per NK keys.
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
-    constexpr int NK = 64, KT = NK / 32, BYTES = NK * 2 * D;
+    constexpr int NK = D == 256 ? 32 : 64, KT = NK / 32, BYTES = NK * 2 * D;
     typedef Pages<D, NK / 4, NK, WHOLE> P;
     constexpr int LOADS = P::LOADS;
+    static_assert(2 * LOADS == KT * D / 32, "as many loads as Columns::step asks for");
     const int w = wave_id(), lane = threadIdx.x & 63;
     const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
     Tile t;
@@ -787,11 +794,14 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
         if (!plain) {
 #pragma unroll
             for (int k = 0; k < KT; k++) {
-                uint32_t here;
-                if constexpr (WHOLE)
-                    here = (there >> (2 * k) & 1 ? 0xffffu : 0) | (there >> (2 * k + 1) & 1 ? 0xffff0000u : 0);
-                else
-                    here = space.present[B][2 * k] | space.present[B][2 * k + 1] << 16;
+                uint32_t here = 0;
+                constexpr int PARTS = 32 / QUARTER;  // waves whose rows make 32
+#pragma unroll
+                for (int v = 0; v < PARTS; v++) {
+                    const uint32_t rows = WHOLE ? there >> (k * PARTS + v) & 1 ? (1u << QUARTER) - 1 : 0
+                                                : space.present[B][k * PARTS + v];
+                    here |= rows << (v * QUARTER);
+                }
                 hide(s[k], c.sees(at + 32 * k, window) & here);
             }
             peak = c.peak(s, scale);
