@@ -62,8 +62,9 @@ struct Values {
 // One workgroup per slice of a row's vocabulary. The row's history is read once by every slice (from L2 after
 // the first); the slice's tokens are counted in LDS, by whole numbers, so that the order of the additions does
 // not matter. Then eight logits per thread at a time, 16 bytes where the rows' alignment allows it. Bound by the
-// logits' bytes in flight where there are many rows, so LDS per token is kept small and slices large; one row by
-// the launch and two round trips to memory.
+// logits' bytes in flight where there are many rows, so LDS per token is kept small and slices large (64 rows of
+// 151936, up to 8192 tokens and 300 biases: 19.1 us, 2.2 TB/s; with a word for each count and each bias 24); one row
+// by the launch and two round trips to memory (4.9 us).
 // NARROW: counts of 16 bits instead of 32, for histories that cannot count further.
 // DENSE: a word per token for its bias, for any number of biases: entry i leaves -(i + 1) there if that is the
 // least, so the last entry of a token stays, and then puts its value there. As floats those numbers are NaN,

@@ -566,7 +566,12 @@ struct Space {
 // One token, or a few, over a long history: bound by the bytes of the keys and values. A workgroup takes a
 // split's keys, each of its four waves a quarter of them with the same 32 columns and buffers of its own, so
 // nothing waits between waves until their outputs are joined. A wave keeps 32 keys' rows and 32 values' rows in
-// LDS: the next keys are requested once the scores are formed and the next values once they are summed.
+// LDS: the next keys are requested once the scores are formed and the next values once they are summed, so
+// that eight waves of a CU have about 100 KB under way. The columns that hold no row are multiplied all the same: the
+// matrix unit is idle most of the time here, which also pays for the weights' remainders (EXACT).
+// 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 216 us with the join, 5.1 TB/s of keys and values (a
+// 2 GiB copy: 4.8); one token over 40960: 28 us and a join of 6; one over 261, 16 heads on 8: 8 us, which are the
+// launch, the sequence's and the page's lookups and three steps of a wave one after the other.
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int ROWS = 32, BYTES = ROWS * 2 * D;
@@ -684,7 +689,13 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
 
 // A chunk of new tokens: bound by the matrix products. The four waves of a workgroup take 32 columns each and
 // share the keys and values in LDS, two buffers of NK rows: while one is used the other is filled, a quarter by
-// each wave, with one barrier per NK keys.
+// each wave, with one barrier per NK keys. Two workgroups share a CU (heads of 256: one), so that one's products
+// run beside the other's lookups and barriers.
+// 2048 tokens after 6144, 32 heads on 8 of 128: 237 us, 1.02 PFLOP/s (a product of two 8192 x 8192 matrices: 1.2, of
+// larger ones 1.37). What bounds it then is power: the clock falls to 1.75 GHz, and the same call on zeros takes
+// 199 us at 2.35. Of the 240 us, without the loads into LDS 30 less, without the softmax 20 less. Two groups of 32
+// columns per wave would halve the LDS reads, but need the second half of the register file, which vector
+// instructions cannot use: 453 us. Heads of 64: 152 us for the same rows, bound by the softmax's vector work.
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int NK = D == 256 ? 32 : 64, KT = NK / 32, BYTES = NK * 2 * D;
