@@ -136,12 +136,22 @@ __device__ __forceinline__ constexpr int swizzle(int r) {
 
 // 64 lanes' 16 bytes from base + offset into LDS at `to` on, without passing registers. The wave waits for
 // it with wait_loads: the compiler does not know of it.
+// STREAM: read non-temporally, what one workgroup alone reads (64 tokens over up to 8448 positions 216 -> 195 us).
+template <bool STREAM>
 __device__ __forceinline__ void load_to_lds(unsigned to, const void *base, unsigned offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
-                 : "memory");
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(offset), "s"(base)
+                     : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base)
+                     : "memory");
 }
+template <bool STREAM>
 __device__ __forceinline__ void load_to_lds(unsigned to, const void *at) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(to), "v"(at) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
 }
 // A wave-uniform value in scalar registers.
 __device__ __forceinline__ int64_t uniform(int64_t x) {
@@ -159,7 +169,7 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // not there read the pool's first rows (the scores' mask leaves them out).
 // WHOLE: the 16 positions from a multiple of 16 on lie in one page, so a place is looked up once for them, 64
 // at a time, one per lane; otherwise every position's place is looked up, 128 at a time, into LDS.
-template <int D, int ROWS, int STEP, bool WHOLE>
+template <int D, int ROWS, int STEP, bool WHOLE, bool STREAM>
 struct Pages {
     static constexpr int PER = 512 / D;        // rows per load
     static constexpr int LOADS = ROWS / PER;   // of keys, and as many of values
@@ -230,10 +240,10 @@ struct Pages {
     // Load i of the step's rows into LDS at `to` (where load 0 goes); from: base() of the load's group.
     __device__ __forceinline__ void load(const char *from, int step, int i, unsigned to) const {
         if constexpr (WHOLE) {
-            load_to_lds(to + i * 1024, from, offset[i % GROUP_LOADS]);
+            load_to_lds<STREAM>(to + i * 1024, from, offset[i % GROUP_LOADS]);
         } else {
             const int64_t at = places[step % AHEAD * ROWS + i * PER + (threadIdx.x & 63) / (D / 8)];
-            load_to_lds(to + i * 1024, from + (at < 0 ? head : at) + offset[i % GROUP_LOADS]);
+            load_to_lds<STREAM>(to + i * 1024, from + (at < 0 ? head : at) + offset[i % GROUP_LOADS]);
         }
     }
     // All loads of the step's rows of one cache.
@@ -569,13 +579,13 @@ struct Space {
 // LDS: the next keys are requested once the scores are formed and the next values once they are summed, so
 // that eight waves of a CU have about 100 KB under way. The columns that hold no row are multiplied all the same: the
 // matrix unit is idle most of the time here, which also pays for the weights' remainders (EXACT).
-// 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 216 us with the join, 5.1 TB/s of keys and values (a
-// 2 GiB copy: 4.8); one token over 40960: 28 us and a join of 6; one over 261, 16 heads on 8: 8 us, which are the
+// 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 195 us with the join, 5.6 TB/s of keys and values (a
+// 2 GiB copy: 4.8); one token over 40960: 36 us with a join of 6; one over 261, 16 heads on 8: 8 us, which are the
 // launch, the sequence's and the page's lookups and three steps of a wave one after the other.
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int ROWS = 32, BYTES = ROWS * 2 * D;
-    typedef Pages<D, ROWS, ROWS, WHOLE> P;
+    typedef Pages<D, ROWS, ROWS, WHOLE, true> P;
     constexpr int LOADS = P::LOADS;
     const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
     const int w = wave_id(), lane = threadIdx.x & 63;
@@ -699,7 +709,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int NK = D == 256 ? 32 : 64, KT = NK / 32, BYTES = NK * 2 * D;
-    typedef Pages<D, NK / 4, NK, WHOLE> P;
+    typedef Pages<D, NK / 4, NK, WHOLE, false> P;
     constexpr int LOADS = P::LOADS;
     static_assert(2 * LOADS == KT * D / 32, "as many loads as Columns::step asks for");
     const int w = wave_id(), lane = threadIdx.x & 63;
