@@ -880,8 +880,9 @@ __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z
 // ------------------------------------------------------------------------------------------
 
 // Workgroups of many rows first: they take longest, and those of few rows, where there are any, fill up beside
-// them (a chunk of 511 after 4095 and another beside 20 single tokens, 16 heads on 8: many first 55 us, in
-// turns 71, few first 69; two windowed chunks and no few rows, whose empty workgroups then come last: 34 / 45 / 34).
+// them. (Kinds in turns put the few ones first into the places there are: two chunks beside 20 single tokens 71 us
+// against 55, with warm caches; two windowed chunks, whose batch then had empty workgroups of few rows in
+// between, 45 against 34.)
 template <int D, bool WHOLE>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArgs l) {
     __shared__ Space<D, WHOLE> space;
@@ -1001,10 +1002,11 @@ struct Plan {
     size_t few_rows, many_rows, floats;  // rows of partial outputs
 
     // A join costs 2 to 3 us, what a workgroup takes for about 640 keys alone (one token, 32 heads on 8, 511 / 1023
-    // / 8191 / 40959 positions: unsplit 8.6 / 12.3 / 64.6 / 425 us, 128 keys or 256 workgroups 9.5 / 10.0 / 16.1 /
-    // 39.7, 512 workgroups 9.6 / 10.1 / 17.8 / 41.3). Sequences of unequal length gain from twice the workgroups
-    // (4 sequences up to 8000 20.4 / 20.4), and from pieces of 1024 keys, or 2048 where there are enough of those
-    // (16 up to 8000, pieces of 2048 / 1024: 67.5 / 60.5; 64 up to 8447, whole / 2048 / 1024: 234 / 216 / 219).
+    // / 8191 / 40959 positions: unsplit 8.6 / 14.8 / 86.7 / 421 us, 128 keys or 256 workgroups 9.5 / 10.7 / 16.0 /
+    // 36.0, 512 workgroups 9.6 / 10.8 / 17.4 / 37.2). Sequences of unequal length gain from twice the workgroups
+    // (4 of up to 8000, 256 / 512: 22.3 / 23.0), and from pieces of 1024 keys, or 2048 where there are enough of
+    // those (16 of up to 8000, pieces of 2048 / 1024: 62.5 / 54.6; 64 of up to 8447, whole / 2048 / 1024: 217 / 195
+    // / 195).
     static int64_t few_splits(int64_t units, int n_seqs, int64_t span) {
         if (span <= 640) return 1;
         const int64_t target = n_seqs > 1 ? 2 * CUS : CUS, piece = units <= CUS ? 1024 : 2048;
@@ -1013,16 +1015,18 @@ struct Plan {
     }
 
     // The least of an estimate in ns: a workgroup's keys, alone on a CU or two to one, the parts' bytes written and
-    // read, and the join's launch. Beside workgroups of few rows at most `most`.
+    // read, and the join's launch. Beside workgroups of few rows at most `most`. (32 heads on 8 of 128, in 1 / 2 / 4 /
+    // 8 / 16 splits: 64 tokens after 8000 131 / 76 / 47 / 35 / 40 us, 512 after 8000 141 / 113 / 85 / 98 / 114, 1024
+    // after none 27 / 35 / 42 / 57 / 57.)
     static int64_t many_splits(int64_t units, int head_dim, int64_t span, int64_t most) {
         int64_t best = 1;
         double least = 0;
         for (int64_t n = 1; n <= std::min<int64_t>(most, (span + 127) / 128); n++) {
             const double groups = (double)units * n, keys = (double)((span + n - 1) / n);
             const double key = head_dim == 256 ? 47.0 * std::max(1.0, groups / CUS)
-                                               : (groups <= CUS ? 24.0 : 35.0 * std::max(1.0, groups / (2 * CUS))) *
+                                               : (groups <= CUS ? 17.5 : 28.0 * std::max(1.0, groups / (2 * CUS))) *
                                                      (head_dim + 64) / 192;
-            const double cost = keys * key + (n > 1 ? 4000 + groups * 128 * (head_dim + 2) * 8 / 4000 : 0);
+            const double cost = keys * key + (n > 1 ? 4000 + groups * 128 * (head_dim + 2) * 8 / 2660 : 0);
             if (n == 1 || cost < least) best = n, least = cost;
         }
         return best;
@@ -1053,9 +1057,9 @@ struct Plan {
                 if (window == 0) break;
             }
         };
-        // Workgroups of few rows need places of their own beside those of many: the mixed step above, 88 tiles x kv
-        // heads in 1 / 2 / 3 / 4 / 6 splits 115 / 84 / 70 / 76 / 84 us; 64 single tokens of up to 8000 beside one
-        // chunk, 128 in 1 / 2 / 3 / 4 276 / 267 / 288 / 310.
+        // Workgroups of few rows need places of their own beside those of many: chunks of 511 and 71 after up to 4095
+        // beside 20 single tokens, 16 heads on 8, in 1 / 2 / 3 / 4 / 6 splits 98 / 74 / 65 / 68 / 77 us; 64 single
+        // tokens of up to 8000 beside a chunk of 511, 32 on 8, in 1 / 2 / 3 / 4 245 / 236 / 258 / 276.
         const int64_t units = (rows + MANY - 1) / MANY * n_kv_heads, most = few ? std::max<int64_t>(1, 288 / units) : 64;
         cut(FEW, [&](int64_t span) { return few_splits((int64_t)n_seqs * n_kv_heads, n_seqs, span); }, few_split, few_chunk);
         cut(MANY, [&](int64_t span) { return many_splits(units, head_dim, span, most); },
