@@ -431,7 +431,8 @@ def swiglu_forward(act, gate, up, n, stream=None):
 
 
 # ---- serving operators over a paged KV cache (include/llm_amd/paged.h). They take tensors alone and
-# read every size and stride from them ----
+# read every size and stride from them. With a `stream` other than the current one the caller keeps the
+# tensors, as they are, until the work on it is done: torch hands a dropped tensor's memory out again ----
 
 ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2
 

@@ -649,6 +649,7 @@ def test_two_captured_graphs_and_streams(gpu):
         for _, out, want, args in made:
             assert torch.equal(bits(out), bits(want))
             out.fill_(3)
+            torch.cuda.synchronize()
             gpu.attention_paged_forward(out, *args, stream=streams[0])
             torch.cuda.synchronize()
             assert torch.equal(bits(out), bits(want))
@@ -780,17 +781,18 @@ def test_native_and_general_way_are_one(gpu, monkeypatch):
             q_out = torch.zeros(b.tokens, 4, 64, device="cuda", dtype=torch.int16)
             out, z = torch.zeros_like(q_out, dtype=torch.bfloat16), torch.zeros_like(x)
             ws = workspace(gpu, b, 4, 40, 9000)
+            where, bias = b.where(), ids.float()  # kept until the other stream has read them
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
-            gpu.qk_norm_rope_paged(q_out, rows[:, :4], rows[:, 4:6], rows[:, 6:], norm, norm, f, kc, vc, *b.where(), 1e-5,
+            gpu.qk_norm_rope_paged(q_out, rows[:, :4], rows[:, 4:6], rows[:, 6:], norm, norm, f, kc, vc, *where, 1e-5,
                                    1.5, True, side)
-            gpu.attention_paged_forward(out, q_out, kc, vc, *b.where(), ws, 0.25, 40, 9000, window=60, stream=side.cuda_stream)
-            gpu.logits_penalty_forward(z, x, ids, n, n, bias_tokens=ids, bias=ids.float(), stream=side)
+            gpu.attention_paged_forward(out, q_out, kc, vc, *where, ws, 0.25, 40, 9000, window=60, stream=side.cuda_stream)
+            gpu.logits_penalty_forward(z, x, ids, n, n, bias_tokens=ids, bias=bias, stream=side)
             torch.cuda.synchronize()
             refusals = []
-            for call in (lambda: gpu.attention_paged_forward(out, q_out, kc, vc, *b.where(), ws, 1, 40, 9000, -1),
-                         lambda: gpu.attention_paged_forward(out, q_out, kc, vc, *b.where(), None, 0.1, 40, 9000),
-                         lambda: gpu.qk_norm_rope_paged(q_out, rows[:, :4], rows[:, 4:6], rows[:, 6:], None, None, f[:4], kc, vc, *b.where(), 1e-5),
+            for call in (lambda: gpu.attention_paged_forward(out, q_out, kc, vc, *where, ws, 1, 40, 9000, -1),
+                         lambda: gpu.attention_paged_forward(out, q_out, kc, vc, *where, None, 0.1, 40, 9000),
+                         lambda: gpu.qk_norm_rope_paged(q_out, rows[:, :4], rows[:, 4:6], rows[:, 6:], None, None, f[:4], kc, vc, *where, 1e-5),
                          lambda: gpu.logits_penalty_forward(z, x[:, :1000], ids, n, n)):
                 with pytest.raises(gpu.LlmError) as e:
                     call()
