@@ -530,8 +530,9 @@ struct Columns {
             float dot = 0.0f;
 #pragma unroll 1
             for (int d = 0; d < D; d += 8) dot = dot8(ld16(query + d), ld16(k + d), dot);
-            const float weight = __builtin_amdgcn_exp2f(fmaf(dot, a.scale_log2, -top));
             const bool seen = p <= position && (a.window <= 0 || p > position - a.window);
+            // what a row does not see weighs 0 even where its score is no number
+            const float weight = seen ? __builtin_amdgcn_exp2f(fmaf(dot, a.scale_log2, -top)) : 0.0f;
 #pragma unroll
             for (int d = 0; d < D / 32; d++)
 #pragma unroll

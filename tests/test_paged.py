@@ -374,6 +374,24 @@ def test_attention_bad_values_stay_with_the_rows_that_see_them(gpu, seqs, window
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs,window,dim", [([(4, 60), (1, 30)], 0, 128), ([(4, 60), (30, 90)], 9, 64),
+                                             ([(200, 230)], 0, 128), ([(200, 230)], 30, 256)])
+@pytest.mark.parametrize("key", [math.nan, 1e38, 20.0])
+def test_attention_bad_keys_with_bad_values(gpu, seqs, window, dim, key):
+    """A key and a value that are no numbers at one position, or a key far ahead of every other there: rows
+    that do not see it are what they are without it."""
+    heads, kv_heads = 4, 2
+    b = Batch(seqs, kv_heads, dim, 16, 12)
+    q = b.normal(b.tokens, heads, dim).abs()
+    for s, (new, n) in enumerate(seqs):
+        for p in (n - 1, n - 3, n - new // 2, n - 26):
+            b.k[b.slot(s, p)] = key
+            b.v[b.slot(s, p)] = math.nan
+    scale = 1 / math.sqrt(dim)
+    check_attend(b, attend(gpu, b, q, scale, window), q, scale, window)
+
+
+@pytest.mark.gpu
 def test_attention_scores_of_minus_infinity(gpu):
     """A score of -inf weighs nothing; a row of none but those gives zeros, as one that sees nothing."""
     b = Batch([(1, 40), (70, 90), (1, 30)], 2, 64, 16, 13)
