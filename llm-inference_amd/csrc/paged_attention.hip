@@ -1140,6 +1140,7 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
         llm_fail("%s: window %d is negative", name, window);
         return;
     }
+    if (window >= 1 << 30) window = 0;  // past every position; positions less the window then stay in range
     if (!(scale > 0.0f) || !isfinite(scale)) {
         llm_fail("%s: scale %g is not positive and finite", name, (double)scale);
         return;

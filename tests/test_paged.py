@@ -323,6 +323,16 @@ def test_attention_whatever_the_expected_lengths(gpu, case, max_q, max_kv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs", [[(5, 2), (8, 3), (1, 40)], [(70, 40), (40, 7)]])
+@pytest.mark.parametrize("window", [2 ** 30 - 1, 2 ** 30, 2 ** 31 - 1])
+def test_attention_window_past_every_length(gpu, seqs, window):
+    """A window past any position is none, for rows whose positions are negative beside others too."""
+    b = Batch(seqs, 2, 64, 16, 21)
+    q = b.normal(b.tokens, 4, 64)
+    check_attend(b, attend(gpu, b, q, 0.125, window), q, 0.125, window)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs,dim,heads", [([(1, 9000)], 128, 4), ([(1, 70000), (1, 3)], 64, 2),
                                             ([(3, 5000), (1, 2500), (1, 1)], 256, 2), ([(150, 6000)], 128, 2)])
 def test_attention_long_histories(gpu, seqs, dim, heads):
