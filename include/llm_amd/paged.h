@@ -34,9 +34,9 @@ extern "C" {
 typedef struct {
     bf16 *key_cache;        /* 16-byte aligned */
     bf16 *value_cache;
-    int64_t page_stride;    /* elements, multiples of 8, not negative */
+    int64_t page_stride;    /* elements, multiples of 8, not negative; to be written into: at least head_dim */
     int64_t slot_stride;    /* at least head_dim, at most 2^26 */
-    int64_t head_stride;
+    int64_t head_stride;    /* like page_stride */
     const int *page_table;  /* [n_seqs, table_pages] */
     const int *q_start;     /* [n_seqs + 1] */
     const int *kv_len;      /* [n_seqs] */
@@ -65,8 +65,8 @@ float rope_frequencies(double *inv_freq, int rotary_dim, double theta, int kind,
  * row's place in the caches (q_out alone where the position is not there, negative ones included).
  * Pair j is the elements j and j + rotary_dim / 2 (interleaved 0) or 2j and 2j + 1 (1). inv_freq: device,
  * [rotary_dim / 2] doubles. q, k and v have rows of heads * head_dim elements q_stride, k_stride and
- * v_stride apart (multiples of 8), as slices of one q/k/v projection have; q_out likewise. q_out may be q;
- * nothing else may overlap. rotary_dim is a multiple of 16, at most head_dim. Two rows with one place in
+ * v_stride apart (multiples of 8), as slices of one q/k/v projection have; q_out likewise. q_out may be q,
+ * row on row; nothing else may overlap. rotary_dim is a multiple of 16, at most head_dim. Two rows with one place in
  * the cache leave either's k and v there, head by head. */
 void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, const bf16 *v,
                         const bf16 *q_norm_w, const bf16 *k_norm_w, const double *inv_freq,
@@ -102,7 +102,7 @@ size_t attention_paged_workspace_floats(int n_tokens, int n_seqs, int n_heads, i
  *   a token whose bit is 0 in `allowed` (bit t % 32 of word t / 32): x = -inf, whatever it was.
  * tokens: [rows, token_stride]; bias_tokens and bias: [rows, bias_stride]; allowed: [rows, allowed_stride]
  * words. prompt_len and token_len are counts within the row's token_stride entries, and bias_len within
- * bias_stride: what is outside is cut off. Tokens outside [0, vocab) are passed over. repetition, frequency and
+ * bias_stride (at most 2^22): what is outside is cut off. Tokens outside [0, vocab) are passed over. repetition, frequency and
  * presence: [rows], each NULL where it is off; tokens NULL: no history; bias_tokens NULL: no biases;
  * allowed NULL: no mask; prompt_len NULL: no prompt; bias_len NULL: all bias_stride entries. Rows of
  * logits and out are logits_stride and out_stride elements apart; out may be logits. */

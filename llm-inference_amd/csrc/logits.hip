@@ -268,6 +268,10 @@ extern "C" void logits_penalty_forward(bf16 *out, const bf16 *logits, const int 
         llm_fail("%s: biases need their values and a bias_stride that is not negative", name);
         return;
     }
+    if (bias_tokens && bias_stride > 1 << 22) {  // more entries' numbers would meet the bits of -inf
+        llm_fail("%s: bias_stride %d is over 4194304", name, bias_stride);
+        return;
+    }
     if (allowed && allowed_stride < (vocab + 31) / 32) {
         llm_fail("%s: allowed_stride %d is under the %d words of %d tokens", name, allowed_stride,
                  (vocab + 31) / 32, vocab);

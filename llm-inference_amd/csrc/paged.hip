@@ -186,6 +186,16 @@ extern "C" void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, co
         !check_rows(name, "q", q, q_stride, q_width) || !check_rows(name, "k", k, k_stride, kv_width) ||
         !check_rows(name, "v", v, v_stride, kv_width))
         return;
+    if (q_out == q && q_out_stride != q_stride) {
+        llm_fail("%s: in place, the rows of q_out and q must be the same", name);
+        return;
+    }
+    // what is written must not lie on itself (as expanded tensors do)
+    if ((batch->n_kv_heads > 1 && batch->head_stride < D) || (batch->n_pages > 1 && batch->page_stride < D)) {
+        llm_fail("%s: pages %lld and kv heads %lld elements apart overlap (head_dim %d)", name,
+                 (long long)batch->page_stride, (long long)batch->head_stride, D);
+        return;
+    }
     a.q_out = q_out;
     a.q = q;
     a.k = k;

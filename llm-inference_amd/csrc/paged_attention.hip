@@ -1141,13 +1141,17 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
         return;
     }
     if (window >= 1 << 30) window = 0;  // past every position; positions less the window then stay in range
-    if (!(scale > 0.0f) || !isfinite(scale)) {
+    if (!(scale > 0.0f) || !isfinite(scale * 1.44269504f)) {
         llm_fail("%s: scale %g is not positive and finite", name, (double)scale);
         return;
     }
     const int D = batch->head_dim;
     const int64_t width = (int64_t)n_heads * D;
     if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width)) return;
+    if (out == q) {
+        llm_fail("%s: out must not be q, which is read again", name);
+        return;
+    }
     const Plan plan(n_tokens, batch->n_seqs, n_heads, batch->n_kv_heads, D, max_q_len, max_kv_len, window);
     if (plan.few_units * plan.few_split + plan.many_units * plan.many_split > INT32_MAX / 64) {
         llm_fail("%s: %d rows in %d sequences of up to %d tokens are too many for one launch", name, n_tokens,

@@ -248,6 +248,15 @@ def test_in_place_needs_one_stride(pkg):
     assert L.llm_last_error() is None
 
 
+def test_too_many_biases_are_refused(pkg):
+    p, L = 0x1000, pkg.lib()
+    L.llm_clear_error()
+    L.logits_penalty_forward(p, p, p, p, p, p, p, p, p, p, p, p, 2, 1000, 8, (1 << 22) + 1, 32, 1000, 1000, None)
+    got = L.llm_last_error()
+    L.llm_clear_error()
+    assert got and "bias_stride 4194305" in got.decode()
+
+
 @pytest.mark.gpu
 def test_wrapper_refusals(gpu):
     import torch

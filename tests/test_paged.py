@@ -746,6 +746,21 @@ def test_attention_refusals(pkg, at, value, message):
     assert message in refused(pkg, "attention_paged_forward", *args)
 
 
+def test_append_where_it_would_write_over_itself(pkg):
+    p = 0x1000
+    for change in (dict(head_stride=56), dict(head_stride=0), dict(page_stride=0)):
+        assert "overlap" in refused(pkg, "qk_norm_rope_paged", p, p, p, p, None, None, p, ctypes.byref(record(pkg, **change)),
+                                    4, 4, 64, 0, 1e-6, 1.0, 256, 256, 128, 128, None)
+    assert "in place" in refused(pkg, "qk_norm_rope_paged", p, p, p, p, None, None, p, ctypes.byref(record(pkg)),
+                                 4, 4, 64, 0, 1e-6, 1.0, 264, 256, 128, 128, None)
+
+
+def test_attention_in_place_and_overflowing_scales_are_refused(pkg):
+    p, b = 0x1000, ctypes.byref(record(pkg))
+    assert "out must not be q" in refused(pkg, "attention_paged_forward", p, p, b, p, 4, 4, 1, 100, 0, 0.1, 256, 256, None)
+    assert "not positive and finite" in refused(pkg, "attention_paged_forward", 0x9000, p, b, p, 4, 4, 1, 100, 0, 3e38, 256, 256, None)
+
+
 def test_no_rows_is_no_launch(pkg):
     p, b = 0x1000, record(pkg)
     assert refused(pkg, "qk_norm_rope_paged", p, p, p, p, None, None, p, ctypes.byref(b), 0, 4, 64, 0, 1e-6, 1.0,
