@@ -1148,10 +1148,6 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
     const int D = batch->head_dim;
     const int64_t width = (int64_t)n_heads * D;
     if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width)) return;
-    if (out == q) {
-        llm_fail("%s: out must not be q, which is read again", name);
-        return;
-    }
     const Plan plan(n_tokens, batch->n_seqs, n_heads, batch->n_kv_heads, D, max_q_len, max_kv_len, window);
     if (plan.few_units * plan.few_split + plan.many_units * plan.many_split > INT32_MAX / 64) {
         llm_fail("%s: %d rows in %d sequences of up to %d tokens are too many for one launch", name, n_tokens,
@@ -1160,6 +1156,10 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
     }
     if (!aligned16(ws) || (plan.floats && !ws)) {
         llm_fail("%s: ws must be a 16-byte aligned device address", name);
+        return;
+    }
+    if (out == q) {
+        llm_fail("%s: out must not be q, which is read again", name);
         return;
     }
     a.out = out;
