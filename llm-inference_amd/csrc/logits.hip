@@ -61,25 +61,25 @@ struct Values {
 
 // One workgroup per slice of a row's vocabulary. The row's history is read once by every slice (from L2 after
 // the first); the slice's tokens are counted in LDS, by whole numbers, so that the order of the additions does
-// not matter. Then eight logits per thread at a time, 16 bytes where the rows' alignment allows it. Bound by the
-// logits' bytes in flight where there are many rows, so LDS per token is kept small and slices large (64 rows of
-// 151936, up to 8192 tokens and 300 biases: 19.1 us, 2.2 TB/s; with a word for each count and each bias 24); one row
-// by the launch and two round trips to memory (4.9 us).
+// not matter. Then eight logits per thread at a time, 16 bytes where the rows' alignment allows it. 64 rows of
+// 151936, up to 8192 tokens and 300 biases: 15.6 us, 2.6 TB/s, of which the history takes 1.6 and the biases 2; what
+// bounds it is one phase of a workgroup waiting for the other (all logits requested in front of the history
+// instead of the first eight per thread: 21.0 against 19.9 then); one row by the launch and two round trips to
+// memory (4.9 us).
 // NARROW: counts of 16 bits instead of 32, for histories that cannot count further.
 // DENSE: a word per token for its bias, for any number of biases: entry i leaves -(i + 1) there if that is the
 // least, so the last entry of a token stays, and then puts its value there. As floats those numbers are NaN,
 // which no value put there is, so no other entry can take a value for its number. Otherwise, for up to T biases,
-// a bit per token, and the values in the order of their tokens: a token's place is the number of bits before
-// its own.
+// a bit per token, and a token's last entry in the first of 2 T places from its own on that no other token has
+// (in the order of the tokens instead, found by counting bits, with three barriers more, 19.9 us instead of 17.4).
 template <bool NARROW, bool DENSE>
 __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
     extern __shared__ uint32_t lds[];
     constexpr int PER = NARROW ? 2 : 1;  // tokens per word of the counts
     constexpr int WORD = DENSE ? 1 : 32;  // tokens per word of the biases
-    constexpr int LISTED = DENSE ? 1 : T;
-    __shared__ __align__(16) int entries[LISTED], ids[LISTED];
-    __shared__ int listed, before[LISTED], totals[T / 64];
-    __shared__ float sorted[LISTED];
+    constexpr int PLACES = DENSE ? 1 : 2 * T;
+    __shared__ uint32_t placed[PLACES];
+    __shared__ float values[DENSE ? 1 : T];
     const int r = blockIdx.y, t0 = blockIdx.x * a.slice, n = min(a.slice, a.vocab - t0);
     uint32_t *met = lds, *biased = lds + (a.tokens ? a.slice / PER : 0);
     const bf16 *from = a.x + r * a.x_stride + t0;
@@ -124,8 +124,7 @@ __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
     const auto in_slice = [&](int token) { return (unsigned)token - (unsigned)t0 < (unsigned)n; };
     const int clear = (a.tokens ? a.slice / PER : 0) + (a.bias_tokens ? a.slice / WORD : 0);
     for (int i = 4 * threadIdx.x; i < clear; i += 4 * T) *(u32x4 *)(lds + i) = u32x4{0, 0, 0, 0};
-    if (threadIdx.x == 0) listed = 0;
-    if (!DENSE) ids[threadIdx.x] = -1;
+    if (!DENSE && a.bias_tokens) placed[threadIdx.x] = placed[threadIdx.x + T] = 0;
     __syncthreads();
     if (history)
         tokens.each(history, [&](int i, int token) {
@@ -149,36 +148,17 @@ __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
             const float v = gptr(bias)[i];
             *at = v == v ? __float_as_uint(v) : 0x7fc00000u;
         }
-    } else if (biases) {
-        const int t = bias_token - t0, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-        bool mine = (int)threadIdx.x < biases && in_slice(bias_token);
-        if (mine) {
-            atomicOr(&biased[t / 32], 1u << (t % 32));
-            const int at = atomicAdd(&listed, 1);
-            entries[at] = threadIdx.x;
-            ids[at] = t;
+    } else if ((int)threadIdx.x < biases && in_slice(bias_token)) {
+        const int t = bias_token - t0;
+        values[threadIdx.x] = value;
+        atomicOr(&biased[t / 32], 1u << (t % 32));
+        const uint32_t entry = (uint32_t)t << 16 | (threadIdx.x + 1);
+        for (uint32_t at = t;; at++) {  // ends: there are more places than entries
+            const uint32_t there = atomicCAS(&placed[at % PLACES], 0, entry);
+            if (there && there >> 16 != (uint32_t)t) continue;
+            if (there) atomicMax(&placed[at % PLACES], entry);
+            break;
         }
-        __syncthreads();
-        for (int k = 0; k < listed; k += 4) {  // is there a later one of the same token?
-            const u32x4 id = *(const u32x4 *)&ids[k], entry = *(const u32x4 *)&entries[k];
-#pragma unroll
-            for (int e = 0; e < 4; e++) mine = mine && ((int)id[e] != t || (int)entry[e] <= (int)threadIdx.x);
-        }
-        const int bits = (int)threadIdx.x < a.slice / 32 ? __popc(biased[threadIdx.x]) : 0;
-        int upto = bits;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int other = __shfl_up(upto, d);
-            if (lane >= d) upto += other;
-        }
-        if (lane == 63) totals[w] = upto;
-        __syncthreads();
-        int first = upto - bits;
-#pragma unroll
-        for (int v = 0; v < T / 64; v++) first += v < w ? totals[v] : 0;
-        before[threadIdx.x] = first;
-        __syncthreads();
-        if (mine) sorted[before[t / 32] + __popc(biased[t / 32] & ((1u << (t % 32)) - 1))] = value;
     }
     __syncthreads();
     for (int i = 8 * threadIdx.x; i < n; i += 8 * T) {
@@ -207,9 +187,12 @@ __global__ __launch_bounds__(T) void penalty_kernel(PenaltyArgs a) {
             const uint32_t all = biased[i / 32];
             if (all >> (i % 32) & 0xff) {
 #pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (all >> (i % 32 + e) & 1)
-                        y[e] += sorted[before[i / 32] + __popc(all & ((1u << (i % 32 + e)) - 1))];
+                for (int e = 0; e < 8; e++) {
+                    if (!(all >> (i % 32 + e) & 1)) continue;
+                    uint32_t at = i + e, entry = placed[at % PLACES];
+                    while (entry >> 16 != (uint32_t)(i + e)) entry = placed[++at % PLACES];  // it is there
+                    y[e] += values[(entry & 0xffff) - 1];
+                }
             }
         }
 #pragma unroll
@@ -277,9 +260,11 @@ extern "C" void logits_penalty_forward(bf16 *out, const bf16 *logits, const int 
                  (vocab + 31) / 32, vocab);
         return;
     }
-    // as large a slice as leaves workgroups enough: histories are read by fewer
     const bool narrow = token_stride < 1 << 15, dense = bias_tokens && bias_stride > T;
-    int slice = narrow && !dense ? 16384 : 4096;
+    // a slice's counts and biases in at most 48 KB of LDS; smaller ones where there are too few workgroups (64 rows
+    // of 151936, up to 8192 tokens and 300 biases, slices of 4096 / 8192 / 12288 / 16384: 17.1 / 15.6 / 16.4 / 16.9 us,
+    // with up to 40000 tokens 25.6 / 21.8 / 25.1; 16 rows, 2048 / 4096 / 8192: 8.7 / 8.0 / 8.4; one, 2048 / 4096: 4.6 / 4.4)
+    int slice = dense && !narrow ? 4096 : 8192;
     while (slice > 2048 && (int64_t)rows * ((vocab + slice - 1) / slice) < 512) slice /= 2;
     PenaltyArgs a = {out, logits, tokens, prompt_len, token_len, repetition, frequency, presence,
                      bias_tokens, bias, bias_len, allowed, vocab, token_stride, bias_stride,

@@ -110,6 +110,20 @@ def test_penalties_against_the_definition(gpu, rows, vocab, history, biases, mas
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 200])
+def test_biases_of_tokens_with_one_place(gpu, rows):
+    """Tokens whose biases begin their search at the same places, each several times, the first tokens of a
+    slice and the last among them."""
+    import torch
+    rng = np.random.default_rng(3)
+    logits = torch.randn(rows, 20000, device="cuda").bfloat16()
+    c = make(rng, rows, 20000, 50, 512, True)
+    near = np.concatenate([np.arange(0, 20000, 1024), np.arange(1023, 20000, 1024), np.arange(1022, 20000, 2048), [8191, 8192]])
+    c["bias_tokens"] = rng.choice(near, (rows, 512)).astype(np.int32)
+    check(run(gpu, logits, c), logits, c)
+
+
+@pytest.mark.gpu
 def test_a_long_history_of_few_tokens(gpu):
     import torch
     rng = np.random.default_rng(1)
