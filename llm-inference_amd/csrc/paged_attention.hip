@@ -890,11 +890,12 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArg
     const bool many = (int)blockIdx.x < l.many_groups;
     const int i = blockIdx.x - (many ? 0 : l.many_groups);
     if (many) {
+        // a unit's splits one after the other, so that tiles that are not there come last
         // where the device holds all of these workgroups at once, two to a CU, the second of a CU is as much
         // shorter as its first is longer
-        int unit = i % l.many_units;
+        int unit = i / l.many.n_split;
         if (l.mirrored && unit >= CUS) unit = l.many_units - 1 - (unit - CUS);
-        attend_many<D, WHOLE>(l.many, unit, i / l.many_units, space);
+        attend_many<D, WHOLE>(l.many, unit, i % l.many.n_split, space);
     } else {
         attend_few<D, WHOLE>(l.few, i % l.few_units, i / l.few_units, space);
     }
@@ -1031,19 +1032,21 @@ struct Plan {
             1, std::min((span + 127) / 128, std::max(target / units, n_seqs > 1 ? (span + piece - 1) / piece : 1)));
     }
 
-    // The least of an estimate in ns: a workgroup's keys, alone on a CU or two to one, the parts' bytes written and
-    // read, and the join's launch. Beside workgroups of few rows at most `most`. (32 heads on 8 of 128, in 1 / 2 / 4 /
-    // 8 / 16 splits: 64 tokens after 8000 131 / 76 / 47 / 35 / 40 us, 512 after 8000 141 / 113 / 85 / 98 / 114, 1024
-    // after none 27 / 35 / 42 / 57 / 57.)
+    // The least of an estimate in ns: a workgroup's keys (alone on a CU; beside another from CUS workgroups on; past
+    // two to a CU in turns), the parts' bytes written and read, and the join. Beside workgroups of few rows at most
+    // `most`. Over 123 shapes (33 to 2048 tokens after 0 to 16000, heads of 64, 128 and 256) what it chooses takes 0.4%
+    // longer than the best of those measured, at most 6%. (32 heads on 8 of 128, in 1 / 2 / 4 / 8 / 16 splits: 64 tokens
+    // after 6144 103 / 63 / 41 / 30 / 27 us, 512 after 6144 110 / 78 / 75 / 91 / 109, 1024 after none 28 / 38 / 53 / 51 / 51.)
     static int64_t many_splits(int64_t units, int head_dim, int64_t span, int64_t most) {
         int64_t best = 1;
         double least = 0;
         for (int64_t n = 1; n <= std::min<int64_t>(most, (span + 127) / 128); n++) {
             const double groups = (double)units * n, keys = (double)((span + n - 1) / n);
-            const double key = head_dim == 256 ? 47.0 * std::max(1.0, groups / CUS)
-                                               : (groups <= CUS ? 17.5 : 28.0 * std::max(1.0, groups / (2 * CUS))) *
-                                                     (head_dim + 64) / 192;
-            const double cost = keys * key + (n > 1 ? 4000 + groups * 128 * (head_dim + 2) * 8 / 2660 : 0);
+            const double shared = groups <= CUS       ? 1.0
+                                  : groups <= 2 * CUS ? 1.3 + 0.55 * (groups - CUS) / CUS
+                                                      : 1.85 * ceil(groups / (2 * CUS));
+            const double key = head_dim == 256 ? 39.0 * ceil(groups / CUS) : 16.3 * shared * (head_dim + 64) / 192;
+            const double cost = keys * key + (n > 1 ? 8000 + groups * 128 * (head_dim + 2) * 8 / 10000 : 0);
             if (n == 1 || cost < least) best = n, least = cost;
         }
         return best;
@@ -1059,9 +1062,12 @@ struct Plan {
         // after all is only slower there)
         const int64_t tokens = FEW / group, rest = n_tokens - n_seqs * tokens;
         few = !many || (n_seqs > 1 && rest <= (int64_t)(n_seqs - 1) * (max_q_len - tokens));
-        // at most one tile of a sequence is not full; one of many rows has over FEW of them
-        const int64_t few_tiles = many ? n_seqs : rows / FEW + std::min<int64_t>(n_seqs, rows);
-        const int64_t many_tiles = rows / MANY + (few ? std::min<int64_t>(n_seqs, rows / (FEW + 1)) : n_seqs);
+        // r rows of a sequence make at most (r + T - 1) / T tiles; one of many rows has over FEW. Empty workgroups
+        // between the others would put two of those on a CU and none on another (with one tile too many 512 tokens
+        // after 6144 in two splits 95 us instead of 78).
+        const int64_t few_tiles = many ? n_seqs : (rows + (FEW - 1) * std::min<int64_t>(n_seqs, rows)) / FEW;
+        const int64_t long_seqs = std::min<int64_t>(n_seqs, few ? rows / (FEW + 1) : rows);
+        const int64_t many_tiles = (rows + (MANY - 1) * long_seqs) / MANY;
         few_units = few ? few_tiles * n_kv_heads : 0;
         many_units = many ? many_tiles * n_kv_heads : 0;
         // a window shortens what the rows see; the workspace is asked for without it, so never more splits than then
