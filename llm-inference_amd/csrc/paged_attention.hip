@@ -580,8 +580,8 @@ struct Space {
 // LDS: the next keys are requested once the scores are formed and the next values once they are summed, so
 // that eight waves of a CU have about 100 KB under way. The columns that hold no row are multiplied all the same: the
 // matrix unit is idle most of the time here, which also pays for the weights' remainders (EXACT).
-// 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 195 us with the join, 5.6 TB/s of keys and values (a
-// 2 GiB copy: 4.8); one token over 40960: 36 us with a join of 6; one over 261, 16 heads on 8: 8 us, which are the
+// 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 192 us with the join, 5.7 TB/s of keys and values (a
+// 2 GiB copy: 4.8); one token over 40960: 34 us with a join of 5; one over 261, 16 heads on 8: 8 us, which are the
 // launch, the sequence's and the page's lookups and three steps of a wave one after the other.
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
@@ -702,7 +702,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
 // share the keys and values in LDS, two buffers of NK rows: while one is used the other is filled, a quarter by
 // each wave, with one barrier per NK keys. Two workgroups share a CU (heads of 256: one), so that one's products
 // run beside the other's lookups and barriers.
-// 2048 tokens after 6144, 32 heads on 8 of 128: 237 us, 1.02 PFLOP/s (a product of two 8192 x 8192 matrices: 1.2, of
+// 2048 tokens after 6144, 32 heads on 8 of 128: 227 to 244 us, 1.0 PFLOP/s (a product of two 8192 x 8192 matrices: 1.2, of
 // larger ones 1.37). What bounds it then is power: the clock falls to 1.75 GHz, and the same call on zeros takes
 // 199 us at 2.35. Of the 240 us, without the loads into LDS 30 less, without the softmax 20 less. Two groups of 32
 // columns per wave would halve the LDS reads, but need the second half of the register file, which vector
@@ -1022,12 +1022,12 @@ struct Plan {
     int few_split, few_chunk, many_split, many_chunk;
     size_t few_rows, many_rows, floats;  // rows of partial outputs
 
-    // A join costs 2 to 3 us, what a workgroup takes for about 640 keys alone (one token, 32 heads on 8, 511 / 1023
-    // / 8191 / 40959 positions: unsplit 8.6 / 14.8 / 86.7 / 421 us, 128 keys or 256 workgroups 9.5 / 10.7 / 16.0 /
-    // 36.0, 512 workgroups 9.6 / 10.8 / 17.4 / 37.2). Sequences of unequal length gain from twice the workgroups
-    // (4 of up to 8000, 256 / 512: 22.3 / 23.0), and from pieces of 1024 keys, or 2048 where there are enough of
-    // those (16 of up to 8000, pieces of 2048 / 1024: 62.5 / 54.6; 64 of up to 8447, whole / 2048 / 1024: 217 / 195
-    // / 195).
+    // A join costs 2 to 3 us, what a workgroup takes for about 600 keys alone (one token, 32 heads on 8, 511 / 1023 /
+    // 4095 positions: unsplit 10.2 / 15.6 / 44.8 us, in pieces of 128 keys 11.1 / 11.4 / 12.4; 40959 positions in 256
+    // workgroups 34.5, in 512 35.7). Several sequences, which may be of
+    // unequal length, take twice the workgroups (4 / 8 / 16 of up to 2000, 256 workgroups 14.0 / 16.3 / 22.7, 512 14.0 /
+    // 16.5 / 22.5), in pieces of 1024 keys, or 2048 where there are enough of those (16 of up to 8000, pieces of 2048 /
+    // 1024: 62.5 / 54.6; 64 of up to 8447, whole / 2048 / 1024: 217 / 195 / 195).
     static int64_t few_splits(int64_t units, int n_seqs, int64_t span) {
         if (span <= 640) return 1;
         const int64_t target = n_seqs > 1 ? 2 * CUS : CUS, piece = units <= CUS ? 1024 : 2048;
