@@ -78,7 +78,9 @@ void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, const bf16 *v
  * max(0, p - window + 1) .. p that are there (window 0: from 0 on), softmax(q . k * scale) over them, and
  * out is the weighted sum of their values. A row that sees nothing, or only scores of -inf, gives
  * zeros. What lies in the caches at positions that a row does not see, NaN and infinities included, does
- * not reach it. Scores, weights and sums are in 32 bits; in front of the values the weights are rounded to
+ * not reach it. A value that it sees and that is infinite makes its element infinite, or no number where its weight
+ * falls below the range of 32 bits; finite values overflow where their size times 2^8 times the number of
+ * positions passes that range. Scores, weights and sums are in 32 bits; in front of the values the weights are rounded to
  * bf16, with what that leaves added back where a sequence has at most 32 rows x heads per kv head (there the
  * bytes of the cache take longer than both products). Query head h reads kv head h / (n_heads / n_kv_heads). Rows of q and out are q_stride and
  * out_stride elements apart; out must not overlap anything. scale > 0.

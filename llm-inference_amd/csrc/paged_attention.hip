@@ -583,15 +583,15 @@ struct Space {
 // 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 192 us with the join, 5.7 TB/s of keys and values (a
 // 2 GiB copy: 4.8); one token over 40960: 34 us with a join of 5; one over 261, 16 heads on 8: 8 us, which are the
 // launch, the sequence's and the page's lookups and three steps of a wave one after the other.
-template <int D, bool WHOLE>
-__device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
+// EXACT: with remainders. The result is then whether an output of the workgroup came out infinite or as no number.
+// A remainder may be 0 or negative, and 0 or a negative number times an infinite value makes no number where the
+// weight itself makes an infinity: such a workgroup does all of it again without remainders.
+template <int D, bool WHOLE, bool EXACT>
+__device__ __forceinline__ bool few_rows(const AttendArgs &a, int kv, const Tile &t, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int ROWS = 32, BYTES = ROWS * 2 * D;
     typedef Pages<D, ROWS, ROWS, WHOLE, true> P;
     constexpr int LOADS = P::LOADS;
-    const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
     const int w = wave_id(), lane = threadIdx.x & 63;
-    Tile t;
-    if (!find_tile<FEW>(a, a.which, tile, t) || z >= t.active) return;
     const int begin = t.begin + z * a.chunk;
     const int end = z == a.n_split - 1 ? t.end : min(t.end, begin + a.chunk);
     const int steps = end > begin ? (end - begin + ROWS - 1) / ROWS : 0;
@@ -626,13 +626,13 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
         }
         c.raise(c.peak(s, a.scale_log2));
         u32x4 hi[2], lo[2];
-        c.template weigh<true>(s[0], a.scale_log2, hi, lo);
+        c.template weigh<EXACT>(s[0], a.scale_log2, hi, lo);
         if (more)
             wait_loads<LOADS>();
         else
             wait_loads<0>();
         if (edge) bad |= clear_unseen<D, LOADS>(values, at, here, t.from, t.to, t.least, t.most);
-        c.template add<true>(values, hi, lo);
+        c.template add<EXACT>(values, hi, lo);
         wait_lds();
         if (more) pages.request(a.b.vc, i + 1, value_at);
     }
@@ -645,6 +645,7 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
     // join the waves: each one's output, maximum and sum through LDS
     float x, y;
     swap_pair<32>(c.sum, x, y);
+    if (EXACT && threadIdx.x == 0) space.bad[0] = 0;  // the second time waves may still have to read it
     __syncthreads();
     if (lane < 32) {
         space.tops[w][lane] = c.top;
@@ -679,6 +680,11 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
 #pragma unroll
             for (int j = 0; j < 4; j++) o[j] = fmaf(f, e[j], o[j]);
         }
+        if constexpr (EXACT) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (!(fabsf(o[j]) < INFINITY)) space.bad[0] = 1;
+        }
         if (t.active > 1) {
             *gptr((f32x4 *)(a.part + (at + row) * D + 4 * k)) = o;
             if (k == 0) {
@@ -692,6 +698,17 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
                    o[1] * f, o[2] * f, o[3] * f);
         }
     }
+    if constexpr (!EXACT) return false;
+    __syncthreads();
+    return space.bad[0] != 0;
+}
+
+template <int D, bool WHOLE>
+__device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
+    const int tile = unit / a.n_kv_heads, kv = unit - tile * a.n_kv_heads;
+    Tile t;
+    if (!find_tile<FEW>(a, a.which, tile, t) || z >= t.active) return;
+    if (few_rows<D, WHOLE, true>(a, kv, t, unit, z, space)) few_rows<D, WHOLE, false>(a, kv, t, unit, z, space);
 }
 
 // ------------------------------------------------------------------------------------------

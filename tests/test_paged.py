@@ -384,6 +384,38 @@ def test_attention_bad_values_stay_with_the_rows_that_see_them(gpu, seqs, window
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("seqs,window,dim,page", [
+    ([(1, 1)], 0, 128, 16), ([(1, 40), (2, 70)], 0, 64, 16), ([(1, 300), (5, 300), (1, 33)], 40, 128, 5),
+    ([(1, 9000)], 0, 128, 64), ([(3, 5000), (1, 2500)], 0, 256, 16), ([(70, 200)], 0, 128, 16),
+    ([(40, 600), (1, 600)], 0, 64, 16), ([(150, 6000)], 200, 256, 64)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_attention_infinite_values_that_every_row_sees(gpu, seqs, window, dim, page, bad):
+    """An infinity among the values that all rows of a sequence see makes an infinity of its sign, both signs in
+    one element no number, and other elements are what they are without it: for few and for many rows, split or
+    not, whatever the position weighs (here down to e^-60)."""
+    import torch
+    heads, kv_heads, scale = 4, 2, 1 / math.sqrt(dim)
+    b = Batch(seqs, kv_heads, dim, page, 43)
+    q = b.normal(b.tokens, heads, dim)
+    q[:, :, 0] = 4.0
+    for s, (new, n) in enumerate(seqs):
+        seen = list(range(max(0, n - window) if window else 0, n - new + 1))  # by every row of the sequence
+        for p in seen[-3:]:
+            b.v[b.slot(s, p) + (0, 3)] = bad
+        b.v[b.slot(s, seen[-1]) + (1, dim - 1)] = bad
+        b.v[b.slot(s, seen[0]) + (1, dim // 2)] = bad
+        if len(seen) > 1:
+            b.v[b.slot(s, seen[0]) + (0, 9)], b.v[b.slot(s, seen[-1]) + (0, 9)] = bad, -bad
+            b.k[b.slot(s, seen[0]) + (1, 0)] = -15 / scale  # 60 below where it would be
+    out = attend(gpu, b, q, scale, window)
+    got, (want, err) = out.cpu().double().numpy(), attended(b, q, scale, window)
+    fine = np.isfinite(want)
+    assert 0 < (~fine).sum() < fine.size // 4
+    assert np.array_equal(got[~fine], want[~fine], equal_nan=True), "other infinities than the definition"
+    close(out.cpu()[torch.from_numpy(fine)], want[fine], err[fine])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("seqs,window,dim", [([(4, 60), (1, 30)], 0, 128), ([(4, 60), (30, 90)], 9, 64),
                                              ([(200, 230)], 0, 128), ([(200, 230)], 30, 256)])
 @pytest.mark.parametrize("key", [math.nan, 1e38, 20.0])
