@@ -93,7 +93,8 @@ void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBatch *batch, 
                              int n_tokens, int n_heads, int max_q_len, int max_kv_len, int window,
                              float scale, int64_t out_stride, int64_t q_stride, hipStream_t stream);
 
-/* Floats attention_paged_forward needs in ws for these sizes on the current device. */
+/* Floats of ws that attention_paged_forward needs at most for these sizes and for any with fewer n_tokens, n_seqs,
+ * max_q_len or max_kv_len (the heads being the same): one workspace for the largest serves every call. */
 size_t attention_paged_workspace_floats(int n_tokens, int n_seqs, int n_heads, int n_kv_heads,
                                         int head_dim, int max_q_len, int max_kv_len);
 

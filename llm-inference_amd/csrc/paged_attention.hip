@@ -1037,7 +1037,34 @@ struct Plan {
     bool few, many;
     int64_t few_units, many_units;  // tiles x kv heads, at most
     int few_split, few_chunk, many_split, many_chunk;
-    size_t few_rows, many_rows, floats;  // rows of partial outputs
+    size_t few_rows, many_rows;  // rows of partial outputs
+
+    // Parts (units x splits) of a call that splits at most, so that the workspace stays within 68 MB and 136 MB (heads of
+    // 128) however many sequences or rows there are: the device is full long before. (Single tokens of 256 / 512 / 1024
+    // sequences of up to 8192, 32 heads on 8 of 128, in 4 splits 779 / 1512 / 3100 us, with 4096 parts at most 752 / 1425 /
+    // 2853, with 2048 741 / 1445 / 2819; 128 sequences 394 / 394 / 412. Chunks of 2080 after 6112 / 2400 after 14000 / 6160
+    // after 2000, by the estimate alone 327 / 670 / 616 us, with 4096 parts 326 / 672 / 685, with 2048 295 / 633 / 507, with
+    // 1024 305 / 669 / 507; 1056 after 7136 179 / 179 / 178 / 193.)
+    static constexpr int64_t FEW_PARTS = 4096, MANY_PARTS = 2048;
+    static constexpr int64_t UNSPLIT = 640, MOST_SPLITS = 64;  // keys that few rows never split; splits of many rows
+
+    // Floats of workspace that the plans of these sizes, and of any with fewer tokens or sequences or with less
+    // expected of them, take at most: every term is one that does not fall as they grow.
+    static size_t floats(int n_tokens, int n_seqs, int n_heads, int n_kv_heads, int head_dim, int max_q_len,
+                         int max_kv_len) {
+        const int64_t group = n_heads / n_kv_heads, rows = n_tokens * group, seqs = std::min(n_seqs, n_tokens);
+        const int64_t pieces = ((int64_t)max_kv_len + 127) / 128;
+        const auto parts = [&](int64_t tile, int64_t splits, int64_t most) {
+            splits = std::min(splits, pieces);
+            return splits > 1 ? std::min(most, (rows + (tile - 1) * seqs) / tile * n_kv_heads * splits) : 0;
+        };
+        const int64_t few_most = max_kv_len <= UNSPLIT ? 1
+                                 : n_seqs > 1 ? std::max<int64_t>(2 * CUS / n_kv_heads, (pieces + 7) / 8)
+                                              : CUS / n_kv_heads;
+        const int64_t few = parts(FEW, few_most, FEW_PARTS);
+        const int64_t many = std::min(max_q_len, n_tokens) * group > FEW ? parts(MANY, MOST_SPLITS, MANY_PARTS) : 0;
+        return (size_t)(few * FEW + many * MANY) * (head_dim + 2);
+    }
 
     // A join costs 2 to 3 us, what a workgroup takes for about 600 keys alone (one token, 32 heads on 8, 511 / 1023 /
     // 4095 positions: unsplit 10.2 / 15.6 / 44.8 us, in pieces of 128 keys 11.1 / 11.4 / 12.4; 40959 positions in 256
@@ -1046,7 +1073,7 @@ struct Plan {
     // 16.5 / 22.5), in pieces of 1024 keys, or 2048 where there are enough of those (16 of up to 8000, pieces of 2048 /
     // 1024: 62.5 / 54.6; 64 of up to 8447, whole / 2048 / 1024: 217 / 195 / 195).
     static int64_t few_splits(int64_t units, int n_seqs, int64_t span) {
-        if (span <= 640) return 1;
+        if (span <= UNSPLIT) return 1;
         const int64_t target = n_seqs > 1 ? 2 * CUS : CUS, piece = units <= CUS ? 1024 : 2048;
         return std::max<int64_t>(
             1, std::min((span + 127) / 128, std::max(target / units, n_seqs > 1 ? (span + piece - 1) / piece : 1)));
@@ -1085,8 +1112,9 @@ struct Plan {
         // r rows of a sequence make at most (r + T - 1) / T tiles; one of many rows has over FEW. Empty workgroups
         // between the others would put two of those on a CU and none on another (with one tile too many 512 tokens
         // after 6144 in two splits 95 us instead of 78).
-        const int64_t few_tiles = many ? n_seqs : (rows + (FEW - 1) * std::min<int64_t>(n_seqs, rows)) / FEW;
-        const int64_t long_seqs = std::min<int64_t>(n_seqs, few ? rows / (FEW + 1) : rows);
+        const int64_t seqs = std::min(n_seqs, n_tokens);  // that have rows
+        const int64_t few_tiles = many ? seqs : (rows + (FEW - 1) * seqs) / FEW;
+        const int64_t long_seqs = few ? std::min(seqs, rows / (FEW + 1)) : seqs;
         const int64_t many_tiles = (rows + (MANY - 1) * long_seqs) / MANY;
         few_units = few ? few_tiles * n_kv_heads : 0;
         many_units = many ? many_tiles * n_kv_heads : 0;
@@ -1103,13 +1131,14 @@ struct Plan {
         // Workgroups of few rows need places of their own beside those of many: chunks of 511 and 71 after up to 4095
         // beside 20 single tokens, 16 heads on 8, in 1 / 2 / 3 / 4 / 6 splits 98 / 74 / 65 / 68 / 77 us; 64 single
         // tokens of up to 8000 beside a chunk of 511, 32 on 8, in 1 / 2 / 3 / 4 245 / 236 / 258 / 276.
-        const int64_t units = (rows + MANY - 1) / MANY * n_kv_heads, most = few ? std::max<int64_t>(1, 288 / units) : 64;
-        cut(FEW, [&](int64_t span) { return few_splits((int64_t)n_seqs * n_kv_heads, n_seqs, span); }, few_split, few_chunk);
-        cut(MANY, [&](int64_t span) { return many_splits(units, head_dim, span, most); },
-            many_split, many_chunk);
+        const int64_t units = (rows + MANY - 1) / MANY * n_kv_heads, beside = few ? 288 / units : MOST_SPLITS;
+        const int64_t few_most = std::max<int64_t>(1, FEW_PARTS / std::max<int64_t>(1, few_units));
+        const int64_t many_most = std::max<int64_t>(1, std::min(beside, MANY_PARTS / std::max<int64_t>(1, many_units)));
+        cut(FEW, [&](int64_t span) { return std::min(few_most, few_splits((int64_t)n_seqs * n_kv_heads, n_seqs, span)); },
+            few_split, few_chunk);
+        cut(MANY, [&](int64_t span) { return many_splits(units, head_dim, span, many_most); }, many_split, many_chunk);
         few_rows = few_split > 1 ? (size_t)few_units * few_split * FEW : 0;
         many_rows = many_split > 1 ? (size_t)many_units * many_split * MANY : 0;
-        floats = (few_rows + many_rows) * (head_dim + 2);
     }
 };
 
@@ -1167,7 +1196,7 @@ extern "C" size_t attention_paged_workspace_floats(int n_tokens, int n_seqs, int
     }
     if (!check_sizes(name, n_tokens, n_heads, max_q_len, max_kv_len)) return 0;
     if (n_tokens == 0) return 0;
-    return Plan(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len, 0).floats;
+    return Plan::floats(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len);
 }
 
 extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBatch *batch, float *ws, int n_tokens,
@@ -1196,7 +1225,7 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
                  batch->n_seqs, max_kv_len);
         return;
     }
-    if (!aligned16(ws) || (plan.floats && !ws)) {
+    if (!aligned16(ws) || (plan.few_rows + plan.many_rows && !ws)) {
         llm_fail("%s: ws must be a 16-byte aligned device address", name);
         return;
     }

@@ -557,6 +557,29 @@ def test_attention_strided_rows(gpu):
     assert (wide[:, 4:] == 7).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_calls_stay_within_the_workspace_of_their_sizes(gpu, dim):
+    """What lies behind the floats that each of several calls asks for is left as it is."""
+    import torch
+    heads, kv_heads = 8, 2
+    for seqs in ([(1, 9000)], [(40, 3000)], [(200, 5000)], [(1, 3000), (3, 900), (1, 1)], [(60, 2000), (1, 4000), (2, 10)],
+                 [(600, 2500), (33, 900)]):
+        b = Batch([(0, 0)], kv_heads, dim, 64, 59)
+        n = [-(-have // 64) for _, have in seqs]
+        b.table = torch.arange(sum(n)).int()[None].expand(len(seqs), -1).contiguous()  # a pool that all share
+        k, v = (torch.randn(sum(n), 64, kv_heads, dim, device="cuda").bfloat16() for _ in range(2))
+        starts = [sum(new for new, _ in seqs[:s]) for s in range(len(seqs) + 1)]
+        where = [t.cuda() for t in (b.table, torch.tensor(starts).int(), torch.tensor([have for _, have in seqs]).int())]
+        q = torch.randn(starts[-1], heads, dim, device="cuda").bfloat16()
+        max_q, max_kv = max(new for new, _ in seqs), max(have for _, have in seqs)
+        for q_told, kv_told in ((max_q, max_kv), (1, max_kv), (max_q, 700), (2 * max_q, 40960)):
+            need = gpu.attention_paged_workspace_floats(starts[-1], len(seqs), heads, kv_heads, dim, q_told, kv_told)
+            ws = torch.full((need + (1 << 20),), 7.0, device="cuda")
+            gpu.attention_paged_forward(torch.empty_like(q), q, k, v, *where, ws[:need], 0.1, q_told, kv_told)
+            assert (ws[need:] == 7).all()
+
+
 # ---------------------------------------------------------------- together
 
 @pytest.mark.gpu
@@ -791,6 +814,31 @@ def test_attention_in_place_and_overflowing_scales_are_refused(pkg):
     p, b = 0x1000, ctypes.byref(record(pkg))
     assert "out must not be q" in refused(pkg, "attention_paged_forward", p, p, b, p, 4, 4, 1, 100, 0, 0.1, 256, 256, None)
     assert "not positive and finite" in refused(pkg, "attention_paged_forward", 0x9000, p, b, p, 4, 4, 1, 100, 0, 3e38, 256, 256, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (16, 8, 128), (16, 4, 256), (24, 4, 64), (40, 1, 64),
+                                                (7, 7, 128), (600, 300, 64)])
+def test_workspace_of_the_largest_call_serves_smaller_ones(pkg, heads, kv_heads, dim):
+    """The count does not fall as a size grows, nor does it grow without end."""
+    def floats(*sizes):
+        n_tokens, n_seqs, max_q, max_kv = sizes
+        return pkg.attention_paged_workspace_floats(n_tokens, n_seqs, heads, kv_heads, dim, max_q, max_kv)
+
+    assert floats(2048, 1, 2048, 8192) >= floats(512, 1, 512, 8192) > 0
+    rng = np.random.default_rng(heads)
+    most = [65536, 4096, 65536, 1 << 20]
+    for _ in range(3000):
+        large = [int(math.exp(rng.uniform(0, math.log(n + 1)))) for n in most]
+        small = [int(rng.integers(1, n + 1)) if rng.random() < 0.6 else n for n in large]
+        assert floats(*small) <= floats(*large), (small, large)
+    for i in range(4):  # one size by one, the others in the middle
+        sizes = [600, 20, 300, 9000]
+        counts = []
+        for n in list(range(1, 700)) + [1000, 2000, 4096]:
+            sizes[i] = n
+            counts.append(floats(*sizes))
+        assert counts == sorted(counts)
+    assert floats(*most) <= (4096 * 32 + 2048 * 128) * (dim + 2)
 
 
 def test_no_rows_is_no_launch(pkg):
