@@ -1220,7 +1220,8 @@ extern "C" void attention_paged_forward(bf16 *out, const bf16 *q, const PagedBat
     const int64_t width = (int64_t)n_heads * D;
     if (!check_rows(name, "out", out, out_stride, width) || !check_rows(name, "q", q, q_stride, width)) return;
     const Plan plan(n_tokens, batch->n_seqs, n_heads, batch->n_kv_heads, D, max_q_len, max_kv_len, window);
-    if (plan.few_units * plan.few_split + plan.many_units * plan.many_split > INT32_MAX / 64) {
+    // a launch has less than 2^32 threads; the join, of units that are split, stays far below
+    if (plan.few_units * plan.few_split + plan.many_units * plan.many_split >= 1 << 24) {
         llm_fail("%s: %d rows in %d sequences of up to %d tokens are too many for one launch", name, n_tokens,
                  batch->n_seqs, max_kv_len);
         return;

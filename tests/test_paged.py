@@ -841,6 +841,15 @@ def test_workspace_of_the_largest_call_serves_smaller_ones(pkg, heads, kv_heads,
     assert floats(*most) <= (4096 * 32 + 2048 * 128) * (dim + 2)
 
 
+def test_more_workgroups_than_a_launch_has_are_refused(pkg):
+    """On the host, by the library's own message: 2^24 workgroups of 256 threads and more."""
+    p, n = 0x1000, 1 << 20
+    for kv_heads in (16, 17, 31):
+        b = ctypes.byref(record(pkg, n_seqs=n, n_kv_heads=kv_heads, slot_stride=64 * kv_heads, page_stride=1024 * kv_heads))
+        assert "too many for one launch" in refused(pkg, "attention_paged_forward", 0x9000, p, b, p, n, kv_heads, 1, 100, 0,
+                                                    0.1, 64 * kv_heads, 64 * kv_heads, None)
+
+
 def test_no_rows_is_no_launch(pkg):
     p, b = 0x1000, record(pkg)
     assert refused(pkg, "qk_norm_rope_paged", p, p, p, p, None, None, p, ctypes.byref(b), 0, 4, 64, 0, 1e-6, 1.0,
