@@ -491,6 +491,7 @@ def _paged_batch(key_cache, value_cache, page_table, q_start, kv_len):
             raise LlmError(f"{name} must have shape [pages, slots, kv heads, head_dim], the last contiguous")
     if key_cache.shape != value_cache.shape or key_cache.stride() != value_cache.stride():
         raise LlmError("key_cache and value_cache must have the same shape and strides")
+    _on_device("page_table", page_table, (torch.int32,))
     if page_table.dim() != 2:
         raise LlmError(f"page_table must have shape [sequences, pages], got {tuple(page_table.shape)}")
     pages, slots, kv_heads, dim = key_cache.shape
@@ -514,6 +515,7 @@ def qk_norm_rope_paged(q_out, q, k, v, q_norm_w, k_norm_w, inv_freq, key_cache, 
         return
     import torch
     batch = _paged_batch(key_cache, value_cache, page_table, q_start, kv_len)
+    _on_device("q", q, _bits16())
     if q.dim() != 3:
         raise LlmError(f"q must have shape [tokens, heads, head_dim], got {tuple(q.shape)}")
     n, heads, dim = q.shape[0], q.shape[1], batch.head_dim
@@ -547,19 +549,21 @@ def attention_paged_forward(out, q, key_cache, value_cache, page_table, q_start,
         return
     import torch
     batch = _paged_batch(key_cache, value_cache, page_table, q_start, kv_len)
+    _on_device("q", q, _bits16())
     if q.dim() != 3:
         raise LlmError(f"q must have shape [tokens, heads, head_dim], got {tuple(q.shape)}")
     n, heads, dim = q.shape[0], q.shape[1], batch.head_dim
     out_at, out_stride = _head_rows("out", out, (n, heads, dim))
     q_at, q_stride = _head_rows("q", q, (n, heads, dim))
+    if ws is not None:
+        _on_device("ws", ws, (torch.float32,))
+        _dense("ws", ws, torch.float32, ws.shape)
     if n and heads % max(batch.n_kv_heads, 1) == 0:
         need = attention_paged_workspace_floats(n, batch.n_seqs, heads, batch.n_kv_heads, dim, max_q_len,
                                                 max_kv_len)
         have = 0 if ws is None else ws.numel()
         if have < need:
             raise LlmError(f"ws holds {have} floats, attention needs {need}")
-    if ws is not None:
-        _dense("ws", ws, torch.float32, ws.shape)
     _call(lib().attention_paged_forward, out_at, q_at, ctypes.byref(batch), _ptr(ws), n, heads, max_q_len,
           max_kv_len, window, scale, out_stride, q_stride, _stream(stream))
 
@@ -576,14 +580,15 @@ def logits_penalty_forward(out, logits, tokens=None, prompt_len=None, token_len=
     import torch
     for name, t in (("out", out), ("logits", logits)):
         _on_device(name, t, _bits16())
+    for name, t in (("out", out), ("logits", logits)):
         if t.dim() != 2 or t.shape != logits.shape or (t.shape[1] > 1 and t.stride(1) != 1):
             raise LlmError(f"{name} must have shape [rows, vocab], the same for both, with contiguous rows")
     rows, vocab = logits.shape
     strides = [t.stride(0) if rows > 1 else max(vocab, 1) for t in (out, logits)]
-    if allowed is not None:
-        _on_device("allowed", allowed, (torch.int32, torch.uint32))
     wide = {}
-    for name, t in (("tokens", tokens), ("bias_tokens", bias_tokens), ("allowed", allowed)):
+    for name, t in (("allowed", allowed), ("tokens", tokens), ("bias_tokens", bias_tokens)):
+        if t is not None:
+            _on_device(name, t, (torch.int32, torch.uint32) if name == "allowed" else (torch.int32,))
         if t is not None and t.dim() != 2:
             raise LlmError(f"{name} must have two dimensions, got {tuple(t.shape)}")
         wide[name] = 0 if t is None else t.shape[1]

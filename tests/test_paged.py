@@ -895,6 +895,37 @@ def test_wrapper_refusals(gpu):
 
 
 @pytest.mark.gpu
+def test_wrappers_name_what_is_no_tensor(gpu):
+    """What is no tensor is refused by the library's own error, whatever else it is."""
+    import torch
+    b = Batch([(2, 20), (1, 5)], 2, 64, 16, 1)
+    kc, vc = b.pools()
+    q, k, v = (b.normal(3, h, 64).cuda() for h in (4, 2, 2))
+    where, f = b.where(), gpu.rope_frequencies(64, 1e4)[0].cuda()
+    append = dict(q_out=torch.empty_like(q), q=q, k=k, v=v, q_norm_w=None, k_norm_w=None, inv_freq=f, key_cache=kc,
+                  value_cache=vc, page_table=where[0], q_start=where[1], kv_len=where[2], eps=1e-6)
+    attend = dict(out=torch.empty_like(q), q=q, key_cache=kc, value_cache=vc, page_table=where[0], q_start=where[1],
+                  kv_len=where[2], ws=workspace(gpu, b, 4, 2, 9000), scale=0.1, max_q_len=2, max_kv_len=9000)
+    ids, n = torch.zeros(2, 5, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    x = torch.zeros(2, 100, dtype=torch.bfloat16, device="cuda")
+    penalty = dict(out=x, logits=x, tokens=ids, token_len=n, bias_tokens=ids, bias=ids.float(), allowed=ids)
+    for call, good, names, none in (
+            (gpu.qk_norm_rope_paged, append, ["q_out", "q", "k", "v", "inv_freq", "key_cache", "value_cache", "page_table",
+                                              "q_start", "kv_len", "q_norm_w"], True),
+            (gpu.attention_paged_forward, attend, ["out", "q", "key_cache", "value_cache", "page_table", "q_start", "kv_len",
+                                                   "ws"], True),
+            (gpu.logits_penalty_forward, penalty, ["out", "logits"], True),
+            (gpu.logits_penalty_forward, penalty, ["tokens", "token_len", "bias_tokens", "bias", "allowed"], False)):
+        for name in names:
+            for value in [[1, 2], 7] + ([None] if none and name != "q_norm_w" else []):
+                with pytest.raises(gpu.LlmError):
+                    call(**dict(good, **{name: value}))
+    with pytest.raises(gpu.LlmError, match="page_table must be a tensor on the GPU"):
+        gpu.attention_paged_forward(**dict(attend, page_table=None))
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_native_and_general_way_are_one(gpu, monkeypatch):
     """The native launchers and the general ctypes way: the same results from the same arguments, and the
     same refusals."""
