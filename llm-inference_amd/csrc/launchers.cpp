@@ -297,6 +297,7 @@ PyObject *native_attention_paged_forward(PyObject *, PyObject *const *o, Py_ssiz
                 !take<int>(o[9], max_q) || !take<int>(o[10], max_kv) || !take<int>(o[11], window) ||
                 !take<hipStream_t>(o[12], stream))
                 return false;
+            if (llm_last_error()) return false;  // from an earlier call: the general way reports it
             const size_t need = attention_paged_workspace_floats((int)n, b.n_seqs, (int)heads, b.n_kv_heads,
                                                                  b.head_dim, max_q.i, max_kv.i);
             if (llm_last_error()) {  // the general way meets and reports it again

@@ -926,6 +926,27 @@ def test_wrappers_name_what_is_no_tensor(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_an_error_from_before_is_reported(gpu, monkeypatch, native):
+    """An error that an earlier call of the library left is reported by the next call, once."""
+    import torch
+    if not native:
+        monkeypatch.setattr(gpu, "_native", None)
+    b = Batch([(1, 20)], 2, 64, 16, 1)
+    q, (kc, vc), where = b.normal(1, 4, 64).cuda(), b.pools(), b.where()
+    out, x = torch.empty_like(q), torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda")
+    f, k = gpu.rope_frequencies(64, 1e4)[0].cuda(), q[:, :2]
+    for call in (lambda: gpu.attention_paged_forward(out, q, kc, vc, *where, None, 0.1, 1, 20),
+                 lambda: gpu.qk_norm_rope_paged(out, q, k, k, None, None, f, kc, vc, *where, 1e-6),
+                 lambda: gpu.logits_penalty_forward(x, x)):
+        gpu.lib().attention_paged_workspace_floats(1, 1, 4, 3, 64, 1, 20)  # no such heads
+        with pytest.raises(gpu.LlmError, match="4 heads on 3"):
+            call()
+        call()
+    torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
 def test_native_and_general_way_are_one(gpu, monkeypatch):
     """The native launchers and the general ctypes way: the same results from the same arguments, and the
     same refusals."""
