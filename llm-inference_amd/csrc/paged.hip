@@ -146,7 +146,10 @@ extern "C" float rope_frequencies(double *inv_freq, int rotary_dim, double theta
         };
         low = fmax(floor(pair_that_turns(32)), 0.0);
         high = fmin(ceil(pair_that_turns(1)), (double)(rotary_dim - 1));
-        if (high == low) high += 0.001;
+        if (pair_that_turns(1) <= 0)
+            low = -1, high = 0;  // none turns once: all are divided
+        else if (high <= low)
+            high = low + 0.001;  // all turn more than 32 times
     }
     for (int j = 0; j < rotary_dim / 2; j++) {
         const double f = pow(theta, -2.0 * j / rotary_dim);

@@ -220,6 +220,17 @@ def test_rope_frequencies(pkg):
             pkg.rope_frequencies(*args)
 
 
+@pytest.mark.parametrize("theta,trained,share", [(1e4, 1, 1), (1e4, 4, 1), (1e6, 6, 1), (10.0, 32768, 0), (1.5, 100000, 0)])
+def test_yarn_where_all_pairs_are_slow_or_fast(pkg, theta, trained, share):
+    """None turns once over the trained length: all are divided. All turn more than 32 times: all are left."""
+    base = theta ** (-2.0 * np.arange(32) / 64)
+    turns = trained * base / (2 * math.pi)
+    assert (turns < 1).all() if share else (turns > 32).all()
+    got, scale = pkg.rope_frequencies(64, theta, pkg.ROPE_YARN, 4.0, trained)
+    assert scale == pytest.approx(0.1 * math.log(4) + 1, rel=1e-6)
+    assert np.allclose(got.numpy(), base / 4 if share else base, rtol=1e-14, atol=0)
+
+
 # ---------------------------------------------------------------- attention over pages
 
 def attended(b, q, scale, window):
