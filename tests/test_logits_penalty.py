@@ -150,6 +150,20 @@ def test_many_biases_and_long_histories(gpu, history, biases, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,history,biases,slices", [(64, 65544, 700, 600, 9), (64, 70001, 300, 513, 9),
+                                                              (32, 65544, 32768, 600, 17), (64, 65544, 32800, 40, 9)])
+def test_penalties_of_many_rows(gpu, rows, vocab, history, biases, slices):
+    """So many rows that the slices are the largest: 8192 tokens, 4096 where counts of 32 bits and a word per
+    token for the biases share the memory."""
+    import torch
+    assert rows * slices >= 512 and -(-vocab // (4096 if slices == 17 else 8192)) == slices
+    rng = np.random.default_rng(history + biases)
+    logits = torch.from_numpy(rng.standard_normal((rows, vocab)).astype(np.float32) * 4).cuda().bfloat16()
+    c = make(rng, rows, vocab, history, biases, True, True)
+    check(run(gpu, logits, c), logits, c)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("off", ["repetition", "frequency", "presence", "prompt_len"])
 def test_each_part_can_be_off(gpu, off):
     import torch

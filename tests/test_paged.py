@@ -174,6 +174,47 @@ def test_append_against_the_definition(gpu, case, fused):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,dim,rotary,interleaved,norm,seqs", [
+    (32, 8, 128, 128, False, True, [(1500, 1700), (1, 5), (31, 31)]), (35, 7, 64, 32, True, False, [(2601, 2601)]),
+    (6, 3, 256, 256, True, True, [(1200, 1200), (0, 4), (601, 640)]), (12, 4, 128, 48, False, False, [(4100, 4100)])])
+def test_append_of_many_rows(gpu, heads, kv_heads, dim, rotary, interleaved, norm, seqs):
+    """So many rows that a wave takes several groups of a row's heads, of q, k and v among each other."""
+    import torch
+    page = 16
+    groups = -(-heads * dim // 512) + 2 * -(-kv_heads * dim // 512)
+    assert sum(n for n, _ in seqs) * groups // 6144 >= 2
+    b = Batch([], kv_heads, dim, page, 47)
+    b.seqs, need = seqs, [-(-n // page) for _, n in seqs]
+    b.pages = sum(need) + 2
+    b.table = torch.full((len(seqs), max(need)), -1, dtype=torch.int32)
+    order = torch.randperm(b.pages, generator=b.g).int()
+    for s, n in enumerate(need):
+        b.table[s, :n] = order[sum(need[:s]):sum(need[:s]) + n]
+    b.starts = [sum(n for n, _ in seqs[:s]) for s in range(len(seqs) + 1)]
+    b.tokens = b.starts[-1] + 1
+    b.q_start, b.kv_len = (torch.tensor(x, dtype=torch.int32) for x in (b.starts, [n for _, n in seqs]))
+    rows = b.normal(b.tokens, heads + 2 * kv_heads, dim)
+    q, k, v = rows[:, :heads], rows[:, heads:heads + kv_heads], rows[:, heads + kv_heads:]
+    qn, kn = (b.normal(dim), b.normal(dim)) if norm else (None, None)
+    inv_freq, scale = gpu.rope_frequencies(rotary, 1e6, gpu.ROPE_YARN, 4.0, 4096)
+    kc, vc = (torch.full((b.pages, page, kv_heads, dim), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    whole = rows.cuda()
+    q_out = torch.full((b.tokens, heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    gpu.qk_norm_rope_paged(q_out, whole[:, :heads], whole[:, heads:heads + kv_heads], whole[:, heads + kv_heads:],
+                           qn.cuda() if norm else None, kn.cuda() if norm else None, inv_freq.cuda(), kc, vc,
+                           *b.where(), 1e-6, scale, interleaved=interleaved)
+    got_q, got_k, got_v = q_out.cpu(), kc.cpu(), vc.cpu()
+    written = torch.zeros(b.pages, page, dtype=torch.bool)
+    for t, s, p in b.rows():
+        slot = b.slot(s, p)
+        written[slot] = True
+        close(got_q[t], *rotated(q[t], qn, p, inv_freq.numpy(), scale, interleaved, 1e-6))
+        close(got_k[slot], *rotated(k[t], kn, p, inv_freq.numpy(), scale, interleaved, 1e-6))
+        assert torch.equal(got_v[slot], v[t])
+    assert (got_q[-1] == 7).all() and (got_k[~written] == 7).all() and (got_v[~written] == 7).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_append_far_positions_and_in_place(gpu, interleaved):
     """A long context's last rows (positions around 2^20): the angle's 64 bits; q_out may be q."""
@@ -566,6 +607,58 @@ def test_attention_strided_rows(gpu):
     gpu.attention_paged_forward(wide[:, :4], rows[:, :4], kc, vc, *b.where(), workspace(gpu, b, 4, 40, 70), 0.125, 40, 70)
     check_attend(b, wide[:, :4].contiguous(), q, 0.125, 0)
     assert (wide[:, 4:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,dim,new,past,window", [(3, 64, 1456, 0, 0), (3, 128, 1450, 30, 60), (5, 256, 840, 3, 0)])
+def test_attention_of_more_workgroups_than_the_device_has_cus(gpu, kv_heads, dim, new, past, window):
+    """Whole tiles without splits, more of them than CUs but not twice as many, an odd number: every row of every
+    tile, against 64 bits a kv head at a time."""
+    import torch
+    group, page, n = 8, 16, new + past
+    units = -(-new * group // 128) * kv_heads
+    assert 256 < units < 512 and units % 2
+    scale = 1 / math.sqrt(dim)
+    g = torch.Generator().manual_seed(dim)
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g).bfloat16()
+
+    pages = -(-n // page)
+    q, k, v = normal(new, kv_heads * group, dim), normal(pages, page, kv_heads, dim), normal(pages, page, kv_heads, dim)
+    table = torch.randperm(pages, generator=g).int()[None]
+    where = [t.cuda() for t in (table, torch.tensor([0, new], dtype=torch.int32), torch.tensor([n], dtype=torch.int32))]
+    floats = gpu.attention_paged_workspace_floats(new, 1, kv_heads * group, kv_heads, dim, new, n)
+    out = torch.zeros(new, kv_heads * group, dim, dtype=torch.bfloat16, device="cuda")
+    gpu.attention_paged_forward(out, q.cuda(), k.cuda(), v.cuda(), *where, torch.empty(max(floats, 1), device="cuda"),
+                                scale, new, n, window=window)
+    got = out.cpu()
+    at, key = np.arange(past, n)[:, None], np.arange(n)[None]
+    hidden = (key > at) | ((key <= at - window) if window else False)
+    for h in range(kv_heads):
+        kk, vv = (x[table[0].long(), :, h].reshape(-1, dim)[:n].double().numpy() for x in (k, v))
+        for j in range(h * group, (h + 1) * group):
+            qq = q[:, j].double().numpy()
+            score = np.where(hidden, -np.inf, qq @ kk.T * scale)
+            off = 2 * (dim * F32 * (np.abs(qq) @ np.abs(kk).T).max(-1) * scale
+                       + 8 * F32 * np.abs(np.where(hidden, 0, score)).max(-1))[:, None]
+            w = np.exp(score - score.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            close(got[:, j], w @ vv, (HALF_STEP + off + (n + 64) * F32) * (w @ np.abs(vv)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("seqs,window,dim,page", [([(1, 261)], 0, 128, 16), ([(1, 40), (4, 300), (1, 900)], 0, 64, 16),
+                                                  ([(1, 3000), (1, 10)], 0, 256, 16), ([(2, 700), (3, 90)], 64, 128, 7)])
+def test_few_rows_keep_what_their_weights_rounding_leaves(gpu, seqs, window, dim, page):
+    """A call whose sequences all have few rows: each weight is a bf16 and a bf16 of the rest, off by half a
+    step of half a step at most, so the bound has 2^-16 where that of many rows has 2^-8."""
+    b = Batch(seqs, 2, dim, page, 53)
+    q, scale = b.normal(b.tokens, 8, dim), 1 / math.sqrt(dim)
+    out = attend(gpu, b, q, scale, window)
+    want, err = attended(b, q, scale, window)
+    b.v = b.v.abs()
+    close(out.cpu(), want, err - (HALF_STEP - HALF_STEP ** 2) * attended(b, q, scale, window)[0])
 
 
 @pytest.mark.gpu
