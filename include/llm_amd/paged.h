@@ -80,10 +80,13 @@ void qk_norm_rope_paged(bf16 *q_out, const bf16 *q, const bf16 *k, const bf16 *v
  * zeros. What lies in the caches at positions that a row does not see, NaN and infinities included, does
  * not reach it. A value that it sees and that is infinite makes its element infinite, or no number where its weight
  * falls below the range of 32 bits; finite values overflow where their size times 2^8 times the number of
- * positions passes that range. Scores, weights and sums are in 32 bits; in front of the values the weights are rounded to
- * bf16, with what that leaves added back where a sequence has at most 32 rows x heads per kv head (there the
- * bytes of the cache take longer than both products). Query head h reads kv head h / (n_heads / n_kv_heads). Rows of q and out are q_stride and
- * out_stride elements apart; out must not overlap anything. scale > 0.
+ * positions passes that range. Query head h reads kv head h / (n_heads / n_kv_heads). Rows of q and out are
+ * q_stride and out_stride elements apart; out must not overlap anything. scale > 0.
+ * Scores, weights and sums are in 32 bits; in front of the values the weights are rounded to bf16. What that leaves
+ * is added back where rows are few, since there the bytes of the cache take longer than both products: in sequences
+ * of at most 32 rows x heads per kv head, and in all of them where max_q_len expects no more. It is not where n_tokens,
+ * n_seqs and max_q_len leave room for no such sequence (one sequence of which more is expected, for instance), nor in
+ * what a workgroup computes (few rows, some keys) if a part of it is infinite or no number.
  * max_q_len and max_kv_len say how many new rows and how many cached tokens a sequence is expected to have at
  * most: the split of the work goes by them. Longer sequences are computed all the
  * same, more slowly. How the work is split changes the order of the sums and with it the last bits.

@@ -1105,8 +1105,8 @@ struct Plan {
         const int64_t longest = std::min<int64_t>(max_q_len, n_tokens) * group;
         many = longest > FEW;
         // with sequences of at most FEW / group tokens of few rows and the others of at most max_q_len, this many
-        // at least have many rows: where that is all of them, all go to attend_many (and one that is short
-        // after all is only slower there)
+        // at least have many rows: where that is all of them, all go to attend_many (one that is short after all
+        // takes longer there, and its weights have no remainders)
         const int64_t tokens = FEW / group, rest = n_tokens - n_seqs * tokens;
         few = !many || (n_seqs > 1 && rest <= (int64_t)(n_seqs - 1) * (max_q_len - tokens));
         // r rows of a sequence make at most (r + T - 1) / T tiles; one of many rows has over FEW. Empty workgroups
