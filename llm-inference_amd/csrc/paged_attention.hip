@@ -927,11 +927,9 @@ __global__ __launch_bounds__(256, D == 256 ? 1 : 2) void attend_kernel(LaunchArg
 
 // A wave joins 256 / D rows, four elements of a row per lane, up to 8 splits' parts requested at a time and
 // added in order. Few rows of many splits: the four waves of a workgroup take a quarter of the splits each and
-// are joined in order through LDS; many rows of few splits: each wave takes rows of its own. Where the parts lie does
-// not depend on the sequence, so the first ones are requested in front of its lookup where there are few sequences
-// (one token after 40960 / 4000 / 64 after 6144: 34.6 / 12.4 / 27.0 us instead of 36.8 / 14.3 / 30.8 with the lookup
-// first). Of many sequences some have no such tile or fewer splits, whose parts would be read in vain (22 sequences,
-// two with chunks: 68.0 us instead of 65.3; 64 of one token 197 and 196; 4 of them 25.0 and 25.8).
+// are joined in order through LDS; many rows of few splits: each wave takes rows of its own. The
+// first parts, whose place does not depend on the sequence, requested in front of its lookup bring nothing (one token
+// after 40960 / 4000, 64 after 6144: 34.8 / 12.6 / 25.7 us both ways; two chunks of 64 after 6144 36.1 instead of 34.6).
 template <int D, int T>
 __device__ __forceinline__ void join_tile(const AttendArgs &a, int unit, int part, int parts, f32x4 (&outs)[4][64],
                                           float (&tops)[4][64], float (&sums)[4][64]) {
@@ -942,7 +940,7 @@ __device__ __forceinline__ void join_tile(const AttendArgs &a, int unit, int par
     const int z0 = SHARED ? a.n_split * w / 4 : 0, upto = SHARED ? a.n_split * (w + 1) / 4 : a.n_split;
     u32x2 stats[U];
     f32x4 e[U];
-    const auto request = [&](int row, int z) {  // row < T
+    const auto request = [&](int row, int z) {
         const int64_t at = (int64_t)unit * a.n_split * T + row;
 #pragma unroll
         for (int u = 0; u < U; u++) {
@@ -950,21 +948,22 @@ __device__ __forceinline__ void join_tile(const AttendArgs &a, int unit, int par
             stats[u] = *gptr((const u32x2 *)(a.stats + from * 2));
             e[u] = *gptr((const f32x4 *)(a.part + from * D + 4 * k));
         }
+        // all of them requested before the first is waited for: otherwise each load goes where its part is added (one token
+        // after 40960 36.8 us instead of 34.6, 64 after 6144 32.3 instead of 25.3)
+        asm volatile(""
+                     : "+v"(e[0]), "+v"(e[1]), "+v"(e[2]), "+v"(e[3]), "+v"(e[4]), "+v"(e[5]), "+v"(e[6]), "+v"(e[7]));
+        static_assert(U == 8, "all of e stand there");
     };
     const int first = part * ROWS * (SHARED ? 1 : 4), own = (SHARED ? 0 : w * ROWS) + lane / CHUNKS;
-    static_assert(T % (4 * ROWS) == 0, "the first rows lie in the tile");
-    bool requested = a.b.n_seqs <= (SHARED ? 8 : 2);
-    if (requested) request(first + own, z0);
     Tile t;
     if (!find_tile<T>(a, a.which, tile, t) || t.active <= 1) return;
     const int z1 = min(upto, t.active);
-    for (int r0 = first; r0 < t.rows; r0 += parts * ROWS * (SHARED ? 1 : 4), requested = false) {
+    for (int r0 = first; r0 < t.rows; r0 += parts * ROWS * (SHARED ? 1 : 4)) {
         const int row = r0 + own;
         float top = LOWEST, sum = 0.0f;
         f32x4 o = {0, 0, 0, 0};
         for (int z = z0; z < z1; z += U) {
-            if (!requested) request(min(row, t.rows - 1), z);
-            requested = false;
+            request(min(row, t.rows - 1), z);
             float m[U], n[U];
             float next = top;
 #pragma unroll
@@ -1066,9 +1065,9 @@ struct Plan {
         return (size_t)(few * FEW + many * MANY) * (head_dim + 2);
     }
 
-    // A join costs 2 to 3 us, what a workgroup takes for about 600 keys alone (one token, 32 heads on 8, 511 / 1023 /
-    // 4095 positions: unsplit 10.2 / 15.6 / 44.8 us, in pieces of 128 keys 11.1 / 11.4 / 12.4; 40959 positions in 256
-    // workgroups 34.5, in 512 35.7). Several sequences, which may be of
+    // A join costs 2 to 3 us, what a workgroup takes for about 600 keys alone (one token, 32 heads on 8, 511 / 639 / 1023 /
+    // 4095 positions: unsplit 9.8 / 10.9 / 16.4 / 46.1 us, in pieces of 128 keys 11.1 / 11.8 / 12.2 / 13.3; 40959 positions
+    // in 256 workgroups 34.5, in 512 35.7). Several sequences, which may be of
     // unequal length, take twice the workgroups (4 / 8 / 16 of up to 2000, 256 workgroups 14.0 / 16.3 / 22.7, 512 14.0 /
     // 16.5 / 22.5), in pieces of 1024 keys, or 2048 where there are enough of those (16 of up to 8000, pieces of 2048 /
     // 1024: 62.5 / 54.6; 64 of up to 8447, whole / 2048 / 1024: 217 / 195 / 195).
