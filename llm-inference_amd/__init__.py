@@ -533,6 +533,7 @@ def qk_norm_rope_paged(q_out, q, k, v, q_norm_w, k_norm_w, inv_freq, key_cache, 
 
 
 def attention_paged_workspace_floats(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim, max_q_len, max_kv_len):
+    """Floats of ws for attention_paged_forward with these sizes and with any smaller ones of these heads."""
     floats = lib().attention_paged_workspace_floats(n_tokens, n_seqs, n_heads, n_kv_heads, head_dim,
                                                     max_q_len, max_kv_len)
     check()

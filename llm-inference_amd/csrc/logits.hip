@@ -59,9 +59,10 @@ struct Values {
     }
 };
 
-// One workgroup per slice of a row's vocabulary. The row's history is read once by every slice (from L2 after
-// the first); the slice's tokens are counted in LDS, by whole numbers, so that the order of the additions does
-// not matter. Then eight logits per thread at a time, 16 bytes where the rows' alignment allows it. 64 rows of
+// One workgroup per slice of a row's vocabulary. The row's history is read once by every slice (from memory by the
+// first on each XCD, then from its L2); the slice's tokens are counted in LDS, by whole numbers, so that the order of
+// the additions does not matter. Then eight logits per thread at a time, 16 bytes where the row's alignment allows it
+// and one by one where not (64 rows of 50256 10.8 us, of 50257, where one row in eight is aligned, 16.1). 64 rows of
 // 151936, up to 8192 tokens and 300 biases: 15.6 us, 2.6 TB/s, of which the history takes 1.6 and the biases 2; what
 // bounds it is one phase of a workgroup waiting for the other (all logits requested in front of the history
 // instead of the first eight per thread: 21.0 against 19.9 then); one row by the launch and two round trips to

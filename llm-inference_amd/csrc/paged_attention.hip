@@ -581,13 +581,15 @@ struct Space {
 // that eight waves of a CU have about 100 KB under way. The columns that hold no row are multiplied all the same: the
 // matrix unit is idle most of the time here, which also pays for the weights' remainders (EXACT).
 // 64 tokens over up to 8448 positions, 32 heads on 8 of 128: 192 us with the join, 5.7 TB/s of keys and values (a
-// 2 GiB copy: 4.8); one token over 40960: 34 us with a join of 5; one over 261, 16 heads on 8: 8 us, which are the
-// launch, the sequence's and the page's lookups and three steps of a wave one after the other.
+// 2 GiB copy: 4.8; the library's read probe: 7.2); one token over 40960: 34 us with a join of 5; one over 261, 16 heads
+// on 8: 8.7 us, which are the launch, the sequence's and the page's lookups and three steps of a wave one after the
+// other. Heads of 256, 16 on 4: 199 and 36 us for the first two, of 64 113 and 22.
 // EXACT: with remainders. The result is then whether an output of the workgroup came out infinite or as no number.
 // A remainder may be 0 or negative, and 0 or a negative number times an infinite value makes no number where the
 // weight itself makes an infinity: such a workgroup does all of it again without remainders.
 template <int D, bool WHOLE, bool EXACT>
-__device__ __forceinline__ bool few_rows(const AttendArgs &a, int kv, const Tile &t, int unit, int z, Space<D, WHOLE> &space) {
+__device__ __forceinline__ bool few_rows(const AttendArgs &a, int kv, const Tile &t, int unit, int z,
+                                         Space<D, WHOLE> &space) {
     constexpr int ROWS = 32, BYTES = ROWS * 2 * D;
     typedef Pages<D, ROWS, ROWS, WHOLE, true> P;
     constexpr int LOADS = P::LOADS;
@@ -719,11 +721,14 @@ __device__ __forceinline__ void attend_few(const AttendArgs &a, int unit, int z,
 // share the keys and values in LDS, two buffers of NK rows: while one is used the other is filled, a quarter by
 // each wave, with one barrier per NK keys. Two workgroups share a CU (heads of 256: one), so that one's products
 // run beside the other's lookups and barriers.
-// 2048 tokens after 6144, 32 heads on 8 of 128: 227 to 244 us, 1.0 PFLOP/s (a product of two 8192 x 8192 matrices: 1.2, of
-// larger ones 1.37). What bounds it then is power: the clock falls to 1.75 GHz, and the same call on zeros takes
+// 2048 tokens after 6144, 32 heads on 8 of 128: 227 to 244 us (card to card), 1.0 PFLOP/s (a product of two 8192 x 8192
+// matrices: 1.2, of larger ones 1.37). What bounds it then is power: the clock falls to 1.75 GHz, and the same call on zeros takes
 // 199 us at 2.35. Of the 240 us, without the loads into LDS 30 less, without the softmax 20 less. Two groups of 32
 // columns per wave would halve the LDS reads, but need the second half of the register file, which vector
-// instructions cannot use: 453 us. Heads of 64: 152 us for the same rows, bound by the softmax's vector work.
+// instructions cannot use: 453 us. As it is six registers are spilled, outside the loop; pages of other sizes than
+// multiples of 16 take 14, of which a step reads two, and a lookup's result from LDS before every load: 337 us with
+// pages of 24, 347 with pages of one. Heads of 64: 143 to 152 us for the same rows, bound by the softmax's vector
+// work; of 256 (16 on 4) 333, with one workgroup per CU, so nothing runs beside a wait.
 template <int D, bool WHOLE>
 __device__ __forceinline__ void attend_many(const AttendArgs &a, int unit, int z, Space<D, WHOLE> &space) {
     constexpr int NK = D == 256 ? 32 : 64, KT = NK / 32, BYTES = NK * 2 * D;
@@ -1127,9 +1132,11 @@ struct Plan {
                 if (window == 0) break;
             }
         };
-        // Workgroups of few rows need places of their own beside those of many: chunks of 511 and 71 after up to 4095
-        // beside 20 single tokens, 16 heads on 8, in 1 / 2 / 3 / 4 / 6 splits 98 / 74 / 65 / 68 / 77 us; 64 single
-        // tokens of up to 8000 beside a chunk of 511, 32 on 8, in 1 / 2 / 3 / 4 245 / 236 / 258 / 276.
+        // Workgroups of few rows need places of their own beside those of many. In at most 1 / 2 / 3 / 4 / 6 / 8 splits:
+        // chunks of 511 and 71 after up to 4095 beside 20 single tokens, 16 heads on 8 of 128, 99 / 69 / 63 / 63 / 63 / 63
+        // us; 32 on 8, 511 after 8000 beside 64 247 / 233 / 265 / 266 / 265 / 266, 128 after 4000 beside 8 81 / 52 / 43 /
+        // 40 / 36 / 37, 256 after 16000 beside 16 312 / 184 / 147 / 146 / 149 / 154, two of 300 after 2000 beside 32
+        // 62 / 52 / 59 / 59 / 59 / 59; 16 on 4 of 256, 256 after 8000 beside 8 339 / 183 / 129 / 105 / 93 / 92.
         const int64_t units = (rows + MANY - 1) / MANY * n_kv_heads, beside = few ? 288 / units : MOST_SPLITS;
         const int64_t few_most = std::max<int64_t>(1, FEW_PARTS / std::max<int64_t>(1, few_units));
         const int64_t many_most = std::max<int64_t>(1, std::min(beside, MANY_PARTS / std::max<int64_t>(1, many_units)));
