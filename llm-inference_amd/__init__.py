@@ -32,6 +32,8 @@ __all__ = [
     "dump_close", "dump_enabled", "attention_forward_noalloc", "EXPORTED_SYMBOLS",
     "qk_norm_rope_attention_one_pass", "attention_one_pass_bytes", "attention_one_pass_supported",
     "ROPE_PLAIN", "ROPE_LINEAR", "ROPE_YARN", "rope_frequencies", "qk_norm_rope_paged",
+    "lora_projection_forward", "lora_projection_workspace_floats", "sample_rows_forward",
+    "sample_rows_workspace_floats",
     "attention_paged_forward", "attention_paged_workspace_floats", "logits_penalty_forward",
 ]
 
@@ -51,7 +53,8 @@ EXPORTED_SYMBOLS = [
     "qk_norm_rope_attention_forward", "qk_norm_rope_attention_one_pass",
     "attention_one_pass_bytes", "attention_one_pass_supported",
     "rope_frequencies", "qk_norm_rope_paged", "attention_paged_forward",
-    "attention_paged_workspace_floats", "logits_penalty_forward",
+    "attention_paged_workspace_floats", "logits_penalty_forward", "lora_projection_forward",
+    "lora_projection_workspace_floats", "sample_rows_forward", "sample_rows_workspace_floats",
 ]
 
 
@@ -75,6 +78,12 @@ class PagedBatch(ctypes.Structure):
                 ("head_stride", _i64), ("page_table", _vp), ("q_start", _vp), ("kv_len", _vp),
                 ("n_seqs", _i), ("n_pages", _i), ("page_size", _i), ("table_pages", _i),
                 ("n_kv_heads", _i), ("head_dim", _i)]
+
+
+class LoraBatch(ctypes.Structure):
+    """include/llm_amd/batch.h LoraBatch."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scale", _vp), ("q_start", _vp), ("adapter", _vp),
+                ("n_seqs", _i), ("n_adapters", _i), ("rank", _i)]
 
 
 _SIGS = {
@@ -107,6 +116,10 @@ _SIGS = {
     "attention_paged_forward": (None, [_vp] * 4 + [_i] * 5 + [_f, _i64, _i64, _vp]),
     "attention_paged_workspace_floats": (_sz, [_i] * 7),
     "logits_penalty_forward": (None, [_vp] * 12 + [_i] * 5 + [_i64, _i64, _vp]),
+    "lora_projection_forward": (None, [_vp] * 6 + [_i] * 3 + [_i64] * 3 + [_vp]),
+    "lora_projection_workspace_floats": (_sz, [_i] * 4),
+    "sample_rows_forward": (None, [_vp] * 9 + [_i, _i, _i64, _vp]),
+    "sample_rows_workspace_floats": (_sz, [_i, _i]),
     "dump_open": (None, [ctypes.c_char_p]),
     "dump_close": (None, []),
     "dump_enabled": (_i, []),
@@ -605,3 +618,107 @@ def logits_penalty_forward(out, logits, tokens=None, prompt_len=None, token_len=
           _dense("bias_len", bias_len, torch.int32, (rows,)),
           allowed if allowed is None else _dense("allowed", allowed, allowed.dtype, (rows, wide["allowed"])),
           rows, vocab, wide["tokens"], wide["bias_tokens"], wide["allowed"], *strides, _stream(stream))
+
+
+# ---- what the requests of a batch bring of their own (include/llm_amd/batch.h); tensors alone, as above ----
+
+def lora_projection_workspace_floats(n_tokens, n_out, n_in, rank):
+    """Floats of ws for lora_projection_forward with these sizes and with fewer tokens or a lower rank (0: no
+    adapters)."""
+    floats = lib().lora_projection_workspace_floats(n_tokens, n_out, n_in, rank)
+    check()
+    return floats
+
+
+def _matrix_rows(name, t, shape):
+    """(address, elements between rows) of rows of 16-bit elements, contiguous within a row."""
+    _on_device(name, t, _bits16())
+    if tuple(t.shape) != tuple(shape) or (shape[1] > 1 and t.stride(1) != 1):
+        raise LlmError(f"{name} must have shape {tuple(shape)} with contiguous rows, got {tuple(t.shape)}")
+    return t.data_ptr() or None, t.stride(0) if shape[0] > 1 else max(shape[1], 1)
+
+
+def _workspace(ws, need, what):
+    import torch
+    if ws is not None:
+        _on_device("ws", ws, (torch.float32,))
+        _dense("ws", ws, torch.float32, ws.shape)
+    have = 0 if ws is None else ws.numel()
+    if have < need:
+        raise LlmError(f"ws holds {have} floats, {what} needs {need}")
+    return _ptr(ws)
+
+
+def lora_projection_forward(out, x, w=None, lora_a=None, lora_b=None, lora_scale=None, q_start=None, adapter=None,
+                            residual=None, ws=None, stream=None):
+    """out [tokens, n_out] = residual + x [tokens, n_in] wT, and for the rows q_start[s] .. q_start[s + 1] - 1 of
+    sequence s with the adapter a = adapter[s] + lora_scale[a] (x lora_a[a]T) lora_b[a]T. w [n_out, n_in], lora_a
+    [adapters, rank, n_in], lora_b [adapters, n_out, rank]; each of w, the adapters (lora_a, lora_b, q_start and
+    adapter together), lora_scale and residual may be None. ws: a float32 tensor of at least
+    lora_projection_workspace_floats(...) floats (None where that is 0), kept between calls that do not overlap."""
+    if _native and _native.lora_projection_forward(out, x, w, lora_a, lora_b, lora_scale, q_start, adapter, residual,
+                                                   ws, stream):
+        return
+    import torch
+    for name, t in (("out", out), ("x", x)):
+        _on_device(name, t, _bits16())
+        if t.dim() != 2:
+            raise LlmError(f"{name} must have two dimensions, got {tuple(t.shape)}")
+    n, n_in, n_out = x.shape[0], x.shape[1], out.shape[1]
+    out_at, out_stride = _matrix_rows("out", out, (n, n_out))
+    x_at, x_stride = _matrix_rows("x", x, (n, n_in))
+    residual_at, residual_stride = (None, n_out) if residual is None else _matrix_rows("residual", residual, (n, n_out))
+    if w is not None:
+        _on_device("w", w, _bits16())
+        _dense("w", w, w.dtype, (n_out, n_in))
+    batch, rank = None, 0
+    parts = dict(lora_a=lora_a, lora_b=lora_b, q_start=q_start, adapter=adapter)
+    if any(t is not None for t in parts.values()) or lora_scale is not None:
+        for name, t in parts.items():
+            if t is None:
+                raise LlmError(f"adapters need lora_a, lora_b, q_start and adapter: {name} is None")
+        for name, t in (("lora_a", lora_a), ("lora_b", lora_b)):
+            _on_device(name, t, _bits16())
+        if lora_a.dim() != 3:
+            raise LlmError(f"lora_a must have shape [adapters, rank, n_in], got {tuple(lora_a.shape)}")
+        _on_device("adapter", adapter, (torch.int32,))
+        adapters, rank, seqs = lora_a.shape[0], lora_a.shape[1], adapter.numel()
+        batch = LoraBatch(_dense("lora_a", lora_a, lora_a.dtype, (adapters, rank, n_in)),
+                          _dense("lora_b", lora_b, lora_b.dtype, (adapters, n_out, rank)),
+                          _dense("lora_scale", lora_scale, torch.float32, (adapters,)),
+                          _dense("q_start", q_start, torch.int32, (seqs + 1,)),
+                          _dense("adapter", adapter, torch.int32, (seqs,)), seqs, adapters, rank)
+    ws_at = _workspace(ws, lora_projection_workspace_floats(n, n_out, n_in, rank), "the projection")
+    _call(lib().lora_projection_forward, out_at, x_at, _ptr(w), residual_at,
+          None if batch is None else ctypes.byref(batch), ws_at, n, n_out, n_in, out_stride, x_stride,
+          residual_stride, _stream(stream))
+
+
+def sample_rows_workspace_floats(rows, vocab):
+    """Floats of ws for sample_rows_forward with these sizes and with smaller ones."""
+    floats = lib().sample_rows_workspace_floats(rows, vocab)
+    check()
+    return floats
+
+
+def sample_rows_forward(out, logits, u, temperature=None, top_k=None, top_p=None, min_p=None, logprob=None, ws=None,
+                        stream=None):
+    """A token of each row of logits [rows, vocab] into out (int32 [rows]), drawn with the given u (float32 [rows],
+    in [0, 1)) from what temperature, top_k, top_p and min_p ([rows] each, or None: off) leave; logprob (float32
+    [rows]): ln of its probability there. ws: a float32 tensor of at least sample_rows_workspace_floats(...) floats
+    (None where that is 0), kept between calls that do not overlap."""
+    if _native and _native.sample_rows_forward(out, logits, u, temperature, top_k, top_p, min_p, logprob, ws, stream):
+        return
+    import torch
+    _on_device("logits", logits, _bits16())
+    if logits.dim() != 2:
+        raise LlmError(f"logits must have shape [rows, vocab], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    logits_at, stride = _matrix_rows("logits", logits, (rows, vocab))
+    f32, i32 = torch.float32, torch.int32
+    columns = [_dense(name, t, dtype, (rows,)) for name, t, dtype in (
+        ("out", out, i32), ("logprob", logprob, f32), ("temperature", temperature, f32), ("top_k", top_k, i32),
+        ("top_p", top_p, f32), ("min_p", min_p, f32), ("u", u, f32))]
+    ws_at = _workspace(ws, sample_rows_workspace_floats(rows, vocab), "the draw")
+    _call(lib().sample_rows_forward, columns[0], columns[1], logits_at, *columns[2:], ws_at, rows, vocab, stride,
+          _stream(stream))

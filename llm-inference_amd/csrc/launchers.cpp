@@ -26,6 +26,7 @@
 #include <type_traits>
 #include <utility>
 
+#include "llm_amd/batch.h"
 #include "llm_amd/kernels.h"
 #include "llm_amd/paged.h"
 
@@ -361,6 +362,115 @@ PyObject *native_logits_penalty_forward(PyObject *, PyObject *const *o, Py_ssize
         });
 }
 
+// Rows [n, width] of 16-bit elements, contiguous within a row.
+bool take_matrix(PyObject *o, int64_t n, int64_t width, bf16 *&out, int64_t &stride) {
+    const at::Tensor *t = tensor_here(o);
+    if (!t || !bits16(*t) || t->dim() != 2 || t->size(0) != n || t->size(1) != width ||
+        (width > 1 && t->stride(1) != 1))
+        return false;
+    out = (bf16 *)t->data_ptr();
+    stride = n > 1 ? t->stride(0) : width;
+    return true;
+}
+
+// A contiguous tensor of 16-bit elements, or None.
+bool take_bits16(PyObject *o, std::initializer_list<int64_t> shape, const bf16 *&out) {
+    out = nullptr;
+    if (o == Py_None) return true;
+    const at::Tensor *t = tensor_here(o);
+    return t && bits16(*t) && take_dense(o, nullptr, shape, out);
+}
+
+// A workspace of the floats that `need` says, or None where that is 0. No error of an earlier call is
+// there, so that one of need() is its own; the general way meets and reports it again.
+template <class Need>
+bool take_workspace(PyObject *o, float *&ws, Need need) {
+    if (llm_last_error()) return false;
+    const size_t floats = need();
+    if (llm_last_error()) {
+        llm_clear_error();
+        return false;
+    }
+    ws = nullptr;
+    if (o == Py_None) return floats == 0;
+    const at::Tensor *t = tensor_here(o);
+    if (!t || t->scalar_type() != at::kFloat || !t->is_contiguous()) return false;
+    ws = (float *)t->data_ptr();
+    return (size_t)t->numel() >= floats;
+}
+
+PyObject *native_lora_projection_forward(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
+    bf16 *out, *x, *residual = nullptr;
+    const bf16 *w;
+    LoraBatch l = {};
+    float *ws;
+    Arg stream;
+    bool adapters = false;
+    int64_t n = 0, n_out = 0, n_in = 0, strides[3];
+    return take_and_launch(
+        [&] {
+            if (n_args != 11) return false;
+            const at::Tensor *to = tensor_here(o[0]), *from = tensor_here(o[1]);
+            if (!to || !from || to->dim() != 2 || from->dim() != 2) return false;
+            n = from->size(0), n_in = from->size(1), n_out = to->size(1);
+            strides[2] = n_out;
+            if (n > INT_MAX || n_in > INT_MAX || n_out > INT_MAX || !n || !n_out || !n_in ||
+                !take_matrix(o[0], n, n_out, out, strides[0]) || !take_matrix(o[1], n, n_in, x, strides[1]) ||
+                !take_bits16(o[2], {n_out, n_in}, w) ||
+                (o[8] != Py_None && !take_matrix(o[8], n, n_out, residual, strides[2])))
+                return false;
+            adapters = o[3] != Py_None;
+            if (adapters) {
+                const at::Tensor *a = tensor_here(o[3]), *which = tensor_here(o[7]);
+                if (!a || !which || a->dim() != 3 || which->dim() != 1 || o[4] == Py_None || o[6] == Py_None) return false;
+                const int64_t count = a->size(0), rank = a->size(1), seqs = which->size(0);
+                if (count > INT_MAX || rank > INT_MAX || seqs >= INT_MAX) return false;
+                l.n_seqs = (int)seqs, l.n_adapters = (int)count, l.rank = (int)rank;
+                if (!take_bits16(o[3], {count, rank, n_in}, l.a) || !take_bits16(o[4], {count, n_out, rank}, l.b) ||
+                    !take_dense(o[5], &FLOAT32, {count}, l.scale) || !take_dense(o[6], &INT32, {seqs + 1}, l.q_start) ||
+                    !take_dense(o[7], &INT32, {seqs}, l.adapter))
+                    return false;
+            } else if (o[4] != Py_None || o[5] != Py_None || o[6] != Py_None || o[7] != Py_None) {
+                return false;
+            }
+            return take_workspace(o[9], ws, [&] {
+                       return lora_projection_workspace_floats((int)n, (int)n_out, (int)n_in, l.rank);
+                   }) && take<hipStream_t>(o[10], stream);
+        },
+        [&] {
+            lora_projection_forward(out, x, w, residual, adapters ? &l : nullptr, ws, (int)n, (int)n_out, (int)n_in,
+                                    strides[0], strides[1], strides[2], (hipStream_t)stream.p);
+        });
+}
+
+PyObject *native_sample_rows_forward(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
+    bf16 *logits;
+    int *out;
+    float *logprob, *ws;
+    const float *u, *temperature, *top_p, *min_p;
+    const int *top_k;
+    Arg stream;
+    int64_t rows = 0, vocab = 0, stride = 0;
+    return take_and_launch(
+        [&] {
+            if (n_args != 10) return false;
+            const at::Tensor *t = tensor_here(o[1]);
+            if (!t || t->dim() != 2) return false;
+            rows = t->size(0), vocab = t->size(1);
+            return rows <= INT_MAX && vocab > 0 && vocab <= INT_MAX && take_matrix(o[1], rows, vocab, logits, stride) &&
+                   take_dense(o[0], &INT32, {rows}, out) && take_dense(o[2], &FLOAT32, {rows}, u) &&
+                   take_dense(o[3], &FLOAT32, {rows}, temperature) && take_dense(o[4], &INT32, {rows}, top_k) &&
+                   take_dense(o[5], &FLOAT32, {rows}, top_p) && take_dense(o[6], &FLOAT32, {rows}, min_p) &&
+                   take_dense(o[7], &FLOAT32, {rows}, logprob) &&
+                   take_workspace(o[8], ws, [&] { return sample_rows_workspace_floats((int)rows, (int)vocab); }) &&
+                   take<hipStream_t>(o[9], stream);
+        },
+        [&] {
+            sample_rows_forward(out, logprob, logits, temperature, top_k, top_p, min_p, u, ws, (int)rows, (int)vocab,
+                                stride, (hipStream_t)stream.p);
+        });
+}
+
 PyObject *init(PyObject *, PyObject *error) {
     Py_INCREF(error);
     Py_XSETREF(g_error, error);
@@ -391,6 +501,8 @@ PyMethodDef methods[] = {
     {"qk_norm_rope_paged", (PyCFunction)(void *)native_qk_norm_rope_paged, METH_FASTCALL, nullptr},
     {"attention_paged_forward", (PyCFunction)(void *)native_attention_paged_forward, METH_FASTCALL, nullptr},
     {"logits_penalty_forward", (PyCFunction)(void *)native_logits_penalty_forward, METH_FASTCALL, nullptr},
+    {"lora_projection_forward", (PyCFunction)(void *)native_lora_projection_forward, METH_FASTCALL, nullptr},
+    {"sample_rows_forward", (PyCFunction)(void *)native_sample_rows_forward, METH_FASTCALL, nullptr},
     {"init", init, METH_O, "The exception class of library errors."},
     {nullptr, nullptr, 0, nullptr},
 };
