@@ -40,7 +40,7 @@ typedef struct {
  * is not there for rows of sequences without one. w: [n_out, n_in], 16-byte aligned, or NULL: no product,
  * as beside a projection computed elsewhere. residual NULL: none; it may be out, row on row. lora NULL: no
  * adapters, and every row is computed. Otherwise nothing may overlap. x has rows x_stride elements apart (a multiple
- * of 8, 16-byte aligned), out and residual rows out_stride and residual_stride apart, of any alignment (multiples
+ * of 8 up to 4194304, 16-byte aligned), out and residual rows out_stride and residual_stride apart, of any alignment (multiples
  * of 8 are faster). n_in is a multiple of 8.
  * Products and sums are in 32 bits and rounded to bf16 once, at the end; a[a] x is kept to 16 bits of its
  * mantissa in front of b[a] (as a bf16 and the bf16 of what that leaves). The order of the sums depends on the

@@ -324,6 +324,22 @@ __device__ __forceinline__ bool wait_gives_up(long long spins, long long limit, 
     return false;
 }
 
+// The number of leading i in [0, n) with pred(i), pred not increasing: 64 probes per round, one per lane.
+// Whatever pred says, the result is in [0, n] and pred is asked about [0, n) alone.
+template <class Pred>
+__device__ __forceinline__ int count_leading(int n, Pred pred) {
+    const int lane = threadIdx.x & 63;
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) / 64;
+        const int64_t at = lo + (int64_t)(lane + 1) * step - 1;  // the last of the lane's share
+        const int met = __popcll(__ballot(at < hi && pred((int)at)));
+        hi = min(hi, lo + met * step + step - 1);
+        lo += met * step;
+    }
+    return lo;
+}
+
 // Larger value wins, equal values keep the lower index; NaN is never taken.
 __device__ __forceinline__ void amax_pair(float &v, int &i, float v2, int i2) {
     if (v2 > v || (v2 == v && i2 < i)) {

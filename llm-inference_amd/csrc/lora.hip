@@ -1,4 +1,10 @@
 // A projection of many rows with the low-rank adapters of their sequences (include/llm_amd/batch.h).
+//
+// out = x Wt + low Bt, low = scale x At: the second term is the first one's sum carried on over the rank, with rows
+// of `low` for rows of x and an adapter's b for W. low is kept as two bf16, the value and what that leaves (16 bits
+// of mantissa), side by side, so the sum goes over twice the rank.
+#include <math.h>
+
 #include <algorithm>
 
 #include "common.h"
@@ -8,84 +14,515 @@ using namespace llm;
 
 namespace {
 
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+#define LLM_LDS __attribute__((address_space(3)))
+typedef LLM_LDS char lds_char;
+
+constexpr int CUS = 256, XCDS = 8;
+constexpr int NO_ADAPTER = -1, NO_SEQUENCE = -2;
 
 struct LoraArgs {
     bf16 *out;
     const bf16 *x, *w, *residual;
-    const bf16 *a, *b;
+    const bf16 *a, *b;       // a null: no adapters, every row is of one sequence
     const float *scale;
     const int *q_start, *adapter;
-    float *low;  // [n_tokens, rank]
+    bf16 *low;               // [n_tokens, 2 rank]: value, remainder
+    int *owner;              // [n_tokens]: the row's adapter, NO_ADAPTER or NO_SEQUENCE
+    float *part;             // [splits, n_tokens, part_width], or null: straight to out
     int64_t out_stride, x_stride, residual_stride;
     int n_tokens, n_out, n_in, n_seqs, n_adapters, rank;
+    int part_width;
+    int splits, split_steps;  // of the product's sum, steps of 64 each
+    int m_tiles, n_tiles, low_groups;
+    bool wide;               // out and residual take 16 bytes at a time
 };
 
-__device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
-                                                   0, 0);
+// What is loaded for places past an operand's end.
+__device__ const u32x4 g_zeros = {0, 0, 0, 0};
+
+template <int S>
+struct Mfma;
+template <>
+struct Mfma<32> {
+    typedef f32x16 Acc;
+    static constexpr int K = 16, REGS = 16;
+    static __device__ __forceinline__ f32x16 mul(const u32x4 &a, const u32x4 &b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    }
+    // The first of the four rows that registers 4 i .. 4 i + 3 hold.
+    static __device__ __forceinline__ int row(int i, int lane) { return 8 * i + 4 * (lane / 32); }
+};
+template <>
+struct Mfma<16> {
+    typedef f32x4 Acc;
+    static constexpr int K = 32, REGS = 4;
+    static __device__ __forceinline__ f32x4 mul(const u32x4 &a, const u32x4 &b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ int row(int, int lane) { return 4 * (lane / 16); }
+};
+
+// 64 lanes' 16 bytes into LDS at `to` on, without passing registers: the wave waits for it with wait_loads.
+__device__ __forceinline__ void load_to_lds(unsigned to, const void *base, unsigned offset) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_to_lds(unsigned to, const void *at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
 }
 
-// The sequence of row t, or -1.
-__device__ __forceinline__ int sequence_of(const LoraArgs &l, int t) {
-    int lo = 0, hi = l.n_seqs;  // the first sequence that ends behind t
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (gptr(l.q_start)[mid + 1] <= t) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo < l.n_seqs && gptr(l.q_start)[lo] <= t && t < gptr(l.q_start)[lo + 1] ? lo : -1;
+// ------------------------------------------------------------------------------------------
+// the rows' sequences
+// ------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ int start_of(const LoraArgs &l, int s) {
+    return max(0, min(l.n_tokens, gptr(l.q_start)[s]));
 }
-// Its adapter: -1 none, -2 no sequence.
-__device__ __forceinline__ int adapter_of(const LoraArgs &l, int t) {
-    if (!l.a) return -1;
-    const int s = sequence_of(l, t);
-    if (s < 0) return -2;
+
+// 16 rows of one sequence at most. A sequence of n rows from f on has at most (f + n) / 16 - f / 16 + 1 tiles, so
+// those of sequence s are found from f / 16 + s on, of n_tokens / 16 + n_seqs.
+struct RowTile {
+    int first, rows, adapter;  // rows 0: no tile
+};
+__device__ __forceinline__ RowTile row_tile(const LoraArgs &l, int i) {
+    RowTile t = {16 * i, 0, NO_ADAPTER};
+    if (!l.a) {
+        t.rows = min(16, l.n_tokens - t.first);
+        return t;
+    }
+    const int s = count_leading(l.n_seqs, [&](int j) { return start_of(l, j) / 16 + j <= i; }) - 1;
+    if (s < 0) return t;
+    const int f = start_of(l, s), n = start_of(l, s + 1) - f, j = i - (f / 16 + s);
+    t.first = f + 16 * j;
+    t.rows = max(0, min(16, n - 16 * j));
     const int a = gptr(l.adapter)[s];
-    return (unsigned)a < (unsigned)l.n_adapters ? a : -1;
+    if ((unsigned)a < (unsigned)l.n_adapters) t.adapter = a;
+    return t;
 }
 
-// low[t] = scale (a x[t]), a wave per row and element.
-__global__ __launch_bounds__(256) void shrink_kernel(LoraArgs l) {
-    const int t = blockIdx.y, j = blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63;
-    const int a = adapter_of(l, t);
-    if (a < 0 || j >= l.rank) return;
-    const bf16 *row = l.a + ((int64_t)a * l.rank + j) * l.n_in, *x = l.x + t * l.x_stride;
-    float sum = 0;
-    for (int i = lane * 8; i < l.n_in; i += 512) sum = dot8(ld16(row + i), ld16(x + i), sum);
-    sum = wave_sum(sum);
-    if (lane == 0) l.low[(int64_t)t * l.rank + j] = sum * (l.scale ? gptr(l.scale)[a] : 1.0f);
+
+// low of 16 rows and LOW elements of the rank: the waves of a workgroup take a part of the sum each.
+constexpr int LOW = 64;
+template <int WAVES>
+__device__ __forceinline__ void shrink(const LoraArgs &l, int tile, int group, float *lds) {
+    const int lane = threadIdx.x & 63, wave = wave_id(), r0 = group * LOW;
+    const RowTile t = row_tile(l, tile);
+    if (group == 0) {
+        if (tile == 0) {
+            const int begin = start_of(l, 0), end = max(begin, start_of(l, l.n_seqs));
+            for (int i = threadIdx.x; i < l.n_tokens; i += 64 * WAVES)
+                if (i < begin || i >= end) gptr(l.owner)[i] = NO_SEQUENCE;
+        }
+        if ((int)threadIdx.x < t.rows) gptr(l.owner)[t.first + threadIdx.x] = t.adapter;
+    }
+    if (t.rows == 0 || t.adapter < 0) return;
+    const bf16 *x = l.x + (t.first + min(lane % 16, t.rows - 1)) * l.x_stride;
+    const bf16 *a = l.a + (int64_t)t.adapter * l.rank * l.n_in;
+    const bf16 *row[LOW / 16];
+#pragma unroll
+    for (int j = 0; j < LOW / 16; j++) row[j] = a + (int64_t)min(r0 + j * 16 + lane % 16, l.rank - 1) * l.n_in;
+    const int tiles = min(LOW / 16, (l.rank - r0 + 15) / 16);
+    const int part = (l.n_in + 32 * WAVES - 1) / (32 * WAVES) * 32, from = wave * part, to = min(l.n_in, from + part);
+    f32x4 acc[LOW / 16] = {};
+    constexpr int U = 4;
+    for (int k0 = from; k0 < to; k0 += 32 * U) {
+        u32x4 xs[U], as[U][LOW / 16];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = k0 + 32 * u + lane / 16 * 8;
+            xs[u] = k < to ? ld16(x + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < LOW / 16; j++) as[u][j] = k < to && j < tiles ? ld16(row[j] + k) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < LOW / 16; j++) acc[j] = Mfma<16>::mul(as[u][j], xs[u], acc[j]);
+    }
+    float *mine = lds + wave * 16 * LOW;
+#pragma unroll
+    for (int j = 0; j < LOW / 16; j++) *(f32x4 *)(mine + lane % 16 * LOW + j * 16 + lane / 16 * 4) = acc[j];
+    __syncthreads();
+    const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
+    for (int i = threadIdx.x; i < 16 * LOW; i += 64 * WAVES) {
+        const int m = i / LOW, r = r0 + i % LOW;
+        if (m >= t.rows || r >= l.rank) continue;
+        float sum = 0;
+        for (int w = 0; w < WAVES; w++) sum += lds[w * 16 * LOW + i];
+        sum *= scale;
+        const float value = round_bf(sum), rest = fabsf(value) < INFINITY ? sum - value : 0.0f;
+        LLM_GLOBAL uint16_t *low = gptr((uint16_t *)l.low) + (int64_t)(t.first + m) * 2 * l.rank + r;
+        low[0] = (uint16_t)f2bf(value);
+        low[l.rank] = (uint16_t)f2bf(rest);
+    }
 }
 
-// 16 rows by 16 columns per wave: lane's row l % 16, columns 4 (l / 16) .. + 3.
-__global__ __launch_bounds__(256) void project_kernel(LoraArgs l) {
-    const int lane = threadIdx.x & 63, n0 = (blockIdx.x * 4 + wave_id()) * 16, t0 = blockIdx.y * 16;
-    if (n0 >= l.n_out) return;
-    const int t = t0 + lane % 16, k0 = lane / 16 * 8;
-    f32x4 acc = {0, 0, 0, 0};
-    if (l.w) {
-        const bf16 *w = l.w + (int64_t)min(n0 + lane % 16, l.n_out - 1) * l.n_in, *x = l.x + min(t, l.n_tokens - 1) * l.x_stride;
-        for (int k = k0; k - k0 < l.n_in; k += 32) {
-            u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-            if (k < l.n_in) a = ld16(w + k), b = ld16(x + k);
-            acc = mfma(a, b, acc);
+// Whether NaN or infinities were among eight elements; they are zeros then.
+__device__ __forceinline__ bool clear_unfit_of(u32x4 &v) {
+    bool found = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        if ((v[j] & 0x7f80u) == 0x7f80u) v[j] &= 0xffff0000u, found = true;
+        if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] &= 0xffffu, found = true;
+    }
+    return found;
+}
+// What those that b has for column n add to row m.
+__device__ __forceinline__ float unfit_term(const LoraArgs &l, int m, int n, int adapter) {
+    const uint16_t *low = (const uint16_t *)l.low + (int64_t)m * 2 * l.rank;
+    const uint16_t *b = (const uint16_t *)l.b + ((int64_t)adapter * l.n_out + n) * l.rank;
+    float y = 0.0f;
+    for (int j = 0; j < l.rank; j++) {
+        const float v = bf2f(gptr(b)[j]);
+        if (!(fabsf(v) < INFINITY)) y += (bf2f(gptr(low)[j]) + bf2f(gptr(low)[l.rank + j])) * v;
+    }
+    return y;
+}
+
+// ------------------------------------------------------------------------------------------
+// the product
+// ------------------------------------------------------------------------------------------
+
+// TM rows by TN columns of a workgroup, in waves of RM by RN, on MFMAs of side S; 64 elements of the sum a step,
+// STAGES steps' operands in LDS. A row's 128 bytes of a step lie as eight 16-byte chunks, chunk c of row r at
+// c ^ (r % 8): the rows that a product reads at one chunk then lie in different banks.
+template <int TM_, int TN_, int RM_, int RN_, int S_, int STAGES_>
+struct Shape {
+    static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, S = S_, STAGES = STAGES_;
+    static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / S, NT = RN / S;
+    static constexpr int BYTES = (TM + TN) * 128;                    // of a stage
+    static constexpr int X_LOADS = (TM / 8 + WAVES - 1) / WAVES;     // per wave; with fewer rows several load the same
+    static constexpr int W_LOADS = TN / 8 / WAVES;
+    static constexpr int LOADS = X_LOADS + W_LOADS;
+    static constexpr int SLAB = S * (RN + 4);                        // floats of a wave's rows on their way out
+    static constexpr int SLABS = WAVES * SLAB * 4;
+    static constexpr int SHRINK = WAVES * 16 * LOW * 4;
+    static constexpr int LDS0 = STAGES * BYTES > SLABS ? STAGES * BYTES : SLABS;
+    static constexpr int LDS = LDS0 > SHRINK ? LDS0 : SHRINK;
+    static_assert(TN / 8 % WAVES == 0 && (TM / 8 % WAVES == 0 || WAVES % (TM / 8) == 0), "loads per wave");
+};
+
+template <class G>
+__global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
+    __shared__ __attribute__((aligned(128))) char lds[G::LDS + G::TM * 4 + 4];
+    int *owner = (int *)(lds + G::LDS), *unfit = owner + G::TM;
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    if ((int)blockIdx.x < l.low_groups) {
+        const int groups = (l.rank + LOW - 1) / LOW;
+        shrink<G::WAVES>(l, blockIdx.x / groups, blockIdx.x % groups, (float *)lds);
+        return;
+    }
+    // the tiles of one XCD, whose workgroups every eighth one is, lie side by side
+    const int tiles = l.m_tiles * l.n_tiles * l.splits, block = blockIdx.x - l.low_groups;
+    const int each = tiles / XCDS, more = tiles % XCDS, xcd = block % XCDS;
+    const int at = xcd * each + min(xcd, more) + block / XCDS;
+    const int m0 = at % l.m_tiles * G::TM, n0 = at / l.m_tiles % l.n_tiles * G::TN, split = at / (l.m_tiles * l.n_tiles);
+    const bool join = l.part != nullptr, adapters = l.a && !join;
+    if (adapters && (int)threadIdx.x < G::TM)
+        owner[threadIdx.x] = m0 + (int)threadIdx.x < l.n_tokens ? gptr(l.owner)[m0 + threadIdx.x] : NO_SEQUENCE;
+    if (threadIdx.x == 0) *unfit = 0;
+
+    // loads: lane's row lane / 8 and chunk lane % 8 of eight rows
+    const unsigned base = (unsigned)(uintptr_t)(lds_char *)lds;
+    const int row = lane / 8, chunk = lane % 8 ^ row;
+    unsigned x_at[G::X_LOADS], w_at[G::W_LOADS];   // bytes from the tile's first row
+    int x_row[G::X_LOADS];
+    const auto x_group = [&](int i) { return G::TM / 8 >= G::WAVES ? wave * G::X_LOADS + i : wave % (G::TM / 8); };
+    const auto w_group = [&](int i) { return wave * G::W_LOADS + i; };
+#pragma unroll
+    for (int i = 0; i < G::X_LOADS; i++) {
+        x_row[i] = x_group(i) * 8 + row;
+        x_at[i] = (unsigned)(min(x_row[i], l.n_tokens - 1 - m0) * l.x_stride * 2) + chunk * 16;
+    }
+#pragma unroll
+    for (int i = 0; i < G::W_LOADS; i++)
+        w_at[i] = (unsigned)min(w_group(i) * 8 + row, l.n_out - 1 - n0) * (unsigned)l.n_in * 2 + chunk * 16;
+    const char *x_from = (const char *)(l.x + m0 * l.x_stride), *w_from = (const char *)(l.w + (int64_t)n0 * l.n_in);
+    const int all_steps = l.w ? (l.n_in + 63) / 64 : 0, whole_steps = l.w ? l.n_in / 64 : 0;
+    int step = split * l.split_steps;
+    const int last_step = min(all_steps, step + l.split_steps);
+    int current = NO_ADAPTER, piece = 0;  // the adapter whose part of the sum comes next
+    unsigned of_adapter = 0;              // stages that hold some of it
+    const int pieces = (2 * l.rank + 63) / 64;
+    __syncthreads();
+
+    // Requests the next step's operands into stage `to`; false after the last.
+    const auto request = [&](int to) {
+        const unsigned xs = base + to * G::BYTES, ws = xs + G::TM * 128;
+        if (step < whole_steps && step < last_step) {
+            const char *x = x_from + (int64_t)step * 128, *w = w_from + (int64_t)step * 128;
+#pragma unroll
+            for (int i = 0; i < G::X_LOADS; i++) load_to_lds(xs + x_group(i) * 1024, x, x_at[i]);
+#pragma unroll
+            for (int i = 0; i < G::W_LOADS; i++) load_to_lds(ws + w_group(i) * 1024, w, w_at[i]);
+            step++;
+            return true;
+        }
+        if (step < last_step) {  // the last step of a width that is no multiple of 64
+            const char *x = x_from + (int64_t)step * 128, *w = w_from + (int64_t)step * 128;
+            const bool there = step * 64 + chunk * 8 < l.n_in;
+#pragma unroll
+            for (int i = 0; i < G::X_LOADS; i++)
+                load_to_lds(xs + x_group(i) * 1024, there ? x + x_at[i] : (const char *)&g_zeros);
+#pragma unroll
+            for (int i = 0; i < G::W_LOADS; i++)
+                load_to_lds(ws + w_group(i) * 1024, there ? w + w_at[i] : (const char *)&g_zeros);
+            step++;
+            return true;
+        }
+        if (!adapters) return false;
+        if (piece == 0) {  // the next higher adapter of the tile's rows
+            int next = INT32_MAX;
+#pragma unroll
+            for (int i = 0; i < (G::TM + 63) / 64; i++) {
+                const int o = owner[min(i * 64 + lane, G::TM - 1)];
+                if (o > current) next = min(next, o);
+            }
+            for (int d = 1; d < 64; d *= 2) next = min(next, __shfl_xor(next, d));
+            current = __builtin_amdgcn_readfirstlane(next);
+        }
+        if (current == INT32_MAX) return false;
+        const int c = piece * 8 + chunk, chunks = l.rank / 8;
+        const char *low = (const char *)(l.low + (int64_t)m0 * 2 * l.rank) + c * 16;
+        const char *b = (const char *)(l.b + ((int64_t)current * l.n_out + n0) * l.rank) + (c >= chunks ? c - chunks : c) * 16;
+        const bool there = c < 2 * chunks;
+#pragma unroll
+        for (int i = 0; i < G::X_LOADS; i++)
+            load_to_lds(xs + x_group(i) * 1024, there && owner[x_row[i]] == current ? low + (int64_t)x_row[i] * 4 * l.rank
+                                                                                  : (const char *)&g_zeros);
+#pragma unroll
+        for (int i = 0; i < G::W_LOADS; i++)
+            load_to_lds(ws + w_group(i) * 1024,
+                        there ? b + (int64_t)min(w_group(i) * 8 + row, l.n_out - 1 - n0) * 2 * l.rank : (const char *)&g_zeros);
+        if (++piece == pieces) piece = 0;
+        of_adapter |= 1u << to;
+        return true;
+    };
+    // NaN and infinities of an adapter become zeros: times the zeros of other rows, or a remainder of zero, they
+    // would be no numbers. The rows that they belong to get them in the end.
+    const auto clear_unfit = [&](int from) {
+        bool found = false;
+        for (int c = threadIdx.x; c < G::TN * 8; c += G::T) {
+            u32x4 *at = (u32x4 *)(lds + from * G::BYTES + G::TM * 128 + c * 16), v = *at;
+            if (clear_unfit_of(v)) *at = v, found = true;
+        }
+        if (found) *unfit = 1;
+        wait_lds();
+        barrier();
+    };
+
+    typename Mfma<G::S>::Acc acc[G::MT][G::NT] = {};
+    const int mine_m = wave % G::WM * G::RM, mine_n = wave / G::WM * G::RN;
+    const auto multiply = [&](int from) {
+        const char *xs = lds + from * G::BYTES, *ws = xs + G::TM * 128;
+        const int r = lane % G::S, c = lane / G::S;
+#pragma unroll
+        for (int k = 0; k < 64 / Mfma<G::S>::K; k++) {
+            const int slot = (k * (64 / G::S) + c) ^ (r & 7);
+            u32x4 xf[G::MT], wf[G::NT];
+#pragma unroll
+            for (int i = 0; i < G::MT; i++) xf[i] = *(const u32x4 *)(xs + (mine_m + i * G::S + r) * 128 + slot * 16);
+#pragma unroll
+            for (int j = 0; j < G::NT; j++) wf[j] = *(const u32x4 *)(ws + (mine_n + j * G::S + r) * 128 + slot * 16);
+#pragma unroll
+            for (int i = 0; i < G::MT; i++)
+#pragma unroll
+                for (int j = 0; j < G::NT; j++) acc[i][j] = Mfma<G::S>::mul(wf[j], xf[i], acc[i][j]);
+        }
+    };
+
+    int pending = 0, stage = 0;
+#pragma unroll
+    for (int i = 0; i < G::STAGES - 1; i++)
+        if (request(i)) pending++;
+    while (pending > 0) {
+        // all but the steps requested behind this one are there, in every wave; the stage before this one is read
+        if (pending == G::STAGES - 1) wait_loads<(G::STAGES - 2) * G::LOADS>();
+        else wait_loads<0>();
+        wait_lds();
+        barrier();
+        const int next = stage == 0 ? G::STAGES - 1 : stage - 1;
+        if (pending == G::STAGES - 1 && request(next)) pending++;
+        if (of_adapter >> stage & 1) {
+            clear_unfit(stage);
+            of_adapter &= ~(1u << stage);
+        }
+        multiply(stage);
+        pending--;
+        stage = stage == G::STAGES - 1 ? 0 : stage + 1;
+    }
+    wait_lds();
+    barrier();
+
+    // out through LDS, S rows of a wave at a time, so that a row's columns are written side by side
+    float *slab = (float *)lds + wave * G::SLAB;
+#pragma unroll
+    for (int i = 0; i < G::MT; i++) {
+#pragma unroll
+        for (int j = 0; j < G::NT; j++)
+#pragma unroll
+            for (int r = 0; r < Mfma<G::S>::REGS / 4; r++)
+                *(f32x4 *)(slab + lane % G::S * (G::RN + 4) + j * G::S + Mfma<G::S>::row(r, lane)) =
+                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+        wait_lds();
+        constexpr int PER = G::RN / 8;  // lanes of a row
+        const int n = n0 + mine_n + lane % PER * 8;
+#pragma unroll 1
+        for (int r = lane / PER; r < G::S; r += 64 / PER) {
+            const int tile_row = mine_m + i * G::S + r, m = m0 + tile_row;
+            if (m >= l.n_tokens || n >= l.n_out || (adapters && owner[tile_row] == NO_SEQUENCE)) continue;
+            const float *from = slab + r * (G::RN + 4) + lane % PER * 8;
+            f32x4 y[2] = {*(const f32x4 *)from, *(const f32x4 *)(from + 4)};
+            if (join) {
+                float *to = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width + n;
+                *gptr((f32x4 *)to) = y[0];
+                if (n + 4 < l.n_out) *gptr((f32x4 *)(to + 4)) = y[1];
+                continue;
+            }
+            if (adapters && *unfit && owner[tile_row] >= 0)
+                for (int e = 0; e < 8 && n + e < l.n_out; e++) y[e / 4][e % 4] += unfit_term(l, m, n + e, owner[tile_row]);
+            bf16 *to = l.out + m * l.out_stride + n;
+            const bf16 *res = l.residual + m * l.residual_stride + n;
+            if (l.wide && n + 8 <= l.n_out) {
+                if (l.residual) {
+                    const u32x4 v = ld16(res);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[e / 4][e % 4] += elem(v, e);
+                }
+                st16(to, u32x4{pack2(y[0][0], y[0][1]), pack2(y[0][2], y[0][3]), pack2(y[1][0], y[1][1]), pack2(y[1][2], y[1][3])});
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (n + e < l.n_out)
+                        gptr(to)[e] = (bf16)f2bf(y[e / 4][e % 4] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f));
+            }
+        }
+        wait_lds();
+    }
+}
+
+// ------------------------------------------------------------------------------------------
+// the join: the parts of the product, the adapters' term and the residual
+// ------------------------------------------------------------------------------------------
+
+// 16 rows of a sequence by 64 columns per wave; a lane has row lane % 16 and four columns of each 16.
+__global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
+    const int lane = threadIdx.x & 63, n0 = (blockIdx.x * 4 + wave_id()) * 64;
+    const RowTile t = row_tile(l, blockIdx.y);
+    if (t.rows == 0 || n0 >= l.n_out) return;
+    const int m = t.first + min(lane % 16, t.rows - 1);
+    f32x4 acc[4] = {};
+    bool unfit = false;
+    if (t.adapter >= 0) {
+        const bf16 *low = l.low + (int64_t)m * 2 * l.rank, *b = l.b + (int64_t)t.adapter * l.n_out * l.rank;
+        const int chunks = l.rank / 8;
+        for (int c0 = 0; c0 < 2 * chunks; c0 += 4) {
+            const int c = c0 + lane / 16, of_b = c >= chunks ? c - chunks : c;
+            const bool there = c < 2 * chunks;
+            const u32x4 x = there ? ld16(low + c * 8) : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int n = min(n0 + j * 16 + lane % 16, l.n_out - 1);
+                u32x4 v = there ? ld16(b + (int64_t)n * l.rank + of_b * 8) : u32x4{0, 0, 0, 0};
+                unfit |= clear_unfit_of(v);
+                acc[j] = Mfma<16>::mul(v, x, acc[j]);
+            }
         }
     }
-    if (t >= l.n_tokens) return;
-    const int a = adapter_of(l, t);
-    if (a == -2) return;
-    for (int e = 0; e < 4; e++) {
-        const int n = n0 + lane / 16 * 4 + e;
+    unfit = __any(unfit);
+    if (lane % 16 >= t.rows) return;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int n = n0 + j * 16 + lane / 16 * 4;
         if (n >= l.n_out) break;
-        float y = acc[e];
-        if (a >= 0) {
-            const bf16 *b = l.b + ((int64_t)a * l.n_out + n) * l.rank;
-            for (int j = 0; j < l.rank; j++) y = fmaf(l.low[(int64_t)t * l.rank + j], bf2f(gptr(b)[j]), y);
+        const float *part = l.part + (int64_t)m * l.part_width + n;
+        f32x4 y = acc[j];
+        for (int s = 0; s < l.splits; s++) y += *gptr((const f32x4 *)(part + (int64_t)s * l.n_tokens * l.part_width));
+        bf16 *to = l.out + m * l.out_stride + n;
+        const bf16 *res = l.residual + m * l.residual_stride + n;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (n + e >= l.n_out) break;
+            float v = y[e] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f);
+            if (unfit) v += unfit_term(l, m, n + e, t.adapter);
+            gptr(to)[e] = (bf16)f2bf(v);
         }
-        if (l.residual) y += bf2f(gptr(l.residual)[t * l.residual_stride + n]);
-        gptr(l.out)[t * l.out_stride + n] = (bf16)f2bf(y);
     }
+}
+
+// ------------------------------------------------------------------------------------------
+// on the host
+// ------------------------------------------------------------------------------------------
+
+typedef Shape<256, 192, 64, 96, 16, 2> Large;
+typedef Shape<128, 128, 64, 64, 16, 2> Middle;
+typedef Shape<64, 64, 64, 16, 16, 4> Small;
+typedef Shape<16, 64, 16, 16, 16, 4> Row;
+
+constexpr int MOST_SPLITS = 32;
+constexpr size_t MOST_PART = 1 << 23;  // floats
+
+// How a call is computed: the product's tiles, its splits, and whether a join adds them and the adapters' term.
+struct Plan {
+    int shape, splits, split_steps;
+    bool join;
+
+    static size_t part_floats(int n_tokens, int n_out) { return (size_t)n_tokens * ((n_out + 3) / 4 * 4); }
+    // Of the parts, for n_tokens and for fewer.
+    static size_t most_part(int n_tokens, int n_out) {
+        return std::min(MOST_PART, MOST_SPLITS * part_floats(n_tokens, n_out));
+    }
+
+    Plan(int n_tokens, int n_out, int n_in, bool product, bool adapters, int rank, int n_seqs, int n_adapters) {
+        const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
+        const int64_t one = (int64_t)part_floats(n_tokens, n_out);
+        const int most = (int)std::min<int64_t>(std::min(MOST_SPLITS, std::max(steps, 1)), MOST_PART / one);
+        const struct { int tm, tn, at_once; double step, alone; } shapes[4] = {
+            {256, 192, 1, 1300, 1300}, {128, 128, 2, 1100, 650}, {64, 64, 2, 420, 350}, {16, 64, 3, 300, 200}};
+        double least = 0;
+        shape = -1;
+        for (int i = 0; i < 4; i++) {
+            const auto &s = shapes[i];
+            const double tiles = (double)((n_tokens + s.tm - 1) / s.tm) * ((n_out + s.tn - 1) / s.tn);
+            const auto consider = [&](int n, bool joined) {
+                const int each = (steps + n - 1) / n;
+                // adapters of a tile's rows, each with steps of its own
+                const double own = !joined && adapters
+                    ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(s.tm, n_tokens) / n_tokens) : 0;
+                const double groups = tiles * n, rounds = groups <= CUS ? 1 : ceil(groups / (s.at_once * CUS));
+                const double cost = 2000 + rounds * (each + own + 2) * (groups <= CUS ? s.alone : s.step) +
+                                    (joined ? 4000 + one * (n + 1.0) * 8 / 5000 : 0);
+                if (shape < 0 || cost < least) shape = i, splits = n, join = joined, least = cost;
+            };
+            consider(1, false);
+            for (int n = adapters || !product ? 1 : 2; n <= most; n++) consider(n, true);
+        }
+        split_steps = (steps + splits - 1) / splits;
+        splits = split_steps ? (steps + split_steps - 1) / split_steps : join ? 0 : 1;
+    }
+};
+
+template <class G>
+void launch_product(LoraArgs l, hipStream_t stream) {
+    l.m_tiles = (l.n_tokens + G::TM - 1) / G::TM;
+    l.n_tiles = (l.n_out + G::TN - 1) / G::TN;
+    const int64_t groups = l.low_groups + (int64_t)l.m_tiles * l.n_tiles * l.splits;
+    if (groups) product_kernel<G><<<groups, G::T, 0, stream>>>(l);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -99,11 +536,14 @@ bool check_sizes(const char *name, int n_tokens, int n_out, int n_in, int rank) 
     return true;
 }
 
+size_t low_floats(int n_tokens, int rank) { return (size_t)n_tokens * rank; }
+size_t owner_floats(int n_tokens, int rank) { return rank ? ((size_t)n_tokens + 3) / 4 * 4 : 0; }
+
 }  // namespace
 
 extern "C" size_t lora_projection_workspace_floats(int n_tokens, int n_out, int n_in, int rank) {
     if (!check_sizes("lora_projection_workspace_floats", n_tokens, n_out, n_in, rank)) return 0;
-    return (size_t)n_tokens * rank;
+    return low_floats(n_tokens, rank) + owner_floats(n_tokens, rank) + Plan::most_part(n_tokens, n_out);
 }
 
 extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w, const bf16 *residual,
@@ -111,10 +551,11 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
                                         int64_t out_stride, int64_t x_stride, int64_t residual_stride,
                                         hipStream_t stream) {
     static const char name[] = "lora_projection";
-    if (!check_sizes(name, n_tokens, n_out, n_in, lora ? lora->rank : 0)) return;
+    const int rank = lora ? lora->rank : 0;
+    if (!check_sizes(name, n_tokens, n_out, n_in, rank)) return;
     if (lora) {
-        if (lora->rank == 0 || lora->n_seqs <= 0 || lora->n_seqs > 1 << 20 || lora->n_adapters <= 0) {
-            llm_fail("%s: rank %d, n_seqs %d (up to 1048576) and n_adapters %d must be positive", name, lora->rank,
+        if (rank == 0 || lora->n_seqs <= 0 || lora->n_seqs > 1 << 20 || lora->n_adapters <= 0) {
+            llm_fail("%s: rank %d, n_seqs %d (up to 1048576) and n_adapters %d must be positive", name, rank,
                      lora->n_seqs, lora->n_adapters);
             return;
         }
@@ -128,8 +569,8 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
         llm_fail("%s: out and x must not be null, x and w 16-byte aligned", name);
         return;
     }
-    if (x_stride < n_in || x_stride % 8) {
-        llm_fail("%s: the rows of x are %lld elements apart, not a multiple of 8 of at least %d", name,
+    if (x_stride < n_in || x_stride % 8 || x_stride > 1 << 22) {
+        llm_fail("%s: the rows of x are %lld elements apart, not a multiple of 8 of at least %d, up to 4194304", name,
                  (long long)x_stride, n_in);
         return;
     }
@@ -146,18 +587,52 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
         llm_fail("%s: out must not be x, which is read again", name);
         return;
     }
-    if (!aligned16(ws) || (lora && !ws)) {
+    const Plan p(n_tokens, n_out, n_in, w != nullptr, lora != nullptr, rank, lora ? lora->n_seqs : 0,
+                 lora ? lora->n_adapters : 0);
+    if (!ws || !aligned16(ws)) {
         llm_fail("%s: ws must be a 16-byte aligned device address", name);
         return;
     }
-    LoraArgs l = {out, x, w, residual, nullptr, nullptr, nullptr, nullptr, nullptr, ws, out_stride, x_stride, residual_stride,
-                  n_tokens, n_out, n_in, 0, 0, 0};
+    LoraArgs l = {};
+    l.out = out, l.x = x, l.w = w, l.residual = residual;
+    l.out_stride = out_stride, l.x_stride = x_stride, l.residual_stride = residual_stride;
+    l.n_tokens = n_tokens, l.n_out = n_out, l.n_in = n_in;
+    l.part_width = (n_out + 3) / 4 * 4;
+    l.splits = p.splits, l.split_steps = p.split_steps;
+    l.wide = out_stride % 8 == 0 && aligned16(out) && (!residual || (residual_stride % 8 == 0 && aligned16(residual)));
+    l.low = (bf16 *)ws;
+    l.owner = (int *)(ws + low_floats(n_tokens, rank));
+    float *part = ws + low_floats(n_tokens, rank) + owner_floats(n_tokens, rank);
+    int tiles = (n_tokens + 15) / 16, low_groups = 0;
     if (lora) {
         l.a = lora->a, l.b = lora->b, l.scale = lora->scale, l.q_start = lora->q_start, l.adapter = lora->adapter;
-        l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = lora->rank;
-        shrink_kernel<<<dim3((l.rank + 3) / 4, n_tokens), 256, 0, stream>>>(l);
+        l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = rank;
+        tiles = n_tokens / 16 + lora->n_seqs;
+        low_groups = tiles * ((rank + LOW - 1) / LOW);
+    }
+    const auto product = [&](const LoraArgs &a) {
+        switch (p.shape) {
+        case 0: launch_product<Large>(a, stream); break;
+        case 1: launch_product<Middle>(a, stream); break;
+        case 2: launch_product<Small>(a, stream); break;
+        default: launch_product<Row>(a, stream);
+        }
+        return LAUNCH_OK();
+    };
+    if (p.join) {
+        l.part = part;
+        l.low_groups = low_groups;
+        if (!product(l)) return;
+        join_kernel<<<dim3((n_out + 255) / 256, tiles), 256, 0, stream>>>(l);
+        LAUNCH_OK();
+        return;
+    }
+    if (lora) {
+        LoraArgs low = l;
+        low.splits = 0;
+        low.low_groups = low_groups;
+        launch_product<Middle>(low, stream);
         if (!LAUNCH_OK()) return;
     }
-    project_kernel<<<dim3((n_out + 63) / 64, (n_tokens + 15) / 16), 256, 0, stream>>>(l);
-    LAUNCH_OK();
+    product(l);
 }
