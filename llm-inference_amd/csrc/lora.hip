@@ -33,11 +33,13 @@ struct LoraArgs {
     bf16 *low;               // [n_tokens, 2 rank]: value, remainder
     int *owner;              // [n_tokens]: the row's adapter, NO_ADAPTER or NO_SEQUENCE
     float *part;             // [splits, n_tokens, part_width], or null: straight to out
+    float *low_part;         // [low_splits, n_tokens, rank], where there are parts
     int64_t out_stride, x_stride, residual_stride;
     int n_tokens, n_out, n_in, n_seqs, n_adapters, rank;
     int part_width;
     int splits, split_steps;  // of the product's sum, steps of 64 each
-    int m_tiles, n_tiles, low_groups;
+    int m_tiles, n_tiles;
+    int low_groups, low_splits;  // workgroups in front of the product's that compute low_part
     bool wide;               // out and residual take 16 bytes at a time
 };
 
@@ -105,71 +107,107 @@ __device__ __forceinline__ RowTile row_tile(const LoraArgs &l, int i) {
         t.rows = min(16, l.n_tokens - t.first);
         return t;
     }
-    const int s = count_leading(l.n_seqs, [&](int j) { return start_of(l, j) / 16 + j <= i; }) - 1;
-    if (s < 0) return t;
-    const int f = start_of(l, s), n = start_of(l, s + 1) - f, j = i - (f / 16 + s);
-    t.first = f + 16 * j;
-    t.rows = max(0, min(16, n - 16 * j));
-    const int a = gptr(l.adapter)[s];
+    const int lane = threadIdx.x & 63;
+    int s0 = 0;  // the sequence is among the 64 from s0 on, which are read at once
+    if (l.n_seqs > 64) s0 = max(0, count_leading(l.n_seqs, [&](int j) { return start_of(l, j) / 16 + j <= i; }) - 1);
+    const int s = min(s0 + lane, l.n_seqs - 1);
+    const int f = start_of(l, s), n = start_of(l, s + 1) - f, adapter = gptr(l.adapter)[s];
+    const uint64_t upto = __ballot(s0 + lane < l.n_seqs && f / 16 + s <= i);
+    if (!upto) return t;
+    const int at = 63 - __builtin_clzll(upto);
+    const int first = __builtin_amdgcn_readlane(f, at), rows = __builtin_amdgcn_readlane(n, at), a = __builtin_amdgcn_readlane(adapter, at);
+    const int j = i - (first / 16 + s0 + at);
+    t.first = first + 16 * j;
+    t.rows = max(0, min(16, rows - 16 * j));
     if ((unsigned)a < (unsigned)l.n_adapters) t.adapter = a;
     return t;
 }
 
+// low of 16 rows and 16 NT elements of the rank, of the sum's elements from `from` on; the waves of the workgroup
+// take SPAN of them each. The sum into sums (LDS, [16][16 NT]).
+template <int NT>
+struct Low {
+    static constexpr int U = NT == 4 ? 4 : 8;  // loads of each operand under way
+    template <int WAVES>
+    static __device__ __forceinline__ void sum(const LoraArgs &l, const RowTile &t, int r0, int from, int span, float *sums) {
+        const int lane = threadIdx.x & 63, wave = wave_id();
+        const bf16 *x = l.x + (t.first + min(lane % 16, t.rows - 1)) * l.x_stride;
+        const bf16 *a = l.a + (int64_t)t.adapter * l.rank * l.n_in;
+        const bf16 *row[NT];
+#pragma unroll
+        for (int j = 0; j < NT; j++) row[j] = a + (int64_t)min(r0 + j * 16 + lane % 16, l.rank - 1) * l.n_in;
+        const int to = min(l.n_in, from + (wave + 1) * span);
+        f32x4 acc[NT] = {};
+        for (int k0 = from + wave * span; k0 < to; k0 += 32 * U) {
+            u32x4 xs[U], as[U][NT];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = k0 + 32 * u + lane / 16 * 8;
+                xs[u] = k < to ? ld16(x + k) : u32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < NT; j++) as[u][j] = k < to ? ld16(row[j] + k) : u32x4{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[j] = Mfma<16>::mul(as[u][j], xs[u], acc[j]);
+        }
+        constexpr int ROW = 16 * NT;
+        float *mine = sums + wave * 16 * ROW;
+#pragma unroll
+        for (int j = 0; j < NT; j++) *(f32x4 *)(mine + lane % 16 * ROW + j * 16 + lane / 16 * 4) = acc[j];
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * ROW; i += 64 * WAVES) {
+            float y = 0.0f;
+            for (int w = 0; w < WAVES; w++) y += sums[w * 16 * ROW + i];
+            sums[i] = y;
+        }
+    }
+};
+constexpr int LOW_SPAN = 1024;  // elements of the sum per workgroup where a join adds their parts
+__host__ __device__ __forceinline__ int low_width(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
-// low of 16 rows and LOW elements of the rank: the waves of a workgroup take a part of the sum each.
-constexpr int LOW = 64;
+// For a join: part low_split of low, in 32 bits and without its scale.
 template <int WAVES>
-__device__ __forceinline__ void shrink(const LoraArgs &l, int tile, int group, float *lds) {
-    const int lane = threadIdx.x & 63, wave = wave_id(), r0 = group * LOW;
-    const RowTile t = row_tile(l, tile);
-    if (group == 0) {
-        if (tile == 0) {
+__device__ __forceinline__ void low_part(const LoraArgs &l, int block, float *lds) {
+    const int width = low_width(l.rank), groups = (l.rank + width - 1) / width;
+    const int split = block % l.low_splits, r0 = block / l.low_splits % groups * width;
+    const RowTile t = row_tile(l, block / l.low_splits / groups);
+    if (t.rows == 0 || t.adapter < 0) return;
+    const int from = split * LOW_SPAN;
+    if (width == 16) Low<1>::sum<WAVES>(l, t, r0, from, LOW_SPAN / WAVES, lds);
+    else if (width == 32) Low<2>::sum<WAVES>(l, t, r0, from, LOW_SPAN / WAVES, lds);
+    else Low<4>::sum<WAVES>(l, t, r0, from, LOW_SPAN / WAVES, lds);
+    float *to = l.low_part + ((int64_t)split * l.n_tokens + t.first) * l.rank + r0;
+    for (int i = threadIdx.x; i < 16 * width; i += 64 * WAVES)
+        if (i / width < t.rows && r0 + i % width < l.rank) gptr(to)[(int64_t)(i / width) * l.rank + i % width] = lds[i];
+}
+
+// Otherwise: low as two bf16, and the rows' owners. 16 waves share the sum.
+constexpr int LOW_WAVES = 16;
+template <int NT>
+__global__ __launch_bounds__(64 * LOW_WAVES) void low_kernel(LoraArgs l) {
+    __shared__ __attribute__((aligned(16))) float sums[LOW_WAVES * 16 * 16 * NT];
+    const int r0 = blockIdx.y * 16 * NT;
+    const RowTile t = row_tile(l, blockIdx.x);
+    if (blockIdx.y == 0) {
+        if (blockIdx.x == 0) {
             const int begin = start_of(l, 0), end = max(begin, start_of(l, l.n_seqs));
-            for (int i = threadIdx.x; i < l.n_tokens; i += 64 * WAVES)
+            for (int i = threadIdx.x; i < l.n_tokens; i += 64 * LOW_WAVES)
                 if (i < begin || i >= end) gptr(l.owner)[i] = NO_SEQUENCE;
         }
         if ((int)threadIdx.x < t.rows) gptr(l.owner)[t.first + threadIdx.x] = t.adapter;
     }
     if (t.rows == 0 || t.adapter < 0) return;
-    const bf16 *x = l.x + (t.first + min(lane % 16, t.rows - 1)) * l.x_stride;
-    const bf16 *a = l.a + (int64_t)t.adapter * l.rank * l.n_in;
-    const bf16 *row[LOW / 16];
-#pragma unroll
-    for (int j = 0; j < LOW / 16; j++) row[j] = a + (int64_t)min(r0 + j * 16 + lane % 16, l.rank - 1) * l.n_in;
-    const int tiles = min(LOW / 16, (l.rank - r0 + 15) / 16);
-    const int part = (l.n_in + 32 * WAVES - 1) / (32 * WAVES) * 32, from = wave * part, to = min(l.n_in, from + part);
-    f32x4 acc[LOW / 16] = {};
-    constexpr int U = 4;
-    for (int k0 = from; k0 < to; k0 += 32 * U) {
-        u32x4 xs[U], as[U][LOW / 16];
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = k0 + 32 * u + lane / 16 * 8;
-            xs[u] = k < to ? ld16(x + k) : u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int j = 0; j < LOW / 16; j++) as[u][j] = k < to && j < tiles ? ld16(row[j] + k) : u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int j = 0; j < LOW / 16; j++) acc[j] = Mfma<16>::mul(as[u][j], xs[u], acc[j]);
-    }
-    float *mine = lds + wave * 16 * LOW;
-#pragma unroll
-    for (int j = 0; j < LOW / 16; j++) *(f32x4 *)(mine + lane % 16 * LOW + j * 16 + lane / 16 * 4) = acc[j];
-    __syncthreads();
     const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
-    for (int i = threadIdx.x; i < 16 * LOW; i += 64 * WAVES) {
-        const int m = i / LOW, r = r0 + i % LOW;
-        if (m >= t.rows || r >= l.rank) continue;
-        float sum = 0;
-        for (int w = 0; w < WAVES; w++) sum += lds[w * 16 * LOW + i];
-        sum *= scale;
-        const float value = round_bf(sum), rest = fabsf(value) < INFINITY ? sum - value : 0.0f;
-        LLM_GLOBAL uint16_t *low = gptr((uint16_t *)l.low) + (int64_t)(t.first + m) * 2 * l.rank + r;
-        low[0] = (uint16_t)f2bf(value);
-        low[l.rank] = (uint16_t)f2bf(rest);
-    }
+    Low<NT>::template sum<LOW_WAVES>(l, t, r0, 0, (l.n_in + 32 * LOW_WAVES - 1) / (32 * LOW_WAVES) * 32, sums);
+    const int i = threadIdx.x, m = i / (16 * NT), r = r0 + i % (16 * NT);
+    if (m >= t.rows || r >= l.rank) return;
+    const float sum = sums[i] * scale;
+    const float value = round_bf(sum), rest = fabsf(value) < INFINITY ? sum - value : 0.0f;
+    LLM_GLOBAL uint16_t *low = gptr((uint16_t *)l.low) + (int64_t)(t.first + m) * 2 * l.rank + r;
+    low[0] = (uint16_t)f2bf(value);
+    low[l.rank] = (uint16_t)f2bf(rest);
 }
 
 // Whether NaN or infinities were among eight elements; they are zeros then.
@@ -182,14 +220,14 @@ __device__ __forceinline__ bool clear_unfit_of(u32x4 &v) {
     }
     return found;
 }
-// What those that b has for column n add to row m.
-__device__ __forceinline__ float unfit_term(const LoraArgs &l, int m, int n, int adapter) {
-    const uint16_t *low = (const uint16_t *)l.low + (int64_t)m * 2 * l.rank;
+// What those that b has for column n add, with low(j).
+template <class Of>
+__device__ __forceinline__ float unfit_term(const LoraArgs &l, int n, int adapter, Of low) {
     const uint16_t *b = (const uint16_t *)l.b + ((int64_t)adapter * l.n_out + n) * l.rank;
     float y = 0.0f;
     for (int j = 0; j < l.rank; j++) {
         const float v = bf2f(gptr(b)[j]);
-        if (!(fabsf(v) < INFINITY)) y += (bf2f(gptr(low)[j]) + bf2f(gptr(low)[l.rank + j])) * v;
+        if (!(fabsf(v) < INFINITY)) y += low(j) * v;
     }
     return y;
 }
@@ -211,9 +249,9 @@ struct Shape {
     static constexpr int LOADS = X_LOADS + W_LOADS;
     static constexpr int SLAB = S * (RN + 4);                        // floats of a wave's rows on their way out
     static constexpr int SLABS = WAVES * SLAB * 4;
-    static constexpr int SHRINK = WAVES * 16 * LOW * 4;
+    static constexpr int SUMS = WAVES * 16 * 64 * 4;                 // of low's parts
     static constexpr int LDS0 = STAGES * BYTES > SLABS ? STAGES * BYTES : SLABS;
-    static constexpr int LDS = LDS0 > SHRINK ? LDS0 : SHRINK;
+    static constexpr int LDS = LDS0 > SUMS ? LDS0 : SUMS;
     static_assert(TN / 8 % WAVES == 0 && (TM / 8 % WAVES == 0 || WAVES % (TM / 8) == 0), "loads per wave");
 };
 
@@ -222,11 +260,7 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     __shared__ __attribute__((aligned(128))) char lds[G::LDS + G::TM * 4 + 4];
     int *owner = (int *)(lds + G::LDS), *unfit = owner + G::TM;
     const int lane = threadIdx.x & 63, wave = wave_id();
-    if ((int)blockIdx.x < l.low_groups) {
-        const int groups = (l.rank + LOW - 1) / LOW;
-        shrink<G::WAVES>(l, blockIdx.x / groups, blockIdx.x % groups, (float *)lds);
-        return;
-    }
+    if ((int)blockIdx.x < l.low_groups) return low_part<G::WAVES>(l, blockIdx.x, (float *)lds);
     // the tiles of one XCD, whose workgroups every eighth one is, lie side by side
     const int tiles = l.m_tiles * l.n_tiles * l.splits, block = blockIdx.x - l.low_groups;
     const int each = tiles / XCDS, more = tiles % XCDS, xcd = block % XCDS;
@@ -394,8 +428,11 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
                 if (n + 4 < l.n_out) *gptr((f32x4 *)(to + 4)) = y[1];
                 continue;
             }
-            if (adapters && *unfit && owner[tile_row] >= 0)
-                for (int e = 0; e < 8 && n + e < l.n_out; e++) y[e / 4][e % 4] += unfit_term(l, m, n + e, owner[tile_row]);
+            if (adapters && *unfit && owner[tile_row] >= 0) {
+                const uint16_t *low = (const uint16_t *)l.low + (int64_t)m * 2 * l.rank;
+                for (int e = 0; e < 8 && n + e < l.n_out; e++)
+                    y[e / 4][e % 4] += unfit_term(l, n + e, owner[tile_row], [&](int j) { return bf2f(gptr(low)[j]) + bf2f(gptr(low)[l.rank + j]); });
+            }
             bf16 *to = l.out + m * l.out_stride + n;
             const bf16 *res = l.residual + m * l.residual_stride + n;
             if (l.wide && n + 8 <= l.n_out) {
@@ -420,27 +457,92 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
 // the join: the parts of the product, the adapters' term and the residual
 // ------------------------------------------------------------------------------------------
 
-// 16 rows of a sequence by 64 columns per wave; a lane has row lane % 16 and four columns of each 16.
+// 16 rows of a sequence by 256 columns per workgroup. The rows' low is added up once, into LDS; what every lane reads
+// besides is requested in front of that.
+constexpr int FEW = 4;      // rows up to which a lane has a column, and the sum over the rank is one of vector operations
+constexpr int PARTS = 4;    // parts under way
+
+// The product's parts of four rows at most, one column per lane.
+__device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, int n, const float *low) {
+    float y[FEW] = {};
+    const int at = min(n, l.n_out - 1);
+    for (int s0 = 0; s0 < l.splits; s0 += PARTS) {
+        float part[FEW][PARTS];
+#pragma unroll
+        for (int i = 0; i < FEW; i++)
+#pragma unroll
+            for (int s = 0; s < PARTS; s++)
+                part[i][s] = i < t.rows && s0 + s < l.splits
+                                 ? gptr(l.part)[((int64_t)(s0 + s) * l.n_tokens + t.first + i) * l.part_width + at] : 0.0f;
+#pragma unroll
+        for (int i = 0; i < FEW; i++)
+#pragma unroll
+            for (int s = 0; s < PARTS; s++) y[i] += part[i][s];
+    }
+    if (l.residual)
+#pragma unroll
+        for (int i = 0; i < FEW; i++)
+            if (i < t.rows) y[i] += bf2f(gptr(l.residual)[(t.first + i) * l.residual_stride + at]);
+    if (t.adapter >= 0) {
+        const bf16 *b = l.b + ((int64_t)t.adapter * l.n_out + at) * l.rank;
+        for (int j = 0; j < l.rank; j += 8) {
+            const u32x4 v = ld16(b + j);
+#pragma unroll
+            for (int i = 0; i < FEW; i++)
+                if (i < t.rows)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) y[i] = fmaf(low[i * l.rank + j + e], elem(v, e), y[i]);
+        }
+    }
+    if (n < l.n_out)
+#pragma unroll
+        for (int i = 0; i < FEW; i++)
+            if (i < t.rows) gptr(l.out)[(t.first + i) * l.out_stride + n] = (bf16)f2bf(y[i]);
+}
+
 __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
-    const int lane = threadIdx.x & 63, n0 = (blockIdx.x * 4 + wave_id()) * 64;
-    const RowTile t = row_tile(l, blockIdx.y);
-    if (t.rows == 0 || n0 >= l.n_out) return;
-    const int m = t.first + min(lane % 16, t.rows - 1);
+    __shared__ float low[16 * 256];
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const RowTile t = row_tile(l, blockIdx.x);
+    if (t.rows == 0) return;
+    if (t.adapter >= 0) {
+        const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
+        const float *from = l.low_part + (int64_t)t.first * l.rank;
+        for (int i = threadIdx.x; i < t.rows * l.rank; i += 256) {
+            float y = 0.0f;
+            for (int s = 0; s < l.low_splits; s++) y += gptr(from)[(int64_t)s * l.n_tokens * l.rank + i];
+            low[i] = y * scale;
+        }
+        __syncthreads();
+    }
+    if (t.rows <= FEW) return join_few(l, t, blockIdx.y * 256 + threadIdx.x, low);
+    // a lane has row lane % 16 and four columns of each 16
+    const int n0 = (blockIdx.y * 4 + wave) * 64, mine = min(lane % 16, t.rows - 1), m = t.first + mine;
+    if (n0 >= l.n_out) return;
     f32x4 acc[4] = {};
     bool unfit = false;
     if (t.adapter >= 0) {
-        const bf16 *low = l.low + (int64_t)m * 2 * l.rank, *b = l.b + (int64_t)t.adapter * l.n_out * l.rank;
-        const int chunks = l.rank / 8;
-        for (int c0 = 0; c0 < 2 * chunks; c0 += 4) {
-            const int c = c0 + lane / 16, of_b = c >= chunks ? c - chunks : c;
-            const bool there = c < 2 * chunks;
-            const u32x4 x = there ? ld16(low + c * 8) : u32x4{0, 0, 0, 0};
+        const bf16 *b = l.b + (int64_t)t.adapter * l.n_out * l.rank;
+        for (int c0 = 0; c0 < l.rank / 8; c0 += 4) {
+            const int c = c0 + lane / 16;
+            const bool there = c < l.rank / 8;
+            u32x4 value = {0, 0, 0, 0}, rest = {0, 0, 0, 0};
+            if (there) {
+                const float *from = low + mine * l.rank + c * 8;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float y0 = from[2 * e], y1 = from[2 * e + 1], v0 = round_bf(y0), v1 = round_bf(y1);
+                    value[e] = pack2(y0, y1);
+                    rest[e] = pack2(fabsf(v0) < INFINITY ? y0 - v0 : 0.0f, fabsf(v1) < INFINITY ? y1 - v1 : 0.0f);
+                }
+            }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int n = min(n0 + j * 16 + lane % 16, l.n_out - 1);
-                u32x4 v = there ? ld16(b + (int64_t)n * l.rank + of_b * 8) : u32x4{0, 0, 0, 0};
+                u32x4 v = there ? ld16(b + (int64_t)n * l.rank + c * 8) : u32x4{0, 0, 0, 0};
                 unfit |= clear_unfit_of(v);
-                acc[j] = Mfma<16>::mul(v, x, acc[j]);
+                acc[j] = Mfma<16>::mul(v, value, acc[j]);
+                acc[j] = Mfma<16>::mul(v, rest, acc[j]);
             }
         }
     }
@@ -459,7 +561,7 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
         for (int e = 0; e < 4; e++) {
             if (n + e >= l.n_out) break;
             float v = y[e] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f);
-            if (unfit) v += unfit_term(l, m, n + e, t.adapter);
+            if (unfit) v += unfit_term(l, n + e, t.adapter, [&](int i) { return low[mine * l.rank + i]; });
             gptr(to)[e] = (bf16)f2bf(v);
         }
     }
@@ -474,7 +576,7 @@ typedef Shape<128, 128, 64, 64, 16, 2> Middle;
 typedef Shape<64, 64, 64, 16, 16, 4> Small;
 typedef Shape<16, 64, 16, 16, 16, 4> Row;
 
-constexpr int MOST_SPLITS = 32;
+constexpr int MOST_SPLITS = 32, MOST_JOINED = 2048;
 constexpr size_t MOST_PART = 1 << 23;  // floats
 
 // How a call is computed: the product's tiles, its splits, and whether a join adds them and the adapters' term.
@@ -510,7 +612,7 @@ struct Plan {
                 if (shape < 0 || cost < least) shape = i, splits = n, join = joined, least = cost;
             };
             consider(1, false);
-            for (int n = adapters || !product ? 1 : 2; n <= most; n++) consider(n, true);
+            for (int n = adapters || !product ? 1 : 2; n <= most && n_tokens <= MOST_JOINED; n++) consider(n, true);
         }
         split_steps = (steps + splits - 1) / splits;
         splits = split_steps ? (steps + split_steps - 1) / split_steps : join ? 0 : 1;
@@ -518,11 +620,14 @@ struct Plan {
 };
 
 template <class G>
-void launch_product(LoraArgs l, hipStream_t stream) {
+bool launch_product(const char *name, LoraArgs l, hipStream_t stream) {
     l.m_tiles = (l.n_tokens + G::TM - 1) / G::TM;
     l.n_tiles = (l.n_out + G::TN - 1) / G::TN;
     const int64_t groups = l.low_groups + (int64_t)l.m_tiles * l.n_tiles * l.splits;
+    if (groups * G::T >= 1ll << 32)  // the threads of a launch
+        return llm_fail("%s: n_tokens %d by n_out %d is too much for one launch", name, l.n_tokens, l.n_out);
     if (groups) product_kernel<G><<<groups, G::T, 0, stream>>>(l);
+    return LAUNCH_OK();
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
@@ -536,14 +641,18 @@ bool check_sizes(const char *name, int n_tokens, int n_out, int n_in, int rank) 
     return true;
 }
 
-size_t low_floats(int n_tokens, int rank) { return (size_t)n_tokens * rank; }
+int low_splits(int n_in) { return (n_in + LOW_SPAN - 1) / LOW_SPAN; }
+// Of low: as two bf16, or of its parts, which a join of at most MOST_JOINED rows adds.
+size_t low_floats(int n_tokens, int n_in, int rank) {
+    return (size_t)rank * std::max(n_tokens, std::min(n_tokens, MOST_JOINED) * low_splits(n_in));
+}
 size_t owner_floats(int n_tokens, int rank) { return rank ? ((size_t)n_tokens + 3) / 4 * 4 : 0; }
 
 }  // namespace
 
 extern "C" size_t lora_projection_workspace_floats(int n_tokens, int n_out, int n_in, int rank) {
     if (!check_sizes("lora_projection_workspace_floats", n_tokens, n_out, n_in, rank)) return 0;
-    return low_floats(n_tokens, rank) + owner_floats(n_tokens, rank) + Plan::most_part(n_tokens, n_out);
+    return low_floats(n_tokens, n_in, rank) + owner_floats(n_tokens, rank) + Plan::most_part(n_tokens, n_out);
 }
 
 extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w, const bf16 *residual,
@@ -601,37 +710,38 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     l.splits = p.splits, l.split_steps = p.split_steps;
     l.wide = out_stride % 8 == 0 && aligned16(out) && (!residual || (residual_stride % 8 == 0 && aligned16(residual)));
     l.low = (bf16 *)ws;
-    l.owner = (int *)(ws + low_floats(n_tokens, rank));
-    float *part = ws + low_floats(n_tokens, rank) + owner_floats(n_tokens, rank);
-    int tiles = (n_tokens + 15) / 16, low_groups = 0;
+    l.low_part = ws;
+    l.low_splits = low_splits(n_in);
+    l.owner = (int *)(ws + low_floats(n_tokens, n_in, rank));
+    float *part = ws + low_floats(n_tokens, n_in, rank) + owner_floats(n_tokens, rank);
+    int tiles = (n_tokens + 15) / 16;
     if (lora) {
         l.a = lora->a, l.b = lora->b, l.scale = lora->scale, l.q_start = lora->q_start, l.adapter = lora->adapter;
         l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = rank;
         tiles = n_tokens / 16 + lora->n_seqs;
-        low_groups = tiles * ((rank + LOW - 1) / LOW);
     }
     const auto product = [&](const LoraArgs &a) {
         switch (p.shape) {
-        case 0: launch_product<Large>(a, stream); break;
-        case 1: launch_product<Middle>(a, stream); break;
-        case 2: launch_product<Small>(a, stream); break;
-        default: launch_product<Row>(a, stream);
+        case 0: return launch_product<Large>(name, a, stream);
+        case 1: return launch_product<Middle>(name, a, stream);
+        case 2: return launch_product<Small>(name, a, stream);
+        default: return launch_product<Row>(name, a, stream);
         }
-        return LAUNCH_OK();
     };
     if (p.join) {
         l.part = part;
-        l.low_groups = low_groups;
+        if (lora) l.low_groups = tiles * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
         if (!product(l)) return;
-        join_kernel<<<dim3((n_out + 255) / 256, tiles), 256, 0, stream>>>(l);
+        join_kernel<<<dim3(tiles, (n_out + 255) / 256), 256, 0, stream>>>(l);
         LAUNCH_OK();
         return;
     }
     if (lora) {
-        LoraArgs low = l;
-        low.splits = 0;
-        low.low_groups = low_groups;
-        launch_product<Middle>(low, stream);
+        const int width = low_width(rank);
+        const dim3 grid(tiles, (rank + width - 1) / width);
+        if (width == 16) low_kernel<1><<<grid, 64 * LOW_WAVES, 0, stream>>>(l);
+        else if (width == 32) low_kernel<2><<<grid, 64 * LOW_WAVES, 0, stream>>>(l);
+        else low_kernel<4><<<grid, 64 * LOW_WAVES, 0, stream>>>(l);
         if (!LAUNCH_OK()) return;
     }
     product(l);
