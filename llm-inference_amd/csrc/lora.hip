@@ -17,6 +17,7 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 #define LLM_LDS __attribute__((address_space(3)))
 typedef LLM_LDS char lds_char;
@@ -40,7 +41,7 @@ struct LoraArgs {
     int splits, split_steps;  // of the product's sum, steps of 64 each
     int m_tiles, n_tiles;
     int low_groups, low_splits;  // workgroups in front of the product's that compute low_part
-    bool wide;               // out and residual take 16 bytes at a time
+    bool wide;               // out and residual take 8 bytes at a time
 };
 
 // What is loaded for places past an operand's end.
@@ -81,7 +82,12 @@ template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+// A builtin, so that the compiler knows that what was read is there and does not wait for newer reads in its place.
+__device__ __forceinline__ void wait_lds() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ void barrier() {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -210,6 +216,21 @@ __global__ __launch_bounds__(64 * LOW_WAVES) void low_kernel(LoraArgs l) {
     low[l.rank] = (uint16_t)f2bf(rest);
 }
 
+// Four columns of a row, with the residual's.
+__device__ __forceinline__ void store4(const LoraArgs &l, bf16 *to, const bf16 *res, f32x4 y, int n) {
+    if (l.wide && n + 4 <= l.n_out) {
+        if (l.residual) {
+            const u32x2 v = *gptr((const u32x2 *)res);
+            y += f32x4{lo_f(v.x), hi_f(v.x), lo_f(v.y), hi_f(v.y)};
+        }
+        *gptr((u32x2 *)to) = u32x2{pack2(y[0], y[1]), pack2(y[2], y[3])};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (n + e < l.n_out) gptr(to)[e] = (bf16)f2bf(y[e] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f));
+    }
+}
+
 // Whether NaN or infinities were among eight elements; they are zeros then.
 __device__ __forceinline__ bool clear_unfit_of(u32x4 &v) {
     bool found = false;
@@ -244,15 +265,11 @@ struct Shape {
     static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, S = S_, STAGES = STAGES_;
     static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / S, NT = RN / S;
     static constexpr int BYTES = (TM + TN) * 128;                    // of a stage
-    static constexpr int X_LOADS = (TM / 8 + WAVES - 1) / WAVES;     // per wave; with fewer rows several load the same
-    static constexpr int W_LOADS = TN / 8 / WAVES;
+    static constexpr int X_LOADS = (TM / 8 + WAVES - 1) / WAVES;     // per wave, of eight rows; the last ones may be
+    static constexpr int W_LOADS = (TN / 8 + WAVES - 1) / WAVES;     // loaded more than once
     static constexpr int LOADS = X_LOADS + W_LOADS;
-    static constexpr int SLAB = S * (RN + 4);                        // floats of a wave's rows on their way out
-    static constexpr int SLABS = WAVES * SLAB * 4;
     static constexpr int SUMS = WAVES * 16 * 64 * 4;                 // of low's parts
-    static constexpr int LDS0 = STAGES * BYTES > SLABS ? STAGES * BYTES : SLABS;
-    static constexpr int LDS = LDS0 > SUMS ? LDS0 : SUMS;
-    static_assert(TN / 8 % WAVES == 0 && (TM / 8 % WAVES == 0 || WAVES % (TM / 8) == 0), "loads per wave");
+    static constexpr int LDS = STAGES * BYTES > SUMS ? STAGES * BYTES : SUMS;
 };
 
 template <class G>
@@ -276,8 +293,8 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     const int row = lane / 8, chunk = lane % 8 ^ row;
     unsigned x_at[G::X_LOADS], w_at[G::W_LOADS];   // bytes from the tile's first row
     int x_row[G::X_LOADS];
-    const auto x_group = [&](int i) { return G::TM / 8 >= G::WAVES ? wave * G::X_LOADS + i : wave % (G::TM / 8); };
-    const auto w_group = [&](int i) { return wave * G::W_LOADS + i; };
+    const auto x_group = [&](int i) { return min(wave * G::X_LOADS + i, G::TM / 8 - 1); };
+    const auto w_group = [&](int i) { return min(wave * G::W_LOADS + i, G::TN / 8 - 1); };
 #pragma unroll
     for (int i = 0; i < G::X_LOADS; i++) {
         x_row[i] = x_group(i) * 8 + row;
@@ -295,15 +312,19 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     const int pieces = (2 * l.rank + 63) / 64;
     __syncthreads();
 
+    // Load i of a step of whole chunks into stage `to`.
+    const auto load_whole = [&](int i, int to) {
+        const unsigned xs = base + to * G::BYTES;
+        if (i < G::X_LOADS) load_to_lds(xs + x_group(i) * 1024, x_from + (int64_t)step * 128, x_at[i]);
+        else load_to_lds(xs + G::TM * 128 + w_group(i - G::X_LOADS) * 1024, w_from + (int64_t)step * 128, w_at[i - G::X_LOADS]);
+    };
     // Requests the next step's operands into stage `to`; false after the last.
+    const int whole_end = min(whole_steps, last_step);
     const auto request = [&](int to) {
         const unsigned xs = base + to * G::BYTES, ws = xs + G::TM * 128;
-        if (step < whole_steps && step < last_step) {
-            const char *x = x_from + (int64_t)step * 128, *w = w_from + (int64_t)step * 128;
+        if (step < whole_end) {
 #pragma unroll
-            for (int i = 0; i < G::X_LOADS; i++) load_to_lds(xs + x_group(i) * 1024, x, x_at[i]);
-#pragma unroll
-            for (int i = 0; i < G::W_LOADS; i++) load_to_lds(ws + w_group(i) * 1024, w, w_at[i]);
+            for (int i = 0; i < G::LOADS; i++) load_whole(i, to);
             step++;
             return true;
         }
@@ -362,94 +383,119 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
 
     typename Mfma<G::S>::Acc acc[G::MT][G::NT] = {};
     const int mine_m = wave % G::WM * G::RM, mine_n = wave / G::WM * G::RN;
-    const auto multiply = [&](int from) {
+    constexpr int KS = 64 / Mfma<G::S>::K;  // products of a step, on operands in alternating registers
+    static_assert(KS % 2 == 0, "registers alternate");
+    u32x4 xf[2][G::MT], wf[2][G::NT];
+    const auto fetch = [&](int from, int k) {
         const char *xs = lds + from * G::BYTES, *ws = xs + G::TM * 128;
-        const int r = lane % G::S, c = lane / G::S;
+        const int r = lane % G::S, slot = (k * (64 / G::S) + lane / G::S) ^ (r & 7);
 #pragma unroll
-        for (int k = 0; k < 64 / Mfma<G::S>::K; k++) {
-            const int slot = (k * (64 / G::S) + c) ^ (r & 7);
-            u32x4 xf[G::MT], wf[G::NT];
+        for (int i = 0; i < G::MT; i++) xf[k % 2][i] = *(const u32x4 *)(xs + (mine_m + i * G::S + r) * 128 + slot * 16);
 #pragma unroll
-            for (int i = 0; i < G::MT; i++) xf[i] = *(const u32x4 *)(xs + (mine_m + i * G::S + r) * 128 + slot * 16);
+        for (int j = 0; j < G::NT; j++) wf[k % 2][j] = *(const u32x4 *)(ws + (mine_n + j * G::S + r) * 128 + slot * 16);
+    };
+    const auto multiply = [&](int k) {
 #pragma unroll
-            for (int j = 0; j < G::NT; j++) wf[j] = *(const u32x4 *)(ws + (mine_n + j * G::S + r) * 128 + slot * 16);
+        for (int i = 0; i < G::MT; i++)
 #pragma unroll
-            for (int i = 0; i < G::MT; i++)
-#pragma unroll
-                for (int j = 0; j < G::NT; j++) acc[i][j] = Mfma<G::S>::mul(wf[j], xf[i], acc[i][j]);
+            for (int j = 0; j < G::NT; j++) acc[i][j] = Mfma<G::S>::mul(wf[k % 2][j], xf[k % 2][i], acc[i][j]);
+    };
+    const auto begin = [&](int from) {
+        if (of_adapter >> from & 1) {
+            clear_unfit(from);
+            of_adapter &= ~(1u << from);
         }
+        fetch(from, 0);
     };
 
-    int pending = 0, stage = 0;
+    int pending = 0, stage = 0;  // steps requested and not yet multiplied; the first one's stage
 #pragma unroll
     for (int i = 0; i < G::STAGES - 1; i++)
         if (request(i)) pending++;
-    while (pending > 0) {
-        // all but the steps requested behind this one are there, in every wave; the stage before this one is read
+    if (pending > 0) {
         if (pending == G::STAGES - 1) wait_loads<(G::STAGES - 2) * G::LOADS>();
         else wait_loads<0>();
-        wait_lds();
         barrier();
-        const int next = stage == 0 ? G::STAGES - 1 : stage - 1;
-        if (pending == G::STAGES - 1 && request(next)) pending++;
-        if (of_adapter >> stage & 1) {
-            clear_unfit(stage);
-            of_adapter &= ~(1u << stage);
+        if (pending == G::STAGES - 1 && request(G::STAGES - 1)) pending++;
+        begin(0);
+    }
+    // the next step is there and this one read, in every wave: its stage takes another one, and the next step's first
+    // operands come beside this one's last products
+    while (pending == G::STAGES && step < whole_end) {
+#pragma unroll
+        for (int k = 0; k + 1 < KS; k++) {
+            fetch(stage, k + 1);
+            multiply(k);
         }
-        multiply(stage);
-        pending--;
+        const int free = stage;
         stage = stage == G::STAGES - 1 ? 0 : stage + 1;
+        wait_lds();
+        wait_loads<(G::STAGES - 2) * G::LOADS>();
+        barrier();
+        fetch(stage, 0);
+#pragma unroll
+        for (int i = 0; i < G::MT; i++) {
+#pragma unroll
+            for (int n = i * G::LOADS / G::MT; n < (i + 1) * G::LOADS / G::MT; n++) load_whole(n, free);
+#pragma unroll
+            for (int j = 0; j < G::NT; j++)
+                acc[i][j] = Mfma<G::S>::mul(wf[(KS - 1) % 2][j], xf[(KS - 1) % 2][i], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        step++;
+    }
+    while (pending > 0) {
+#pragma unroll
+        for (int k = 0; k + 1 < KS; k++) {
+            fetch(stage, k + 1);
+            multiply(k);
+        }
+        if (pending > 1) {
+            const int free = stage;
+            stage = stage == G::STAGES - 1 ? 0 : stage + 1;
+            wait_lds();
+            if (pending == G::STAGES) wait_loads<(G::STAGES - 2) * G::LOADS>();
+            else wait_loads<0>();
+            barrier();
+            if (pending == G::STAGES && request(free)) pending++;
+            begin(stage);
+        }
+        multiply(KS - 1);
+        pending--;
     }
     wait_lds();
     barrier();
 
-    // out through LDS, S rows of a wave at a time, so that a row's columns are written side by side
-    float *slab = (float *)lds + wave * G::SLAB;
+    // a lane has four columns side by side of a row
 #pragma unroll
     for (int i = 0; i < G::MT; i++) {
+        const int tile_row = mine_m + i * G::S + lane % G::S, m = m0 + tile_row;
+        if (m >= l.n_tokens || (adapters && owner[tile_row] == NO_SEQUENCE)) continue;
+        bf16 *to = l.out + m * l.out_stride;
+        const bf16 *res = l.residual + m * l.residual_stride;
+        float *part = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width;
 #pragma unroll
         for (int j = 0; j < G::NT; j++)
 #pragma unroll
-            for (int r = 0; r < Mfma<G::S>::REGS / 4; r++)
-                *(f32x4 *)(slab + lane % G::S * (G::RN + 4) + j * G::S + Mfma<G::S>::row(r, lane)) =
-                    f32x4{acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-        wait_lds();
-        constexpr int PER = G::RN / 8;  // lanes of a row
-        const int n = n0 + mine_n + lane % PER * 8;
-#pragma unroll 1
-        for (int r = lane / PER; r < G::S; r += 64 / PER) {
-            const int tile_row = mine_m + i * G::S + r, m = m0 + tile_row;
-            if (m >= l.n_tokens || n >= l.n_out || (adapters && owner[tile_row] == NO_SEQUENCE)) continue;
-            const float *from = slab + r * (G::RN + 4) + lane % PER * 8;
-            f32x4 y[2] = {*(const f32x4 *)from, *(const f32x4 *)(from + 4)};
-            if (join) {
-                float *to = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width + n;
-                *gptr((f32x4 *)to) = y[0];
-                if (n + 4 < l.n_out) *gptr((f32x4 *)(to + 4)) = y[1];
-                continue;
+            for (int r = 0; r < Mfma<G::S>::REGS / 4; r++) {
+                const int n = n0 + mine_n + j * G::S + Mfma<G::S>::row(r, lane);
+                if (n >= l.n_out) continue;
+                const f32x4 y = {acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
+                if (join) *gptr((f32x4 *)(part + n)) = y;
+                else store4(l, to + n, res + n, y, n);
             }
-            if (adapters && *unfit && owner[tile_row] >= 0) {
-                const uint16_t *low = (const uint16_t *)l.low + (int64_t)m * 2 * l.rank;
-                for (int e = 0; e < 8 && n + e < l.n_out; e++)
-                    y[e / 4][e % 4] += unfit_term(l, n + e, owner[tile_row], [&](int j) { return bf2f(gptr(low)[j]) + bf2f(gptr(low)[l.rank + j]); });
-            }
-            bf16 *to = l.out + m * l.out_stride + n;
-            const bf16 *res = l.residual + m * l.residual_stride + n;
-            if (l.wide && n + 8 <= l.n_out) {
-                if (l.residual) {
-                    const u32x4 v = ld16(res);
-#pragma unroll
-                    for (int e = 0; e < 8; e++) y[e / 4][e % 4] += elem(v, e);
-                }
-                st16(to, u32x4{pack2(y[0][0], y[0][1]), pack2(y[0][2], y[0][3]), pack2(y[1][0], y[1][1]), pack2(y[1][2], y[1][3])});
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (n + e < l.n_out)
-                        gptr(to)[e] = (bf16)f2bf(y[e / 4][e % 4] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f));
-            }
+    }
+    if (adapters && *unfit) {  // infinities and NaN, behind what was written
+        __syncthreads();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");
+        for (int i = threadIdx.x; i < G::TM * G::TN; i += G::T) {
+            const int m = m0 + i / G::TN, n = n0 + i % G::TN, a = owner[i / G::TN];
+            if (a < 0 || n >= l.n_out) continue;
+            const uint16_t *low = (const uint16_t *)l.low + (int64_t)m * 2 * l.rank;
+            const float more = unfit_term(l, n, a, [&](int j) { return bf2f(gptr(low)[j]) + bf2f(gptr(low)[l.rank + j]); });
+            LLM_GLOBAL bf16 *to = gptr(l.out) + m * l.out_stride + n;
+            if (!(fabsf(more) < INFINITY)) *to = (bf16)f2bf(bf2f(*to) + more);
         }
-        wait_lds();
     }
 }
 
@@ -457,41 +503,82 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
 // the join: the parts of the product, the adapters' term and the residual
 // ------------------------------------------------------------------------------------------
 
-// 16 rows of a sequence by 256 columns per workgroup. The rows' low is added up once, into LDS; what every lane reads
-// besides is requested in front of that.
+// 16 rows of a sequence by 256 columns per workgroup. The rows' low is added up once, into LDS; the first parts of the
+// product, and what b and the residual hold for few rows, are requested in front of that, so that all of it comes in
+// one round trip behind the lookup of the rows.
 constexpr int FEW = 4;      // rows up to which a lane has a column, and the sum over the rank is one of vector operations
-constexpr int PARTS = 4;    // parts under way
+constexpr int PARTS = 4;    // parts, and chunks of b, under way
 
-// The product's parts of four rows at most, one column per lane.
-__device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, int n, const float *low) {
-    float y[FEW] = {};
+// low of the tile's rows, from its parts.
+__device__ __forceinline__ void join_low(const LoraArgs &l, const RowTile &t, float *low) {
+    const float *from = l.low_part + (int64_t)t.first * l.rank;
+    for (int i = threadIdx.x; i < t.rows * l.rank; i += 256) {
+        float y = 0.0f;
+        constexpr int U = 8;
+        for (int s0 = 0; s0 < l.low_splits; s0 += U) {
+            float part[U];
+#pragma unroll
+            for (int s = 0; s < U; s++)
+                part[s] = s0 + s < l.low_splits ? gptr(from)[(int64_t)(s0 + s) * l.n_tokens * l.rank + i] : 0.0f;
+#pragma unroll
+            for (int s = 0; s < U; s++) y += part[s];
+        }
+        low[i] = y;
+    }
+    const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
+    for (int i = threadIdx.x; i < t.rows * l.rank; i += 256) low[i] *= scale;
+    __syncthreads();
+}
+
+__device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, int n, float *low) {
     const int at = min(n, l.n_out - 1);
-    for (int s0 = 0; s0 < l.splits; s0 += PARTS) {
-        float part[FEW][PARTS];
+    const auto part_at = [&](int i, int s) {
+        return i < t.rows && s < l.splits ? gptr(l.part)[((int64_t)s * l.n_tokens + t.first + i) * l.part_width + at] : 0.0f;
+    };
+    float part[FEW][PARTS], res[FEW], y[FEW] = {};
+    u32x4 v[PARTS];
+    const bf16 *b = l.b + ((int64_t)max(t.adapter, 0) * l.n_out + at) * l.rank;
+    const int rank = t.adapter >= 0 ? l.rank : 0;
+#pragma unroll
+    for (int c = 0; c < PARTS; c++)
+        if (c * 8 < rank) v[c] = ld16(b + c * 8);
+#pragma unroll
+    for (int i = 0; i < FEW; i++) {
+#pragma unroll
+        for (int s = 0; s < PARTS; s++) part[i][s] = part_at(i, s);
+        res[i] = l.residual && i < t.rows ? bf2f(gptr(l.residual)[(t.first + i) * l.residual_stride + at]) : 0.0f;
+    }
+    if (rank) join_low(l, t, low);
+#pragma unroll
+    for (int i = 0; i < FEW; i++)
+#pragma unroll
+        for (int s = 0; s < PARTS; s++) y[i] += part[i][s];
+    for (int s0 = PARTS; s0 < l.splits; s0 += PARTS) {
 #pragma unroll
         for (int i = 0; i < FEW; i++)
 #pragma unroll
-            for (int s = 0; s < PARTS; s++)
-                part[i][s] = i < t.rows && s0 + s < l.splits
-                                 ? gptr(l.part)[((int64_t)(s0 + s) * l.n_tokens + t.first + i) * l.part_width + at] : 0.0f;
+            for (int s = 0; s < PARTS; s++) part[i][s] = part_at(i, s0 + s);
 #pragma unroll
         for (int i = 0; i < FEW; i++)
 #pragma unroll
             for (int s = 0; s < PARTS; s++) y[i] += part[i][s];
     }
-    if (l.residual)
 #pragma unroll
-        for (int i = 0; i < FEW; i++)
-            if (i < t.rows) y[i] += bf2f(gptr(l.residual)[(t.first + i) * l.residual_stride + at]);
-    if (t.adapter >= 0) {
-        const bf16 *b = l.b + ((int64_t)t.adapter * l.n_out + at) * l.rank;
-        for (int j = 0; j < l.rank; j += 8) {
-            const u32x4 v = ld16(b + j);
+    for (int i = 0; i < FEW; i++) y[i] += res[i];
+    for (int j0 = 0; j0 < rank; j0 += 8 * PARTS) {
+        u32x4 next[PARTS];
+#pragma unroll
+        for (int c = 0; c < PARTS; c++)
+            if (j0 + (PARTS + c) * 8 < rank) next[c] = ld16(b + j0 + (PARTS + c) * 8);
+#pragma unroll
+        for (int c = 0; c < PARTS; c++) {
+            if (j0 + c * 8 >= rank) break;
 #pragma unroll
             for (int i = 0; i < FEW; i++)
                 if (i < t.rows)
 #pragma unroll
-                    for (int e = 0; e < 8; e++) y[i] = fmaf(low[i * l.rank + j + e], elem(v, e), y[i]);
+                    for (int e = 0; e < 8; e++) y[i] = fmaf(low[i * rank + j0 + c * 8 + e], elem(v[c], e), y[i]);
+            v[c] = next[c];
         }
     }
     if (n < l.n_out)
@@ -505,44 +592,68 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     const RowTile t = row_tile(l, blockIdx.x);
     if (t.rows == 0) return;
-    if (t.adapter >= 0) {
-        const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
-        const float *from = l.low_part + (int64_t)t.first * l.rank;
-        for (int i = threadIdx.x; i < t.rows * l.rank; i += 256) {
-            float y = 0.0f;
-            for (int s = 0; s < l.low_splits; s++) y += gptr(from)[(int64_t)s * l.n_tokens * l.rank + i];
-            low[i] = y * scale;
-        }
-        __syncthreads();
-    }
     if (t.rows <= FEW) return join_few(l, t, blockIdx.y * 256 + threadIdx.x, low);
     // a lane has row lane % 16 and four columns of each 16
     const int n0 = (blockIdx.y * 4 + wave) * 64, mine = min(lane % 16, t.rows - 1), m = t.first + mine;
+    const auto part_at = [&](int j, int s) {
+        if (s >= l.splits) return f32x4{0, 0, 0, 0};
+        const int n = min(n0 + j * 16 + lane / 16 * 4, l.part_width - 4);
+        return *gptr((const f32x4 *)(l.part + ((int64_t)s * l.n_tokens + m) * l.part_width + n));
+    };
+    f32x4 part[4][PARTS], y[4] = {};
+#pragma unroll
+    for (int s = 0; s < PARTS; s++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) part[j][s] = part_at(j, s);
+    if (t.adapter >= 0) join_low(l, t, low);
     if (n0 >= l.n_out) return;
+#pragma unroll
+    for (int s = 0; s < PARTS; s++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) y[j] += part[j][s];
+    for (int s0 = PARTS; s0 < l.splits; s0 += PARTS) {
+#pragma unroll
+        for (int s = 0; s < PARTS; s++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) part[j][s] = part_at(j, s0 + s);
+#pragma unroll
+        for (int s = 0; s < PARTS; s++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) y[j] += part[j][s];
+    }
     f32x4 acc[4] = {};
     bool unfit = false;
     if (t.adapter >= 0) {
         const bf16 *b = l.b + (int64_t)t.adapter * l.n_out * l.rank;
-        for (int c0 = 0; c0 < l.rank / 8; c0 += 4) {
-            const int c = c0 + lane / 16;
-            const bool there = c < l.rank / 8;
-            u32x4 value = {0, 0, 0, 0}, rest = {0, 0, 0, 0};
-            if (there) {
-                const float *from = low + mine * l.rank + c * 8;
+        constexpr int U = 2;
+        for (int c0 = 0; c0 < l.rank / 8; c0 += 4 * U) {
+            u32x4 v[U][4];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float y0 = from[2 * e], y1 = from[2 * e + 1], v0 = round_bf(y0), v1 = round_bf(y1);
-                    value[e] = pack2(y0, y1);
-                    rest[e] = pack2(fabsf(v0) < INFINITY ? y0 - v0 : 0.0f, fabsf(v1) < INFINITY ? y1 - v1 : 0.0f);
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int c = c0 + 4 * u + lane / 16, n = min(n0 + j * 16 + lane % 16, l.n_out - 1);
+                    v[u][j] = c < l.rank / 8 ? ld16(b + (int64_t)n * l.rank + c * 8) : u32x4{0, 0, 0, 0};
                 }
-            }
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int n = min(n0 + j * 16 + lane % 16, l.n_out - 1);
-                u32x4 v = there ? ld16(b + (int64_t)n * l.rank + c * 8) : u32x4{0, 0, 0, 0};
-                unfit |= clear_unfit_of(v);
-                acc[j] = Mfma<16>::mul(v, value, acc[j]);
-                acc[j] = Mfma<16>::mul(v, rest, acc[j]);
+            for (int u = 0; u < U; u++) {
+                const int c = c0 + 4 * u + lane / 16;
+                u32x4 value = {0, 0, 0, 0}, rest = {0, 0, 0, 0};
+                if (c < l.rank / 8) {
+                    const float *from = low + mine * l.rank + c * 8;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y0 = from[2 * e], y1 = from[2 * e + 1], v0 = round_bf(y0), v1 = round_bf(y1);
+                        value[e] = pack2(y0, y1);
+                        rest[e] = pack2(fabsf(v0) < INFINITY ? y0 - v0 : 0.0f, fabsf(v1) < INFINITY ? y1 - v1 : 0.0f);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    unfit |= clear_unfit_of(v[u][j]);
+                    acc[j] = Mfma<16>::mul(v[u][j], value, acc[j]);
+                    acc[j] = Mfma<16>::mul(v[u][j], rest, acc[j]);
+                }
             }
         }
     }
@@ -552,18 +663,12 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
     for (int j = 0; j < 4; j++) {
         const int n = n0 + j * 16 + lane / 16 * 4;
         if (n >= l.n_out) break;
-        const float *part = l.part + (int64_t)m * l.part_width + n;
-        f32x4 y = acc[j];
-        for (int s = 0; s < l.splits; s++) y += *gptr((const f32x4 *)(part + (int64_t)s * l.n_tokens * l.part_width));
-        bf16 *to = l.out + m * l.out_stride + n;
-        const bf16 *res = l.residual + m * l.residual_stride + n;
+        y[j] += acc[j];
+        if (unfit)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (n + e >= l.n_out) break;
-            float v = y[e] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f);
-            if (unfit) v += unfit_term(l, n + e, t.adapter, [&](int i) { return low[mine * l.rank + i]; });
-            gptr(to)[e] = (bf16)f2bf(v);
-        }
+            for (int e = 0; e < 4; e++)
+                if (n + e < l.n_out) y[j][e] += unfit_term(l, n + e, t.adapter, [&](int i) { return low[mine * l.rank + i]; });
+        store4(l, l.out + m * l.out_stride + n, l.residual + m * l.residual_stride + n, y[j], n);
     }
 }
 
@@ -571,10 +676,24 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
 // on the host
 // ------------------------------------------------------------------------------------------
 
-typedef Shape<256, 192, 64, 96, 16, 2> Large;
-typedef Shape<128, 128, 64, 64, 16, 2> Middle;
+// Shapes of the product, with what an estimate goes by, in ns: workgroups that a CU holds at once, a step where few
+// CUs have a workgroup and where all do, and a tile's first loads and stores.
+struct Pace {
+    int tm, tn, at_once;
+    double alone, full, fixed;
+};
+typedef Shape<256, 192, 64, 96, 16, 2> Wide;
+typedef Shape<224, 256, 112, 64, 16, 2> High;
+typedef Shape<192, 256, 96, 64, 16, 2> Square;
+typedef Shape<128, 256, 64, 64, 16, 3> Half;
+typedef Shape<128, 128, 32, 64, 16, 2> Quarter;
+typedef Shape<64, 128, 64, 32, 16, 3> Low64;
 typedef Shape<64, 64, 64, 16, 16, 4> Small;
 typedef Shape<16, 64, 16, 16, 16, 4> Row;
+constexpr Pace PACES[] = {{256, 192, 1, 930, 1130, 11000}, {224, 256, 1, 1050, 1250, 11000}, {192, 256, 1, 920, 1050, 11000},
+                          {128, 256, 1, 620, 780, 8000},   {128, 128, 2, 560, 760, 6000},    {64, 128, 2, 400, 500, 4500},
+                          {64, 64, 2, 300, 400, 4000},     {16, 64, 3, 250, 350, 3500}};
+constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 
 constexpr int MOST_SPLITS = 32, MOST_JOINED = 2048;
 constexpr size_t MOST_PART = 1 << 23;  // floats
@@ -594,21 +713,19 @@ struct Plan {
         const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
         const int64_t one = (int64_t)part_floats(n_tokens, n_out);
         const int most = (int)std::min<int64_t>(std::min(MOST_SPLITS, std::max(steps, 1)), MOST_PART / one);
-        const struct { int tm, tn, at_once; double step, alone; } shapes[4] = {
-            {256, 192, 1, 1300, 1300}, {128, 128, 2, 1100, 650}, {64, 64, 2, 420, 350}, {16, 64, 3, 300, 200}};
         double least = 0;
         shape = -1;
-        for (int i = 0; i < 4; i++) {
-            const auto &s = shapes[i];
+        for (int i = 0; i < SHAPES; i++) {
+            const Pace &s = PACES[i];
             const double tiles = (double)((n_tokens + s.tm - 1) / s.tm) * ((n_out + s.tn - 1) / s.tn);
             const auto consider = [&](int n, bool joined) {
-                const int each = (steps + n - 1) / n;
                 // adapters of a tile's rows, each with steps of its own
                 const double own = !joined && adapters
                     ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(s.tm, n_tokens) / n_tokens) : 0;
-                const double groups = tiles * n, rounds = groups <= CUS ? 1 : ceil(groups / (s.at_once * CUS));
-                const double cost = 2000 + rounds * (each + own + 2) * (groups <= CUS ? s.alone : s.step) +
-                                    (joined ? 4000 + one * (n + 1.0) * 8 / 5000 : 0);
+                const double groups = tiles * n, rounds = ceil(groups / (s.at_once * CUS)), busy = std::min(1.0, groups / CUS);
+                const double step = s.alone + (s.full - s.alone) * busy;
+                const double cost = rounds * (((steps + n - 1) / n + own) * step + s.fixed) +
+                                    (joined ? 5000 + one * (n * 8.0 + 4) / 4500 : adapters ? 5000 : 0);
                 if (shape < 0 || cost < least) shape = i, splits = n, join = joined, least = cost;
             };
             consider(1, false);
@@ -708,7 +825,8 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     l.n_tokens = n_tokens, l.n_out = n_out, l.n_in = n_in;
     l.part_width = (n_out + 3) / 4 * 4;
     l.splits = p.splits, l.split_steps = p.split_steps;
-    l.wide = out_stride % 8 == 0 && aligned16(out) && (!residual || (residual_stride % 8 == 0 && aligned16(residual)));
+    l.wide = out_stride % 4 == 0 && (uintptr_t)out % 8 == 0 &&
+             (!residual || (residual_stride % 4 == 0 && (uintptr_t)residual % 8 == 0));
     l.low = (bf16 *)ws;
     l.low_part = ws;
     l.low_splits = low_splits(n_in);
@@ -722,9 +840,13 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     }
     const auto product = [&](const LoraArgs &a) {
         switch (p.shape) {
-        case 0: return launch_product<Large>(name, a, stream);
-        case 1: return launch_product<Middle>(name, a, stream);
-        case 2: return launch_product<Small>(name, a, stream);
+        case 0: return launch_product<Wide>(name, a, stream);
+        case 1: return launch_product<High>(name, a, stream);
+        case 2: return launch_product<Square>(name, a, stream);
+        case 3: return launch_product<Half>(name, a, stream);
+        case 4: return launch_product<Quarter>(name, a, stream);
+        case 5: return launch_product<Low64>(name, a, stream);
+        case 6: return launch_product<Small>(name, a, stream);
         default: return launch_product<Row>(name, a, stream);
         }
     };
