@@ -6,6 +6,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "llm_amd/batch.h"
@@ -18,6 +19,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 
 #define LLM_LDS __attribute__((address_space(3)))
 typedef LLM_LDS char lds_char;
@@ -32,15 +34,15 @@ struct LoraArgs {
     const float *scale;
     const int *q_start, *adapter;
     bf16 *low;               // [n_tokens, 2 rank]: value, remainder
+    float *low_part;         // [low_splits, n_tokens, rank]: its parts, without the scale
     int *owner;              // [n_tokens]: the row's adapter, NO_ADAPTER or NO_SEQUENCE
     float *part;             // [splits, n_tokens, part_width], or null: straight to out
-    float *low_part;         // [low_splits, n_tokens, rank], where there are parts
     int64_t out_stride, x_stride, residual_stride;
     int n_tokens, n_out, n_in, n_seqs, n_adapters, rank;
     int part_width;
     int splits, split_steps;  // of the product's sum, steps of 64 each
     int m_tiles, n_tiles;
-    int low_groups, low_splits;  // workgroups in front of the product's that compute low_part
+    int low_groups, low_splits;  // workgroups behind the product's that compute low_part; its parts
     bool wide;               // out and residual take 8 bytes at a time
 };
 
@@ -72,8 +74,12 @@ struct Mfma<16> {
 };
 
 // 64 lanes' 16 bytes into LDS at `to` on, without passing registers: the wave waits for it with wait_loads.
+template <bool STREAM = false>
 __device__ __forceinline__ void load_to_lds(unsigned to, const void *base, unsigned offset) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
+    if constexpr (STREAM)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(to), "v"(offset), "s"(base) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void load_to_lds(unsigned to, const void *at) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(at) : "memory");
@@ -102,118 +108,162 @@ __device__ __forceinline__ int start_of(const LoraArgs &l, int s) {
     return max(0, min(l.n_tokens, gptr(l.q_start)[s]));
 }
 
-// 16 rows of one sequence at most. A sequence of n rows from f on has at most (f + n) / 16 - f / 16 + 1 tiles, so
-// those of sequence s are found from f / 16 + s on, of n_tokens / 16 + n_seqs.
+// R rows of one sequence at most. A sequence of n rows from f on has at most (f + n) / R - f / R + 1 tiles, so those
+// of sequence s are found from f / R + s on, of n_tokens / R + n_seqs.
 struct RowTile {
     int first, rows, adapter;  // rows 0: no tile
 };
+template <int R>
 __device__ __forceinline__ RowTile row_tile(const LoraArgs &l, int i) {
-    RowTile t = {16 * i, 0, NO_ADAPTER};
-    if (!l.a) {
-        t.rows = min(16, l.n_tokens - t.first);
-        return t;
-    }
+    RowTile t = {0, 0, NO_ADAPTER};
     const int lane = threadIdx.x & 63;
     int s0 = 0;  // the sequence is among the 64 from s0 on, which are read at once
-    if (l.n_seqs > 64) s0 = max(0, count_leading(l.n_seqs, [&](int j) { return start_of(l, j) / 16 + j <= i; }) - 1);
+    if (l.n_seqs > 64) s0 = max(0, count_leading(l.n_seqs, [&](int j) { return start_of(l, j) / R + j <= i; }) - 1);
     const int s = min(s0 + lane, l.n_seqs - 1);
     const int f = start_of(l, s), n = start_of(l, s + 1) - f, adapter = gptr(l.adapter)[s];
-    const uint64_t upto = __ballot(s0 + lane < l.n_seqs && f / 16 + s <= i);
+    const uint64_t upto = __ballot(s0 + lane < l.n_seqs && f / R + s <= i);
     if (!upto) return t;
     const int at = 63 - __builtin_clzll(upto);
     const int first = __builtin_amdgcn_readlane(f, at), rows = __builtin_amdgcn_readlane(n, at), a = __builtin_amdgcn_readlane(adapter, at);
-    const int j = i - (first / 16 + s0 + at);
-    t.first = first + 16 * j;
-    t.rows = max(0, min(16, rows - 16 * j));
+    const int j = i - (first / R + s0 + at);
+    t.first = first + R * j;
+    t.rows = max(0, min(R, rows - R * j));
     if ((unsigned)a < (unsigned)l.n_adapters) t.adapter = a;
     return t;
 }
 
-// low of 16 rows and 16 NT elements of the rank, of the sum's elements from `from` on; the waves of the workgroup
-// take SPAN of them each. The sum into sums (LDS, [16][16 NT]).
-template <int NT>
-struct Low {
-    static constexpr int U = NT == 4 ? 4 : 8;  // loads of each operand under way
-    template <int WAVES>
-    static __device__ __forceinline__ void sum(const LoraArgs &l, const RowTile &t, int r0, int from, int span, float *sums) {
-        const int lane = threadIdx.x & 63, wave = wave_id();
-        const bf16 *x = l.x + (t.first + min(lane % 16, t.rows - 1)) * l.x_stride;
-        const bf16 *a = l.a + (int64_t)t.adapter * l.rank * l.n_in;
-        const bf16 *row[NT];
+// ------------------------------------------------------------------------------------------
+// low
+// ------------------------------------------------------------------------------------------
+
+// A part of low, over SPAN elements of its sum per wave, of 16 MT rows and 16 NT elements of the rank.
+template <int MT, int NT, int WAVES, int SPAN>
+__device__ __forceinline__ void low_sums(const LoraArgs &l, const RowTile &t, int r0, int split, float *sums) {
+    constexpr int U = MT == 1 && NT < 4 ? SPAN / 32 : 4;  // loads of each row under way
+    constexpr int ROW = 16 * NT;
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const bf16 *a = l.a + (int64_t)t.adapter * l.rank * l.n_in, *x[MT], *row[NT];
 #pragma unroll
-        for (int j = 0; j < NT; j++) row[j] = a + (int64_t)min(r0 + j * 16 + lane % 16, l.rank - 1) * l.n_in;
-        const int to = min(l.n_in, from + (wave + 1) * span);
-        f32x4 acc[NT] = {};
-        for (int k0 = from + wave * span; k0 < to; k0 += 32 * U) {
-            u32x4 xs[U], as[U][NT];
+    for (int i = 0; i < MT; i++) x[i] = l.x + (t.first + min(i * 16 + lane % 16, t.rows - 1)) * l.x_stride;
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int k = k0 + 32 * u + lane / 16 * 8;
-                xs[u] = k < to ? ld16(x + k) : u32x4{0, 0, 0, 0};
+    for (int j = 0; j < NT; j++) row[j] = a + (int64_t)min(r0 + j * 16 + lane % 16, l.rank - 1) * l.n_in;
+    const int begin = (split * WAVES + wave) * SPAN, end = min(l.n_in, begin + SPAN);
+    f32x4 acc[MT][NT] = {};
+    for (int k0 = begin; k0 < end; k0 += 32 * U) {
+        u32x4 xs[U][MT], as[U][NT];
+        const auto request = [&](const bf16 *p, int u) {
+            const int k = k0 + 32 * u + lane / 16 * 8;
+            return k < end ? ld16(p + k) : u32x4{0, 0, 0, 0};
+        };
+        // the halves of a line one after the other
 #pragma unroll
-                for (int j = 0; j < NT; j++) as[u][j] = k < to ? ld16(row[j] + k) : u32x4{0, 0, 0, 0};
-            }
+        for (int i = 0; i < MT; i++)
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++) xs[u][i] = request(x[i], u);
 #pragma unroll
-                for (int j = 0; j < NT; j++) acc[j] = Mfma<16>::mul(as[u][j], xs[u], acc[j]);
-        }
-        constexpr int ROW = 16 * NT;
-        float *mine = sums + wave * 16 * ROW;
+        for (int j = 0; j < NT; j++)
 #pragma unroll
-        for (int j = 0; j < NT; j++) *(f32x4 *)(mine + lane % 16 * ROW + j * 16 + lane / 16 * 4) = acc[j];
-        __syncthreads();
-        for (int i = threadIdx.x; i < 16 * ROW; i += 64 * WAVES) {
-            float y = 0.0f;
-            for (int w = 0; w < WAVES; w++) y += sums[w * 16 * ROW + i];
-            sums[i] = y;
-        }
+            for (int u = 0; u < U; u++) as[u][j] = request(row[j], u);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) acc[i][j] = Mfma<16>::mul(as[u][j], xs[u][i], acc[i][j]);
     }
-};
-constexpr int LOW_SPAN = 1024;  // elements of the sum per workgroup where a join adds their parts
+    // rows 16 bytes further apart: side by side those of a product's 16 would meet in the same banks
+    constexpr int ALL = 16 * MT * (ROW + 4);
+    float *mine = sums + wave * ALL;
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) *(f32x4 *)(mine + (i * 16 + lane % 16) * (ROW + 4) + j * 16 + lane / 16 * 4) = acc[i][j];
+    __syncthreads();
+    float *to = l.low_part + ((int64_t)split * l.n_tokens + t.first) * l.rank + r0;
+    for (int i = 4 * threadIdx.x; i < 16 * MT * ROW; i += 4 * 64 * WAVES) {
+        const int m = i / ROW, r = i % ROW;
+        if (m >= t.rows || r0 + r >= l.rank) continue;
+        f32x4 y = {0, 0, 0, 0};
+        for (int w = 0; w < WAVES; w++) y += *(const f32x4 *)(sums + w * ALL + m * (ROW + 4) + r);
+        *gptr((f32x4 *)(to + (int64_t)m * l.rank + r)) = y;
+    }
+}
 __host__ __device__ __forceinline__ int low_width(int rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
-// For a join: part low_split of low, in 32 bits and without its scale.
-template <int WAVES>
+// A part of low of R rows, in 32 bits and without the scale; and the rows' owners.
+template <int R, int WAVES, int SPAN>
 __device__ __forceinline__ void low_part(const LoraArgs &l, int block, float *lds) {
     const int width = low_width(l.rank), groups = (l.rank + width - 1) / width;
     const int split = block % l.low_splits, r0 = block / l.low_splits % groups * width;
-    const RowTile t = row_tile(l, block / l.low_splits / groups);
-    if (t.rows == 0 || t.adapter < 0) return;
-    const int from = split * LOW_SPAN;
-    if (width == 16) Low<1>::sum<WAVES>(l, t, r0, from, LOW_SPAN / WAVES, lds);
-    else if (width == 32) Low<2>::sum<WAVES>(l, t, r0, from, LOW_SPAN / WAVES, lds);
-    else Low<4>::sum<WAVES>(l, t, r0, from, LOW_SPAN / WAVES, lds);
-    float *to = l.low_part + ((int64_t)split * l.n_tokens + t.first) * l.rank + r0;
-    for (int i = threadIdx.x; i < 16 * width; i += 64 * WAVES)
-        if (i / width < t.rows && r0 + i % width < l.rank) gptr(to)[(int64_t)(i / width) * l.rank + i % width] = lds[i];
-}
-
-// Otherwise: low as two bf16, and the rows' owners. 16 waves share the sum.
-constexpr int LOW_WAVES = 16;
-template <int NT>
-__global__ __launch_bounds__(64 * LOW_WAVES) void low_kernel(LoraArgs l) {
-    __shared__ __attribute__((aligned(16))) float sums[LOW_WAVES * 16 * 16 * NT];
-    const int r0 = blockIdx.y * 16 * NT;
-    const RowTile t = row_tile(l, blockIdx.x);
-    if (blockIdx.y == 0) {
-        if (blockIdx.x == 0) {
+    const int tile = block / l.low_splits / groups;
+    const RowTile t = row_tile<R>(l, tile);
+    if (split == 0 && r0 == 0) {
+        if (tile == 0) {
             const int begin = start_of(l, 0), end = max(begin, start_of(l, l.n_seqs));
-            for (int i = threadIdx.x; i < l.n_tokens; i += 64 * LOW_WAVES)
+            for (int i = threadIdx.x; i < l.n_tokens; i += 64 * WAVES)
                 if (i < begin || i >= end) gptr(l.owner)[i] = NO_SEQUENCE;
         }
         if ((int)threadIdx.x < t.rows) gptr(l.owner)[t.first + threadIdx.x] = t.adapter;
     }
     if (t.rows == 0 || t.adapter < 0) return;
-    const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
-    Low<NT>::template sum<LOW_WAVES>(l, t, r0, 0, (l.n_in + 32 * LOW_WAVES - 1) / (32 * LOW_WAVES) * 32, sums);
-    const int i = threadIdx.x, m = i / (16 * NT), r = r0 + i % (16 * NT);
-    if (m >= t.rows || r >= l.rank) return;
-    const float sum = sums[i] * scale;
-    const float value = round_bf(sum), rest = fabsf(value) < INFINITY ? sum - value : 0.0f;
-    LLM_GLOBAL uint16_t *low = gptr((uint16_t *)l.low) + (int64_t)(t.first + m) * 2 * l.rank + r;
-    low[0] = (uint16_t)f2bf(value);
-    low[l.rank] = (uint16_t)f2bf(rest);
+    const auto sum = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        if (width == 16) low_sums<MT, 1, WAVES, SPAN>(l, t, r0, split, lds);
+        else if (width == 32) low_sums<MT, 2, WAVES, SPAN>(l, t, r0, split, lds);
+        else low_sums<MT, 4, WAVES, SPAN>(l, t, r0, split, lds);
+    };
+    if (t.rows <= 16) sum(std::integral_constant<int, 1>{});
+    else sum(std::integral_constant<int, R / 16>{});
+}
+
+// Elements of the sum per workgroup: of 64 rows so few that the workgroups fill the CUs, of 16 beside the product more,
+// for fewer parts to add up.
+constexpr int LOW_WAVES = 4, LOW_ROWS = 64, LOW_SPAN = 512, JOIN_LOW_SPAN = 1024;
+__global__ __launch_bounds__(64 * LOW_WAVES) void low_kernel(LoraArgs l) {
+    __shared__ __attribute__((aligned(16))) float sums[LOW_WAVES * LOW_ROWS * 68];
+    low_part<LOW_ROWS, LOW_WAVES, LOW_SPAN / LOW_WAVES>(l, blockIdx.x, sums);
+}
+
+// Element i of a row's low: the parts in order, and the scale.
+__device__ __forceinline__ f32x4 low_sum(const LoraArgs &l, int64_t at, float scale) {
+    f32x4 y = {0, 0, 0, 0};
+    constexpr int U = 4;
+    for (int s0 = 0; s0 < l.low_splits; s0 += U) {
+        f32x4 part[U];
+#pragma unroll
+        for (int s = 0; s < U; s++)
+            part[s] = s0 + s < l.low_splits ? *gptr((const f32x4 *)(l.low_part + (int64_t)(s0 + s) * l.n_tokens * l.rank + at))
+                                            : f32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < U; s++) y += part[s];
+    }
+    return y * scale;
+}
+// Two numbers as bf16, and what that leaves of them.
+__device__ __forceinline__ void in_two(float y0, float y1, uint32_t &value, uint32_t &rest) {
+    const float v0 = round_bf(y0), v1 = round_bf(y1);
+    value = pack2(y0, y1);
+    rest = pack2(fabsf(v0) < INFINITY ? y0 - v0 : 0.0f, fabsf(v1) < INFINITY ? y1 - v1 : 0.0f);
+}
+
+// low from its parts: four elements per thread.
+__global__ __launch_bounds__(256) void low_sum_kernel(LoraArgs l) {
+    const int per = l.rank / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int m = (int)(i / per), r = (int)(i % per) * 4;
+    if (m >= l.n_tokens) return;
+    const int owner = gptr(l.owner)[m];
+    if (owner < 0) return;
+    const f32x4 y = low_sum(l, (int64_t)m * l.rank + r, l.scale ? gptr(l.scale)[owner] : 1.0f);
+    u32x2 value, rest;
+    uint32_t v, w;
+    in_two(y[0], y[1], v, w);
+    value.x = v, rest.x = w;
+    in_two(y[2], y[3], v, w);
+    value.y = v, rest.y = w;
+    bf16 *low = l.low + (int64_t)m * 2 * l.rank + r;
+    *gptr((u32x2 *)low) = value;
+    *gptr((u32x2 *)(low + l.rank)) = rest;
 }
 
 // Four columns of a row, with the residual's.
@@ -260,33 +310,36 @@ __device__ __forceinline__ float unfit_term(const LoraArgs &l, int n, int adapte
 // TM rows by TN columns of a workgroup, in waves of RM by RN, on MFMAs of side S; 64 elements of the sum a step,
 // STAGES steps' operands in LDS. A row's 128 bytes of a step lie as eight 16-byte chunks, chunk c of row r at
 // c ^ (r % 8): the rows that a product reads at one chunk then lie in different banks.
-template <int TM_, int TN_, int RM_, int RN_, int S_, int STAGES_>
+template <int TM_, int TN_, int RM_, int RN_, int S_, int STAGES_, bool STREAM_ = false>
 struct Shape {
+    static constexpr bool STREAM = STREAM_;                          // W is read once, past the caches
     static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, S = S_, STAGES = STAGES_;
     static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / S, NT = RN / S;
+    static constexpr bool JOINS = TM <= 64;                          // also in front of join_kernel
     static constexpr int BYTES = (TM + TN) * 128;                    // of a stage
+    static_assert(!JOINS || STAGES * BYTES >= WAVES * 16 * 68 * 4, "low_part's sums");
     static constexpr int X_LOADS = (TM / 8 + WAVES - 1) / WAVES;     // per wave, of eight rows; the last ones may be
     static constexpr int W_LOADS = (TN / 8 + WAVES - 1) / WAVES;     // loaded more than once
     static constexpr int LOADS = X_LOADS + W_LOADS;
-    static constexpr int SUMS = WAVES * 16 * 64 * 4;                 // of low's parts
-    static constexpr int LDS = STAGES * BYTES > SUMS ? STAGES * BYTES : SUMS;
 };
 
 template <class G>
 __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
-    __shared__ __attribute__((aligned(128))) char lds[G::LDS + G::TM * 4 + 4];
-    int *owner = (int *)(lds + G::LDS), *unfit = owner + G::TM;
+    __shared__ __attribute__((aligned(128))) char lds[G::STAGES * G::BYTES + G::TM * 8 + 8];
+    int *owner = (int *)(lds + G::STAGES * G::BYTES), *list = owner + G::TM, *count = list + G::TM, *unfit = count + 1;
     const int lane = threadIdx.x & 63, wave = wave_id();
-    if ((int)blockIdx.x < l.low_groups) return low_part<G::WAVES>(l, blockIdx.x, (float *)lds);
+    if (G::JOINS && (int)blockIdx.x >= l.m_tiles * l.n_tiles * l.splits)
+        return low_part<16, G::WAVES, JOIN_LOW_SPAN / G::WAVES>(l, blockIdx.x - l.m_tiles * l.n_tiles * l.splits, (float *)lds);
     // the tiles of one XCD, whose workgroups every eighth one is, lie side by side
-    const int tiles = l.m_tiles * l.n_tiles * l.splits, block = blockIdx.x - l.low_groups;
+    const int tiles = l.m_tiles * l.n_tiles * l.splits, block = blockIdx.x;
     const int each = tiles / XCDS, more = tiles % XCDS, xcd = block % XCDS;
     const int at = xcd * each + min(xcd, more) + block / XCDS;
     const int m0 = at % l.m_tiles * G::TM, n0 = at / l.m_tiles % l.n_tiles * G::TN, split = at / (l.m_tiles * l.n_tiles);
-    const bool join = l.part != nullptr, adapters = l.a && !join;
-    if (adapters && (int)threadIdx.x < G::TM)
+    const bool join = l.part != nullptr, adapters = l.a && !l.low_groups && split == l.splits - 1;
+    const bool owned = l.a && !l.low_groups;  // otherwise join_kernel looks them up
+    if (owned && (int)threadIdx.x < G::TM)
         owner[threadIdx.x] = m0 + (int)threadIdx.x < l.n_tokens ? gptr(l.owner)[m0 + threadIdx.x] : NO_SEQUENCE;
-    if (threadIdx.x == 0) *unfit = 0;
+    if (threadIdx.x == 0) *unfit = *count = 0;
 
     // loads: lane's row lane / 8 and chunk lane % 8 of eight rows
     const unsigned base = (unsigned)(uintptr_t)(lds_char *)lds;
@@ -305,18 +358,46 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
         w_at[i] = (unsigned)min(w_group(i) * 8 + row, l.n_out - 1 - n0) * (unsigned)l.n_in * 2 + chunk * 16;
     const char *x_from = (const char *)(l.x + m0 * l.x_stride), *w_from = (const char *)(l.w + (int64_t)n0 * l.n_in);
     const int all_steps = l.w ? (l.n_in + 63) / 64 : 0, whole_steps = l.w ? l.n_in / 64 : 0;
-    int step = split * l.split_steps;
-    const int last_step = min(all_steps, step + l.split_steps);
-    int current = NO_ADAPTER, piece = 0;  // the adapter whose part of the sum comes next
-    unsigned of_adapter = 0;              // stages that hold some of it
+    const int last_step = min(all_steps, (split + 1) * l.split_steps);
+    int step = split * l.split_steps, next = 0, piece = 0;  // what is requested next: the product's, then adapters'
+    unsigned of_adapter = 0;                                // stages that hold some of these
     const int pieces = (2 * l.rank + 63) / 64;
     __syncthreads();
+    if (adapters && wave == 0) {  // the adapters of the tile's rows, each once: entry 64 q + lane in entry[q]
+        constexpr int Q = (G::TM + 63) / 64;
+        int entry[Q], n = 0;
+#pragma unroll
+        for (int q = 0; q < Q; q++) entry[q] = NO_ADAPTER;
+#pragma unroll 1
+        for (int q = 0; q < Q; q++) {
+            const int i = q * 64 + lane, mine = i < G::TM ? owner[i] : NO_SEQUENCE;
+            uint64_t starts = __ballot(mine >= 0 && (i == 0 || owner[i - 1] != mine));
+            while (starts) {  // of rows with one adapter, one after the other
+                const int a = __builtin_amdgcn_readlane(mine, __builtin_ctzll(starts));
+                starts &= starts - 1;
+                bool there = false;
+#pragma unroll
+                for (int p = 0; p < Q; p++) there |= entry[p] == a;
+                if (__any(there)) continue;
+#pragma unroll
+                for (int p = 0; p < Q; p++)
+                    if (p * 64 + lane == n) entry[p] = a;
+                n++;
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+            if (q * 64 + lane < n) list[q * 64 + lane] = entry[q];
+        if (lane == 0) *count = n;
+    }
+    if (adapters) __syncthreads();
+    const int listed = adapters ? __builtin_amdgcn_readfirstlane(*count) : 0;
 
     // Load i of a step of whole chunks into stage `to`.
     const auto load_whole = [&](int i, int to) {
         const unsigned xs = base + to * G::BYTES;
         if (i < G::X_LOADS) load_to_lds(xs + x_group(i) * 1024, x_from + (int64_t)step * 128, x_at[i]);
-        else load_to_lds(xs + G::TM * 128 + w_group(i - G::X_LOADS) * 1024, w_from + (int64_t)step * 128, w_at[i - G::X_LOADS]);
+        else load_to_lds<G::STREAM>(xs + G::TM * 128 + w_group(i - G::X_LOADS) * 1024, w_from + (int64_t)step * 128, w_at[i - G::X_LOADS]);
     };
     // Requests the next step's operands into stage `to`; false after the last.
     const int whole_end = min(whole_steps, last_step);
@@ -340,18 +421,8 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
             step++;
             return true;
         }
-        if (!adapters) return false;
-        if (piece == 0) {  // the next higher adapter of the tile's rows
-            int next = INT32_MAX;
-#pragma unroll
-            for (int i = 0; i < (G::TM + 63) / 64; i++) {
-                const int o = owner[min(i * 64 + lane, G::TM - 1)];
-                if (o > current) next = min(next, o);
-            }
-            for (int d = 1; d < 64; d *= 2) next = min(next, __shfl_xor(next, d));
-            current = __builtin_amdgcn_readfirstlane(next);
-        }
-        if (current == INT32_MAX) return false;
+        if (next == listed) return false;
+        const int current = __builtin_amdgcn_readfirstlane(list[next]);
         const int c = piece * 8 + chunk, chunks = l.rank / 8;
         const char *low = (const char *)(l.low + (int64_t)m0 * 2 * l.rank) + c * 16;
         const char *b = (const char *)(l.b + ((int64_t)current * l.n_out + n0) * l.rank) + (c >= chunks ? c - chunks : c) * 16;
@@ -364,24 +435,11 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
         for (int i = 0; i < G::W_LOADS; i++)
             load_to_lds(ws + w_group(i) * 1024,
                         there ? b + (int64_t)min(w_group(i) * 8 + row, l.n_out - 1 - n0) * 2 * l.rank : (const char *)&g_zeros);
-        if (++piece == pieces) piece = 0;
+        if (++piece == pieces) piece = 0, next++;
         of_adapter |= 1u << to;
         return true;
     };
-    // NaN and infinities of an adapter become zeros: times the zeros of other rows, or a remainder of zero, they
-    // would be no numbers. The rows that they belong to get them in the end.
-    const auto clear_unfit = [&](int from) {
-        bool found = false;
-        for (int c = threadIdx.x; c < G::TN * 8; c += G::T) {
-            u32x4 *at = (u32x4 *)(lds + from * G::BYTES + G::TM * 128 + c * 16), v = *at;
-            if (clear_unfit_of(v)) *at = v, found = true;
-        }
-        if (found) *unfit = 1;
-        wait_lds();
-        barrier();
-    };
-
-    typename Mfma<G::S>::Acc acc[G::MT][G::NT] = {};
+    typename Mfma<G::S>::Acc acc[G::MT][G::NT];
     const int mine_m = wave % G::WM * G::RM, mine_n = wave / G::WM * G::RN;
     constexpr int KS = 64 / Mfma<G::S>::K;  // products of a step, on operands in alternating registers
     static_assert(KS % 2 == 0, "registers alternate");
@@ -400,14 +458,36 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
 #pragma unroll
             for (int j = 0; j < G::NT; j++) acc[i][j] = Mfma<G::S>::mul(wf[k % 2][j], xf[k % 2][i], acc[i][j]);
     };
+    // NaN and infinities of an adapter, times the zeros of other rows or a remainder of zero, would be no numbers
+    // everywhere. Where there are some, which the largest exponent tells, the tile is computed again with zeros in
+    // their place, and the rows that they belong to get them in the end.
+    u16x2 largest = {0, 0};
+    bool clear = false;
     const auto begin = [&](int from) {
-        if (of_adapter >> from & 1) {
-            clear_unfit(from);
-            of_adapter &= ~(1u << from);
+        if (of_adapter >> from & 1 && clear) {
+            for (int c = threadIdx.x; c < G::TN * 8; c += G::T) {
+                u32x4 *at = (u32x4 *)(lds + from * G::BYTES + G::TM * 128 + c * 16), v = *at;
+                if (clear_unfit_of(v)) *at = v;
+            }
+            wait_lds();
+            barrier();
         }
         fetch(from, 0);
     };
+    const auto look_at = [&](int from, int k) {
+        if (!(of_adapter >> from & 1)) return;
+#pragma unroll
+        for (int j = 0; j < G::NT; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, wf[k % 2][j][e] & 0x7fff7fffu));
+    };
 
+again:
+#pragma unroll
+    for (int i = 0; i < G::MT; i++)
+#pragma unroll
+        for (int j = 0; j < G::NT; j++) acc[i][j] = {};
     int pending = 0, stage = 0;  // steps requested and not yet multiplied; the first one's stage
 #pragma unroll
     for (int i = 0; i < G::STAGES - 1; i++)
@@ -445,19 +525,22 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
         step++;
     }
     while (pending > 0) {
+        const int at = stage;
 #pragma unroll
         for (int k = 0; k + 1 < KS; k++) {
-            fetch(stage, k + 1);
+            fetch(at, k + 1);
+            look_at(at, k);
             multiply(k);
         }
+        look_at(at, KS - 1);
+        of_adapter &= ~(1u << at);
         if (pending > 1) {
-            const int free = stage;
             stage = stage == G::STAGES - 1 ? 0 : stage + 1;
             wait_lds();
             if (pending == G::STAGES) wait_loads<(G::STAGES - 2) * G::LOADS>();
             else wait_loads<0>();
             barrier();
-            if (pending == G::STAGES && request(free)) pending++;
+            if (pending == G::STAGES && request(at)) pending++;
             begin(stage);
         }
         multiply(KS - 1);
@@ -465,12 +548,23 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     }
     wait_lds();
     barrier();
+    if (adapters && !clear) {
+        if (largest[0] >= 0x7f80 || largest[1] >= 0x7f80) *unfit = 1;
+        wait_lds();
+        barrier();
+        clear = __builtin_amdgcn_readfirstlane(*unfit);
+        if (clear) {
+            step = split * l.split_steps;
+            next = 0;
+            goto again;
+        }
+    }
 
     // a lane has four columns side by side of a row
 #pragma unroll
     for (int i = 0; i < G::MT; i++) {
         const int tile_row = mine_m + i * G::S + lane % G::S, m = m0 + tile_row;
-        if (m >= l.n_tokens || (adapters && owner[tile_row] == NO_SEQUENCE)) continue;
+        if (m >= l.n_tokens || (owned && owner[tile_row] == NO_SEQUENCE)) continue;
         bf16 *to = l.out + m * l.out_stride;
         const bf16 *res = l.residual + m * l.residual_stride;
         float *part = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width;
@@ -485,7 +579,7 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
                 else store4(l, to + n, res + n, y, n);
             }
     }
-    if (adapters && *unfit) {  // infinities and NaN, behind what was written
+    if (clear) {  // the infinities and NaN, behind what was written
         __syncthreads();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "agent");
         for (int i = threadIdx.x; i < G::TM * G::TN; i += G::T) {
@@ -493,106 +587,111 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
             if (a < 0 || n >= l.n_out) continue;
             const uint16_t *low = (const uint16_t *)l.low + (int64_t)m * 2 * l.rank;
             const float more = unfit_term(l, n, a, [&](int j) { return bf2f(gptr(low)[j]) + bf2f(gptr(low)[l.rank + j]); });
+            if (fabsf(more) < INFINITY) continue;
+            LLM_GLOBAL float *part = gptr(l.part) + ((int64_t)split * l.n_tokens + m) * l.part_width + n;
             LLM_GLOBAL bf16 *to = gptr(l.out) + m * l.out_stride + n;
-            if (!(fabsf(more) < INFINITY)) *to = (bf16)f2bf(bf2f(*to) + more);
+            if (join) *part += more;
+            else *to = (bf16)f2bf(bf2f(*to) + more);
         }
     }
 }
 
-// ------------------------------------------------------------------------------------------
-// the join: the parts of the product, the adapters' term and the residual
-// ------------------------------------------------------------------------------------------
-
-// 16 rows of a sequence by 256 columns per workgroup. The rows' low is added up once, into LDS; the first parts of the
-// product, and what b and the residual hold for few rows, are requested in front of that, so that all of it comes in
-// one round trip behind the lookup of the rows.
-constexpr int FEW = 4;      // rows up to which a lane has a column, and the sum over the rank is one of vector operations
-constexpr int PARTS = 4;    // parts, and chunks of b, under way
-
-// low of the tile's rows, from its parts.
-__device__ __forceinline__ void join_low(const LoraArgs &l, const RowTile &t, float *low) {
-    const float *from = l.low_part + (int64_t)t.first * l.rank;
-    for (int i = threadIdx.x; i < t.rows * l.rank; i += 256) {
-        float y = 0.0f;
-        constexpr int U = 8;
-        for (int s0 = 0; s0 < l.low_splits; s0 += U) {
-            float part[U];
+// out of the product's parts: four columns of a row per thread.
+__global__ __launch_bounds__(256) void sum_kernel(LoraArgs l) {
+    const int per = l.part_width / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int m = (int)(i / per), n = (int)(i % per) * 4;
+    if (m >= l.n_tokens || (l.a && gptr(l.owner)[m] == NO_SEQUENCE)) return;
+    const float *part = l.part + (int64_t)m * l.part_width + n;
+    const int64_t next = (int64_t)l.n_tokens * l.part_width;
+    f32x4 y = {0, 0, 0, 0};
+    constexpr int U = 4;
+    for (int s0 = 0; s0 < l.splits; s0 += U) {
+        f32x4 v[U];
 #pragma unroll
-            for (int s = 0; s < U; s++)
-                part[s] = s0 + s < l.low_splits ? gptr(from)[(int64_t)(s0 + s) * l.n_tokens * l.rank + i] : 0.0f;
+        for (int s = 0; s < U; s++)
+            v[s] = s0 + s < l.splits ? *gptr((const f32x4 *)(part + (s0 + s) * next)) : f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int s = 0; s < U; s++) y += part[s];
-        }
-        low[i] = y;
+        for (int s = 0; s < U; s++) y += v[s];
     }
-    const float scale = l.scale ? gptr(l.scale)[t.adapter] : 1.0f;
-    for (int i = threadIdx.x; i < t.rows * l.rank; i += 256) low[i] *= scale;
+    store4(l, l.out + m * l.out_stride + n, l.residual + m * l.residual_stride + n, y, n);
+}
+
+// ------------------------------------------------------------------------------------------
+// the join: the product's parts, the adapters' terms and the residual
+// ------------------------------------------------------------------------------------------
+
+// 16 rows of a sequence by 256 columns per workgroup. What the lanes read besides the parts of low is requested in
+// front of those, so that all of it comes in one round trip behind the lookup of the rows.
+constexpr int FEW = 4;      // rows up to which a lane has a column, and the sum over the rank is one of vector operations
+
+// low of the tile's rows, into LDS.
+__device__ __forceinline__ void join_low(const LoraArgs &l, const RowTile &t, float scale, float *low) {
+    for (int i = 4 * threadIdx.x; i < t.rows * l.rank; i += 4 * 256)
+        *(f32x4 *)(low + i) = low_sum(l, (int64_t)t.first * l.rank + i, scale);
     __syncthreads();
 }
 
-__device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, int n, float *low) {
-    const int at = min(n, l.n_out - 1);
+// ROWS: rows of the tile at most.
+template <int ROWS>
+__device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, int n, float scale, float *low) {
+    constexpr int P = ROWS == 1 ? 8 : 4, CHUNKS = 4;  // parts, and chunks of b, under way
+    const int at = min(n, l.n_out - 1), rank = t.adapter >= 0 ? l.rank : 0;
     const auto part_at = [&](int i, int s) {
         return i < t.rows && s < l.splits ? gptr(l.part)[((int64_t)s * l.n_tokens + t.first + i) * l.part_width + at] : 0.0f;
     };
-    float part[FEW][PARTS], res[FEW], y[FEW] = {};
-    u32x4 v[PARTS];
+    float part[ROWS][P], y[ROWS];
+    u32x4 v[CHUNKS];
     const bf16 *b = l.b + ((int64_t)max(t.adapter, 0) * l.n_out + at) * l.rank;
-    const int rank = t.adapter >= 0 ? l.rank : 0;
 #pragma unroll
-    for (int c = 0; c < PARTS; c++)
+    for (int c = 0; c < CHUNKS; c++)
         if (c * 8 < rank) v[c] = ld16(b + c * 8);
 #pragma unroll
-    for (int i = 0; i < FEW; i++) {
+    for (int i = 0; i < ROWS; i++) {
+        y[i] = l.residual && i < t.rows ? bf2f(gptr(l.residual)[(t.first + i) * l.residual_stride + at]) : 0.0f;
 #pragma unroll
-        for (int s = 0; s < PARTS; s++) part[i][s] = part_at(i, s);
-        res[i] = l.residual && i < t.rows ? bf2f(gptr(l.residual)[(t.first + i) * l.residual_stride + at]) : 0.0f;
+        for (int s = 0; s < P; s++) part[i][s] = part_at(i, s);
     }
-    if (rank) join_low(l, t, low);
+    if (rank) join_low(l, t, scale, low);
+    for (int s0 = 0;;) {
 #pragma unroll
-    for (int i = 0; i < FEW; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
-        for (int s = 0; s < PARTS; s++) y[i] += part[i][s];
-    for (int s0 = PARTS; s0 < l.splits; s0 += PARTS) {
+            for (int s = 0; s < P; s++) y[i] += part[i][s];
+        if ((s0 += P) >= l.splits) break;
 #pragma unroll
-        for (int i = 0; i < FEW; i++)
+        for (int i = 0; i < ROWS; i++)
 #pragma unroll
-            for (int s = 0; s < PARTS; s++) part[i][s] = part_at(i, s0 + s);
-#pragma unroll
-        for (int i = 0; i < FEW; i++)
-#pragma unroll
-            for (int s = 0; s < PARTS; s++) y[i] += part[i][s];
+            for (int s = 0; s < P; s++) part[i][s] = part_at(i, s0 + s);
     }
+    for (int j0 = 0; j0 < rank; j0 += 8 * CHUNKS) {
 #pragma unroll
-    for (int i = 0; i < FEW; i++) y[i] += res[i];
-    for (int j0 = 0; j0 < rank; j0 += 8 * PARTS) {
-        u32x4 next[PARTS];
-#pragma unroll
-        for (int c = 0; c < PARTS; c++)
-            if (j0 + (PARTS + c) * 8 < rank) next[c] = ld16(b + j0 + (PARTS + c) * 8);
-#pragma unroll
-        for (int c = 0; c < PARTS; c++) {
+        for (int c = 0; c < CHUNKS; c++) {
             if (j0 + c * 8 >= rank) break;
 #pragma unroll
-            for (int i = 0; i < FEW; i++)
+            for (int i = 0; i < ROWS; i++)
                 if (i < t.rows)
 #pragma unroll
                     for (int e = 0; e < 8; e++) y[i] = fmaf(low[i * rank + j0 + c * 8 + e], elem(v[c], e), y[i]);
-            v[c] = next[c];
         }
+#pragma unroll
+        for (int c = 0; c < CHUNKS; c++)
+            if (j0 + (CHUNKS + c) * 8 < rank) v[c] = ld16(b + j0 + (CHUNKS + c) * 8);
     }
     if (n < l.n_out)
 #pragma unroll
-        for (int i = 0; i < FEW; i++)
+        for (int i = 0; i < ROWS; i++)
             if (i < t.rows) gptr(l.out)[(t.first + i) * l.out_stride + n] = (bf16)f2bf(y[i]);
 }
 
 __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
-    __shared__ float low[16 * 256];
+    __shared__ __attribute__((aligned(16))) float low[16 * 256];
     const int lane = threadIdx.x & 63, wave = wave_id();
-    const RowTile t = row_tile(l, blockIdx.x);
+    const RowTile t = row_tile<16>(l, blockIdx.x);
     if (t.rows == 0) return;
-    if (t.rows <= FEW) return join_few(l, t, blockIdx.y * 256 + threadIdx.x, low);
+    const float scale = l.scale && t.adapter >= 0 ? gptr(l.scale)[t.adapter] : 1.0f;
+    if (t.rows == 1) return join_few<1>(l, t, blockIdx.y * 256 + threadIdx.x, scale, low);
+    if (t.rows <= FEW) return join_few<FEW>(l, t, blockIdx.y * 256 + threadIdx.x, scale, low);
     // a lane has row lane % 16 and four columns of each 16
     const int n0 = (blockIdx.y * 4 + wave) * 64, mine = min(lane % 16, t.rows - 1), m = t.first + mine;
     const auto part_at = [&](int j, int s) {
@@ -600,26 +699,24 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
         const int n = min(n0 + j * 16 + lane / 16 * 4, l.part_width - 4);
         return *gptr((const f32x4 *)(l.part + ((int64_t)s * l.n_tokens + m) * l.part_width + n));
     };
-    f32x4 part[4][PARTS], y[4] = {};
+    constexpr int P = 4;
+    f32x4 part[4][P], y[4] = {};
 #pragma unroll
-    for (int s = 0; s < PARTS; s++)
+    for (int s = 0; s < P; s++)
 #pragma unroll
         for (int j = 0; j < 4; j++) part[j][s] = part_at(j, s);
-    if (t.adapter >= 0) join_low(l, t, low);
+    if (t.adapter >= 0) join_low(l, t, scale, low);
     if (n0 >= l.n_out) return;
+    for (int s0 = 0;;) {
 #pragma unroll
-    for (int s = 0; s < PARTS; s++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) y[j] += part[j][s];
-    for (int s0 = PARTS; s0 < l.splits; s0 += PARTS) {
-#pragma unroll
-        for (int s = 0; s < PARTS; s++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) part[j][s] = part_at(j, s0 + s);
-#pragma unroll
-        for (int s = 0; s < PARTS; s++)
+        for (int s = 0; s < P; s++)
 #pragma unroll
             for (int j = 0; j < 4; j++) y[j] += part[j][s];
+        if ((s0 += P) >= l.splits) break;
+#pragma unroll
+        for (int s = 0; s < P; s++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) part[j][s] = part_at(j, s0 + s);
     }
     f32x4 acc[4] = {};
     bool unfit = false;
@@ -629,9 +726,9 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
         for (int c0 = 0; c0 < l.rank / 8; c0 += 4 * U) {
             u32x4 v[U][4];
 #pragma unroll
-            for (int u = 0; u < U; u++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
+                for (int u = 0; u < U; u++) {
                     const int c = c0 + 4 * u + lane / 16, n = min(n0 + j * 16 + lane % 16, l.n_out - 1);
                     v[u][j] = c < l.rank / 8 ? ld16(b + (int64_t)n * l.rank + c * 8) : u32x4{0, 0, 0, 0};
                 }
@@ -643,9 +740,10 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
                     const float *from = low + mine * l.rank + c * 8;
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const float y0 = from[2 * e], y1 = from[2 * e + 1], v0 = round_bf(y0), v1 = round_bf(y1);
-                        value[e] = pack2(y0, y1);
-                        rest[e] = pack2(fabsf(v0) < INFINITY ? y0 - v0 : 0.0f, fabsf(v1) < INFINITY ? y1 - v1 : 0.0f);
+                        uint32_t two, left;
+                        in_two(from[2 * e], from[2 * e + 1], two, left);
+                        value[e] = two;
+                        rest[e] = left;
                     }
                 }
 #pragma unroll
@@ -687,18 +785,20 @@ typedef Shape<224, 256, 112, 64, 16, 2> High;
 typedef Shape<192, 256, 96, 64, 16, 2> Square;
 typedef Shape<128, 256, 64, 64, 16, 3> Half;
 typedef Shape<128, 128, 32, 64, 16, 2> Quarter;
-typedef Shape<64, 128, 64, 32, 16, 3> Low64;
-typedef Shape<64, 64, 64, 16, 16, 4> Small;
-typedef Shape<16, 64, 16, 16, 16, 4> Row;
-constexpr Pace PACES[] = {{256, 192, 1, 930, 1130, 11000}, {224, 256, 1, 1050, 1250, 11000}, {192, 256, 1, 920, 1050, 11000},
-                          {128, 256, 1, 620, 780, 8000},   {128, 128, 2, 560, 760, 6000},    {64, 128, 2, 400, 500, 4500},
-                          {64, 64, 2, 300, 400, 4000},     {16, 64, 3, 250, 350, 3500}};
+typedef Shape<64, 128, 64, 32, 16, 3, true> Few128;
+typedef Shape<64, 64, 64, 16, 16, 4, true> Few64;
+typedef Shape<32, 64, 32, 16, 16, 4, true> Few32;
+typedef Shape<16, 64, 16, 16, 16, 4, true> Few16;
+constexpr Pace PACES[] = {{256, 192, 1, 930, 1130, 11000}, {224, 256, 1, 1050, 1250, 11000}, {192, 256, 1, 960, 1120, 11000},
+                          {128, 256, 1, 620, 760, 8000},   {128, 128, 2, 560, 850, 6000},    {64, 128, 2, 400, 500, 4500},
+                          {64, 64, 2, 300, 460, 4000},     {32, 64, 3, 270, 370, 3700},      {16, 64, 3, 250, 350, 3500}};
 constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 
-constexpr int MOST_SPLITS = 32, MOST_JOINED = 2048;
+constexpr int MOST_SPLITS = 32;
 constexpr size_t MOST_PART = 1 << 23;  // floats
 
-// How a call is computed: the product's tiles, its splits, and whether a join adds them and the adapters' term.
+// How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the
+// product, or join_kernel's.
 struct Plan {
     int shape, splits, split_steps;
     bool join;
@@ -712,26 +812,31 @@ struct Plan {
     Plan(int n_tokens, int n_out, int n_in, bool product, bool adapters, int rank, int n_seqs, int n_adapters) {
         const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
         const int64_t one = (int64_t)part_floats(n_tokens, n_out);
-        const int most = (int)std::min<int64_t>(std::min(MOST_SPLITS, std::max(steps, 1)), MOST_PART / one);
         double least = 0;
         shape = -1;
         for (int i = 0; i < SHAPES; i++) {
             const Pace &s = PACES[i];
             const double tiles = (double)((n_tokens + s.tm - 1) / s.tm) * ((n_out + s.tn - 1) / s.tn);
-            const auto consider = [&](int n, bool joined) {
-                // adapters of a tile's rows, each with steps of its own
-                const double own = !joined && adapters
-                    ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(s.tm, n_tokens) / n_tokens) : 0;
+            // adapters of a tile's rows, each with steps of its own
+            const double own = adapters ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(s.tm, n_tokens) / n_tokens) : 0;
+            for (int n = 1; n <= std::min(MOST_SPLITS, std::max(steps, 1)) && (n == 1 || n * one <= (int64_t)MOST_PART); n++) {
                 const double groups = tiles * n, rounds = ceil(groups / (s.at_once * CUS)), busy = std::min(1.0, groups / CUS);
-                const double step = s.alone + (s.full - s.alone) * busy;
-                const double cost = rounds * (((steps + n - 1) / n + own) * step + s.fixed) +
-                                    (joined ? 5000 + one * (n * 8.0 + 4) / 4500 : adapters ? 5000 : 0);
-                if (shape < 0 || cost < least) shape = i, splits = n, join = joined, least = cost;
-            };
-            consider(1, false);
-            for (int n = adapters || !product ? 1 : 2; n <= most && n_tokens <= MOST_JOINED; n++) consider(n, true);
+                const double step = s.alone + (s.full - s.alone) * busy, each = (steps + n - 1) / n;
+                const double parts = one * (n * 8.0 + 4) / 4500, memory = product ? 2.0 * n_out * n_in / 5500 : 0;
+                const double cost = std::max(rounds * (each + own) * step, memory) + rounds * s.fixed +
+                                    (n > 1 ? 5000 + parts : 0) + (adapters ? 11000 : 0);
+                if (shape < 0 || cost < least) shape = i, splits = n, join = false, least = cost;
+                if (!adapters || s.tm > 64 || n * one > (int64_t)MOST_PART) continue;
+                // parts that the join has under way at once
+                const int at_once = n_tokens <= n_seqs ? 8 : 4;
+                const double joined = std::max(rounds * each * step, memory) + rounds * s.fixed + parts + 5000 +
+                                      1200 * ceil((double)n / at_once);
+                if (joined < least) shape = i, splits = n, join = true, least = joined;
+            }
         }
-        split_steps = (steps + splits - 1) / splits;
+        // the last split has the adapters' steps
+        const double own = adapters && !join ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(PACES[shape].tm, n_tokens) / n_tokens) : 0;
+        split_steps = std::min(steps, (int)((steps + own + splits - 1) / splits));
         splits = split_steps ? (steps + split_steps - 1) / split_steps : join ? 0 : 1;
     }
 };
@@ -740,10 +845,10 @@ template <class G>
 bool launch_product(const char *name, LoraArgs l, hipStream_t stream) {
     l.m_tiles = (l.n_tokens + G::TM - 1) / G::TM;
     l.n_tiles = (l.n_out + G::TN - 1) / G::TN;
-    const int64_t groups = l.low_groups + (int64_t)l.m_tiles * l.n_tiles * l.splits;
+    const int64_t groups = (int64_t)l.m_tiles * l.n_tiles * l.splits + l.low_groups;
     if (groups * G::T >= 1ll << 32)  // the threads of a launch
         return llm_fail("%s: n_tokens %d by n_out %d is too much for one launch", name, l.n_tokens, l.n_out);
-    if (groups) product_kernel<G><<<groups, G::T, 0, stream>>>(l);
+    product_kernel<G><<<groups, G::T, 0, stream>>>(l);
     return LAUNCH_OK();
 }
 
@@ -758,11 +863,9 @@ bool check_sizes(const char *name, int n_tokens, int n_out, int n_in, int rank) 
     return true;
 }
 
+// low and its parts, of which there are the most without a join.
 int low_splits(int n_in) { return (n_in + LOW_SPAN - 1) / LOW_SPAN; }
-// Of low: as two bf16, or of its parts, which a join of at most MOST_JOINED rows adds.
-size_t low_floats(int n_tokens, int n_in, int rank) {
-    return (size_t)rank * std::max(n_tokens, std::min(n_tokens, MOST_JOINED) * low_splits(n_in));
-}
+size_t low_floats(int n_tokens, int n_in, int rank) { return (size_t)n_tokens * rank * (1 + low_splits(n_in)); }
 size_t owner_floats(int n_tokens, int rank) { return rank ? ((size_t)n_tokens + 3) / 4 * 4 : 0; }
 
 }  // namespace
@@ -828,43 +931,43 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     l.wide = out_stride % 4 == 0 && (uintptr_t)out % 8 == 0 &&
              (!residual || (residual_stride % 4 == 0 && (uintptr_t)residual % 8 == 0));
     l.low = (bf16 *)ws;
-    l.low_part = ws;
-    l.low_splits = low_splits(n_in);
+    l.low_part = ws + (size_t)n_tokens * rank;
+    l.low_splits = p.join ? (n_in + JOIN_LOW_SPAN - 1) / JOIN_LOW_SPAN : low_splits(n_in);
     l.owner = (int *)(ws + low_floats(n_tokens, n_in, rank));
-    float *part = ws + low_floats(n_tokens, n_in, rank) + owner_floats(n_tokens, rank);
-    int tiles = (n_tokens + 15) / 16;
+    if (p.splits > 1 || p.join) l.part = ws + low_floats(n_tokens, n_in, rank) + owner_floats(n_tokens, rank);
+    int tiles = 0;
     if (lora) {
         l.a = lora->a, l.b = lora->b, l.scale = lora->scale, l.q_start = lora->q_start, l.adapter = lora->adapter;
         l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = rank;
-        tiles = n_tokens / 16 + lora->n_seqs;
-    }
-    const auto product = [&](const LoraArgs &a) {
-        switch (p.shape) {
-        case 0: return launch_product<Wide>(name, a, stream);
-        case 1: return launch_product<High>(name, a, stream);
-        case 2: return launch_product<Square>(name, a, stream);
-        case 3: return launch_product<Half>(name, a, stream);
-        case 4: return launch_product<Quarter>(name, a, stream);
-        case 5: return launch_product<Low64>(name, a, stream);
-        case 6: return launch_product<Small>(name, a, stream);
-        default: return launch_product<Row>(name, a, stream);
+        tiles = n_tokens / (p.join ? 16 : LOW_ROWS) + lora->n_seqs;
+        const int64_t groups = (int64_t)tiles * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
+        if (groups >= 1 << 23) {  // the threads of a launch
+            llm_fail("%s: %d sequences of rank %d over n_in %d are too many for one launch", name, lora->n_seqs, rank, n_in);
+            return;
         }
-    };
-    if (p.join) {
-        l.part = part;
-        if (lora) l.low_groups = tiles * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
-        if (!product(l)) return;
-        join_kernel<<<dim3(tiles, (n_out + 255) / 256), 256, 0, stream>>>(l);
-        LAUNCH_OK();
-        return;
+        if (p.join) {
+            l.low_groups = (int)groups;
+        } else {
+            low_kernel<<<groups, 64 * LOW_WAVES, 0, stream>>>(l);
+            if (!LAUNCH_OK()) return;
+            low_sum_kernel<<<((int64_t)n_tokens * (rank / 4) + 255) / 256, 256, 0, stream>>>(l);
+            if (!LAUNCH_OK()) return;
+        }
     }
-    if (lora) {
-        const int width = low_width(rank);
-        const dim3 grid(tiles, (rank + width - 1) / width);
-        if (width == 16) low_kernel<1><<<grid, 64 * LOW_WAVES, 0, stream>>>(l);
-        else if (width == 32) low_kernel<2><<<grid, 64 * LOW_WAVES, 0, stream>>>(l);
-        else low_kernel<4><<<grid, 64 * LOW_WAVES, 0, stream>>>(l);
-        if (!LAUNCH_OK()) return;
+    bool ok = false;
+    switch (p.shape) {
+    case 0: ok = launch_product<Wide>(name, l, stream); break;
+    case 1: ok = launch_product<High>(name, l, stream); break;
+    case 2: ok = launch_product<Square>(name, l, stream); break;
+    case 3: ok = launch_product<Half>(name, l, stream); break;
+    case 4: ok = launch_product<Quarter>(name, l, stream); break;
+    case 5: ok = launch_product<Few128>(name, l, stream); break;
+    case 6: ok = launch_product<Few64>(name, l, stream); break;
+    case 7: ok = launch_product<Few32>(name, l, stream); break;
+    default: ok = launch_product<Few16>(name, l, stream);
     }
-    product(l);
+    if (!ok) return;
+    if (p.join) join_kernel<<<dim3(tiles, (n_out + 255) / 256), 256, 0, stream>>>(l);
+    else if (p.splits > 1) sum_kernel<<<((int64_t)n_tokens * (l.part_width / 4) + 255) / 256, 256, 0, stream>>>(l);
+    LAUNCH_OK();
 }
