@@ -310,16 +310,17 @@ __device__ __forceinline__ float unfit_term(const LoraArgs &l, int n, int adapte
 // TM rows by TN columns of a workgroup, in waves of RM by RN, on MFMAs of side S; 64 elements of the sum a step,
 // STAGES steps' operands in LDS. A row's 128 bytes of a step lie as eight 16-byte chunks, chunk c of row r at
 // c ^ (r % 8): the rows that a product reads at one chunk then lie in different banks.
-template <int TM_, int TN_, int RM_, int RN_, int S_, int STAGES_, bool STREAM_ = false>
+template <int TM_, int TN_, int RM_, int RN_, int BK_, int STAGES_, bool STREAM_ = false>
 struct Shape {
     static constexpr bool STREAM = STREAM_;                          // W is read once, past the caches
-    static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, S = S_, STAGES = STAGES_;
+    static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, BK = BK_, S = 16, STAGES = STAGES_;
     static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / S, NT = RN / S;
     static constexpr bool JOINS = TM <= 64;                          // also in front of join_kernel
-    static constexpr int BYTES = (TM + TN) * 128;                    // of a stage
+    static constexpr int CHUNKS = BK / 8, ROW = 2 * BK, PER = 64 / CHUNKS;  // of a row: chunks, bytes; rows of a load
+    static constexpr int BYTES = (TM + TN) * ROW;                    // of a stage
     static_assert(!JOINS || STAGES * BYTES >= WAVES * 16 * 68 * 4, "low_part's sums");
-    static constexpr int X_LOADS = (TM / 8 + WAVES - 1) / WAVES;     // per wave, of eight rows; the last ones may be
-    static constexpr int W_LOADS = (TN / 8 + WAVES - 1) / WAVES;     // loaded more than once
+    static constexpr int X_LOADS = (TM / PER + WAVES - 1) / WAVES;   // per wave, of PER rows; the last ones may be
+    static constexpr int W_LOADS = (TN / PER + WAVES - 1) / WAVES;   // loaded more than once
     static constexpr int LOADS = X_LOADS + W_LOADS;
 };
 
@@ -341,27 +342,27 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
         owner[threadIdx.x] = m0 + (int)threadIdx.x < l.n_tokens ? gptr(l.owner)[m0 + threadIdx.x] : NO_SEQUENCE;
     if (threadIdx.x == 0) *unfit = *count = 0;
 
-    // loads: lane's row lane / 8 and chunk lane % 8 of eight rows
+    // loads: lane's row and chunk of PER rows
     const unsigned base = (unsigned)(uintptr_t)(lds_char *)lds;
-    const int row = lane / 8, chunk = lane % 8 ^ row;
+    const int row = lane / G::CHUNKS;
     unsigned x_at[G::X_LOADS], w_at[G::W_LOADS];   // bytes from the tile's first row
-    int x_row[G::X_LOADS];
-    const auto x_group = [&](int i) { return min(wave * G::X_LOADS + i, G::TM / 8 - 1); };
-    const auto w_group = [&](int i) { return min(wave * G::W_LOADS + i, G::TN / 8 - 1); };
+    const auto x_group = [&](int i) { return min(wave * G::X_LOADS + i, G::TM / G::PER - 1); };
+    const auto w_group = [&](int i) { return min(wave * G::W_LOADS + i, G::TN / G::PER - 1); };
+    const auto x_row = [&](int i) { return x_group(i) * G::PER + row; };
+    const auto w_row = [&](int i) { return w_group(i) * G::PER + row; };
+    const auto chunk_of = [&](int r) { return (lane % G::CHUNKS) ^ (r & (G::CHUNKS - 1)); };
 #pragma unroll
-    for (int i = 0; i < G::X_LOADS; i++) {
-        x_row[i] = x_group(i) * 8 + row;
-        x_at[i] = (unsigned)(min(x_row[i], l.n_tokens - 1 - m0) * l.x_stride * 2) + chunk * 16;
-    }
+    for (int i = 0; i < G::X_LOADS; i++)
+        x_at[i] = (unsigned)(min(x_row(i), l.n_tokens - 1 - m0) * l.x_stride * 2) + chunk_of(x_row(i)) * 16;
 #pragma unroll
     for (int i = 0; i < G::W_LOADS; i++)
-        w_at[i] = (unsigned)min(w_group(i) * 8 + row, l.n_out - 1 - n0) * (unsigned)l.n_in * 2 + chunk * 16;
+        w_at[i] = (unsigned)min(w_row(i), l.n_out - 1 - n0) * (unsigned)l.n_in * 2 + chunk_of(w_row(i)) * 16;
     const char *x_from = (const char *)(l.x + m0 * l.x_stride), *w_from = (const char *)(l.w + (int64_t)n0 * l.n_in);
-    const int all_steps = l.w ? (l.n_in + 63) / 64 : 0, whole_steps = l.w ? l.n_in / 64 : 0;
+    const int all_steps = l.w ? (l.n_in + G::BK - 1) / G::BK : 0, whole_steps = l.w ? l.n_in / G::BK : 0;
     const int last_step = min(all_steps, (split + 1) * l.split_steps);
     int step = split * l.split_steps, next = 0, piece = 0;  // what is requested next: the product's, then adapters'
     unsigned of_adapter = 0;                                // stages that hold some of these
-    const int pieces = (2 * l.rank + 63) / 64;
+    const int pieces = (2 * l.rank + G::BK - 1) / G::BK;
     __syncthreads();
     if (adapters && wave == 0) {  // the adapters of the tile's rows, each once: entry 64 q + lane in entry[q]
         constexpr int Q = (G::TM + 63) / 64;
@@ -396,13 +397,13 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     // Load i of a step of whole chunks into stage `to`.
     const auto load_whole = [&](int i, int to) {
         const unsigned xs = base + to * G::BYTES;
-        if (i < G::X_LOADS) load_to_lds(xs + x_group(i) * 1024, x_from + (int64_t)step * 128, x_at[i]);
-        else load_to_lds<G::STREAM>(xs + G::TM * 128 + w_group(i - G::X_LOADS) * 1024, w_from + (int64_t)step * 128, w_at[i - G::X_LOADS]);
+        if (i < G::X_LOADS) load_to_lds(xs + x_group(i) * 1024, x_from + (int64_t)step * G::ROW, x_at[i]);
+        else load_to_lds<G::STREAM>(xs + G::TM * G::ROW + w_group(i - G::X_LOADS) * 1024, w_from + (int64_t)step * G::ROW, w_at[i - G::X_LOADS]);
     };
     // Requests the next step's operands into stage `to`; false after the last.
     const int whole_end = min(whole_steps, last_step);
     const auto request = [&](int to) {
-        const unsigned xs = base + to * G::BYTES, ws = xs + G::TM * 128;
+        const unsigned xs = base + to * G::BYTES, ws = xs + G::TM * G::ROW;
         if (step < whole_end) {
 #pragma unroll
             for (int i = 0; i < G::LOADS; i++) load_whole(i, to);
@@ -410,47 +411,51 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
             return true;
         }
         if (step < last_step) {  // the last step of a width that is no multiple of 64
-            const char *x = x_from + (int64_t)step * 128, *w = w_from + (int64_t)step * 128;
-            const bool there = step * 64 + chunk * 8 < l.n_in;
+            const char *x = x_from + (int64_t)step * G::ROW, *w = w_from + (int64_t)step * G::ROW;
+            const auto there = [&](int r) { return step * G::BK + chunk_of(r) * 8 < l.n_in; };
 #pragma unroll
             for (int i = 0; i < G::X_LOADS; i++)
-                load_to_lds(xs + x_group(i) * 1024, there ? x + x_at[i] : (const char *)&g_zeros);
+                load_to_lds(xs + x_group(i) * 1024, there(x_row(i)) ? x + x_at[i] : (const char *)&g_zeros);
 #pragma unroll
             for (int i = 0; i < G::W_LOADS; i++)
-                load_to_lds(ws + w_group(i) * 1024, there ? w + w_at[i] : (const char *)&g_zeros);
+                load_to_lds(ws + w_group(i) * 1024, there(w_row(i)) ? w + w_at[i] : (const char *)&g_zeros);
             step++;
             return true;
         }
         if (next == listed) return false;
         const int current = __builtin_amdgcn_readfirstlane(list[next]);
-        const int c = piece * 8 + chunk, chunks = l.rank / 8;
-        const char *low = (const char *)(l.low + (int64_t)m0 * 2 * l.rank) + c * 16;
-        const char *b = (const char *)(l.b + ((int64_t)current * l.n_out + n0) * l.rank) + (c >= chunks ? c - chunks : c) * 16;
-        const bool there = c < 2 * chunks;
+        const int chunks = l.rank / 8;
+        const char *low = (const char *)(l.low + (int64_t)m0 * 2 * l.rank);
+        const char *b = (const char *)(l.b + ((int64_t)current * l.n_out + n0) * l.rank);
 #pragma unroll
-        for (int i = 0; i < G::X_LOADS; i++)
-            load_to_lds(xs + x_group(i) * 1024, there && owner[x_row[i]] == current ? low + (int64_t)x_row[i] * 4 * l.rank
-                                                                                  : (const char *)&g_zeros);
+        for (int i = 0; i < G::X_LOADS; i++) {
+            const int r = x_row(i), c = piece * G::CHUNKS + chunk_of(r);
+            load_to_lds(xs + x_group(i) * 1024, c < 2 * chunks && owner[r] == current ? low + ((int64_t)r * 2 * chunks + c) * 16
+                                                                                     : (const char *)&g_zeros);
+        }
 #pragma unroll
-        for (int i = 0; i < G::W_LOADS; i++)
+        for (int i = 0; i < G::W_LOADS; i++) {
+            const int r = w_row(i), c = piece * G::CHUNKS + chunk_of(r);
             load_to_lds(ws + w_group(i) * 1024,
-                        there ? b + (int64_t)min(w_group(i) * 8 + row, l.n_out - 1 - n0) * 2 * l.rank : (const char *)&g_zeros);
+                        c < 2 * chunks ? b + ((int64_t)min(r, l.n_out - 1 - n0) * chunks + (c >= chunks ? c - chunks : c)) * 16
+                                       : (const char *)&g_zeros);
+        }
         if (++piece == pieces) piece = 0, next++;
         of_adapter |= 1u << to;
         return true;
     };
     typename Mfma<G::S>::Acc acc[G::MT][G::NT];
     const int mine_m = wave % G::WM * G::RM, mine_n = wave / G::WM * G::RN;
-    constexpr int KS = 64 / Mfma<G::S>::K;  // products of a step, on operands in alternating registers
+    constexpr int KS = G::BK / Mfma<G::S>::K;  // products of a step, on operands in alternating registers
     static_assert(KS % 2 == 0, "registers alternate");
     u32x4 xf[2][G::MT], wf[2][G::NT];
     const auto fetch = [&](int from, int k) {
-        const char *xs = lds + from * G::BYTES, *ws = xs + G::TM * 128;
-        const int r = lane % G::S, slot = (k * (64 / G::S) + lane / G::S) ^ (r & 7);
+        const char *xs = lds + from * G::BYTES, *ws = xs + G::TM * G::ROW;
+        const int r = lane % G::S, slot = (k * (64 / G::S) + lane / G::S) ^ (r & (G::CHUNKS - 1));
 #pragma unroll
-        for (int i = 0; i < G::MT; i++) xf[k % 2][i] = *(const u32x4 *)(xs + (mine_m + i * G::S + r) * 128 + slot * 16);
+        for (int i = 0; i < G::MT; i++) xf[k % 2][i] = *(const u32x4 *)(xs + (mine_m + i * G::S + r) * G::ROW + slot * 16);
 #pragma unroll
-        for (int j = 0; j < G::NT; j++) wf[k % 2][j] = *(const u32x4 *)(ws + (mine_n + j * G::S + r) * 128 + slot * 16);
+        for (int j = 0; j < G::NT; j++) wf[k % 2][j] = *(const u32x4 *)(ws + (mine_n + j * G::S + r) * G::ROW + slot * 16);
     };
     const auto multiply = [&](int k) {
 #pragma unroll
@@ -465,8 +470,8 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     bool clear = false;
     const auto begin = [&](int from) {
         if (of_adapter >> from & 1 && clear) {
-            for (int c = threadIdx.x; c < G::TN * 8; c += G::T) {
-                u32x4 *at = (u32x4 *)(lds + from * G::BYTES + G::TM * 128 + c * 16), v = *at;
+            for (int c = threadIdx.x; c < G::TN * G::CHUNKS; c += G::T) {
+                u32x4 *at = (u32x4 *)(lds + from * G::BYTES + G::TM * G::ROW + c * 16), v = *at;
                 if (clear_unfit_of(v)) *at = v;
             }
             wait_lds();
@@ -780,15 +785,15 @@ struct Pace {
     int tm, tn, at_once;
     double alone, full, fixed;
 };
-typedef Shape<256, 192, 64, 96, 16, 2> Wide;
-typedef Shape<224, 256, 112, 64, 16, 2> High;
-typedef Shape<192, 256, 96, 64, 16, 2> Square;
-typedef Shape<128, 256, 64, 64, 16, 3> Half;
-typedef Shape<128, 128, 32, 64, 16, 2> Quarter;
-typedef Shape<64, 128, 64, 32, 16, 3, true> Few128;
-typedef Shape<64, 64, 64, 16, 16, 4, true> Few64;
-typedef Shape<32, 64, 32, 16, 16, 4, true> Few32;
-typedef Shape<16, 64, 16, 16, 16, 4, true> Few16;
+typedef Shape<256, 192, 64, 96, 64, 2> Wide;
+typedef Shape<224, 256, 112, 64, 64, 2> High;
+typedef Shape<192, 256, 96, 64, 64, 2> Square;
+typedef Shape<128, 256, 64, 64, 64, 3> Half;
+typedef Shape<128, 128, 32, 64, 64, 2> Quarter;
+typedef Shape<64, 128, 64, 32, 64, 3, true> Few128;
+typedef Shape<64, 64, 64, 16, 64, 4, true> Few64;
+typedef Shape<32, 64, 32, 16, 64, 4, true> Few32;
+typedef Shape<16, 64, 16, 16, 64, 4, true> Few16;
 constexpr Pace PACES[] = {{256, 192, 1, 930, 1130, 11000}, {224, 256, 1, 1050, 1250, 11000}, {192, 256, 1, 960, 1120, 11000},
                           {128, 256, 1, 620, 760, 8000},   {128, 128, 2, 560, 850, 6000},    {64, 128, 2, 400, 500, 4500},
                           {64, 64, 2, 300, 460, 4000},     {32, 64, 3, 270, 370, 3700},      {16, 64, 3, 250, 350, 3500}};
