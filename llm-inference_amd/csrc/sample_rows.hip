@@ -7,6 +7,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "llm_amd/batch.h"
@@ -43,13 +44,15 @@ __device__ __forceinline__ int place_of(uint32_t b) {
 __device__ __forceinline__ uint32_t bits_at(int place) { return place & 0x8000 ? place : 0x7fff - place; }
 
 struct Row {
-    uint32_t counts[BINS / 2];   // n0 + 2^16 n1 of two values, modulo 2^32
+    alignas(16) uint32_t counts[BINS / 2];  // n0 + 2^16 n1 of two values, modulo 2^32
     double mass[CHUNKS + 1];     // in front of each chunk of values
     int tokens[CHUNKS + 1];
     int carries;                 // how often a sum passed what it is held in:
     uint32_t carry[MOST_CARRIES];  // 2 w: n0 of word w passed a multiple of 2^16, 2 w + 1: the word one of 2^32
-    int found[WAVES];
+    int found[WAVES], sums[WAVES];
     int entries;
+    int place, nth;              // of the token drawn: its value, and how many of that are in front of it
+    double ratio;               // of its weight to the sum of what is left
 };
 
 __device__ __forceinline__ void clear(Row &row) {
@@ -85,157 +88,182 @@ __device__ __forceinline__ void counts_of(const Row &row, int carries, uint32_t 
     second = (int)((whole - first) >> 16);
 }
 
-// f(index, bits) for the logits from `first` to `last`, eight per thread at a time from aligned addresses on, four
-// times under way.
-template <class F>
-__device__ __forceinline__ void each_logit(const bf16 *x, int first, int last, F f) {
-    constexpr int U = 4;
-    const int head = min(last, first + (int)((16 - ((uintptr_t)(x + first) & 15)) / 2 & 7));
-    const int body = head + (last - head) / 8 * 8;
-    for (int i0 = head + 8 * (int)threadIdx.x; i0 < body; i0 += U * 8 * T) {
-        u32x4 v[U];
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (i0 + u * 8 * T < body) v[u] = ld16(x + i0 + u * 8 * T);
-#pragma unroll
-        for (int u = 0; u < U; u++)
-            if (i0 + u * 8 * T < body) {
-#pragma unroll
-                for (int e = 0; e < 8; e++) f(i0 + u * 8 * T + e, v[u][e / 2] >> (e % 2 * 16) & 0xffff);
-            }
+// The logits from `first` to `last`, eight per thread at a time from aligned addresses on, the next two under way: the
+// first ones are requested when this is made, in front of what else there is to do.
+struct Logits {
+    const bf16 *x;
+    int first, last, head, body, i;
+    u32x4 v, next;
+    __device__ __forceinline__ u32x4 request(int at) const { return at < body ? ld16(x + at) : u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ Logits(const bf16 *x_, int first_, int last_) : x(x_), first(first_), last(last_) {
+        head = min(last, first + (int)((16 - ((uintptr_t)(x + first) & 15)) / 2 & 7));
+        body = head + (last - head) / 8 * 8;
+        i = head + 8 * (int)threadIdx.x;
+        v = request(i);
+        next = request(i + 8 * T);
     }
-    if (first + (int)threadIdx.x < head) f(first + threadIdx.x, (uint32_t)gptr(x)[first + threadIdx.x]);
-    if (body + (int)threadIdx.x < last) f(body + threadIdx.x, (uint32_t)gptr(x)[body + threadIdx.x]);
-}
+    // f(bits) for each.
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+#pragma unroll 1
+        for (; i < body; i += 8 * T) {
+            const u32x4 now = v;
+            v = next;
+            next = request(i + 2 * 8 * T);
+#pragma unroll
+            for (int e = 0; e < 8; e++) f(now[e / 2] >> (e % 2 * 16) & 0xffff);
+        }
+        // what is in front of the first aligned address, and behind the last one
+        const int rest = (int)threadIdx.x < head - first ? first + threadIdx.x : body + (threadIdx.x - (head - first));
+        if (rest < last && (rest < head || rest >= body)) f((uint32_t)gptr(x)[rest]);
+    }
+};
 
-template <int S>
-__device__ __forceinline__ double xor_lane(double v) {
-    return __hiloint2double(llm::xor_lane<S>(__double2hiint(v)), llm::xor_lane<S>(__double2loint(v)));
-}
-__device__ __forceinline__ double sum_lanes(double v) {
-    v += xor_lane<1>(v), v += xor_lane<2>(v), v += xor_lane<4>(v), v += xor_lane<8>(v), v += xor_lane<16>(v);
-    return v + xor_lane<32>(v);
-}
 __device__ __forceinline__ int sum_lanes(int v) {
     v += llm::xor_lane<1>(v), v += llm::xor_lane<2>(v), v += llm::xor_lane<4>(v), v += llm::xor_lane<8>(v), v += llm::xor_lane<16>(v);
     return v + llm::xor_lane<32>(v);
 }
-// Sums of the lanes in front of this one.
-__device__ __forceinline__ void sum_before(double &v, int &n) {
+__device__ __forceinline__ int least_lane(int v) {
+    v = min(v, llm::xor_lane<1>(v)), v = min(v, llm::xor_lane<2>(v)), v = min(v, llm::xor_lane<4>(v));
+    v = min(v, llm::xor_lane<8>(v)), v = min(v, llm::xor_lane<16>(v));
+    return min(v, llm::xor_lane<32>(v));
+}
+
+// Sums of the lanes up to this one: within rows of 16 lanes of those 1, 2, 4 and 8 in front (DPP row_shr, 0 past the
+// row's first), then the last one of the row in front (row_bcast15, into rows 1 and 3), then that of the first half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int moved(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, true);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+    return __hiloint2double(moved<CTRL, ROWS>(__double2hiint(v)), moved<CTRL, ROWS>(__double2loint(v)));
+}
+template <class V>
+__device__ __forceinline__ V sum_upto(V v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);
+    return v + moved<0x143, 0xc>(v);
+}
+// Of the lane in front (wave_shr:1), 0 for the first.
+__device__ __forceinline__ int in_front(int v) { return __builtin_amdgcn_update_dpp(0, v, 0x138, 0xf, 0xf, true); }
+__device__ __forceinline__ double in_front(double v) {
+    return __hiloint2double(in_front(__double2hiint(v)), in_front(__double2loint(v)));
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ double lane_value(double v, int lane) {
+    return __hiloint2double(lane_value(__double2hiint(v), lane), lane_value(__double2loint(v), lane));
+}
+
+// The smallest of the threads' places and the sum of their counts, in every thread (behind a barrier, with what is in
+// LDS before it).
+__device__ __forceinline__ void gather(Row &row, int &least, int &n) {
+    least = least_lane(least);
+    n = sum_lanes(n);
+    if ((threadIdx.x & 63) == 0) row.found[wave_id()] = least, row.sums[wave_id()] = n;
+    __syncthreads();
     const int lane = threadIdx.x & 63;
-    const int tokens = n;
+    least = __builtin_amdgcn_readfirstlane(least_lane(row.found[lane % WAVES]));
+    n = __builtin_amdgcn_readfirstlane(sum_lanes(lane < WAVES ? row.sums[lane] : 0));
+}
+
+// In front of each chunk, from each chunk's own: the first wave, eight chunks per lane.
+template <class V>
+__device__ __forceinline__ void sum_chunks(V *chunks) {
+    constexpr int EIGHT = CHUNKS / 64;
+    const int lane = threadIdx.x & 63;
+    V sum = 0, own[EIGHT];
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double a = __shfl_up(v, d);
-        const int b = __shfl_up(n, d);
-        if (lane >= d) v += a, n += b;
+    for (int i = 0; i < EIGHT; i++) sum += own[i] = chunks[lane * EIGHT + i];
+    sum = in_front(sum_upto(sum));
+#pragma unroll
+    for (int i = 0; i < EIGHT; i++) {
+        chunks[lane * EIGHT + i] = sum;
+        sum += own[i];
     }
-    v = __shfl_up(v, 1);  // not less its own, which would round
-    if (lane == 0) v = 0.0;
-    n -= tokens;
+    if (lane == 63) chunks[CHUNKS] = sum;
 }
 
-// The draw from a row's counts, by every wave alike.
-struct Draw {
-    const Row &row;
-    int carries;
-    double top, by;  // the largest value, 1 / temperature
-
-    __device__ __forceinline__ double weight(int place) const {
-        const double x = (double)__uint_as_float(bits_at(place) << 16);
-        // beside +inf nothing else weighs
-        return x == top ? 1.0 : top > 3.5e38 ? 0.0 : exp((x - top) * by);
+// A wave looks at the counts four chunks at a time, a lane having four words (eight values) of one of them: group i of
+// the wave's are the chunks from 4 (i WAVES + wave) on. Those that are not empty, as a mask.
+constexpr int GROUPS = CHUNKS / 4 / WAVES;
+__device__ __forceinline__ int word_of(int i) { return ((i * WAVES + wave_id()) * 64 + (threadIdx.x & 63)) * 4; }
+__device__ __forceinline__ uint32_t groups_with_some(const Row &row) {
+    uint32_t some = 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS; i++) {
+        const u32x4 v = *(const u32x4 *)(row.counts + word_of(i));
+        if (__any((v[0] | v[1] | v[2] | v[3]) != 0)) some |= 1u << i;
     }
-
-    // A chunk's values, two per lane, with mass and tokens in front of them.
-    struct Lane {
-        double w0, w1, before;
-        int n0, n1, tokens;
-    };
-    __device__ __forceinline__ Lane lane_of(int chunk) const {
-        Lane l;
-        const int word = chunk * 64 + (threadIdx.x & 63);
-        counts_of(row, carries, word, row.counts[word], l.n0, l.n1);
-        l.w0 = l.n0 ? weight(2 * word) : 0.0;
-        l.w1 = l.n1 ? weight(2 * word + 1) : 0.0;
-        l.before = l.n0 * l.w0 + l.n1 * l.w1;
-        l.tokens = l.n0 + l.n1;
-        sum_before(l.before, l.tokens);
-        l.before += row.mass[chunk];
-        l.tokens += row.tokens[chunk];
-        return l;
-    }
-
-    // The last chunk whose front passes `fits` (which the fronts stop doing, and the first does).
-    template <class V, class Fits>
-    __device__ __forceinline__ int chunk_at(const V *front, Fits fits) const {
-        const int lane = threadIdx.x & 63, group = max(0, __popcll(__ballot(fits(front[lane * 8]))) - 1);
-        return group * 8 + max(0, __popcll(__ballot(lane < 8 && fits(front[group * 8 + (lane & 7)]))) - 1);
-    }
-
-    // A place in the order of the tokens: so many in front of it and their mass; the value of the token there, how
-    // many of that value are in front of it, and its weight.
-    struct Spot {
-        int tokens, place, nth;
-        double mass, weight;
-    };
-    // Of this lane's two values, k0 and k1 tokens are in front of the spot: the lane where that stops.
-    __device__ __forceinline__ Spot spot(int chunk, const Lane &l, int k0, int k1) const {
-        const uint64_t stops = __ballot(k0 + k1 < l.n0 + l.n1);
-        const int at = stops ? __builtin_ctzll(stops) : 63, lane = threadIdx.x & 63;
-        const bool second = k0 == l.n0;
-        Spot s = {l.tokens + k0 + k1, 2 * (chunk * 64 + lane) + (second ? 1 : 0), second ? k1 : k0,
-                  l.before + (k0 * l.w0 + k1 * l.w1), second ? l.w1 : l.w0};
-        s.tokens = __shfl(s.tokens, at);
-        s.place = __shfl(s.place, at);
-        s.nth = __shfl(s.nth, at);
-        s.mass = __shfl(s.mass, at);
-        s.weight = __shfl(s.weight, at);
-        return s;
-    }
-    // The spot behind n tokens.
-    __device__ __forceinline__ Spot behind(int n) const {
-        const int chunk = chunk_at(row.tokens, [&](int t) { return t <= n; });
-        const Lane l = lane_of(chunk);
-        const int k0 = max(0, min(l.n0, n - l.tokens));
-        return spot(chunk, l, k0, max(0, min(l.n1, n - l.tokens - l.n0)));
-    }
-    // The spot behind the last token up to which the mass is less than `at` (EQUAL: not more).
-    template <bool EQUAL>
-    __device__ __forceinline__ Spot within(double at) const {
-        const auto fits = [&](double m) { return EQUAL ? m <= at : m < at; };
-        const int chunk = chunk_at(row.mass, fits);
-        const Lane l = lane_of(chunk);
-        // how many of n tokens of weight w fit behind m
-        const auto part = [&](double m, double w, int n) {
-            if (n == 0 || !fits(m)) return 0;
-            int k = w > 0 ? (int)fmin(fmax((at - m) / w, 0.0), (double)n) : n;
-            if (k > 0 && !fits(m + k * w)) k--;
-            if (k < n && fits(m + (k + 1) * w)) k++;
-            return k;
-        };
-        const int k0 = part(l.before, l.w0, l.n0), k1 = k0 < l.n0 ? 0 : part(l.before + l.n0 * l.w0, l.w1, l.n1);
-        // all of the chunk, where its sum falls short of the next one's front by a rounding, or it is empty
-        if (!__any(k0 + k1 < l.n0 + l.n1)) return behind(row.tokens[chunk + 1]);
-        return spot(chunk, l, k0, k1);
-    }
-};
-
-// The smallest of the threads' places, in every thread (two barriers, with what is in LDS before them).
-__device__ __forceinline__ int least_of(Row &row, int least) {
-    for (int d = 1; d < 64; d *= 2) least = min(least, __shfl_xor(least, d));
-    if ((threadIdx.x & 63) == 0) row.found[wave_id()] = least;
-    __syncthreads();
-    least = row.found[threadIdx.x % WAVES];
-    for (int d = 1; d < WAVES; d *= 2) least = min(least, __shfl_xor(least, d));
-    __syncthreads();
-    return __builtin_amdgcn_readfirstlane(least);
+    return some;
+}
+// The sum over a lane's row of 16, in its last lane.
+template <class V>
+__device__ __forceinline__ V sum_of_row(V v) {
+    v += moved<0x111, 0xf>(v);
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    return v + moved<0x118, 0xf>(v);
 }
 
-// Row r's token from its counts. least: the place of the largest value (BINS: none). where(place, nth, first, last)
-// says among which tokens the nth of that value is, and leaves in nth how many of it are in front of it there.
+// The tokens in front of every chunk, and the groups of this wave that are not empty.
+__device__ __forceinline__ uint32_t sum_tokens(Row &row, int carries) {
+    const int lane = threadIdx.x & 63;
+    if (threadIdx.x < CHUNKS) row.tokens[threadIdx.x] = 0, row.mass[threadIdx.x] = 0.0;
+    const uint32_t some = carries ? (1u << GROUPS) - 1 : groups_with_some(row);
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t rest = some; rest; rest &= rest - 1) {
+        const int word = word_of(__builtin_ctz(rest));
+        const u32x4 v = *(const u32x4 *)(row.counts + word);
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            int n0, n1;
+            counts_of(row, carries, word + j, v[j], n0, n1);
+            n += n0 + n1;
+        }
+        n = sum_of_row(n);
+        if (lane % 16 == 15) row.tokens[word / 64] = n;
+    }
+    __syncthreads();
+    if (wave_id() == 0) sum_chunks(row.tokens);
+    __syncthreads();
+    return some;
+}
+
+// e^x for x <= 0: k = rint(x log2 e), r = x - k ln 2 with ln 2 in two parts, the series of e^r to r^13 (|r| <= 0.347:
+// the next term is below 2^-58), times 2^k.
+__device__ __forceinline__ double exp_d(double x) {
+    x = fmax(x, -1100.0);
+    const double k = rint(x * 0x1.71547652b82fep+0);
+    double r = fma(-k, 0x1.62e42fefa39efp-1, x);
+    r = fma(-k, 0x1.abc9e3b39803fp-56, r);
+    double p = 1.0 / 6227020800.0;
+    p = fma(p, r, 1.0 / 479001600.0);
+    p = fma(p, r, 1.0 / 39916800.0);
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return __builtin_ldexp(p, (int)k);
+}
+
+// Row r's token from its counts. least: the place of the largest value (BINS: none); some: of sum_tokens.
+// where(place, nth, first, last) says among which tokens the nth of that value is, and leaves in nth how many of it
+// are in front of it there.
 template <class Where>
-__device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int least, Where where) {
+__device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int least, uint32_t some, Where where) {
     const int lane = threadIdx.x & 63, wave = wave_id();
     if (least == BINS) {
         if (threadIdx.x == 0) {
@@ -248,250 +276,370 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int l
     const int top_k = a.top_k ? gptr(a.top_k)[r] : 0;
     const float top_p = a.top_p ? gptr(a.top_p)[r] : 1.0f, min_p = a.min_p ? gptr(a.min_p)[r] : 0.0f, u = gptr(a.u)[r];
     const int carries = row.carries;
-    const Draw d = {row, carries, (double)__uint_as_float(bits_at(least) << 16), 1.0 / (double)temperature};
+    const double top = (double)__uint_as_float(bits_at(least) << 16), by = 1.0 / (double)temperature;
+    const auto weight = [&](int place) {
+        const double x = (double)__uint_as_float(bits_at(place) << 16), y = exp_d((x - top) * by);
+        // beside +inf nothing else weighs
+        return x == top ? 1.0 : top > 3.5e38 ? 0.0 : y;
+    };
+    // a chunk's values, two per lane
+    int n[2];
+    double w[2];
+    const auto weights = [&](int chunk) {
+        const int word = chunk * 64 + lane;
+        counts_of(row, carries, word, row.counts[word], n[0], n[1]);
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const double each = weight(2 * word + e);
+            w[e] = n[e] ? each : 0.0;
+        }
+    };
     int place = least, nth = 0;
-    double logprob = 0.0;
+    double ratio = 1.0;
     if (temperature > 0.0f) {
-        constexpr int EACH = CHUNKS / WAVES;  // chunks of a wave, every WAVES-th one
-        uint32_t words[EACH];
-#pragma unroll
-        for (int i = 0; i < EACH; i++) words[i] = row.counts[(i * WAVES + wave) * 64 + lane];
-#pragma unroll
-        for (int i = 0; i < EACH; i++) {
-            const int chunk = i * WAVES + wave;
-            double m = 0.0;
-            int n = 0;
-            if (__any(words[i] != 0) || carries) {
-                int n0, n1;
-                counts_of(row, carries, chunk * 64 + lane, words[i], n0, n1);
-                if (n0) m = n0 * d.weight(2 * (chunk * 64 + lane));
-                if (n1) m += n1 * d.weight(2 * (chunk * 64 + lane) + 1);
-                m = sum_lanes(m);
-                n = sum_lanes(n0 + n1);
-            }
-            if (lane == 0) row.mass[chunk] = m, row.tokens[chunk] = n;
-        }
-        __syncthreads();
-        if (wave == 0) {  // what lies in front of each chunk, eight chunks per lane
-            constexpr int EIGHT = CHUNKS / 64;
-            double before = 0.0, own[EIGHT];
-            int n = 0, tokens[EIGHT];
-#pragma unroll
-            for (int i = 0; i < EIGHT; i++) {
-                before += own[i] = row.mass[lane * EIGHT + i];
-                n += tokens[i] = row.tokens[lane * EIGHT + i];
-            }
-            sum_before(before, n);
-#pragma unroll
-            for (int i = 0; i < EIGHT; i++) {
-                row.mass[lane * EIGHT + i] = before;
-                row.tokens[lane * EIGHT + i] = n;
-                before += own[i];
-                n += tokens[i];
-            }
-            if (lane == 63) row.mass[CHUNKS] = before, row.tokens[CHUNKS] = n;
-        }
-        __syncthreads();
         int left = row.tokens[CHUNKS];
-        double total = row.mass[CHUNKS];
-        if (top_k > 0 && top_k < left) {
-            left = top_k;
-            total = d.behind(left).mass;
-        }
-        if (top_p < 1.0f) {  // those in front of the one that reaches p, and that one
-            const Draw::Spot s = d.template within<false>((double)top_p * total);
-            if (s.tokens + 1 < left) {
-                left = s.tokens + 1;
-                total = s.mass + s.weight;
+        if (top_k > 0) left = min(left, top_k);
+        // the mass of the chunks that hold some of the first top_k
+#pragma unroll 1
+        for (uint32_t rest = some; rest; rest &= rest - 1) {
+            const int word = word_of(__builtin_ctz(rest));
+            if (row.tokens[word / 256 * 4] >= left) break;  // in front of the group
+            const u32x4 v = *(const u32x4 *)(row.counts + word);
+            double part[8], m = 0.0;  // side by side
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                counts_of(row, carries, word + j, v[j], n[0], n[1]);
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const double each = weight(2 * (word + j) + e);
+                    part[2 * j + e] = n[e] ? n[e] * each : 0.0;
+                }
             }
+#pragma unroll
+            for (int j = 0; j < 8; j++) m += part[j];
+            m = sum_of_row(m);
+            if (lane % 16 == 15) row.mass[word / 64] = m;
         }
-        if (min_p > 0.0f) {
-            // the last place of enough weight, by 64ths and then one by one of what is left: weights do not grow
-            // along the places
-            int lo = least, hi = 0xff7f + 1;
-            while (hi - lo > 1) {
-                const int step = (hi - lo + 63) / 64, at = lo + (lane + 1) * step;
-                const int fit = __popcll(__ballot(at < hi && d.weight(at) >= (double)min_p));
-                hi = min(hi, lo + (fit + 1) * step);
-                lo += fit * step;
-            }
-            const int chunk = lo / CHUNK;
-            const Draw::Lane l = d.lane_of(chunk);
-            const int k0 = lane < lo % CHUNK / 2 || 2 * lane == lo % CHUNK || 2 * lane + 1 == lo % CHUNK ? l.n0 : 0;
-            const int k1 = lane < lo % CHUNK / 2 || 2 * lane + 1 == lo % CHUNK ? l.n1 : 0;
-            const Draw::Spot s = d.spot(chunk, l, k0, k1);
-            const bool one = min_p > 1.0f;  // more than the first one weighs
-            if (one || s.tokens < left) {
-                left = one ? 1 : s.tokens;
-                total = one ? 1.0 : s.mass;
-            }
-        }
-        const double at = (double)u * total;
-        Draw::Spot s = u != u ? d.behind(0) : d.template within<true>(at);
-        // past the last one: to that; or to the last one of positive weight
-        if (s.tokens >= left) s = d.behind(left - 1);
-        if (!(at < total) && u == u) {
-            const Draw::Spot last = d.template within<false>(total);
-            if (last.tokens < s.tokens) s = last;
-        }
-        place = s.place;
-        nth = s.nth;
-        logprob = log(s.weight / total);
+        __syncthreads();
+        if (wave == 0) sum_chunks(row.mass);
+        __syncthreads();
     }
+    if (temperature > 0.0f && wave == 0) {
+        int left = row.tokens[CHUNKS];
+        if (top_k > 0) left = min(left, top_k);
+        double total = row.mass[CHUNKS];
+
+        // Spots in the order of the tokens: behind a number of them, behind those up to a value, or behind the last
+        // one up to which the mass is below `at` (BELOW) or not past it (WITHIN).
+        enum { TOKENS, VALUES, BELOW, WITHIN };
+        enum { TOP_K, TOP_P, MIN_P, PICK, BACK, DONE };
+        int spot_tokens = 0;
+#pragma unroll 1
+        for (int step = TOP_K; step < DONE;) {
+            int how = TOKENS, behind = 0;
+            double at = 0.0;
+            bool needed = true;
+            if (step == TOP_K) {
+                needed = left < row.tokens[CHUNKS];
+                behind = left;
+            } else if (step == TOP_P) {
+                needed = top_p < 1.0f;
+                how = BELOW;
+                at = (double)top_p * total;
+            } else if (step == MIN_P) {
+                needed = min_p > 0.0f;
+                how = VALUES;
+                // the last place of enough weight, by 64ths of what is left: weights do not grow along the places
+                int lo = least, hi = needed ? 0xff7f + 1 : least + 1;
+#pragma unroll 1
+                while (hi - lo > 1) {
+                    const int by64 = (hi - lo + 63) / 64, mine = lo + (lane + 1) * by64;
+                    const int fit = __popcll(__ballot(mine < hi && weight(mine) >= (double)min_p));
+                    hi = min(hi, lo + (fit + 1) * by64);
+                    lo += fit * by64;
+                }
+                behind = lo;
+            } else if (step == PICK) {
+                at = (double)u * total;
+                how = u != u ? TOKENS : at < total ? WITHIN : BELOW;  // a u of 1 or more: the last one of positive weight
+                at = fmin(at, total);
+            } else {  // past the last one by a rounding: that
+                needed = spot_tokens >= left;
+                behind = left - 1;
+            }
+            if (!needed) {
+                step++;
+                continue;
+            }
+            const auto fits = [&](double m) { return how == WITHIN ? m <= at : m < at; };
+            int chunk, k0, k1;
+            uint64_t stops;
+            double before;
+            int tokens;
+            for (;;) {
+                // the last chunk whose front is not past the spot; fronts do not fall
+                const auto front = [&](int c) { return how == TOKENS ? row.tokens[c] <= behind : fits(row.mass[c]); };
+                const int group = max(0, __popcll(__ballot(front(lane * 8))) - 1);
+                chunk = group * 8 + max(0, __popcll(__ballot(lane < 8 && front(group * 8 + (lane & 7)))) - 1);
+                if (how == VALUES) chunk = behind / CHUNK;
+                weights(chunk);
+                before = row.mass[chunk] + in_front(sum_upto(n[0] * w[0] + n[1] * w[1]));
+                tokens = row.tokens[chunk] + in_front(sum_upto(n[0] + n[1]));
+                // how many tokens of the lane's two values are in front of the spot
+                if (how == TOKENS) {
+                    k0 = max(0, min(n[0], behind - tokens));
+                    k1 = max(0, min(n[1], behind - tokens - n[0]));
+                } else if (how == VALUES) {
+                    k0 = 2 * (chunk * 64 + lane) <= behind ? n[0] : 0;
+                    k1 = 2 * (chunk * 64 + lane) + 1 <= behind ? n[1] : 0;
+                } else {
+                    const auto part = [&](double m, double each, int most) {
+                        if (most == 0 || !fits(m)) return 0;
+                        int k = each > 0 ? (int)fmin(fmax((at - m) / each, 0.0), (double)most) : most;
+                        if (k > 0 && !fits(m + k * each)) k--;
+                        if (k < most && fits(m + (k + 1) * each)) k++;
+                        return k;
+                    };
+                    k0 = part(before, w[0], n[0]);
+                    k1 = k0 < n[0] ? 0 : part(before + n[0] * w[0], w[1], n[1]);
+                }
+                stops = __ballot(k0 + k1 < n[0] + n[1]);
+                if (stops || how == TOKENS || how == VALUES) break;
+                // all of the chunk, where its sum falls short of the next one's front by a rounding, or it is empty
+                how = TOKENS;
+                behind = row.tokens[chunk + 1];
+            }
+            const int from = stops ? (int)__builtin_ctzll(stops) : 63;
+            const bool second = k0 == n[0];
+            spot_tokens = lane_value(tokens + k0 + k1, from);
+            const double mass = lane_value(before + (k0 * w[0] + k1 * w[1]), from);
+            const double each = lane_value(second ? w[1] : w[0], from);
+            if (step == TOP_K) {
+                total = mass;
+            } else if (step == TOP_P) {  // with the one that reaches p
+                if (spot_tokens + 1 < left) left = spot_tokens + 1, total = mass + each;
+            } else if (step == MIN_P) {
+                if (min_p > 1.0f) left = 1, total = 1.0;  // more than the first one weighs
+                else if (spot_tokens < left) left = spot_tokens, total = mass;
+            } else {
+                place = lane_value(2 * (chunk * 64 + lane) + (second ? 1 : 0), from);
+                nth = lane_value(second ? k1 : k0, from);
+                ratio = each / total;
+            }
+            step++;
+        }
+    }
+    if (threadIdx.x == 0) row.place = place, row.nth = nth, row.ratio = ratio;
+    __syncthreads();
+    place = row.place;
+    nth = row.nth;
+    ratio = row.ratio;
     int first, last;
     where(place, nth, first, last);
-    // each wave counts the value in its part of these tokens, then one looks through its own
+    // each wave counts the value in its part of these tokens, 32 per lane at a time, then one looks through its own
     const uint32_t bits = bits_at(place);
-    const auto same = [&](uint32_t b) { return b == bits || (bits == 0 && b == 0x8000); };
     const bf16 *x = a.x + r * a.x_stride;
-    // parts of whole 512 tokens from an aligned address on
-    const int begin = first - (int)((uintptr_t)(x + first) % 16 / 2), part = (last - begin + 512 * WAVES - 1) / (512 * WAVES) * 512;
-    const auto request = [&](int i) {  // eight tokens from i on, as a mask of those of the value
+    constexpr int ROUND = 64 * 32;
+    const int begin = first - (int)((uintptr_t)(x + first) % 16 / 2);
+    const int part = (last - begin + ROUND * WAVES - 1) / (ROUND * WAVES) * ROUND, mine = begin + wave * part;
+    const auto look_at = [&](int i) {  // the lane's 32 tokens from i on: which have the value
         uint32_t mask = 0;
-        if (i >= first && i + 8 <= last) {
-            const u32x4 v = ld16(x + i);
+        if (i >= first && i + 32 <= last) {
+            u32x4 v[4];
 #pragma unroll
-            for (int e = 0; e < 8; e++) mask |= same(v[e / 2] >> (e % 2 * 16) & 0xffff) ? 1u << e : 0;
+            for (int j = 0; j < 4; j++) v[j] = ld16(x + i + 8 * j);
+#pragma unroll
+            for (int j = 0; j < 32; j++) {
+                uint32_t b = v[j / 8][j % 8 / 2] >> (j % 2 * 16) & 0xffff;
+                if (b == 0x8000) b = 0;
+                mask |= b == bits ? 1u << j : 0;
+            }
         } else {
-            for (int e = 0; e < 8; e++)
-                if (i + e >= first && i + e < last && same(gptr(x)[i + e])) mask |= 1u << e;
+#pragma unroll 1
+            for (int j = max(0, first - i); j < min(32, last - i); j++) {
+                uint32_t b = gptr(x)[i + j];
+                if (b == 0x8000) b = 0;
+                mask |= b == bits ? 1u << j : 0;
+            }
         }
         return mask;
     };
-    const int mine = begin + wave * part, end = min(last, mine + part);
-    int met = 0;
-#pragma unroll 4
-    for (int i = mine; i < end; i += 512) met += __popc(request(i + 8 * lane));
-    met = sum_lanes(met);
-    __syncthreads();
-    if (lane == 0) row.found[wave] = met;
-    __syncthreads();
-    int before = 0;
-    for (int i = 0; i < wave; i++) before += row.found[i];
-    if (nth < before || nth >= before + met) return;
-    nth -= before;
-    for (int i = mine; i < end; i += 512) {
-        const uint32_t mask = request(i + 8 * lane);
-        int upto = __popc(mask);
-        const int own = upto;
-#pragma unroll
-        for (int k = 1; k < 64; k *= 2) {
-            const int v = __shfl_up(upto, k);
-            if (lane >= k) upto += v;
+    int met = 0, at = mine;
+    uint32_t mask = 0;
+#pragma unroll 1
+    for (bool counted = false;;) {
+        // once to count; where that takes one round, its mask is that of the second time
+        if (!counted) {
+            for (int i = mine; i < min(last, mine + part); i += ROUND) {
+                mask = look_at(i + 32 * lane);
+                met += __popc(mask);
+            }
+            met = sum_lanes(met);
+            if (lane == 0) row.sums[wave] = met;
+            __syncthreads();
+            const int before = __builtin_amdgcn_readfirstlane(sum_lanes(lane < wave ? row.sums[lane] : 0));
+            if (nth < before || nth >= before + met) return;
+            nth -= before;
+            counted = true;
+            if (part > ROUND) continue;
+        } else {
+            mask = look_at(at + 32 * lane);
         }
-        const int all = __shfl(upto, 63);
+        const int upto = sum_upto((int)__popc(mask)), all = lane_value(upto, 63);
         if (nth < all) {
-            int rest = nth - (upto - own);
-            if (rest < 0 || rest >= own) return;
-            for (int e = 0; e < 8; e++)
-                if (mask >> e & 1 && rest-- == 0) {
-                    a.out[r] = i + 8 * lane + e;
-                    if (a.logprob) a.logprob[r] = (float)logprob;
-                }
+            int rest = nth - (upto - __popc(mask));
+            if (rest < 0 || rest >= __popc(mask)) return;
+            for (; rest > 0; rest--) mask &= mask - 1;
+            a.out[r] = at + 32 * lane + __builtin_ctz(mask);
+            if (a.logprob) a.logprob[r] = (float)log(ratio);
             return;
         }
         nth -= all;
+        at += ROUND;
     }
 }
 
+// Counts with add(exact), which gives the smallest place and the number of what it counted; again, with carries, where
+// the sum of the counts says that some passed 16 bits.
+template <class Add>
+__device__ __forceinline__ uint32_t count_all(Row &row, int &least, Add add) {
+    int n = 0;
+    least = BINS;
+    add(std::false_type{}, least, n);
+    __syncthreads();
+    gather(row, least, n);
+    uint32_t some = sum_tokens(row, 0);
+    if (row.tokens[CHUNKS] == n) return some;
+    __syncthreads();
+    clear(row);
+    add(std::true_type{}, least, n);
+    __syncthreads();
+    return sum_tokens(row, row.carries);
+}
+
 // One workgroup per row.
-template <bool CARRY>
 __global__ __launch_bounds__(T) void sample_kernel(SampleArgs a) {
     __shared__ Row row;
     const int r = blockIdx.x;
+    Logits logits(a.x + r * a.x_stride, 0, a.vocab);
     clear(row);
-    int least = BINS;
-    each_logit(a.x + r * a.x_stride, 0, a.vocab, [&](int, uint32_t b) {
-        const int p = place_of(b);
-        if (p == NONE) return;
-        least = min(least, p);
-        count<CARRY>(row, p, 1);
+    int least;
+    const uint32_t some = count_all(row, least, [&](auto carry, int &least, int &n) {
+        if (carry) logits = Logits(a.x + r * a.x_stride, 0, a.vocab);  // again
+        logits.each([&](uint32_t b) {
+            const int p = place_of(b);
+            if (p == NONE) return;
+            least = min(least, p);
+            n++;
+            count<decltype(carry)::value>(row, p, 1);
+        });
     });
-    least = least_of(row, least);
-    draw(a, row, r, least, [&](int, int &, int &first, int &last) { first = 0, last = a.vocab; });
+    draw(a, row, r, least, some, [&](int, int &, int &first, int &last) { first = 0, last = a.vocab; });
 }
 
 // A slice of a row: its values and their counts as a list.
 __global__ __launch_bounds__(T) void slice_kernel(SampleArgs a) {
     __shared__ Row row;
-    const int r = blockIdx.y, lane = threadIdx.x & 63, wave = wave_id();
+    const int r = blockIdx.y, lane = threadIdx.x & 63;
     const int first = blockIdx.x * a.slice, last = min(a.vocab, first + a.slice);
+    Logits logits(a.x + r * a.x_stride, first, last);
     clear(row);
-    each_logit(a.x + r * a.x_stride, first, last, [&](int, uint32_t b) {
+    logits.each([&](uint32_t b) {
         const int p = place_of(b);
         if (p != NONE) count<false>(row, p, 1);  // a slice has less than 2^16 tokens
     });
     __syncthreads();
     const int at = r * a.slices + blockIdx.x;
     uint32_t *list = a.lists + (int64_t)at * a.slice;
-    constexpr int EACH = CHUNKS / WAVES;
-    uint32_t words[EACH];
+    const uint32_t some = groups_with_some(row);
+    const auto entries = [](const u32x4 &v) {
+        int n = 0;
 #pragma unroll
-    for (int i = 0; i < EACH; i++) words[i] = row.counts[(i * WAVES + wave) * 64 + lane];
+        for (int j = 0; j < 4; j++) n += ((v[j] & 0xffff) != 0) + (v[j] >> 16 != 0);
+        return n;
+    };
+    int all = 0;
+#pragma unroll 1
+    for (uint32_t rest = some; rest; rest &= rest - 1) all += entries(*(const u32x4 *)(row.counts + word_of(__builtin_ctz(rest))));
+    const int upto = sum_upto(all);
+    int to = 0;
+    if (lane == 63) to = atomicAdd(&row.entries, upto);
+    to = lane_value(to, 63) + upto - all;  // a lane's entries lie side by side
+#pragma unroll 1
+    for (uint32_t rest = some; rest; rest &= rest - 1) {
+        const int word = word_of(__builtin_ctz(rest));
+        const u32x4 v = *(const u32x4 *)(row.counts + word);
 #pragma unroll
-    for (int i = 0; i < EACH; i++) {
-        const uint64_t some0 = __ballot((words[i] & 0xffff) != 0), some1 = __ballot(words[i] >> 16 != 0);
-        if (!(some0 | some1)) continue;
-        int to = 0;
-        if (lane == 0) to = atomicAdd(&row.entries, __popcll(some0) + __popcll(some1));
-        to = __builtin_amdgcn_readfirstlane(to);
-        const uint64_t before = (1ull << lane) - 1;
-        const uint32_t place = 2 * ((i * WAVES + wave) * 64 + lane);
-        if (words[i] & 0xffff) gptr(list)[to + __popcll(some0 & before)] = place << 16 | (words[i] & 0xffff);
-        if (words[i] >> 16) gptr(list)[to + __popcll(some0) + __popcll(some1 & before)] = (place + 1) << 16 | words[i] >> 16;
+        for (int j = 0; j < 4; j++) {
+            const uint32_t place = 2 * (word + j);
+            if (v[j] & 0xffff) gptr(list)[to++] = place << 16 | (v[j] & 0xffff);
+            if (v[j] >> 16) gptr(list)[to++] = (place + 1) << 16 | v[j] >> 16;
+        }
     }
     __syncthreads();
     if (threadIdx.x == 0) gptr(a.entries)[at] = row.entries;
 }
 
 // The draw from a row's slices.
-template <bool CARRY>
 __global__ __launch_bounds__(T) void merge_kernel(SampleArgs a) {
     __shared__ Row row;
     __shared__ int of_slice[MOST_SLICES];  // how many of the drawn value
     const int r = blockIdx.x;
-    int sizes[MOST_SLICES];
+    int sizes[MOST_SLICES], most = 0;
 #pragma unroll
     for (int s = 0; s < MOST_SLICES; s++) sizes[s] = s < a.slices ? gptr(a.entries)[r * a.slices + s] : 0;
-    clear(row);
-    int least = BINS;
+#pragma unroll
+    for (int s = 0; s < MOST_SLICES; s++) most = max(most, sizes[s]);
     const uint32_t *lists = a.lists + (int64_t)r * a.slices * a.slice;
-    constexpr int U = 4;
+    // an entry of every slice at a time; the first ones stay in registers
+    constexpr int KEPT = 3;
+    uint32_t kept[KEPT][MOST_SLICES];
+    const auto request = [&](int i, uint32_t (&v)[MOST_SLICES]) {
 #pragma unroll
-    for (int s = 0; s < MOST_SLICES; s++) {
-        const uint32_t *list = lists + (int64_t)s * a.slice;
-        for (int i0 = threadIdx.x; i0 < sizes[s]; i0 += U * T) {
-            uint32_t v[U];
+        for (int s = 0; s < MOST_SLICES; s++) v[s] = i < sizes[s] ? gptr(lists)[(int64_t)s * a.slice + i] : 0;
+    };
 #pragma unroll
-            for (int u = 0; u < U; u++) v[u] = i0 + u * T < sizes[s] ? gptr(list)[i0 + u * T] : 0;
+    for (int k = 0; k < KEPT; k++) request(k * T + threadIdx.x, kept[k]);
+    const auto each_entry = [&](auto f) {
+        const auto all = [&](const uint32_t (&v)[MOST_SLICES]) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (v[u]) {
-                    least = min(least, (int)(v[u] >> 16));
-                    count<CARRY>(row, v[u] >> 16, v[u] & 0xffff);
-                }
+            for (int s = 0; s < MOST_SLICES; s++)
+                if (v[s]) f(s, (int)(v[s] >> 16), v[s] & 0xffff);
+        };
+#pragma unroll
+        for (int k = 0; k < KEPT; k++)
+            if (k * T < most) all(kept[k]);
+#pragma unroll 1
+        for (int i = KEPT * T + threadIdx.x; i < most; i += T) {
+            uint32_t v[MOST_SLICES];
+            request(i, v);
+            all(v);
         }
-    }
-    least = least_of(row, least);
-    draw(a, row, r, least, [&](int place, int &nth, int &first, int &last) {
+    };
+    clear(row);
+    int least;
+    const uint32_t some = count_all(row, least, [&](auto carry, int &least, int &n) {
+        each_entry([&](int, int place, uint32_t m) {
+            least = min(least, place);
+            n += m;
+            count<decltype(carry)::value>(row, place, m);
+        });
+    });
+    draw(a, row, r, least, some, [&](int place, int &nth, int &first, int &last) {
         if (threadIdx.x < MOST_SLICES) of_slice[threadIdx.x] = 0;
         __syncthreads();
+        each_entry([&](int s, int p, uint32_t m) {
+            if (p == place) of_slice[s] = m;
+        });
+        __syncthreads();
+        int which = 0;
+        bool there = false;
 #pragma unroll
         for (int s = 0; s < MOST_SLICES; s++) {
-            const uint32_t *list = lists + (int64_t)s * a.slice;
-            for (int i0 = threadIdx.x; i0 < sizes[s]; i0 += U * T) {
-                uint32_t v[U];
-#pragma unroll
-                for (int u = 0; u < U; u++) v[u] = i0 + u * T < sizes[s] ? gptr(list)[i0 + u * T] : 0;
-#pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (v[u] && (int)(v[u] >> 16) == place) of_slice[s] = v[u] & 0xffff;
-            }
+            there |= nth < of_slice[s];
+            if (!there && s + 1 < a.slices) nth -= of_slice[s], which = s + 1;
         }
-        __syncthreads();
-        int s = 0;
-        while (s + 1 < a.slices && nth >= of_slice[s]) nth -= of_slice[s++];
-        first = s * a.slice, last = min(a.vocab, first + a.slice);
+        first = which * a.slice, last = min(a.vocab, first + a.slice);
     });
 }
 
@@ -541,7 +689,6 @@ extern "C" void sample_rows_forward(int *out, float *logprob, const bf16 *logits
     }
     SampleArgs a = {out, logprob, logits, temperature, top_k, top_p, min_p, u, vocab, logits_stride, nullptr, nullptr, 1, vocab};
     const int slices = slices_of(rows, vocab);
-    const bool carry = vocab > 65535;
     if (slices > 1 && slices <= MOST_SLICES) {
         // from multiples of 8 on, so that slices are as aligned as their row
         a.slice = ((vocab + slices - 1) / slices + 7) / 8 * 8;
@@ -550,12 +697,9 @@ extern "C" void sample_rows_forward(int *out, float *logprob, const bf16 *logits
         a.lists = (uint32_t *)ws + ((size_t)rows * a.slices + 3) / 4 * 4;
         slice_kernel<<<dim3(a.slices, rows), T, 0, stream>>>(a);
         if (!LAUNCH_OK()) return;
-        if (carry) merge_kernel<true><<<rows, T, 0, stream>>>(a);
-        else merge_kernel<false><<<rows, T, 0, stream>>>(a);
-    } else if (carry) {
-        sample_kernel<true><<<rows, T, 0, stream>>>(a);
+        merge_kernel<<<rows, T, 0, stream>>>(a);
     } else {
-        sample_kernel<false><<<rows, T, 0, stream>>>(a);
+        sample_kernel<<<rows, T, 0, stream>>>(a);
     }
     LAUNCH_OK();
 }
