@@ -33,6 +33,7 @@ struct SampleArgs {
 constexpr int T = 1024, WAVES = T / 64;
 constexpr int BINS = 1 << 16, CHUNK = 128, CHUNKS = BINS / CHUNK;
 constexpr int MAX_VOCAB = 1 << 22, MOST_CARRIES = 128;  // over vocab / 2^16 + vocab / 2^32
+constexpr uint32_t NO_VALUE = 0xffffffffu;  // two NaN
 constexpr int NONE = -1, MOST_SLICES = 8, MOST_SLICE = 65528;  // a multiple of 8 that 16 bits count
 
 // The place of a value among the values, largest first, from its bits; NONE for what is never taken.
@@ -395,7 +396,8 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int l
                 } else {
                     const auto part = [&](double m, double each, int most) {
                         if (most == 0 || !fits(m)) return 0;
-                        int k = each > 0 ? (int)fmin(fmax((at - m) / each, 0.0), (double)most) : most;
+                        // the reciprocal's 26 bits are enough for one too many or too few of up to 2^22
+                        int k = each > 0 ? (int)fmin(fmax((at - m) * __builtin_amdgcn_rcp(each), 0.0), (double)most) : most;
                         if (k > 0 && !fits(m + k * each)) k--;
                         if (k < most && fits(m + (k + 1) * each)) k++;
                         return k;
@@ -443,24 +445,27 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int l
     const int begin = first - (int)((uintptr_t)(x + first) % 16 / 2);
     const int part = (last - begin + ROUND * WAVES - 1) / (ROUND * WAVES) * ROUND, mine = begin + wave * part;
     const auto look_at = [&](int i) {  // the lane's 32 tokens from i on: which have the value
+        u32x4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int c = i + 8 * j;
+            v[j] = u32x4{NO_VALUE, NO_VALUE, NO_VALUE, NO_VALUE};
+            if (c >= first && c + 8 <= last) {
+                v[j] = ld16(x + c);
+            } else if (c + 8 > first && c < last) {  // at an end that is not aligned
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (c + e >= first && c + e < last)
+                        v[j][e / 2] = e % 2 ? (v[j][e / 2] & 0xffff) | (uint32_t)gptr(x)[c + e] << 16
+                                            : (v[j][e / 2] & 0xffff0000u) | gptr(x)[c + e];
+            }
+        }
         uint32_t mask = 0;
-        if (i >= first && i + 32 <= last) {
-            u32x4 v[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = ld16(x + i + 8 * j);
-#pragma unroll
-            for (int j = 0; j < 32; j++) {
-                uint32_t b = v[j / 8][j % 8 / 2] >> (j % 2 * 16) & 0xffff;
-                if (b == 0x8000) b = 0;
-                mask |= b == bits ? 1u << j : 0;
-            }
-        } else {
-#pragma unroll 1
-            for (int j = max(0, first - i); j < min(32, last - i); j++) {
-                uint32_t b = gptr(x)[i + j];
-                if (b == 0x8000) b = 0;
-                mask |= b == bits ? 1u << j : 0;
-            }
+        for (int j = 0; j < 32; j++) {
+            uint32_t b = v[j / 8][j % 8 / 2] >> (j % 2 * 16) & 0xffff;
+            if (b == 0x8000) b = 0;
+            mask |= b == bits ? 1u << j : 0;
         }
         return mask;
     };
