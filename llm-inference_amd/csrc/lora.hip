@@ -315,7 +315,7 @@ struct Shape {
     static constexpr bool STREAM = STREAM_;                          // W is read once, past the caches
     static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, BK = BK_, S = 16, STAGES = STAGES_;
     static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / S, NT = RN / S;
-    static constexpr bool JOINS = TM <= 64;                          // also in front of join_kernel
+    static constexpr bool JOINS = TM <= 128;                         // also in front of join_kernel
     static constexpr int CHUNKS = BK / 8, ROW = 2 * BK, PER = 64 / CHUNKS;  // of a row: chunks, bytes; rows of a load
     static constexpr int BYTES = (TM + TN) * ROW;                    // of a stage
     static_assert(!JOINS || STAGES * BYTES >= WAVES * 16 * 68 * 4, "low_part's sums");
@@ -794,16 +794,18 @@ typedef Shape<64, 128, 64, 32, 64, 3, true> Few128;
 typedef Shape<64, 64, 64, 16, 64, 4, true> Few64;
 typedef Shape<32, 64, 32, 16, 64, 4, true> Few32;
 typedef Shape<16, 64, 16, 16, 64, 4, true> Few16;
-constexpr Pace PACES[] = {{256, 192, 1, 930, 1130, 11000}, {224, 256, 1, 1050, 1250, 11000}, {192, 256, 1, 960, 1120, 11000},
-                          {128, 256, 1, 620, 760, 8000},   {128, 128, 2, 560, 850, 6000},    {64, 128, 2, 400, 500, 4500},
-                          {64, 64, 2, 300, 460, 4000},     {32, 64, 3, 270, 370, 3700},      {16, 64, 3, 250, 350, 3500}};
+constexpr Pace PACES[] = {{256, 192, 1, 1110, 1060, 8550}, {224, 256, 1, 1080, 1390, 8470}, {192, 256, 1, 760, 1080, 9150},
+                          {128, 256, 1, 595, 695, 4600},   {128, 128, 2, 565, 875, 2180},   {64, 128, 2, 270, 690, 1820},
+                          {64, 64, 2, 195, 290, 1830},     {32, 64, 3, 215, 195, 1940},     {16, 64, 3, 125, 365, 1660}};
 constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 
 constexpr int MOST_SPLITS = 32;
 constexpr size_t MOST_PART = 1 << 23;  // floats
 
 // How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the
-// product, or join_kernel's.
+// product, or join_kernel's. The least of an estimate fitted to 101 calls (1 to 4079 rows, 1 to 128 sequences, ranks of 8
+// to 128, 500 to 151936 columns), each in every shape and many splits: what it chooses takes 3% longer on average
+// than the best of those, at most 29%.
 struct Plan {
     int shape, splits, split_steps;
     bool join;
@@ -816,31 +818,37 @@ struct Plan {
 
     Plan(int n_tokens, int n_out, int n_in, bool product, bool adapters, int rank, int n_seqs, int n_adapters) {
         const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
-        const int64_t one = (int64_t)part_floats(n_tokens, n_out);
+        const double rows = n_tokens, seqs = n_seqs, one = (double)part_floats(n_tokens, n_out);
+        // bytes of low's operands with tiles of 64 rows, and of b with tiles of 16
+        const double low = adapters ? (std::min(rows, rows / LOW_ROWS + seqs) * rank + rows) * n_in * 2 : 0;
+        const double b = adapters ? std::min(rows, rows / 16 + seqs) * n_out * rank * 2 : 0;
+        // adapters of a tile's rows, each with steps of its own
+        const auto own_steps = [&](const Pace &s) {
+            return adapters ? pieces * std::min<double>(n_adapters, 1 + seqs * std::min<double>(s.tm, rows) / rows) : 0.0;
+        };
         double least = 0;
         shape = -1;
         for (int i = 0; i < SHAPES; i++) {
             const Pace &s = PACES[i];
-            const double tiles = (double)((n_tokens + s.tm - 1) / s.tm) * ((n_out + s.tn - 1) / s.tn);
-            // adapters of a tile's rows, each with steps of its own
-            const double own = adapters ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(s.tm, n_tokens) / n_tokens) : 0;
-            for (int n = 1; n <= std::min(MOST_SPLITS, std::max(steps, 1)) && (n == 1 || n * one <= (int64_t)MOST_PART); n++) {
-                const double groups = tiles * n, rounds = ceil(groups / (s.at_once * CUS)), busy = std::min(1.0, groups / CUS);
-                const double step = s.alone + (s.full - s.alone) * busy, each = (steps + n - 1) / n;
-                const double parts = one * (n * 8.0 + 4) / 4500, memory = product ? 2.0 * n_out * n_in / 5500 : 0;
-                const double cost = std::max(rounds * (each + own) * step, memory) + rounds * s.fixed +
-                                    (n > 1 ? 5000 + parts : 0) + (adapters ? 11000 : 0);
+            const double m_tiles = ceil(rows / s.tm), tiles = m_tiles * ceil((double)n_out / s.tn);
+            const double again = s.tm <= 64 ? 0.5 * std::min(m_tiles - 1, 8.0) : 0;  // W past the caches, for more rows
+            const double memory = product ? 2.0 * n_out * n_in * (1 + again) / 4800 : 0;
+            for (int n = 1; n <= std::min(MOST_SPLITS, std::max(steps, 1)) && (n == 1 || n * one <= (double)MOST_PART); n++) {
+                const double groups = tiles * n, step = s.alone + (s.full - s.alone) * std::min(1.0, groups / CUS);
+                const double rounds = ceil(groups / (s.at_once * CUS)), each = (steps + n - 1) / n, parts = one * (8 * n + 4);
+                const double cost = 2500 + std::max(rounds * (each + own_steps(s)) * step, memory) + rounds * s.fixed +
+                                    (n > 1 ? 2500 + parts / 7300 : one * 2 / 7700) + (adapters ? 12500 + low / 6700 : 0);
                 if (shape < 0 || cost < least) shape = i, splits = n, join = false, least = cost;
-                if (!adapters || s.tm > 64 || n * one > (int64_t)MOST_PART) continue;
-                // parts that the join has under way at once
-                const int at_once = n_tokens <= n_seqs ? 8 : 4;
-                const double joined = std::max(rounds * each * step, memory) + rounds * s.fixed + parts + 5000 +
-                                      1200 * ceil((double)n / at_once);
+                if (!adapters || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
+                const double product_cost = product ? std::max(rounds * each * step, memory) + rounds * s.fixed : 0;
+                const int at_once = n_tokens <= n_seqs ? 8 : 4;  // parts that the join has under way
+                const double joined = 2500 + product_cost + 3900 + 1140 * ceil((double)n / at_once) + parts / 5100 + b / 6700 +
+                                      low / 6700;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
             }
         }
         // the last split has the adapters' steps
-        const double own = adapters && !join ? pieces * std::min<double>(n_adapters, 1.0 + (double)n_seqs * std::min(PACES[shape].tm, n_tokens) / n_tokens) : 0;
+        const double own = join ? 0 : own_steps(PACES[shape]);
         split_steps = std::min(steps, (int)((steps + own + splits - 1) / splits));
         splits = split_steps ? (steps + split_steps - 1) / split_steps : join ? 0 : 1;
     }
