@@ -794,9 +794,9 @@ typedef Shape<64, 128, 64, 32, 64, 3, true> Few128;
 typedef Shape<64, 64, 64, 16, 64, 4, true> Few64;
 typedef Shape<32, 64, 32, 16, 64, 4, true> Few32;
 typedef Shape<16, 64, 16, 16, 64, 4, true> Few16;
-constexpr Pace PACES[] = {{256, 192, 1, 1110, 1060, 8550}, {224, 256, 1, 1080, 1390, 8470}, {192, 256, 1, 760, 1080, 9150},
-                          {128, 256, 1, 595, 695, 4600},   {128, 128, 2, 565, 875, 2180},   {64, 128, 2, 270, 690, 1820},
-                          {64, 64, 2, 195, 290, 1830},     {32, 64, 3, 215, 195, 1940},     {16, 64, 3, 125, 365, 1660}};
+constexpr Pace PACES[] = {{256, 192, 1, 900, 1250, 8600}, {224, 256, 1, 1070, 1340, 8900}, {192, 256, 1, 980, 1150, 9200},
+                          {128, 256, 1, 630, 770, 5600},  {128, 128, 2, 560, 810, 4800},   {64, 128, 2, 420, 620, 2500},
+                          {64, 64, 2, 430, 280, 3000},    {32, 64, 3, 330, 350, 2200},     {16, 64, 3, 290, 280, 1900}};
 constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 
 constexpr int MOST_SPLITS = 32;
@@ -819,31 +819,35 @@ struct Plan {
     Plan(int n_tokens, int n_out, int n_in, bool product, bool adapters, int rank, int n_seqs, int n_adapters) {
         const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
         const double rows = n_tokens, seqs = n_seqs, one = (double)part_floats(n_tokens, n_out);
-        // bytes of low's operands with tiles of 64 rows, and of b with tiles of 16
+        // bytes of low's operands with tiles of 64 rows and of 16, and of b with the latter
         const double low = adapters ? (std::min(rows, rows / LOW_ROWS + seqs) * rank + rows) * n_in * 2 : 0;
+        const double low16 = adapters ? (std::min(rows, rows / 16 + seqs) * rank + rows) * n_in * 2 : 0;
         const double b = adapters ? std::min(rows, rows / 16 + seqs) * n_out * rank * 2 : 0;
-        // adapters of a tile's rows, each with steps of its own
+        // adapters of a tile's rows, each with steps of its own: between those of sequences of one length, and as many
+        // as there can be, where the short ones lie side by side
         const auto own_steps = [&](const Pace &s) {
-            return adapters ? pieces * std::min<double>(n_adapters, 1 + seqs * std::min<double>(s.tm, rows) / rows) : 0.0;
+            if (!adapters) return 0.0;
+            const double tile = std::min<double>(s.tm, rows), even = std::min<double>(n_adapters, 1 + seqs * tile / rows);
+            return pieces * sqrt(even * std::min({(double)n_adapters, seqs, tile}));
         };
         double least = 0;
         shape = -1;
         for (int i = 0; i < SHAPES; i++) {
             const Pace &s = PACES[i];
             const double m_tiles = ceil(rows / s.tm), tiles = m_tiles * ceil((double)n_out / s.tn);
-            const double again = s.tm <= 64 ? 0.5 * std::min(m_tiles - 1, 8.0) : 0;  // W past the caches, for more rows
-            const double memory = product ? 2.0 * n_out * n_in * (1 + again) / 4800 : 0;
+            const double again = s.tm <= 64 ? 0.6 * std::min(m_tiles - 1, 8.0) : 0;  // W past the caches, for more rows
+            const double memory = product ? 2.0 * n_out * n_in * (1 + again) / 5100 : 0;
             for (int n = 1; n <= std::min(MOST_SPLITS, std::max(steps, 1)) && (n == 1 || n * one <= (double)MOST_PART); n++) {
                 const double groups = tiles * n, step = s.alone + (s.full - s.alone) * std::min(1.0, groups / CUS);
                 const double rounds = ceil(groups / (s.at_once * CUS)), each = (steps + n - 1) / n, parts = one * (8 * n + 4);
-                const double cost = 2500 + std::max(rounds * (each + own_steps(s)) * step, memory) + rounds * s.fixed +
-                                    (n > 1 ? 2500 + parts / 7300 : one * 2 / 7700) + (adapters ? 12500 + low / 6700 : 0);
+                const double cost = 2100 + std::max(rounds * (each + own_steps(s)) * step, memory) + rounds * s.fixed +
+                                    (n > 1 ? 3400 + parts / 8900 : one * 2 / 9100) + (adapters ? 9200 + low / 9700 : 0);
                 if (shape < 0 || cost < least) shape = i, splits = n, join = false, least = cost;
                 if (!adapters || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
                 const double product_cost = product ? std::max(rounds * each * step, memory) + rounds * s.fixed : 0;
                 const int at_once = n_tokens <= n_seqs ? 8 : 4;  // parts that the join has under way
-                const double joined = 2500 + product_cost + 3900 + 1140 * ceil((double)n / at_once) + parts / 5100 + b / 6700 +
-                                      low / 6700;
+                const double joined = 2100 + product_cost + 4500 + 1140 * ceil((double)n / at_once) + parts / 6000 + b / 7800 +
+                                      low16 / 9700;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
             }
         }
