@@ -500,7 +500,7 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int l
             return;
         }
         nth -= all;
-        at += ROUND;
+        if ((at += ROUND) >= last) return;
     }
 }
 

@@ -155,6 +155,22 @@ def test_counts_past_16_bits(gpu, first, second):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab", [(130, 140000), (2, 600000), (1, 524225), (3, 524224), (127, 65536), (128, 16384)])
+def test_rows_with_and_without_slices(gpu, rows, vocab):
+    """Both sides of the sizes from which rows are cut and slices are too many, with counts past 16 bits."""
+    import torch
+    rng = np.random.default_rng(vocab)
+    logits = torch.from_numpy(rng.choice([1.0, 1.0, 2.0, -1.0], (rows, vocab)).astype(np.float32)).cuda().bfloat16()
+    logits[0] = 3.0
+    c = make(rng, rows)
+    c["top_k"] = rng.integers(1, vocab, rows).astype(np.int32)
+    check(run(gpu, logits, c), logits, c)
+    logits = (torch.randn(rows, vocab, device="cuda") * 3).bfloat16()
+    c = make(rng, rows, **ALL)
+    check(run(gpu, logits, c), logits, c)
+
+
+@pytest.mark.gpu
 def test_every_value(gpu):
     """Every bf16 value once, in a random order, NaN and infinities among them; then every one that is finite."""
     import torch
