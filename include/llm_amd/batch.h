@@ -31,7 +31,7 @@ typedef struct {
     const float *scale;     /* [n_adapters], or NULL: 1 */
     const int *q_start;     /* [n_seqs + 1] */
     const int *adapter;     /* [n_seqs] */
-    int n_seqs;             /* at most 2^20 */
+    int n_seqs;             /* at most 2^20, empty ones among them */
     int n_adapters;
     int rank;               /* a multiple of 8, at most 256 */
 } LoraBatch;
@@ -40,13 +40,14 @@ typedef struct {
  * is not there for rows of sequences without one. w: [n_out, n_in], 16-byte aligned, or NULL: no product,
  * as beside a projection computed elsewhere. residual NULL: none; it may be out, row on row. lora NULL: no
  * adapters, and every row is computed. Otherwise nothing may overlap. x has rows x_stride elements apart (a multiple
- * of 8 up to 4194304, 16-byte aligned), out and residual rows out_stride and residual_stride apart, of any alignment (multiples
- * of 8 are faster). n_in is a multiple of 8.
- * Products and sums are in 32 bits and rounded to bf16 once, at the end; a[a] x is kept to 16 bits of its
- * mantissa in front of b[a] (as a bf16 and the bf16 of what that leaves). The order of the sums depends on the
+ * of 8 up to 4194304, 16-byte aligned), out and residual rows out_stride and residual_stride apart, of any
+ * alignment (multiples of 8 bytes are faster). n_in is a multiple of 8. Up to 2^20 rows, 2^20 of n_in and 2^22 of
+ * n_out; a call that would take a launch of 2^31 threads or more is refused.
+ * Products and sums are in 32 bits and rounded to bf16 once, at the end; scale a[a] x is kept to at least 16 bits
+ * of its mantissa in front of b[a] (as a bf16 and the bf16 of what that leaves). The order of the sums depends on the
  * sizes and lengths alone. NaN and infinities of a row or an adapter reach no other row.
  * ws: lora_projection_workspace_floats() floats, 16-byte aligned, needing no preparation; calls that share it
- * must not overlap (NULL where the count is 0). */
+ * must not overlap. */
 void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w, const bf16 *residual,
                              const LoraBatch *lora, float *ws, int n_tokens, int n_out, int n_in,
                              int64_t out_stride, int64_t x_stride, int64_t residual_stride,

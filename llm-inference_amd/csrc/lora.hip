@@ -9,13 +9,13 @@
 #include <type_traits>
 
 #include "common.h"
+#include "internal.h"
 #include "llm_amd/batch.h"
 
 using namespace llm;
 
 namespace {
 
-typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -49,29 +49,10 @@ struct LoraArgs {
 // What is loaded for places past an operand's end.
 __device__ const u32x4 g_zeros = {0, 0, 0, 0};
 
-template <int S>
-struct Mfma;
-template <>
-struct Mfma<32> {
-    typedef f32x16 Acc;
-    static constexpr int K = 16, REGS = 16;
-    static __device__ __forceinline__ f32x16 mul(const u32x4 &a, const u32x4 &b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
-                                                       c, 0, 0, 0);
-    }
-    // The first of the four rows that registers 4 i .. 4 i + 3 hold.
-    static __device__ __forceinline__ int row(int i, int lane) { return 8 * i + 4 * (lane / 32); }
-};
-template <>
-struct Mfma<16> {
-    typedef f32x4 Acc;
-    static constexpr int K = 32, REGS = 4;
-    static __device__ __forceinline__ f32x4 mul(const u32x4 &a, const u32x4 &b, f32x4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
-                                                       c, 0, 0, 0);
-    }
-    static __device__ __forceinline__ int row(int, int lane) { return 4 * (lane / 16); }
-};
+__device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0,
+                                                   0, 0);
+}
 
 // 64 lanes' 16 bytes into LDS at `to` on, without passing registers: the wave waits for it with wait_loads.
 template <bool STREAM = false>
@@ -106,6 +87,12 @@ __device__ __forceinline__ void barrier() {
 
 __device__ __forceinline__ int start_of(const LoraArgs &l, int s) {
     return max(0, min(l.n_tokens, gptr(l.q_start)[s]));
+}
+
+// What low_part wrote for row m. Starts that decrease leave rows that it does not know of, which are no sequence's.
+__device__ __forceinline__ int owner_of(const LoraArgs &l, int m) {
+    const int owner = gptr(l.owner)[m];
+    return owner >= NO_SEQUENCE && owner < l.n_adapters ? owner : NO_SEQUENCE;
 }
 
 // R rows of one sequence at most. A sequence of n rows from f on has at most (f + n) / R - f / R + 1 tiles, so those
@@ -169,7 +156,7 @@ __device__ __forceinline__ void low_sums(const LoraArgs &l, const RowTile &t, in
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
-                for (int j = 0; j < NT; j++) acc[i][j] = Mfma<16>::mul(as[u][j], xs[u][i], acc[i][j]);
+                for (int j = 0; j < NT; j++) acc[i][j] = mfma(as[u][j], xs[u][i], acc[i][j]);
     }
     // rows 16 bytes further apart: side by side those of a product's 16 would meet in the same banks
     constexpr int ALL = 16 * MT * (ROW + 4);
@@ -252,7 +239,7 @@ __global__ __launch_bounds__(256) void low_sum_kernel(LoraArgs l) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int m = (int)(i / per), r = (int)(i % per) * 4;
     if (m >= l.n_tokens) return;
-    const int owner = gptr(l.owner)[m];
+    const int owner = owner_of(l, m);
     if (owner < 0) return;
     const f32x4 y = low_sum(l, (int64_t)m * l.rank + r, l.scale ? gptr(l.scale)[owner] : 1.0f);
     u32x2 value, rest;
@@ -307,17 +294,19 @@ __device__ __forceinline__ float unfit_term(const LoraArgs &l, int n, int adapte
 // the product
 // ------------------------------------------------------------------------------------------
 
-// TM rows by TN columns of a workgroup, in waves of RM by RN, on MFMAs of side S; 64 elements of the sum a step,
-// STAGES steps' operands in LDS. A row's 128 bytes of a step lie as eight 16-byte chunks, chunk c of row r at
-// c ^ (r % 8): the rows that a product reads at one chunk then lie in different banks.
+// TM rows by TN columns of a workgroup, in waves of RM by RN, on 16x16x32 MFMAs (on 32x32x16 ones 2048 rows of 6144
+// over 2560 took 72 us where these took 56); BK elements of the sum a step, STAGES steps' operands in LDS, where
+// they come from memory without passing registers. Chunk c (16 bytes) of row r lies at c ^ (r % chunks): the rows that
+// a product reads at one chunk are in different banks then.
 template <int TM_, int TN_, int RM_, int RN_, int BK_, int STAGES_, bool STREAM_ = false>
 struct Shape {
     static constexpr bool STREAM = STREAM_;                          // W is read once, past the caches
-    static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, BK = BK_, S = 16, STAGES = STAGES_;
-    static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / S, NT = RN / S;
+    static constexpr int TM = TM_, TN = TN_, RM = RM_, RN = RN_, BK = BK_, STAGES = STAGES_;
+    static constexpr int WM = TM / RM, WN = TN / RN, WAVES = WM * WN, T = 64 * WAVES, MT = RM / 16, NT = RN / 16;
     static constexpr bool JOINS = TM <= 128;                         // also in front of join_kernel
     static constexpr int CHUNKS = BK / 8, ROW = 2 * BK, PER = 64 / CHUNKS;  // of a row: chunks, bytes; rows of a load
     static constexpr int BYTES = (TM + TN) * ROW;                    // of a stage
+    static_assert(TM <= T, "a thread per row looks up its owner");
     static_assert(!JOINS || STAGES * BYTES >= WAVES * 16 * 68 * 4, "low_part's sums");
     static constexpr int X_LOADS = (TM / PER + WAVES - 1) / WAVES;   // per wave, of PER rows; the last ones may be
     static constexpr int W_LOADS = (TN / PER + WAVES - 1) / WAVES;   // loaded more than once
@@ -339,7 +328,7 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     const bool join = l.part != nullptr, adapters = l.a && !l.low_groups && split == l.splits - 1;
     const bool owned = l.a && !l.low_groups;  // otherwise join_kernel looks them up
     if (owned && (int)threadIdx.x < G::TM)
-        owner[threadIdx.x] = m0 + (int)threadIdx.x < l.n_tokens ? gptr(l.owner)[m0 + threadIdx.x] : NO_SEQUENCE;
+        owner[threadIdx.x] = m0 + (int)threadIdx.x < l.n_tokens ? owner_of(l, m0 + threadIdx.x) : NO_SEQUENCE;
     if (threadIdx.x == 0) *unfit = *count = 0;
 
     // loads: lane's row and chunk of PER rows
@@ -444,24 +433,24 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
         of_adapter |= 1u << to;
         return true;
     };
-    typename Mfma<G::S>::Acc acc[G::MT][G::NT];
+    f32x4 acc[G::MT][G::NT];
     const int mine_m = wave % G::WM * G::RM, mine_n = wave / G::WM * G::RN;
-    constexpr int KS = G::BK / Mfma<G::S>::K;  // products of a step, on operands in alternating registers
+    constexpr int KS = G::BK / 32;  // products of a step, on operands in alternating registers
     static_assert(KS % 2 == 0, "registers alternate");
     u32x4 xf[2][G::MT], wf[2][G::NT];
     const auto fetch = [&](int from, int k) {
         const char *xs = lds + from * G::BYTES, *ws = xs + G::TM * G::ROW;
-        const int r = lane % G::S, slot = (k * (64 / G::S) + lane / G::S) ^ (r & (G::CHUNKS - 1));
+        const int r = lane % 16, slot = (k * 4 + lane / 16) ^ (r & (G::CHUNKS - 1));
 #pragma unroll
-        for (int i = 0; i < G::MT; i++) xf[k % 2][i] = *(const u32x4 *)(xs + (mine_m + i * G::S + r) * G::ROW + slot * 16);
+        for (int i = 0; i < G::MT; i++) xf[k % 2][i] = *(const u32x4 *)(xs + (mine_m + i * 16 + r) * G::ROW + slot * 16);
 #pragma unroll
-        for (int j = 0; j < G::NT; j++) wf[k % 2][j] = *(const u32x4 *)(ws + (mine_n + j * G::S + r) * G::ROW + slot * 16);
+        for (int j = 0; j < G::NT; j++) wf[k % 2][j] = *(const u32x4 *)(ws + (mine_n + j * 16 + r) * G::ROW + slot * 16);
     };
     const auto multiply = [&](int k) {
 #pragma unroll
         for (int i = 0; i < G::MT; i++)
 #pragma unroll
-            for (int j = 0; j < G::NT; j++) acc[i][j] = Mfma<G::S>::mul(wf[k % 2][j], xf[k % 2][i], acc[i][j]);
+            for (int j = 0; j < G::NT; j++) acc[i][j] = mfma(wf[k % 2][j], xf[k % 2][i], acc[i][j]);
     };
     // NaN and infinities of an adapter, times the zeros of other rows or a remainder of zero, would be no numbers
     // everywhere. Where there are some, which the largest exponent tells, the tile is computed again with zeros in
@@ -524,7 +513,7 @@ again:
             for (int n = i * G::LOADS / G::MT; n < (i + 1) * G::LOADS / G::MT; n++) load_whole(n, free);
 #pragma unroll
             for (int j = 0; j < G::NT; j++)
-                acc[i][j] = Mfma<G::S>::mul(wf[(KS - 1) % 2][j], xf[(KS - 1) % 2][i], acc[i][j]);
+                acc[i][j] = mfma(wf[(KS - 1) % 2][j], xf[(KS - 1) % 2][i], acc[i][j]);
             __builtin_amdgcn_sched_barrier(0);
         }
         step++;
@@ -568,21 +557,18 @@ again:
     // a lane has four columns side by side of a row
 #pragma unroll
     for (int i = 0; i < G::MT; i++) {
-        const int tile_row = mine_m + i * G::S + lane % G::S, m = m0 + tile_row;
+        const int tile_row = mine_m + i * 16 + lane % 16, m = m0 + tile_row;
         if (m >= l.n_tokens || (owned && owner[tile_row] == NO_SEQUENCE)) continue;
         bf16 *to = l.out + m * l.out_stride;
         const bf16 *res = l.residual + m * l.residual_stride;
         float *part = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width;
 #pragma unroll
-        for (int j = 0; j < G::NT; j++)
-#pragma unroll
-            for (int r = 0; r < Mfma<G::S>::REGS / 4; r++) {
-                const int n = n0 + mine_n + j * G::S + Mfma<G::S>::row(r, lane);
-                if (n >= l.n_out) continue;
-                const f32x4 y = {acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-                if (join) *gptr((f32x4 *)(part + n)) = y;
-                else store4(l, to + n, res + n, y, n);
-            }
+        for (int j = 0; j < G::NT; j++) {
+            const int n = n0 + mine_n + j * 16 + lane / 16 * 4;
+            if (n >= l.n_out) continue;
+            if (join) *gptr((f32x4 *)(part + n)) = acc[i][j];
+            else store4(l, to + n, res + n, acc[i][j], n);
+        }
     }
     if (clear) {  // the infinities and NaN, behind what was written
         __syncthreads();
@@ -606,7 +592,7 @@ __global__ __launch_bounds__(256) void sum_kernel(LoraArgs l) {
     const int per = l.part_width / 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int m = (int)(i / per), n = (int)(i % per) * 4;
-    if (m >= l.n_tokens || (l.a && gptr(l.owner)[m] == NO_SEQUENCE)) return;
+    if (m >= l.n_tokens || (l.a && owner_of(l, m) == NO_SEQUENCE)) return;
     const float *part = l.part + (int64_t)m * l.part_width + n;
     const int64_t next = (int64_t)l.n_tokens * l.part_width;
     f32x4 y = {0, 0, 0, 0};
@@ -754,8 +740,8 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     unfit |= clear_unfit_of(v[u][j]);
-                    acc[j] = Mfma<16>::mul(v[u][j], value, acc[j]);
-                    acc[j] = Mfma<16>::mul(v[u][j], rest, acc[j]);
+                    acc[j] = mfma(v[u][j], value, acc[j]);
+                    acc[j] = mfma(v[u][j], rest, acc[j]);
                 }
             }
         }
@@ -802,10 +788,15 @@ constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 constexpr int MOST_SPLITS = 32;
 constexpr size_t MOST_PART = 1 << 23;  // floats
 
+// For tests: a plan that is taken wherever it can be.
+struct {
+    int shape = -1, splits, join;
+} g_forced;
+
 // How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the
 // product, or join_kernel's. The least of an estimate fitted to 101 calls (1 to 4079 rows, 1 to 128 sequences, ranks of 8
-// to 128, 500 to 151936 columns), each in every shape and many splits: what it chooses takes 3% longer on average
-// than the best of those, at most 29%.
+// to 128, 500 to 151936 columns), each in every shape and many splits: what it chooses takes 4% longer on average
+// than the best of those, at most 30%.
 struct Plan {
     int shape, splits, split_steps;
     bool join;
@@ -830,6 +821,8 @@ struct Plan {
             const double tile = std::min<double>(s.tm, rows), even = std::min<double>(n_adapters, 1 + seqs * tile / rows);
             return pieces * sqrt(even * std::min({(double)n_adapters, seqs, tile}));
         };
+        // join_kernel's workgroups, most of which find nothing where most sequences are empty
+        const bool joins = adapters && (rows / 16 + seqs) * ceil(n_out / 256.0) < 1 << 23;
         double least = 0;
         shape = -1;
         for (int i = 0; i < SHAPES; i++) {
@@ -843,13 +836,19 @@ struct Plan {
                 const double cost = 2100 + std::max(rounds * (each + own_steps(s)) * step, memory) + rounds * s.fixed +
                                     (n > 1 ? 3400 + parts / 8900 : one * 2 / 9100) + (adapters ? 9200 + low / 9700 : 0);
                 if (shape < 0 || cost < least) shape = i, splits = n, join = false, least = cost;
-                if (!adapters || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
+                if (!joins || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
                 const double product_cost = product ? std::max(rounds * each * step, memory) + rounds * s.fixed : 0;
                 const int at_once = n_tokens <= n_seqs ? 8 : 4;  // parts that the join has under way
                 const double joined = 2100 + product_cost + 4500 + 1140 * ceil((double)n / at_once) + parts / 6000 + b / 7800 +
                                       low16 / 9700;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
             }
+        }
+        if (g_forced.shape >= 0) {
+            shape = g_forced.shape;
+            join = g_forced.join && joins && PACES[shape].tm <= 128;
+            splits = std::max(1, std::min(g_forced.splits, steps));
+            if (splits * one > (double)MOST_PART) splits = 1, join = join && (one <= (double)MOST_PART || !product);
         }
         // the last split has the adapters' steps
         const double own = join ? 0 : own_steps(PACES[shape]);
@@ -886,6 +885,13 @@ size_t low_floats(int n_tokens, int n_in, int rank) { return (size_t)n_tokens * 
 size_t owner_floats(int n_tokens, int rank) { return rank ? ((size_t)n_tokens + 3) / 4 * 4 : 0; }
 
 }  // namespace
+
+extern "C" int llm_lora_force(int shape, int splits, int join) {
+    g_forced.shape = shape < SHAPES ? shape : -1;
+    g_forced.splits = splits;
+    g_forced.join = join;
+    return SHAPES;
+}
 
 extern "C" size_t lora_projection_workspace_floats(int n_tokens, int n_out, int n_in, int rank) {
     if (!check_sizes("lora_projection_workspace_floats", n_tokens, n_out, n_in, rank)) return 0;

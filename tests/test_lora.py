@@ -489,3 +489,78 @@ def test_raw_bits_and_the_general_way_give_the_same(gpu, monkeypatch):
                 m.setattr(gpu, "_native", None)
             for form in (c, raw):
                 assert torch.equal(run(gpu, form, torch.full_like(want, 7.0)), want)
+
+
+@pytest.fixture
+def force(gpu):
+    """force(shape, splits, join): the plan of the calls until the test ends. The number of shapes."""
+    L = gpu.lib()
+    yield L.llm_lora_force
+    L.llm_lora_force(-1, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", range(9))
+@pytest.mark.parametrize("splits", [1, 2, 7])
+@pytest.mark.parametrize("join", [False, True])
+def test_every_way_to_compute(gpu, force, shape, splits, join):
+    """Every tile with and without splits, its adapters as steps of the product or joined: ragged rows and columns, sums
+    that end within a step, fewer steps than stages, no product, no adapters."""
+    import torch
+    assert force(shape, splits, int(join)) == 9
+    for n_in, n_out, lengths, rank, spare in [(136, 270, [3, 1, 0, 300, 1, 1, 40], 24, 3), (8, 1, [5, 17], 8, 0),
+                                              (1000, 515, [1] * 70 + [2, 3, 4], 40, 0), (512, 192, [257], 128, 1),
+                                              (72, 1030, [600, 600], 16, 0)]:
+        for kw in (dict(residual=True), dict(product=False), dict(adapters=0)):
+            c = make(n_in + len(lengths), lengths, n_in, n_out, rank, **dict(dict(adapters=5), **kw), spare=spare)
+            both(gpu, c, n_out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", range(9))
+@pytest.mark.parametrize("splits,join", [(1, 0), (3, 0), (1, 1), (3, 1)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_no_number_of_an_adapter_in_every_way(gpu, force, shape, splits, join, bad):
+    """Elements of an adapter's b that are no numbers, in each way to compute: only the rows of its sequences, in their
+    columns; infinities of the right sign also where the low product is a bf16 exactly, so that its remainder is zero."""
+    import torch
+    force(shape, splits, join)
+    lengths, which = [40, 1, 1, 90, 2, 1, 30], [0, 1, 2, 1, -1, 3, 2]
+    c = make(21, lengths, 200, 280, 16, adapters=4, which=which, residual=True, spare=2, scale=False)
+    clean = {k: v if v is None else v.clone() for k, v in c.items()}
+    c["lora_b"][1, 33, 5] = bad
+    c["lora_b"][1, 279, 15] = bad
+    c["lora_a"][1, 5].zero_()
+    c["lora_a"][1, 5, 0] = 1.0
+    c["x"][:, 0] = 3.0  # low[5] is 3
+    clean["lora_a"], clean["x"] = c["lora_a"], c["x"]
+    clean["lora_b"][1, 33, 5] = clean["lora_b"][1, 279, 15] = 0
+    out = torch.full((c["x"].shape[0], 280), 7.0, device="cuda", dtype=torch.bfloat16)
+    run(gpu, c, out)
+    touched = torch.zeros(out.shape, dtype=torch.bool, device="cuda")
+    starts = c["q_start"].tolist()
+    for s, a in enumerate(which):
+        if a == 1:
+            touched[starts[s]:starts[s + 1], [33, 279]] = True
+            if not math.isnan(bad):
+                assert (out[starts[s]:starts[s + 1], 33] == bad).all()
+    assert not out[touched].isfinite().any()
+    want, err, written = defined(clean, *out.shape)
+    fine = written[:, None] & ~touched
+    off = (out.double() - want).abs() - (HALF_STEP * (want.abs() + err) + err)
+    assert (off[fine] <= 0).all() and (out[~written] == 7).all()
+
+
+@pytest.mark.gpu
+def test_starts_that_decrease_stay_within_the_rows(gpu, force):
+    """What the documentation does not allow reads and writes nothing outside of the call's tensors: rows of
+    sequences that do not overlap are right, whatever the others hold."""
+    import torch
+    for shape, join in ((4, 0), (4, 1), (8, 1), (0, 0)):
+        force(shape, 2, join)
+        c = make(22, [60], 128, 192, 8, adapters=3)
+        c["q_start"] = torch.tensor([0, 20, 10, 55, 2 ** 31 - 1, -5, 60], dtype=torch.int32, device="cuda")
+        c["adapter"] = torch.tensor([0, 1, 2, 0, 1, 2], dtype=torch.int32, device="cuda")
+        wide = torch.full((64, 200), 7.0, device="cuda", dtype=torch.bfloat16)
+        run(gpu, c, wide[2:62, 4:196])
+        assert (wide[:2] == 7).all() and (wide[62:] == 7).all() and (wide[:, :4] == 7).all() and (wide[:, 196:] == 7).all()
