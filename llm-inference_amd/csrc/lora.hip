@@ -43,7 +43,7 @@ struct LoraArgs {
     int splits, split_steps;  // of the product's sum, steps of 64 each
     int m_tiles, n_tiles;
     int low_groups, low_splits;  // workgroups behind the product's that compute low_part; its parts
-    bool wide;               // out and residual take 8 bytes at a time
+    int wide;                // elements of out and residual that lie in aligned memory from each multiple of it on: 8, 4, 1
 };
 
 // What is loaded for places past an operand's end.
@@ -255,7 +255,7 @@ __global__ __launch_bounds__(256) void low_sum_kernel(LoraArgs l) {
 
 // Four columns of a row, with the residual's.
 __device__ __forceinline__ void store4(const LoraArgs &l, bf16 *to, const bf16 *res, f32x4 y, int n) {
-    if (l.wide && n + 4 <= l.n_out) {
+    if (l.wide >= 4 && n + 4 <= l.n_out) {
         if (l.residual) {
             const u32x2 v = *gptr((const u32x2 *)res);
             y += f32x4{lo_f(v.x), hi_f(v.x), lo_f(v.y), hi_f(v.y)};
@@ -265,6 +265,23 @@ __device__ __forceinline__ void store4(const LoraArgs &l, bf16 *to, const bf16 *
 #pragma unroll
         for (int e = 0; e < 4; e++)
             if (n + e < l.n_out) gptr(to)[e] = (bf16)f2bf(y[e] + (l.residual ? bf2f(gptr(res)[e]) : 0.0f));
+    }
+}
+
+// Eight columns of a row, past the caches: eight lanes side by side write whole lines so. 2582 rows of 9728 over 2560
+// take 135 us with such stores, 166 with four columns a lane of 16 rows at a time, through the caches (157 past them), and
+// 161 with whole lines through the caches; 64 rows of 151936 148, 158, 156 and 156.
+__device__ __forceinline__ void store8(const LoraArgs &l, bf16 *to, const bf16 *res, f32x4 y, f32x4 z, int n) {
+    if (l.wide == 8 && n + 8 <= l.n_out) {
+        if (l.residual) {
+            const u32x4 v = *(gptr((const u32x4 *)res));
+            y += f32x4{lo_f(v[0]), hi_f(v[0]), lo_f(v[1]), hi_f(v[1])};
+            z += f32x4{lo_f(v[2]), hi_f(v[2]), lo_f(v[3]), hi_f(v[3])};
+        }
+        __builtin_nontemporal_store((u32x4{pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(z[0], z[1]), pack2(z[2], z[3])}), gptr((u32x4 *)to));
+    } else {
+        store4(l, to, res, y, n);
+        if (n + 4 < l.n_out) store4(l, to + 4, res + 4, z, n + 4);
     }
 }
 
@@ -307,7 +324,10 @@ struct Shape {
     static constexpr int CHUNKS = BK / 8, ROW = 2 * BK, PER = 64 / CHUNKS;  // of a row: chunks, bytes; rows of a load
     static constexpr int BYTES = (TM + TN) * ROW;                    // of a stage
     static_assert(TM <= T, "a thread per row looks up its owner");
-    static_assert(!JOINS || STAGES * BYTES >= WAVES * 16 * 68 * 4, "low_part's sums");
+    // rows of low_part beside it, whose sums are in LDS: 64 where a workgroup has a CU to itself and there are many rows
+    // (924 rows of 2560 over 9728, of 22 sequences: 82 us, with 16 rows 87)
+    static constexpr int LOW_ROWS = TM == 128 && TN == 256 ? 64 : 16;
+    static_assert(!JOINS || STAGES * BYTES >= WAVES * LOW_ROWS * 68 * 4, "low_part's sums");
     static constexpr int X_LOADS = (TM / PER + WAVES - 1) / WAVES;   // per wave, of PER rows; the last ones may be
     static constexpr int W_LOADS = (TN / PER + WAVES - 1) / WAVES;   // loaded more than once
     static constexpr int LOADS = X_LOADS + W_LOADS;
@@ -319,7 +339,7 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     int *owner = (int *)(lds + G::STAGES * G::BYTES), *list = owner + G::TM, *count = list + G::TM, *unfit = count + 1;
     const int lane = threadIdx.x & 63, wave = wave_id();
     if (G::JOINS && (int)blockIdx.x >= l.m_tiles * l.n_tiles * l.splits)
-        return low_part<16, G::WAVES, JOIN_LOW_SPAN / G::WAVES>(l, blockIdx.x - l.m_tiles * l.n_tiles * l.splits, (float *)lds);
+        return low_part<G::LOW_ROWS, G::WAVES, JOIN_LOW_SPAN / G::WAVES>(l, blockIdx.x - l.m_tiles * l.n_tiles * l.splits, (float *)lds);
     // the tiles of one XCD, whose workgroups every eighth one is, lie side by side
     const int tiles = l.m_tiles * l.n_tiles * l.splits, block = blockIdx.x;
     const int each = tiles / XCDS, more = tiles % XCDS, xcd = block % XCDS;
@@ -554,21 +574,36 @@ again:
         }
     }
 
-    // a lane has four columns side by side of a row
+    // parts from the registers, a lane having four columns side by side of a row; out through LDS, a wave's 16 rows at a
+    // time, so that what goes out is whole lines
+    constexpr int PITCH = G::RN + 4, EIGHTS = G::RN / 8;
+    static_assert(G::WAVES * 16 * PITCH * 4 <= G::STAGES * G::BYTES, "rows on their way out");
+    float *rows = (float *)lds + wave * 16 * PITCH;
 #pragma unroll
     for (int i = 0; i < G::MT; i++) {
-        const int tile_row = mine_m + i * 16 + lane % 16, m = m0 + tile_row;
-        if (m >= l.n_tokens || (owned && owner[tile_row] == NO_SEQUENCE)) continue;
-        bf16 *to = l.out + m * l.out_stride;
-        const bf16 *res = l.residual + m * l.residual_stride;
-        float *part = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width;
+        if (join) {
+            const int m = m0 + mine_m + i * 16 + lane % 16;
+            if (m >= l.n_tokens) continue;
+            float *part = l.part + ((int64_t)split * l.n_tokens + m) * l.part_width;
 #pragma unroll
-        for (int j = 0; j < G::NT; j++) {
-            const int n = n0 + mine_n + j * 16 + lane / 16 * 4;
-            if (n >= l.n_out) continue;
-            if (join) *gptr((f32x4 *)(part + n)) = acc[i][j];
-            else store4(l, to + n, res + n, acc[i][j], n);
+            for (int j = 0; j < G::NT; j++) {
+                const int n = n0 + mine_n + j * 16 + lane / 16 * 4;
+                if (n < l.n_out) *gptr((f32x4 *)(part + n)) = acc[i][j];
+            }
+            continue;
         }
+#pragma unroll
+        for (int j = 0; j < G::NT; j++) *(f32x4 *)(rows + lane % 16 * PITCH + j * 16 + lane / 16 * 4) = acc[i][j];
+        wait_lds();
+#pragma unroll
+        for (int p = lane; p < 16 * EIGHTS; p += 64) {
+            const int tile_row = mine_m + i * 16 + p / EIGHTS, m = m0 + tile_row, c = p % EIGHTS * 8, n = n0 + mine_n + c;
+            if (m >= l.n_tokens || (owned && owner[tile_row] == NO_SEQUENCE) || n >= l.n_out) continue;
+            const float *from = rows + p / EIGHTS * PITCH + c;
+            store8(l, l.out + m * l.out_stride + n, l.residual + m * l.residual_stride + n, *(const f32x4 *)from,
+                   *(const f32x4 *)(from + 4), n);
+        }
+        wait_lds();
     }
     if (clear) {  // the infinities and NaN, behind what was written
         __syncthreads();
@@ -676,7 +711,8 @@ __device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, in
 }
 
 __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
-    __shared__ __attribute__((aligned(16))) float low[16 * 256];
+    constexpr int PITCH = 64 + 4;
+    __shared__ __attribute__((aligned(16))) float low[16 * 256], lines[4 * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = wave_id();
     const RowTile t = row_tile<16>(l, blockIdx.x);
     if (t.rows == 0) return;
@@ -747,17 +783,26 @@ __global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
         }
     }
     unfit = __any(unfit);
-    if (lane % 16 >= t.rows) return;
+    // a wave's rows through LDS, so that what goes out is whole lines
+    float *rows = lines + wave * 16 * PITCH;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int n = n0 + j * 16 + lane / 16 * 4;
-        if (n >= l.n_out) break;
         y[j] += acc[j];
-        if (unfit)
+        if (unfit && lane % 16 < t.rows)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (n + e < l.n_out) y[j][e] += unfit_term(l, n + e, t.adapter, [&](int i) { return low[mine * l.rank + i]; });
-        store4(l, l.out + m * l.out_stride + n, l.residual + m * l.residual_stride + n, y[j], n);
+        *(f32x4 *)(rows + lane % 16 * PITCH + j * 16 + lane / 16 * 4) = y[j];
+    }
+    wait_lds();
+#pragma unroll
+    for (int p = lane; p < 16 * 8; p += 64) {
+        const int i = p / 8, c = p % 8 * 8, n = n0 + c;
+        if (i >= t.rows || n >= l.n_out) continue;
+        const float *from = rows + i * PITCH + c;
+        store8(l, l.out + (t.first + i) * l.out_stride + n, l.residual + (t.first + i) * l.residual_stride + n,
+               *(const f32x4 *)from, *(const f32x4 *)(from + 4), n);
     }
 }
 
@@ -783,6 +828,8 @@ typedef Shape<16, 64, 16, 16, 64, 4, true> Few16;
 constexpr Pace PACES[] = {{256, 192, 1, 900, 1250, 8600}, {224, 256, 1, 1070, 1340, 8900}, {192, 256, 1, 980, 1150, 9200},
                           {128, 256, 1, 630, 770, 5600},  {128, 128, 2, 560, 810, 4800},   {64, 128, 2, 420, 620, 2500},
                           {64, 64, 2, 430, 280, 3000},    {32, 64, 3, 330, 350, 2200},     {16, 64, 3, 290, 280, 1900}};
+constexpr int LOW_ROWS_BESIDE[] = {Wide::LOW_ROWS,    High::LOW_ROWS,   Square::LOW_ROWS, Half::LOW_ROWS, Quarter::LOW_ROWS,
+                                   Few128::LOW_ROWS, Few64::LOW_ROWS, Few32::LOW_ROWS,  Few16::LOW_ROWS};
 constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 
 constexpr int MOST_SPLITS = 32;
@@ -951,19 +998,21 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     l.n_tokens = n_tokens, l.n_out = n_out, l.n_in = n_in;
     l.part_width = (n_out + 3) / 4 * 4;
     l.splits = p.splits, l.split_steps = p.split_steps;
-    l.wide = out_stride % 4 == 0 && (uintptr_t)out % 8 == 0 &&
-             (!residual || (residual_stride % 4 == 0 && (uintptr_t)residual % 8 == 0));
+    const auto aligned = [&](int n) {
+        return out_stride % n == 0 && (uintptr_t)out % (2 * n) == 0 &&
+               (!residual || (residual_stride % n == 0 && (uintptr_t)residual % (2 * n) == 0));
+    };
+    l.wide = aligned(8) ? 8 : aligned(4) ? 4 : 1;
     l.low = (bf16 *)ws;
     l.low_part = ws + (size_t)n_tokens * rank;
     l.low_splits = p.join ? (n_in + JOIN_LOW_SPAN - 1) / JOIN_LOW_SPAN : low_splits(n_in);
     l.owner = (int *)(ws + low_floats(n_tokens, n_in, rank));
     if (p.splits > 1 || p.join) l.part = ws + low_floats(n_tokens, n_in, rank) + owner_floats(n_tokens, rank);
-    int tiles = 0;
     if (lora) {
         l.a = lora->a, l.b = lora->b, l.scale = lora->scale, l.q_start = lora->q_start, l.adapter = lora->adapter;
         l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = rank;
-        tiles = n_tokens / (p.join ? 16 : LOW_ROWS) + lora->n_seqs;
-        const int64_t groups = (int64_t)tiles * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
+        const int low_rows = p.join ? LOW_ROWS_BESIDE[p.shape] : LOW_ROWS;
+        const int64_t groups = (int64_t)(n_tokens / low_rows + lora->n_seqs) * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
         if (groups >= 1 << 23) {  // the threads of a launch
             llm_fail("%s: %d sequences of rank %d over n_in %d are too many for one launch", name, lora->n_seqs, rank, n_in);
             return;
@@ -990,7 +1039,7 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     default: ok = launch_product<Few16>(name, l, stream);
     }
     if (!ok) return;
-    if (p.join) join_kernel<<<dim3(tiles, (n_out + 255) / 256), 256, 0, stream>>>(l);
+    if (p.join) join_kernel<<<dim3(n_tokens / 16 + lora->n_seqs, (n_out + 255) / 256), 256, 0, stream>>>(l);
     else if (p.splits > 1) sum_kernel<<<((int64_t)n_tokens * (l.part_width / 4) + 255) / 256, 256, 0, stream>>>(l);
     LAUNCH_OK();
 }
