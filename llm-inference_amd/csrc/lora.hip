@@ -825,9 +825,9 @@ typedef Shape<64, 128, 64, 32, 64, 3, true> Few128;
 typedef Shape<64, 64, 64, 16, 64, 4, true> Few64;
 typedef Shape<32, 64, 32, 16, 64, 4, true> Few32;
 typedef Shape<16, 64, 16, 16, 64, 4, true> Few16;
-constexpr Pace PACES[] = {{256, 192, 1, 900, 1250, 8600}, {224, 256, 1, 1070, 1340, 8900}, {192, 256, 1, 980, 1150, 9200},
-                          {128, 256, 1, 630, 770, 5600},  {128, 128, 2, 560, 810, 4800},   {64, 128, 2, 420, 620, 2500},
-                          {64, 64, 2, 430, 280, 3000},    {32, 64, 3, 330, 350, 2200},     {16, 64, 3, 290, 280, 1900}};
+constexpr Pace PACES[] = {{256, 192, 1, 920, 1380, 5800}, {224, 256, 1, 970, 1450, 5900}, {192, 256, 1, 960, 1220, 6100},
+                          {128, 256, 1, 650, 720, 3900},  {128, 128, 2, 520, 740, 3900},  {64, 128, 2, 440, 610, 1900},
+                          {64, 64, 2, 460, 250, 2400},    {32, 64, 3, 310, 280, 2100},    {16, 64, 3, 270, 230, 1700}};
 constexpr int LOW_ROWS_BESIDE[] = {Wide::LOW_ROWS,    High::LOW_ROWS,   Square::LOW_ROWS, Half::LOW_ROWS, Quarter::LOW_ROWS,
                                    Few128::LOW_ROWS, Few64::LOW_ROWS, Few32::LOW_ROWS,  Few16::LOW_ROWS};
 constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
@@ -841,9 +841,9 @@ struct {
 } g_forced;
 
 // How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the
-// product, or join_kernel's. The least of an estimate fitted to 101 calls (1 to 4079 rows, 1 to 128 sequences, ranks of 8
+// product, or join_kernel's. The least of an estimate fitted to 107 calls (1 to 4079 rows, 1 to 128 sequences, ranks of 8
 // to 128, 500 to 151936 columns), each in every shape and many splits: what it chooses takes 4% longer on average
-// than the best of those, at most 30%.
+// than the best of those, at most 29%.
 struct Plan {
     int shape, splits, split_steps;
     bool join;
@@ -857,9 +857,8 @@ struct Plan {
     Plan(int n_tokens, int n_out, int n_in, bool product, bool adapters, int rank, int n_seqs, int n_adapters) {
         const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
         const double rows = n_tokens, seqs = n_seqs, one = (double)part_floats(n_tokens, n_out);
-        // bytes of low's operands with tiles of 64 rows and of 16, and of b with the latter
-        const double low = adapters ? (std::min(rows, rows / LOW_ROWS + seqs) * rank + rows) * n_in * 2 : 0;
-        const double low16 = adapters ? (std::min(rows, rows / 16 + seqs) * rank + rows) * n_in * 2 : 0;
+        // bytes of low's operands with tiles of so many rows, and of b with tiles of 16
+        const auto low = [&](int tile) { return adapters ? (std::min(rows, rows / tile + seqs) * rank + rows) * n_in * 2 : 0; };
         const double b = adapters ? std::min(rows, rows / 16 + seqs) * n_out * rank * 2 : 0;
         // adapters of a tile's rows, each with steps of its own: between those of sequences of one length, and as many
         // as there can be, where the short ones lie side by side
@@ -875,19 +874,22 @@ struct Plan {
         for (int i = 0; i < SHAPES; i++) {
             const Pace &s = PACES[i];
             const double m_tiles = ceil(rows / s.tm), tiles = m_tiles * ceil((double)n_out / s.tn);
-            const double again = s.tm <= 64 ? 0.6 * std::min(m_tiles - 1, 8.0) : 0;  // W past the caches, for more rows
-            const double memory = product ? 2.0 * n_out * n_in * (1 + again) / 5100 : 0;
+            const double again = s.tm <= 64 ? 0.63 * std::min(m_tiles - 1, 8.0) : 0;  // W past the caches, for more rows
+            const double memory = product ? 2.0 * n_out * n_in * (1 + again) / 5770 : 0;
             for (int n = 1; n <= std::min(MOST_SPLITS, std::max(steps, 1)) && (n == 1 || n * one <= (double)MOST_PART); n++) {
                 const double groups = tiles * n, step = s.alone + (s.full - s.alone) * std::min(1.0, groups / CUS);
                 const double rounds = ceil(groups / (s.at_once * CUS)), each = (steps + n - 1) / n, parts = one * (8 * n + 4);
-                const double cost = 2100 + std::max(rounds * (each + own_steps(s)) * step, memory) + rounds * s.fixed +
-                                    (n > 1 ? 3400 + parts / 8900 : one * 2 / 9100) + (adapters ? 9200 + low / 9700 : 0);
+                const double own = own_steps(s), rest = rounds * s.fixed;
+                const double product_cost = product ? std::max(rounds * each * step, memory) : 0;
+                const double cost = 1930 + product_cost + rounds * own * step + rest +
+                                    (n > 1 ? 3010 + parts / 9350 : one * 2 / 9030) + (adapters ? 11100 + low(LOW_ROWS) / 8570 : 0);
                 if (shape < 0 || cost < least) shape = i, splits = n, join = false, least = cost;
                 if (!joins || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
-                const double product_cost = product ? std::max(rounds * each * step, memory) + rounds * s.fixed : 0;
+                // without a product smaller tiles of low (128 rows of 4096, rank 16: 15 us, with 64 rows 17)
+                if (!product && LOW_ROWS_BESIDE[i] > 16) continue;
                 const int at_once = n_tokens <= n_seqs ? 8 : 4;  // parts that the join has under way
-                const double joined = 2100 + product_cost + 4500 + 1140 * ceil((double)n / at_once) + parts / 6000 + b / 7800 +
-                                      low16 / 9700;
+                const double joined = 1930 + product_cost + (product ? rest : 0) + 4500 + 1270 * ceil((double)n / at_once) +
+                                      parts / 4960 + b / 7670 + low(LOW_ROWS_BESIDE[i]) / 8570;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
             }
         }
