@@ -3,6 +3,15 @@
 // out = x Wt + low Bt, low = scale x At: the second term is the first one's sum carried on over the rank, with rows
 // of `low` for rows of x and an adapter's b for W. low is kept as two bf16, the value and what that leaves (16 bits
 // of mantissa), side by side, so the sum goes over twice the rank.
+//
+// A call takes one of three ways, by the estimate in Plan:
+//   many rows, where the product's operations count: low, then one product whose last steps are the adapters';
+//   few rows, where W's bytes and the launches count: parts of the product's sum and, in the same launch behind them,
+//   of low's; then join_kernel adds the parts up, with b's product and the residual;
+//   without adapters: the product, and sum_kernel where its sum is split.
+// 64 rows of 4096 over 2560, each with one of 48 adapters of rank 16, take 16.8 us (the product alone, from a library:
+// 19.3), 2582 rows of five prompts of 9728 over 2560, rank 32, 136 (115), 924 rows of 22 sequences of 2560 over 9728,
+// rank 64, 82 (66).
 #include <math.h>
 
 #include <algorithm>
@@ -203,6 +212,8 @@ __device__ __forceinline__ void low_part(const LoraArgs &l, int block, float *ld
     else sum(std::integral_constant<int, R / 16>{});
 }
 
+// Bound by its round trips, launch, starts, operands: 10 us for 2582 rows over 2560 and rank 32, 13 MB of x. (Unsplit, with
+// sixteen waves a sum and low_sum_kernel's work at its end, a call took as long or, at rank 128, 5 us longer.)
 // Elements of the sum per workgroup: of 64 rows so few that the workgroups fill the CUs, of 16 beside the product more,
 // for fewer parts to add up.
 constexpr int LOW_WAVES = 4, LOW_ROWS = 64, LOW_SPAN = 512, JOIN_LOW_SPAN = 1024;
@@ -333,6 +344,11 @@ struct Shape {
     static constexpr int LOADS = X_LOADS + W_LOADS;
 };
 
+// Large tiles are bound by the card's power: 2582 rows of 9728 over 2560 take 118 us, 1.09 PFLOP/s (a library product of
+// 8192 x 8192 x 8192: 1.40). Each step's operands come from LDS while the step before it is multiplied, and the loads of
+// the step behind the stages go between the products; an XCD has tiles side by side, which share operands in its L2.
+// Tiles of up to 64 rows are bound by W: 64 rows of 151936 over 2560 at 5.4 TB/s, which neither longer steps,
+// more stages, another order of tiles nor another start of each tile's sum changes.
 template <class G>
 __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
     __shared__ __attribute__((aligned(128))) char lds[G::STAGES * G::BYTES + G::TM * 8 + 8];
@@ -622,7 +638,7 @@ again:
     }
 }
 
-// out of the product's parts: four columns of a row per thread.
+// out of the product's parts, in their order: four columns of a row per thread. Bound by their bytes.
 __global__ __launch_bounds__(256) void sum_kernel(LoraArgs l) {
     const int per = l.part_width / 4;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -647,7 +663,8 @@ __global__ __launch_bounds__(256) void sum_kernel(LoraArgs l) {
 // the join: the product's parts, the adapters' terms and the residual
 // ------------------------------------------------------------------------------------------
 
-// 16 rows of a sequence by 256 columns per workgroup. What the lanes read besides the parts of low is requested in
+// 16 rows of a sequence by 256 columns per workgroup. Bound by its round trips for few rows (7 us for 64 rows of 4096), by
+// the parts' and b's bytes for many (924 rows of 2560, three parts, rank 64: 19 us, 3.8 TB/s). What the lanes read besides the parts of low is requested in
 // front of those, so that all of it comes in one round trip behind the lookup of the rows.
 constexpr int FEW = 4;      // rows up to which a lane has a column, and the sum over the rank is one of vector operations
 

@@ -4,6 +4,10 @@
 // values: weight and count of each, in the order of the values. Weights and sums are in 64 bits: a pick falls on
 // the other side of a token's edge where the sums differ by more than what lies between u and the edge, and with
 // sums in 32 bits that happened to one row in a few hundred.
+//
+// Bound by what a workgroup does one after the other, not by bytes: for one row of 151936 (22 us in two launches) 7 us
+// for the slices' lists and 16 to merge and draw, of which clearing the counts takes 0.8, the weights and their sums 3, each
+// filter about 1 and the search for the token 2 to 3. 64 such rows take 31 us, 200 rows of 32003 in one launch 18.
 #include <math.h>
 
 #include <algorithm>
