@@ -9,7 +9,7 @@
 //   few rows, where W's bytes and the launches count: parts of the product's sum and, in the same launch behind them,
 //   of low's; then join_kernel adds the parts up, with b's product and the residual;
 //   without adapters: the product, and sum_kernel where its sum is split.
-// 64 rows of 4096 over 2560, each with one of 48 adapters of rank 16, take 16.8 us (the product alone, from a library:
+// 64 rows of 4096 over 2560, each with one of 48 adapters of rank 16, take 14 us (the product alone, from a library:
 // 19.3), 2582 rows of five prompts of 9728 over 2560, rank 32, 136 (115), 924 rows of 22 sequences of 2560 over 9728,
 // rank 64, 82 (66).
 #include <math.h>
@@ -663,7 +663,7 @@ __global__ __launch_bounds__(256) void sum_kernel(LoraArgs l) {
 // the join: the product's parts, the adapters' terms and the residual
 // ------------------------------------------------------------------------------------------
 
-// 16 rows of a sequence by 256 columns per workgroup. Bound by its round trips for few rows (7 us for 64 rows of 4096), by
+// 16 rows of a sequence by 256 columns per workgroup. Bound by its round trips for few rows (5 us for 64 rows of 4096), by
 // the parts' and b's bytes for many (924 rows of 2560, three parts, rank 64: 19 us, 3.8 TB/s). What the lanes read besides the parts of low is requested in
 // front of those, so that all of it comes in one round trip behind the lookup of the rows.
 constexpr int FEW = 4;      // rows up to which a lane has a column, and the sum over the rank is one of vector operations
@@ -727,15 +727,18 @@ __device__ __forceinline__ void join_few(const LoraArgs &l, const RowTile &t, in
             if (i < t.rows) gptr(l.out)[(t.first + i) * l.out_stride + n] = (bf16)f2bf(y[i]);
 }
 
-__global__ __launch_bounds__(256) void join_kernel(LoraArgs l) {
+// R: rows of a tile at most, FEW or 16. Tiles of few rows are bound by their round trips, so by how many workgroups a CU
+// takes at once: with a kernel of their own, six (three where all tiles shared one), 64 single tokens take 14 us (16.6).
+template <int R>
+__global__ __launch_bounds__(256, R == FEW ? 6 : 3) void join_kernel(LoraArgs l) {
     constexpr int PITCH = 64 + 4;
-    __shared__ __attribute__((aligned(16))) float low[16 * 256], lines[4 * 16 * PITCH];
+    __shared__ __attribute__((aligned(16))) float low[R * 256], lines[R == FEW ? 1 : 4 * 16 * PITCH];
     const int lane = threadIdx.x & 63, wave = wave_id();
-    const RowTile t = row_tile<16>(l, blockIdx.x);
+    const RowTile t = row_tile<R>(l, blockIdx.x);
     if (t.rows == 0) return;
     const float scale = l.scale && t.adapter >= 0 ? gptr(l.scale)[t.adapter] : 1.0f;
     if (t.rows == 1) return join_few<1>(l, t, blockIdx.y * 256 + threadIdx.x, scale, low);
-    if (t.rows <= FEW) return join_few<FEW>(l, t, blockIdx.y * 256 + threadIdx.x, scale, low);
+    if (R == FEW || t.rows <= FEW) return join_few<FEW>(l, t, blockIdx.y * 256 + threadIdx.x, scale, low);
     // a lane has row lane % 16 and four columns of each 16
     const int n0 = (blockIdx.y * 4 + wave) * 64, mine = min(lane % 16, t.rows - 1), m = t.first + mine;
     const auto part_at = [&](int j, int s) {
@@ -857,6 +860,11 @@ struct {
     int shape = -1, splits, join;
 } g_forced;
 
+// Few rows in all or of each sequence, on average: join_kernel has tiles of FEW rows. 60 rows of one sequence, 4096 over 2560
+// and rank 16, take 15 us so and 19 with tiles of 16; 64 sequences of two rows 18 and 21; 120 rows of one, 6144 over 2560 and
+// rank 128, 32 and 30; 128 sequences of four, 2560 over 9728 and rank 64, 95 and 89.
+bool few_each(int n_tokens, int n_seqs) { return n_tokens <= std::max(128, 2 * n_seqs); }
+
 // How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the
 // product, or join_kernel's. The least of an estimate fitted to 107 calls (1 to 4079 rows, 1 to 128 sequences, ranks of 8
 // to 128, 500 to 151936 columns), each in every shape and many splits: what it chooses takes 4% longer on average
@@ -885,7 +893,7 @@ struct Plan {
             return pieces * sqrt(even * std::min({(double)n_adapters, seqs, tile}));
         };
         // join_kernel's workgroups, most of which find nothing where most sequences are empty
-        const bool joins = adapters && (rows / 16 + seqs) * ceil(n_out / 256.0) < 1 << 23;
+        const bool joins = adapters && (rows / (few_each(n_tokens, n_seqs) ? FEW : 16) + seqs) * ceil(n_out / 256.0) < 1 << 23;
         double least = 0;
         shape = -1;
         for (int i = 0; i < SHAPES; i++) {
@@ -904,7 +912,7 @@ struct Plan {
                 if (!joins || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
                 // without a product smaller tiles of low (128 rows of 4096, rank 16: 15 us, with 64 rows 17)
                 if (!product && LOW_ROWS_BESIDE[i] > 16) continue;
-                const int at_once = n_tokens <= n_seqs ? 8 : 4;  // parts that the join has under way
+                const int at_once = few_each(n_tokens, n_seqs) ? 8 : 4;  // parts that the join has under way
                 const double joined = 1930 + product_cost + (product ? rest : 0) + 4500 + 1270 * ceil((double)n / at_once) +
                                       parts / 4960 + b / 7670 + low(LOW_ROWS_BESIDE[i]) / 8570;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
@@ -1058,7 +1066,9 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     default: ok = launch_product<Few16>(name, l, stream);
     }
     if (!ok) return;
-    if (p.join) join_kernel<<<dim3(n_tokens / 16 + lora->n_seqs, (n_out + 255) / 256), 256, 0, stream>>>(l);
+    const int n_tiles = (n_out + 255) / 256;
+    if (p.join && few_each(n_tokens, lora->n_seqs)) join_kernel<FEW><<<dim3(n_tokens / FEW + lora->n_seqs, n_tiles), 256, 0, stream>>>(l);
+    else if (p.join) join_kernel<16><<<dim3(n_tokens / 16 + lora->n_seqs, n_tiles), 256, 0, stream>>>(l);
     else if (p.splits > 1) sum_kernel<<<((int64_t)n_tokens * (l.part_width / 4) + 255) / 256, 256, 0, stream>>>(l);
     LAUNCH_OK();
 }
