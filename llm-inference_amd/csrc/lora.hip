@@ -882,9 +882,10 @@ struct Plan {
     Plan(int n_tokens, int n_out, int n_in, bool product, bool adapters, int rank, int n_seqs, int n_adapters) {
         const int steps = product ? (n_in + 63) / 64 : 0, pieces = (2 * rank + 63) / 64;
         const double rows = n_tokens, seqs = n_seqs, one = (double)part_floats(n_tokens, n_out);
-        // bytes of low's operands with tiles of so many rows, and of b with tiles of 16
+        const bool few = few_each(n_tokens, n_seqs);
+        // bytes of low's operands with tiles of so many rows, and of b with join_kernel's
         const auto low = [&](int tile) { return adapters ? (std::min(rows, rows / tile + seqs) * rank + rows) * n_in * 2 : 0; };
-        const double b = adapters ? std::min(rows, rows / 16 + seqs) * n_out * rank * 2 : 0;
+        const double b = adapters ? std::min(rows, rows / (few ? FEW : 16) + seqs) * n_out * rank * 2 : 0;
         // adapters of a tile's rows, each with steps of its own: between those of sequences of one length, and as many
         // as there can be, where the short ones lie side by side
         const auto own_steps = [&](const Pace &s) {
@@ -893,7 +894,7 @@ struct Plan {
             return pieces * sqrt(even * std::min({(double)n_adapters, seqs, tile}));
         };
         // join_kernel's workgroups, most of which find nothing where most sequences are empty
-        const bool joins = adapters && (rows / (few_each(n_tokens, n_seqs) ? FEW : 16) + seqs) * ceil(n_out / 256.0) < 1 << 23;
+        const bool joins = adapters && (rows / (few ? FEW : 16) + seqs) * ceil(n_out / 256.0) < 1 << 23;
         double least = 0;
         shape = -1;
         for (int i = 0; i < SHAPES; i++) {
@@ -910,10 +911,9 @@ struct Plan {
                                     (n > 1 ? 3010 + parts / 9350 : one * 2 / 9030) + (adapters ? 11100 + low(LOW_ROWS) / 8570 : 0);
                 if (shape < 0 || cost < least) shape = i, splits = n, join = false, least = cost;
                 if (!joins || s.tm > 128 || (product && n * one > (double)MOST_PART)) continue;
-                // without a product smaller tiles of low (128 rows of 4096, rank 16: 15 us, with 64 rows 17)
-                if (!product && LOW_ROWS_BESIDE[i] > 16) continue;
-                const int at_once = few_each(n_tokens, n_seqs) ? 8 : 4;  // parts that the join has under way
-                const double joined = 1930 + product_cost + (product ? rest : 0) + 4500 + 1270 * ceil((double)n / at_once) +
+                if (!product && i < SHAPES - 1) continue;  // low alone: the smallest workgroups
+                const int at_once = few ? 8 : 4;  // parts that the join has under way
+                const double joined = 1930 + product_cost + (product ? rest : 0) + (few ? 3000 : 4500) + 1270 * ceil((double)n / at_once) +
                                       parts / 4960 + b / 7670 + low(LOW_ROWS_BESIDE[i]) / 8570;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
             }
