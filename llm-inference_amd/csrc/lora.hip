@@ -4,7 +4,8 @@
 // of `low` for rows of x and an adapter's b for W. low is kept as two bf16, the value and what that leaves (16 bits
 // of mantissa), side by side, so the sum goes over twice the rank.
 //
-// A call takes one of three ways, by the estimate in Plan:
+// A call takes one of four ways, the first by its size, the others by the estimate in Plan:
+//   one or two rows, little rank and a small W: one launch, in which each workgroup computes low for itself;
 //   many rows, where the product's operations count: low, then one product whose last steps are the adapters';
 //   few rows, where W's bytes and the launches count: parts of the product's sum and, in the same launch behind them,
 //   of low's; then join_kernel adds the parts up, with b's product and the residual;
@@ -827,6 +828,109 @@ __global__ __launch_bounds__(256, R == FEW ? 6 : 3) void join_kernel(LoraArgs l)
 }
 
 // ------------------------------------------------------------------------------------------
+// one or two rows with little rank: everything in one launch
+// ------------------------------------------------------------------------------------------
+
+constexpr int ONE_COLUMNS = 16, ONE_LOW = 16, ONE_SEQS = 64;  // columns of a workgroup; elements of low, sequences at most
+
+// The adapter of row m, found among up to 64 sequences in one round trip.
+__device__ __forceinline__ int owner_among(const LoraArgs &l, int first, int end, int adapter, int m) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t mine = __ballot(lane < l.n_seqs && first <= m && m < end);
+    if (!mine) return NO_SEQUENCE;
+    const int a = __builtin_amdgcn_readlane(adapter, __builtin_ctzll(mine));
+    return (unsigned)a < (unsigned)l.n_adapters ? a : NO_ADAPTER;
+}
+
+// A wave has four columns, and four elements of low, which every workgroup computes for itself, by vector operations in 32
+// bits: at most as much is read of A as of W, and A comes from L2. Bound by two round trips, the lookup's and the operands'
+// (W's first ones are requested in front of the lookup): 5 us for 2048 over 1024, rank 8.
+template <int ROWS>
+__global__ __launch_bounds__(256) void one_kernel(LoraArgs l) {
+    constexpr int U = 2;
+    __shared__ float low[ONE_LOW];
+    const int lane = threadIdx.x & 63, wave = wave_id(), n0 = blockIdx.x * ONE_COLUMNS + wave * 4, s = min(lane, l.n_seqs - 1);
+    const int first = start_of(l, s), end = start_of(l, s + 1), adapter = gptr(l.adapter)[s];
+    const bf16 *w[4], *x[ROWS];
+    const int chunks = l.n_in / 8;
+#pragma unroll
+    for (int j = 0; j < 4; j++) w[j] = l.w + (int64_t)min(n0 + j, l.n_out - 1) * l.n_in;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) x[i] = l.x + i * l.x_stride;
+    u32x4 xs[U][ROWS], ws[U][4], as[U][4];
+    const auto request = [&](const bf16 *p, int c) { return c < chunks ? ld16(p + c * 8) : u32x4{0, 0, 0, 0}; };
+    const auto request_w = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) xs[u][i] = request(x[i], c0 + 64 * u);
+#pragma unroll
+            for (int j = 0; j < 4; j++) ws[u][j] = l.w ? request(w[j], c0 + 64 * u) : u32x4{0, 0, 0, 0};
+        }
+    };
+    request_w(lane);
+    int owner[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) owner[i] = owner_among(l, first, end, adapter, i);
+    // elements 4 wave .. 4 wave + 3 of low, which are of one row, as the rank is a multiple of 8
+    const int element = wave * 4, of = element / l.rank, r = element % l.rank;
+    const int mine = of == 0 ? owner[0] : of < ROWS ? owner[ROWS - 1] : NO_SEQUENCE;
+    const bf16 *a = l.a + ((int64_t)max(mine, 0) * l.rank + r) * l.n_in;
+    const int some = mine >= 0 ? chunks : 0;
+    const auto request_a = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                as[u][j] = c0 + 64 * u < some ? ld16(a + (int64_t)j * l.n_in + (c0 + 64 * u) * 8) : u32x4{0, 0, 0, 0};
+    };
+    request_a(lane);
+    // what lane 4 i + j needs for column j of row i
+    const int row = lane / 4 % ROWS, n = n0 + lane % 4, at = min(n, l.n_out - 1), its = row == 0 ? owner[0] : owner[ROWS - 1];
+    const bf16 *b = l.b + ((int64_t)max(its, 0) * l.n_out + at) * l.rank;
+    const u32x4 b0 = ld16(b), b1 = l.rank > 8 ? ld16(b + 8) : u32x4{0, 0, 0, 0};
+    const float scale = l.scale && mine >= 0 ? gptr(l.scale)[mine] : 1.0f;
+    float y = l.residual ? bf2f(gptr(l.residual)[row * l.residual_stride + at]) : 0.0f;
+    float acc[ROWS][4] = {}, sum[4] = {};
+    for (int c0 = lane;;) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+#pragma unroll
+                    for (int i = 0; i < ROWS; i++) acc[i][j] = fmaf(elem(xs[u][i], e), elem(ws[u][j], e), acc[i][j]);
+                    sum[j] = fmaf(elem(of == 0 ? xs[u][0] : xs[u][ROWS - 1], e), elem(as[u][j], e), sum[j]);
+                }
+        c0 += 64 * U;
+        if (c0 - lane >= chunks) break;
+        request_w(c0);
+        request_a(c0);
+    }
+    const auto all = [&](float v) {
+        v += xor_lane<1>(v), v += xor_lane<2>(v), v += xor_lane<4>(v), v += xor_lane<8>(v), v += xor_lane<16>(v);
+        return v + xor_lane<32>(v);
+    };
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        sum[j] = all(sum[j]) * scale;
+        if (lane == 0 && element + j < ROWS * l.rank) low[element + j] = sum[j];
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) {
+            acc[i][j] = all(acc[i][j]);
+            if (l.w && row == i && lane % 4 == j) y += acc[i][j];
+        }
+    }
+    __syncthreads();
+    if (its >= 0)
+#pragma unroll
+        for (int e = 0; e < 16; e++)
+            if (e < l.rank) y = fmaf(low[row * l.rank + e], elem(e < 8 ? b0 : b1, e % 8), y);
+    if (lane < 4 * ROWS && n < l.n_out && its != NO_SEQUENCE) gptr(l.out)[row * l.out_stride + n] = (bf16)f2bf(y);
+}
+
+// ------------------------------------------------------------------------------------------
 // on the host
 // ------------------------------------------------------------------------------------------
 
@@ -942,6 +1046,14 @@ bool launch_product(const char *name, LoraArgs l, hipStream_t stream) {
     return LAUNCH_OK();
 }
 
+// What one_kernel takes. One row of 2048 over 1024 takes 5.6 us (two launches 8.9), of 6144 over 2560 10.0 (11.3), of 9728
+// over 2560, rank 16, 15.8 (15.5); two of 2048 over 1024 5.4 (6.8), of 2560 over 4096 10.0 (9.7); without W one of 2048 over
+// 1024 4.1 (6.1), of 4096 over 2560 6.1 (6.1).
+bool takes_one(int n_tokens, int n_out, int n_in, bool product, int rank, int n_seqs) {
+    return n_tokens <= 2 && n_tokens * rank <= ONE_LOW && n_seqs <= ONE_SEQS &&
+           (int64_t)n_tokens * n_out * n_in <= (product ? 1 << 24 : 1 << 23);
+}
+
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 bool check_sizes(const char *name, int n_tokens, int n_out, int n_in, int rank) {
@@ -1038,6 +1150,13 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     if (lora) {
         l.a = lora->a, l.b = lora->b, l.scale = lora->scale, l.q_start = lora->q_start, l.adapter = lora->adapter;
         l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = rank;
+        if (g_forced.shape < 0 && takes_one(n_tokens, n_out, n_in, w != nullptr, rank, lora->n_seqs)) {
+            const int groups = (n_out + ONE_COLUMNS - 1) / ONE_COLUMNS;
+            if (n_tokens == 1) one_kernel<1><<<groups, 256, 0, stream>>>(l);
+            else one_kernel<2><<<groups, 256, 0, stream>>>(l);
+            LAUNCH_OK();
+            return;
+        }
         const int low_rows = p.join ? LOW_ROWS_BESIDE[p.shape] : LOW_ROWS;
         const int64_t groups = (int64_t)(n_tokens / low_rows + lora->n_seqs) * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
         if (groups >= 1 << 23) {  // the threads of a launch

@@ -564,3 +564,44 @@ def test_starts_that_decrease_stay_within_the_rows(gpu, force):
         wide = torch.full((64, 200), 7.0, device="cuda", dtype=torch.bfloat16)
         run(gpu, c, wide[2:62, 4:196])
         assert (wide[:2] == 7).all() and (wide[62:] == 7).all() and (wide[:, :4] == 7).all() and (wide[:, 196:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,rank", [(1, 8), (1, 16), (2, 8)])
+@pytest.mark.parametrize("n_in,n_out", [(8, 1), (72, 19), (1024, 2048), (520, 515), (2560, 1030)])
+def test_one_or_two_rows(gpu, rows, rank, n_in, n_out):
+    """The sizes of a single launch: sequences of one and two rows, empty ones around them, up to 64 of them and one more,
+    rows of no sequence, no adapter, each part off."""
+    import torch
+    for lengths, which in [([rows], [1]), ([0, 1] + [0] * 61 + [rows - 1], [0, 2] + [1] * 61 + [3]), ([0] * 40 + [rows], None),
+                           ([0] * 64 + [rows], None), ([1] * rows, [-1, 7][:rows]), ([0, 0], [0, 1])]:
+        spare = rows - sum(lengths)
+        for kw in (dict(residual=True), dict(product=False, residual=True), dict(product=False), dict(scale=False)):
+            c = make(len(lengths) + n_in, lengths, n_in, n_out, rank, adapters=4, which=which, spare=spare, **kw)
+            both(gpu, c, n_out)
+    for starts in ([0, 1], [1, rows], [-3, 9], [2 ** 31 - 1, -1], [rows, 0]):
+        c = make(5, [rows], n_in, n_out, rank, adapters=2, which=[1], residual=True)
+        c["q_start"] = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        both(gpu, c, n_out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("product", [False, True])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_no_number_in_one_of_two_rows(gpu, product, bad):
+    """A row, an adapter's a, b or scale that are no numbers, beside a row that has none of it."""
+    import torch
+    for where in ("x", "lora_a", "lora_b", "lora_scale"):
+        c = make(9, [1, 1], 264, 70, 8, adapters=2, which=[1, 0], product=product, residual=True)
+        clean = {k: v if v is None else v.clone() for k, v in c.items()}
+        dict(x=lambda t: t[0, 3:4], lora_a=lambda t: t[1, 2, 5:6], lora_b=lambda t: t[1, 33, 5:6],
+             lora_scale=lambda t: t[1:2])[where](c[where]).fill_(bad)
+        out = torch.zeros(2, 70, device="cuda", dtype=torch.bfloat16)
+        run(gpu, c, out)
+        want = torch.zeros_like(out)
+        run(gpu, clean, want)
+        assert torch.equal(out[1], want[1]) and not out[0, 33].isfinite()
+    c["adapter"][1] = -1  # without an adapter and, without w, the residual alone
+    c["x"][1, 3] = bad
+    run(gpu, c, out)
+    assert product or torch.equal(out[1], c["residual"][1])
