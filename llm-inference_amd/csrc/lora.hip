@@ -238,11 +238,14 @@ __device__ __forceinline__ f32x4 low_sum(const LoraArgs &l, int64_t at, float sc
     }
     return y * scale;
 }
-// Two numbers as bf16, and what that leaves of them.
+// Two numbers as bf16, and what that leaves of them. Of finite ones past the largest bf16 that leaves less than 2^120, which
+// is rounded by 2^111 at most, 2^-16 of the value.
 __device__ __forceinline__ void in_two(float y0, float y1, uint32_t &value, uint32_t &rest) {
-    const float v0 = round_bf(y0), v1 = round_bf(y1);
-    value = pack2(y0, y1);
-    rest = pack2(fabsf(v0) < INFINITY ? y0 - v0 : 0.0f, fabsf(v1) < INFINITY ? y1 - v1 : 0.0f);
+    constexpr float MOST = 0x1.fep127f;
+    const bool finite0 = fabsf(y0) < INFINITY, finite1 = fabsf(y1) < INFINITY;
+    const float v0 = finite0 ? fminf(fmaxf(y0, -MOST), MOST) : y0, v1 = finite1 ? fminf(fmaxf(y1, -MOST), MOST) : y1;
+    value = pack2(v0, v1);
+    rest = pack2(finite0 ? y0 - round_bf(v0) : 0.0f, finite1 ? y1 - round_bf(v1) : 0.0f);
 }
 
 // low from its parts: four elements per thread.

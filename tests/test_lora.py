@@ -605,3 +605,25 @@ def test_no_number_in_one_of_two_rows(gpu, product, bad):
     c["x"][1, 3] = bad
     run(gpu, c, out)
     assert product or torch.equal(out[1], c["residual"][1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,join", [(-1, 0)] + [(s, j) for s in range(9) for j in (0, 1)])
+@pytest.mark.parametrize("last", [1.0, 1.5])
+def test_low_products_at_the_end_of_the_range(gpu, force, shape, join, last):
+    """Finite in 32 bits, but past the largest bf16 by half its step and more: 8 (255 2^120 + last 2^119) 2^-100 is exact in
+    32 bits, and the nearest bf16 (the even one, where last is 1) is 2^31."""
+    import torch
+    force(shape, 1, join)
+    for lengths in ([1], [3], [20, 1, 40], [300, 2]):
+        c = make(7, lengths, 64, 130, 8, adapters=1, which=[0] * len(lengths), product=False, scale=False)
+        for k in ("x", "lora_a"):
+            c[k].zero_()
+        sign = torch.where(torch.arange(sum(lengths), device="cuda") % 3 == 1, -1.0, 1.0)
+        c["x"][:, :2] = sign[:, None] * 2.0 ** 64
+        c["lora_a"][:, :, 0] = 255 * 2.0 ** 56
+        c["lora_a"][:, :, 1] = last * 2.0 ** 55
+        c["lora_b"].fill_(2.0 ** -100)
+        out = torch.zeros(sum(lengths), 130, device="cuda", dtype=torch.bfloat16)
+        run(gpu, c, out)
+        assert (out == sign[:, None] * 2.0 ** 31).all()
