@@ -300,13 +300,14 @@ __device__ __forceinline__ void store8(const LoraArgs &l, bf16 *to, const bf16 *
     }
 }
 
-// Whether NaN or infinities were among eight elements; they are zeros then.
+// Whether NaN or infinities were among eight elements; they are 2^-126 of the same sign then: zero for rows whose low is
+// zero, infinite where it is infinite, as the product would be, and lost beside the term of unfit_term otherwise.
 __device__ __forceinline__ bool clear_unfit_of(u32x4 &v) {
     bool found = false;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-        if ((v[j] & 0x7f80u) == 0x7f80u) v[j] &= 0xffff0000u, found = true;
-        if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] &= 0xffffu, found = true;
+        if ((v[j] & 0x7f80u) == 0x7f80u) v[j] = (v[j] & 0xffff8000u) | 0x0080u, found = true;
+        if ((v[j] & 0x7f800000u) == 0x7f800000u) v[j] = (v[j] & 0x8000ffffu) | 0x00800000u, found = true;
     }
     return found;
 }
@@ -493,7 +494,7 @@ __global__ __launch_bounds__(G::T) void product_kernel(LoraArgs l) {
             for (int j = 0; j < G::NT; j++) acc[i][j] = mfma(wf[k % 2][j], xf[k % 2][i], acc[i][j]);
     };
     // NaN and infinities of an adapter, times the zeros of other rows or a remainder of zero, would be no numbers
-    // everywhere. Where there are some, which the largest exponent tells, the tile is computed again with zeros in
+    // everywhere. Where there are some, which the largest exponent tells, the tile is computed again with small numbers in
     // their place, and the rows that they belong to get them in the end.
     u16x2 largest = {0, 0};
     bool clear = false;

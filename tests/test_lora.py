@@ -627,3 +627,33 @@ def test_low_products_at_the_end_of_the_range(gpu, force, shape, join, last):
         out = torch.zeros(sum(lengths), 130, device="cuda", dtype=torch.bfloat16)
         run(gpu, c, out)
         assert (out == sign[:, None] * 2.0 ** 31).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,splits,join", [(-1, 0, 0)] + [(s, n, j) for s in range(9) for n, j in ((1, 0), (3, 0), (1, 1))])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_infinite_low_products_meet_infinities(gpu, force, shape, splits, join, bad):
+    """An element of b that is no number, where the low product that it meets is infinite: their product, as in 64 bits."""
+    import torch
+    force(shape, splits, join)
+    for lengths, which in ([[1], [1]], [[1, 1], [0, 1]], [[40, 1, 1, 90, 2, 1, 30], [0, 1, 2, 1, -1, 3, 2]]):
+        c = make(23, lengths, 200, 280, 8, adapters=4, which=which, residual=True, scale=False)
+        rows = sum(lengths)
+        sign = torch.where(torch.arange(rows, device="cuda") % 3 == 1, -1.0, 1.0)
+        c["x"][:, 0] = 3 * sign
+        c["lora_a"][1, 5, 0] = math.inf  # low[5] is an infinity of x[:, 0]'s sign
+        c["lora_b"][1, :, 5] = torch.where(c["lora_b"][1, :, 5] == 0, 1.0, c["lora_b"][1, :, 5])
+        clean = defined(dict(c, lora_a=c["lora_a"].nan_to_num(0, 0, 0)), rows, 280)
+        c["lora_b"][1, 33, 5] = bad
+        out = torch.full((rows, 280), 7.0, device="cuda", dtype=torch.bfloat16)
+        run(gpu, c, out)
+        starts = c["q_start"].tolist()
+        for s, a in enumerate(which):
+            own = slice(starts[s], starts[s + 1])
+            if a == 1:
+                want = sign[own, None] * c["lora_b"][1, :, 5].float() * math.inf
+                assert torch.equal(out[own].isnan(), want.isnan())
+                assert torch.equal(out[own].float().nan_to_num(), want.nan_to_num())
+            else:
+                value, err, _ = (t[own] if t.dim() == 2 else t for t in clean)
+                assert ((out[own].double() - value).abs() <= HALF_STEP * (value.abs() + err) + err).all()
