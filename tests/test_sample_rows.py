@@ -376,3 +376,34 @@ def test_wrapper_refusals(gpu, monkeypatch, native):
             gpu.sample_rows_forward(**dict(dict(out=i, logits=x, u=f, ws=ws), **args))
     gpu.sample_rows_forward(i, x, f, ws=ws)  # and no error is left
     torch.cuda.synchronize()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [3, 700, 40000, 151936])
+def test_random_numbers_of_one_and_more(gpu, vocab):
+    """No running sum passes them: the last token of positive weight, also where the first one's weight is the whole sum in
+    64 bits, and where those behind weigh nothing."""
+    import torch
+    rng = np.random.default_rng(11)
+    x = np.full((12, vocab), -60.0, np.float32)  # e^-60 is less than half a step of 1
+    x[:, vocab // 2] = 0.0
+    x[1, :vocab // 3 + 1] = -700.0
+    x[2] = rng.choice([-60.0, -2000.0], vocab)  # e^-2000 is 0
+    x[2, vocab // 2] = 0.0
+    x[3] = -2000.0
+    x[3, vocab // 2] = 1.0
+    x[4, vocab - 1] = np.inf
+    x[5] = rng.standard_normal(vocab)
+    x[6:] = x[:6]
+    logits = torch.from_numpy(x).cuda().bfloat16()
+    for u in (1.0, 7.0, np.inf):
+        c = make(rng, 12)
+        c["u"] = np.full(12, u, np.float32)
+        check(run(gpu, logits, c), logits, c, exact_edges=True)
+        c["top_k"] = np.tile([0, 1, 2, 5, 600, 1], 2).astype(np.int32)
+        check(run(gpu, logits, c), logits, c, exact_edges=True)
+        c["min_p"] = np.repeat([0.0, 1e-30], 6).astype(np.float32)
+        check(run(gpu, logits, c), logits, c, exact_edges=True)
+        c["top_p"] = np.full(12, 0.75, np.float32)
+        c["temperature"] = np.full(12, 1.5, np.float32)
+        check(run(gpu, logits, c), logits, c, exact_edges=True)
