@@ -956,8 +956,16 @@ typedef Shape<16, 64, 16, 16, 64, 4, true> Few16;
 constexpr Pace PACES[] = {{256, 192, 1, 920, 1380, 5800}, {224, 256, 1, 970, 1450, 5900}, {192, 256, 1, 960, 1220, 6100},
                           {128, 256, 1, 650, 720, 3900},  {128, 128, 2, 520, 740, 3900},  {64, 128, 2, 440, 610, 1900},
                           {64, 64, 2, 460, 250, 2400},    {32, 64, 3, 310, 280, 2100},    {16, 64, 3, 270, 230, 1700}};
-constexpr int LOW_ROWS_BESIDE[] = {Wide::LOW_ROWS,    High::LOW_ROWS,   Square::LOW_ROWS, Half::LOW_ROWS, Quarter::LOW_ROWS,
-                                   Few128::LOW_ROWS, Few64::LOW_ROWS, Few32::LOW_ROWS,  Few16::LOW_ROWS};
+// And what a launch goes by.
+struct Tile {
+    int tm, tn, threads, low_rows;
+};
+template <class G>
+constexpr Tile tile_of() {
+    return {G::TM, G::TN, G::T, G::LOW_ROWS};
+}
+constexpr Tile TILES[] = {tile_of<Wide>(),   tile_of<High>(),  tile_of<Square>(), tile_of<Half>(), tile_of<Quarter>(),
+                          tile_of<Few128>(), tile_of<Few64>(), tile_of<Few32>(),  tile_of<Few16>()};
 constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 
 constexpr int MOST_SPLITS = 32;
@@ -1022,7 +1030,7 @@ struct Plan {
                 if (!product && i < SHAPES - 1) continue;  // low alone: the smallest workgroups
                 const int at_once = few ? 8 : 4;  // parts that the join has under way
                 const double joined = 1930 + product_cost + (product ? rest : 0) + (few ? 3000 : 4500) + 1270 * ceil((double)n / at_once) +
-                                      parts / 4960 + b / 7670 + low(LOW_ROWS_BESIDE[i]) / 8570;
+                                      parts / 4960 + b / 7670 + low(TILES[i].low_rows) / 8570;
                 if (joined < least) shape = i, splits = n, join = true, least = joined;
             }
         }
@@ -1039,14 +1047,12 @@ struct Plan {
     }
 };
 
+// Threads that a launch has fewer than.
+constexpr int64_t MOST_THREADS = 1ll << 31;
+
 template <class G>
-bool launch_product(const char *name, LoraArgs l, hipStream_t stream) {
-    l.m_tiles = (l.n_tokens + G::TM - 1) / G::TM;
-    l.n_tiles = (l.n_out + G::TN - 1) / G::TN;
-    const int64_t groups = (int64_t)l.m_tiles * l.n_tiles * l.splits + l.low_groups;
-    if (groups * G::T >= 1ll << 32)  // the threads of a launch
-        return llm_fail("%s: n_tokens %d by n_out %d is too much for one launch", name, l.n_tokens, l.n_out);
-    product_kernel<G><<<groups, G::T, 0, stream>>>(l);
+bool launch_product(const LoraArgs &l, hipStream_t stream) {
+    product_kernel<G><<<l.m_tiles * l.n_tiles * l.splits + l.low_groups, G::T, 0, stream>>>(l);
     return LAUNCH_OK();
 }
 
@@ -1151,6 +1157,7 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
     l.low_splits = p.join ? (n_in + JOIN_LOW_SPAN - 1) / JOIN_LOW_SPAN : low_splits(n_in);
     l.owner = (int *)(ws + low_floats(n_tokens, n_in, rank));
     if (p.splits > 1 || p.join) l.part = ws + low_floats(n_tokens, n_in, rank) + owner_floats(n_tokens, rank);
+    int64_t low_groups = 0;
     if (lora) {
         l.a = lora->a, l.b = lora->b, l.scale = lora->scale, l.q_start = lora->q_start, l.adapter = lora->adapter;
         l.n_seqs = lora->n_seqs, l.n_adapters = lora->n_adapters, l.rank = rank;
@@ -1161,32 +1168,38 @@ extern "C" void lora_projection_forward(bf16 *out, const bf16 *x, const bf16 *w,
             LAUNCH_OK();
             return;
         }
-        const int low_rows = p.join ? LOW_ROWS_BESIDE[p.shape] : LOW_ROWS;
-        const int64_t groups = (int64_t)(n_tokens / low_rows + lora->n_seqs) * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
-        if (groups >= 1 << 23) {  // the threads of a launch
+        const int low_rows = p.join ? TILES[p.shape].low_rows : LOW_ROWS;
+        low_groups = (int64_t)(n_tokens / low_rows + lora->n_seqs) * ((rank + low_width(rank) - 1) / low_width(rank)) * l.low_splits;
+        if (low_groups * 64 * LOW_WAVES >= MOST_THREADS) {
             llm_fail("%s: %d sequences of rank %d over n_in %d are too many for one launch", name, lora->n_seqs, rank, n_in);
             return;
         }
-        if (p.join) {
-            l.low_groups = (int)groups;
-        } else {
-            low_kernel<<<groups, 64 * LOW_WAVES, 0, stream>>>(l);
-            if (!LAUNCH_OK()) return;
-            low_sum_kernel<<<((int64_t)n_tokens * (rank / 4) + 255) / 256, 256, 0, stream>>>(l);
-            if (!LAUNCH_OK()) return;
-        }
+        if (p.join) l.low_groups = (int)low_groups;
+    }
+    const Tile &tile = TILES[p.shape];
+    l.m_tiles = (n_tokens + tile.tm - 1) / tile.tm;
+    l.n_tiles = (n_out + tile.tn - 1) / tile.tn;
+    if (((int64_t)l.m_tiles * l.n_tiles * l.splits + l.low_groups) * tile.threads >= MOST_THREADS) {
+        llm_fail("%s: n_tokens %d by n_out %d is too much for one launch", name, n_tokens, n_out);
+        return;
+    }
+    if (lora && !p.join) {
+        low_kernel<<<low_groups, 64 * LOW_WAVES, 0, stream>>>(l);
+        if (!LAUNCH_OK()) return;
+        low_sum_kernel<<<((int64_t)n_tokens * (rank / 4) + 255) / 256, 256, 0, stream>>>(l);
+        if (!LAUNCH_OK()) return;
     }
     bool ok = false;
     switch (p.shape) {
-    case 0: ok = launch_product<Wide>(name, l, stream); break;
-    case 1: ok = launch_product<High>(name, l, stream); break;
-    case 2: ok = launch_product<Square>(name, l, stream); break;
-    case 3: ok = launch_product<Half>(name, l, stream); break;
-    case 4: ok = launch_product<Quarter>(name, l, stream); break;
-    case 5: ok = launch_product<Few128>(name, l, stream); break;
-    case 6: ok = launch_product<Few64>(name, l, stream); break;
-    case 7: ok = launch_product<Few32>(name, l, stream); break;
-    default: ok = launch_product<Few16>(name, l, stream);
+    case 0: ok = launch_product<Wide>(l, stream); break;
+    case 1: ok = launch_product<High>(l, stream); break;
+    case 2: ok = launch_product<Square>(l, stream); break;
+    case 3: ok = launch_product<Half>(l, stream); break;
+    case 4: ok = launch_product<Quarter>(l, stream); break;
+    case 5: ok = launch_product<Few128>(l, stream); break;
+    case 6: ok = launch_product<Few64>(l, stream); break;
+    case 7: ok = launch_product<Few32>(l, stream); break;
+    default: ok = launch_product<Few16>(l, stream);
     }
     if (!ok) return;
     const int n_tiles = (n_out + 255) / 256;

@@ -657,3 +657,23 @@ def test_infinite_low_products_meet_infinities(gpu, force, shape, splits, join, 
             else:
                 value, err, _ = (t[own] if t.dim() == 2 else t for t in clean)
                 assert ((out[own].double() - value).abs() <= HALF_STEP * (value.abs() + err) + err).all()
+
+
+@pytest.mark.parametrize("n_out", [250000, 1 << 22])  # of the first, 2^31 to 2^32 threads with most tiles
+@pytest.mark.parametrize("adapters", [False, True])
+def test_products_of_too_many_threads(pkg, n_out, adapters):
+    """Refused before anything is launched, low in front of the product neither."""
+    sizes = dict(n_tokens=1 << 20, n_out=n_out, out_stride=n_out)
+    if adapters:
+        message = _call(pkg, **sizes)
+    else:
+        L, p = pkg.lib(), 0x1000
+        L.llm_clear_error()
+        L.lora_projection_forward(0x2000, p, p, None, None, p, 1 << 20, n_out, 128, n_out, 128, n_out, None)
+        message = L.llm_last_error().decode()
+        L.llm_clear_error()
+    assert "too much for one launch" in message
+
+
+def test_sequences_of_too_many_threads(pkg):
+    assert "too many for one launch" in _call(pkg, lora=dict(n_seqs=1 << 20), n_in=1 << 15, x_stride=1 << 15)
