@@ -1056,12 +1056,18 @@ bool launch_product(const LoraArgs &l, hipStream_t stream) {
     return LAUNCH_OK();
 }
 
-// What one_kernel takes. One row of 2048 over 1024 takes 5.6 us (two launches 8.9), of 6144 over 2560 10.0 (11.3), of 9728
-// over 2560, rank 16, 15.8 (15.5); two of 2048 over 1024 5.4 (6.8), of 2560 over 4096 10.0 (9.7); without W one of 2048 over
-// 1024 4.1 (6.1), of 4096 over 2560 6.1 (6.1).
+// What one_kernel takes: sums of few round trips (of 1024 elements each; the other ways have the sum in up to 32 parts), and
+// columns that the CUs take at once. us of a captured call among others, beside the other way's:
+//   one row of rank 8: 2048 over 1024 4.7 (6.7), 16 over 4096 6.6 (7.1), 16 over 5120 7.7 (7.7), 16 over 9728 12.8 (8.5), 4096
+//   over 4096 11.3 (11.6), 8192 over 1024 7.3 (8.5), 9728 over 1024 9.8 (9.4), 8192 over 2048 12.4 (10.7);
+//   of rank 16: 4096 over 2560 8.9 (9.7), 1024 over 4096 8.1 (7.9), 2048 over 4096 10.2 (9.1);
+//   two rows: 2048 over 1024 5.4 (6.8), 2048 over 2048 7.8 (7.7), 16 over 2560 6.9 (6.6), 4096 over 2048 10.1 (9.0);
+//   without W, one row of rank 8: 4096 over 1024 4.1 (6.0), 2048 over 2560 6.0 (6.0), 16 over 4096 6.6 (5.5); two: 2048 over
+//   1024 4.8 (6.0), 16 over 2560 6.8 (5.7).
 bool takes_one(int n_tokens, int n_out, int n_in, bool product, int rank, int n_seqs) {
-    return n_tokens <= 2 && n_tokens * rank <= ONE_LOW && n_seqs <= ONE_SEQS &&
-           (int64_t)n_tokens * n_out * n_in <= (product ? 1 << 24 : 1 << 23);
+    const int trips = n_tokens == 2 ? 2 : product && rank == 8 ? 4 : 3;
+    return n_tokens <= 2 && n_tokens * rank <= ONE_LOW && n_seqs <= ONE_SEQS && n_in <= trips * 1024 && n_out <= 8192 &&
+           (int64_t)n_tokens * n_out * n_in <= (product ? (1 << 24) - 1 : 1 << 23);
 }
 
 bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }

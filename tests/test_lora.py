@@ -677,3 +677,19 @@ def test_products_of_too_many_threads(pkg, n_out, adapters):
 
 def test_sequences_of_too_many_threads(pkg):
     assert "too many for one launch" in _call(pkg, lora=dict(n_seqs=1 << 20), n_in=1 << 15, x_stride=1 << 15)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,rank,n_in,n_out,product,one", [
+    (1, 8, 1024, 2048, True, True), (1, 8, 4096, 2560, True, True), (1, 16, 2560, 4096, True, True), (2, 8, 1024, 2048, True, True),
+    (1, 16, 1024, 8192, False, True), (1, 8, 9728, 16, True, False), (1, 8, 9728, 256, True, False), (1, 16, 9728, 1024, True, False),
+    (1, 16, 4096, 1024, True, False), (1, 8, 1 << 16, 16, True, False), (1, 8, 1 << 20, 16, True, False), (2, 8, 4096, 257, True, False),
+    (2, 8, 9728, 16, True, False), (1, 8, 9728, 64, False, False), (2, 8, 1 << 16, 16, False, False), (1, 8, 512, 9728, False, False)])
+def test_a_single_launch_where_it_is_shorter(gpu, rows, rank, n_in, n_out, product, one):
+    """Few columns of a long sum are not left to a workgroup each, nor so many columns that the workgroups take turns. The
+    single launch does without the workspace."""
+    import torch
+    c = make(rows + n_in, [1] * rows, n_in, n_out, rank, adapters=2, which=[1, 0][:rows], product=product, residual=True)
+    ws = torch.full((gpu.lora_projection_workspace_floats(rows, n_out, n_in, rank),), math.nan, device="cuda")
+    both(gpu, c, n_out, ws=ws)
+    assert bool(ws.isnan().all()) == one
