@@ -65,6 +65,7 @@ __device__ __forceinline__ f32x4 mfma(const u32x4 &a, const u32x4 &b, f32x4 c) {
 }
 
 // 64 lanes' 16 bytes into LDS at `to` on, without passing registers: the wave waits for it with wait_loads.
+// (m0 is reserved: it cannot be named as written, and the compiler has no use for it in these kernels.)
 template <bool STREAM = false>
 __device__ __forceinline__ void load_to_lds(unsigned to, const void *base, unsigned offset) {
     if constexpr (STREAM)
