@@ -27,8 +27,8 @@ extern "C" void llm_exp_bits(float *out, unsigned first, unsigned n, int branche
 // after an error); then, with set 1 or 0, all are taken or free.
 extern "C" int llm_sample_slots(int set);
 
-// For tests, with no call in flight: lora_projection_forward takes tiles of that shape, in so many splits, and join_kernel
-// if join, wherever a call can (shape < 0: as it chooses). Returns the number of shapes.
+// For tests: the calling thread's lora_projection_forward takes tiles of that shape, in so many splits, and join_kernel if
+// join, wherever a call can (shape < 0: as it chooses). Returns the number of shapes.
 extern "C" int llm_lora_force(int shape, int splits, int join);
 
 // inv_freq_j = 1 / fp32(pow(theta, fp32(2j / D))) for j < D/2 (D <= 256), cached per (theta, D).

@@ -972,8 +972,8 @@ constexpr int SHAPES = sizeof(PACES) / sizeof(PACES[0]);
 constexpr int MOST_SPLITS = 32;
 constexpr size_t MOST_PART = 1 << 23;  // floats
 
-// For tests: a plan that is taken wherever it can be.
-struct {
+// For tests: a plan that is taken wherever it can be, in the calls of the thread that set it.
+thread_local struct {
     int shape = -1, splits, join;
 } g_forced;
 

@@ -693,3 +693,26 @@ def test_a_single_launch_where_it_is_shorter(gpu, rows, rank, n_in, n_out, produ
     ws = torch.full((gpu.lora_projection_workspace_floats(rows, n_out, n_in, rank),), math.nan, device="cuda")
     both(gpu, c, n_out, ws=ws)
     assert bool(ws.isnan().all()) == one
+
+
+@pytest.mark.gpu
+def test_a_plan_for_tests_stays_with_its_thread(gpu, force):
+    """The plan that a test forces is not another thread's: that one's single launch leaves the workspace alone."""
+    import threading
+    import torch
+    c = make(31, [1], 1024, 64, 8, adapters=2, which=[1])
+    floats = gpu.lora_projection_workspace_floats(1, 64, 1024, 8)
+    ws = [torch.full((floats,), math.nan, device="cuda") for _ in range(2)]
+    force(4, 2, 0)
+    both(gpu, c, 64, ws=ws[0])
+    failed = []
+
+    def other():
+        try:
+            both(gpu, c, 64, ws=ws[1])
+        except BaseException as e:
+            failed.append(e)
+    thread = threading.Thread(target=other)
+    thread.start()
+    thread.join()
+    assert not failed and not ws[0].isnan().all() and ws[1].isnan().all()
