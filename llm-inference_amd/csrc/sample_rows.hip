@@ -655,12 +655,17 @@ __global__ __launch_bounds__(T) void merge_kernel(SampleArgs a) {
     });
 }
 
-constexpr int SPLIT_VOCAB = 16384, SPLIT_ROWS = 128;  // rows of at least so many tokens, and fewer of them, are cut
+// Rows of at least SPLIT_VOCAB tokens are cut, into as many slices as let all workgroups of a launch have a CU to themselves;
+// from SPLIT_ROWS on those of LONG_VOCAB alone, and from LONG_ROWS on none. us of a captured call with temperature, top-k and
+// top-p, uncut and in the slices of this rule: one row of 32000 17.4 and 20.4, of 50257 22.3 and 21.1, of 65536 24.2 and 21.2,
+// of 151936 39.7 and 23.0; 64 of 50257 23.5 and 23.6, of 65536 25.3 and 24.3; 96 of 65536 25.8 and 27.4, of 100352 33.9 and
+// 32.4; 127 of 151936 45.4 and 42.4, 160 45.7 and 43.1, 200 46.5 and 52.4.
+constexpr int SPLIT_VOCAB = 49152, SPLIT_ROWS = 65, LONG_VOCAB = 98304, LONG_ROWS = 128;
 
 // Slices of a row.
 int slices_of(int rows, int vocab) {
-    if (vocab < SPLIT_VOCAB || rows >= SPLIT_ROWS) return 1;
-    const int slices = std::max(2, std::min({MOST_SLICES, 256 / rows, vocab / 4096}));
+    if (vocab < SPLIT_VOCAB || rows >= (vocab < LONG_VOCAB ? SPLIT_ROWS : LONG_ROWS)) return 1;
+    const int slices = std::max(2, std::min(MOST_SLICES, 256 / rows));
     return std::max(slices, (vocab + MOST_SLICE - 1) / MOST_SLICE);
 }
 
@@ -679,7 +684,7 @@ size_t list_floats(int vocab) { return (size_t)vocab + 10 * MOST_SLICES; }
 
 extern "C" size_t sample_rows_workspace_floats(int rows, int vocab) {
     if (!check_sizes("sample_rows_workspace_floats", rows, vocab) || vocab < SPLIT_VOCAB) return 0;
-    return std::min(rows, SPLIT_ROWS - 1) * list_floats(std::min(vocab, MOST_SLICES * MOST_SLICE));
+    return std::min(rows, LONG_ROWS - 1) * list_floats(std::min(vocab, MOST_SLICES * MOST_SLICE));
 }
 
 extern "C" void sample_rows_forward(int *out, float *logprob, const bf16 *logits, const float *temperature,

@@ -407,3 +407,18 @@ def test_random_numbers_of_one_and_more(gpu, vocab):
         c["top_p"] = np.full(12, 0.75, np.float32)
         c["temperature"] = np.full(12, 1.5, np.float32)
         check(run(gpu, logits, c), logits, c, exact_edges=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,vocab,cut", [
+    (1, 16384, False), (64, 32003, False), (1, 49151, False), (1, 49152, True), (64, 50257, True), (65, 65536, False),
+    (65, 98303, False), (65, 98304, True), (127, 151936, True), (128, 151936, False)])
+def test_rows_are_cut_where_that_is_shorter(gpu, rows, vocab, cut):
+    """Rows that a workgroup each counts in less time than two launches take are left whole: these do without a workspace."""
+    import torch
+    rng = np.random.default_rng(rows + vocab)
+    logits = torch.from_numpy(rng.standard_normal((rows, vocab)).astype(np.float32) * 3).cuda().bfloat16()
+    c = make(rng, rows, **ALL)
+    ws = torch.full((max(gpu.sample_rows_workspace_floats(rows, vocab), 4),), math.nan, device="cuda")
+    check(run(gpu, logits, c, ws=ws), logits, c)
+    assert bool(ws.isnan().all()) == (not cut)
