@@ -354,23 +354,22 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Row &row, int r, int l
             } else if (step == MIN_P) {
                 // of a u of 1 or more, which no running sum passes, the pick is the last token of positive weight: those of
                 // none go here, as a sum need not show the difference
-                const double enough = fmax((double)min_p, u >= 1.0f ? 0x1p-1074 : 0.0);
-                needed = enough > 0.0;
+                needed = min_p > 0.0f || u >= 1.0f;
                 how = VALUES;
                 // the last place of enough weight, by 64ths of what is left: weights do not grow along the places
                 int lo = least, hi = needed ? 0xff7f + 1 : least + 1;
 #pragma unroll 1
                 while (hi - lo > 1) {
                     const int by64 = (hi - lo + 63) / 64, mine = lo + (lane + 1) * by64;
-                    const int fit = __popcll(__ballot(mine < hi && weight(mine) >= enough));
+                    const double each = weight(mine);
+                    const int fit = __popcll(__ballot(mine < hi && each > 0.0 && !(each < (double)min_p)));
                     hi = min(hi, lo + (fit + 1) * by64);
                     lo += fit * by64;
                 }
                 behind = lo;
             } else if (step == PICK) {
-                at = (double)u * total;
-                how = u < 1.0f ? WITHIN : TOKENS;
-                behind = u >= 1.0f ? left - 1 : 0;
+                how = u != u ? TOKENS : WITHIN;
+                at = u < 1.0f ? (double)u * total : INFINITY;  // 1 or more: all of them, so the last one
             } else {  // past the last one by a rounding: that
                 needed = spot_tokens >= left;
                 behind = left - 1;
