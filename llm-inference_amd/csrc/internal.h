@@ -30,6 +30,8 @@ extern "C" int llm_sample_slots(int set);
 // For tests: the calling thread's lora_projection_forward takes tiles of that shape, in so many splits, and join_kernel if
 // join, wherever a call can (shape < 0: as it chooses). Returns the number of shapes.
 extern "C" int llm_lora_force(int shape, int splits, int join);
+// For tests: the shape of tiles, of those, that lora_projection_forward takes beside a product (rank 0: no adapters).
+extern "C" int llm_lora_plan(int n_tokens, int n_out, int n_in, int rank, int n_seqs, int n_adapters);
 
 // inv_freq_j = 1 / fp32(pow(theta, fp32(2j / D))) for j < D/2 (D <= 256), cached per (theta, D).
 void rope_inv_freq_table(float theta, int D, float *out);

@@ -716,3 +716,12 @@ def test_a_plan_for_tests_stays_with_its_thread(gpu, force):
     thread.start()
     thread.join()
     assert not failed and not ws[0].isnan().all() and ws[1].isnan().all()
+
+
+@pytest.mark.parametrize("rows,n_out,n_in,rank,n_seqs,large", [
+    (1344, 6144, 2560, 0, 0, True), (1344, 6144, 2560, 32, 5, True), (1324, 1040, 4976, 0, 0, True), (1600, 2560, 9728, 0, 0, True),
+    (1987, 6144, 2560, 16, 2, True), (64, 4096, 2560, 16, 64, False), (64, 151936, 2560, 0, 0, False), (17, 2560, 9728, 64, 17, False)])
+def test_tiles_of_few_rows_are_for_few_rows(pkg, rows, n_out, n_in, rank, n_seqs, large):
+    """Shapes 5 to 8 have up to 64 rows and read w past the caches, as often as there are such rows of tiles: 114 us in place
+    of 50 for the first of these calls."""
+    assert (pkg.lib().llm_lora_plan(rows, n_out, n_in, rank, n_seqs, 4 if rank else 0) < 5) == large
