@@ -11,8 +11,8 @@
 //   of low's; then join_kernel adds the parts up, with b's product and the residual;
 //   without adapters: the product, and sum_kernel where its sum is split.
 // 64 rows of 4096 over 2560, each with one of 48 adapters of rank 16, take 14 us (the product alone, from a library:
-// 19.3), 2582 rows of five prompts of 9728 over 2560, rank 32, 136 (115), 924 rows of 22 sequences of 2560 over 9728,
-// rank 64, 82 (66).
+// 19.3), 2582 rows of five prompts of 9728 over 2560, rank 32, 132 to 143 (115), 924 rows of 22 sequences of 2560 over 9728,
+// rank 64, 80 to 84 (66).
 #include <math.h>
 
 #include <algorithm>
@@ -100,7 +100,8 @@ __device__ __forceinline__ int start_of(const LoraArgs &l, int s) {
     return max(0, min(l.n_tokens, gptr(l.q_start)[s]));
 }
 
-// What low_part wrote for row m. Starts that decrease leave rows that it does not know of, which are no sequence's.
+// What low_part wrote for row m. Starts that decrease, which no call may have, leave rows that it wrote nothing for: what is
+// there from before is kept to the adapters that there are, so that it leads to no address outside of the call's tensors.
 __device__ __forceinline__ int owner_of(const LoraArgs &l, int m) {
     const int owner = gptr(l.owner)[m];
     return owner >= NO_SEQUENCE && owner < l.n_adapters ? owner : NO_SEQUENCE;
@@ -284,9 +285,10 @@ __device__ __forceinline__ void store4(const LoraArgs &l, bf16 *to, const bf16 *
     }
 }
 
-// Eight columns of a row, past the caches: eight lanes side by side write whole lines so. 2582 rows of 9728 over 2560
-// take 135 us with such stores, 166 with four columns a lane of 16 rows at a time, through the caches (157 past them), and
-// 161 with whole lines through the caches; 64 rows of 151936 148, 158, 156 and 156.
+// Eight columns of a row, past the caches: the eight lanes side by side of a wave of 64 columns write whole lines so, those of
+// 32 (tiles of 64 by 128) halves, of 16 (the smaller ones) quarters. 2582 rows of 9728 over 2560 take 135 us with such
+// stores, 166 with four columns a lane of 16 rows at a time, through the caches (157 past them), and 161 with whole lines
+// through the caches; 64 rows of 151936, in halves of lines, 148, 158, 156 and 156.
 __device__ __forceinline__ void store8(const LoraArgs &l, bf16 *to, const bf16 *res, f32x4 y, f32x4 z, int n) {
     if (l.wide == 8 && n + 8 <= l.n_out) {
         if (l.residual) {
@@ -350,8 +352,9 @@ struct Shape {
     static constexpr int LOADS = X_LOADS + W_LOADS;
 };
 
-// Large tiles are bound by the card's power: 2582 rows of 9728 over 2560 take 118 us, 1.09 PFLOP/s (a library product of
-// 8192 x 8192 x 8192: 1.40). Each step's operands come from LDS while the step before it is multiplied, and the loads of
+// Large tiles: 2582 rows of 9728 over 2560 take 118 us, 1.09 PFLOP/s (a library product of 8192 x 8192 x 8192: 1.40), in 456
+// tiles, two rounds that are 89% full, each with 6 us of first loads and stores; the matrix units are busy 42% of the time with
+// operands from memory. Each step's operands come from LDS while the step before it is multiplied, and the loads of
 // the step behind the stages go between the products; an XCD has tiles side by side, which share operands in its L2.
 // Tiles of up to 64 rows are bound by W: 64 rows of 151936 over 2560 at 5.4 TB/s, which neither longer steps,
 // more stages, another order of tiles nor another start of each tile's sum changes.
@@ -597,7 +600,7 @@ again:
     }
 
     // parts from the registers, a lane having four columns side by side of a row; out through LDS, a wave's 16 rows at a
-    // time, so that what goes out is whole lines
+    // time, so that what goes out is whole lines, or as much of them as the wave has columns
     constexpr int PITCH = G::RN + 4, EIGHTS = G::RN / 8;
     static_assert(G::WAVES * 16 * PITCH * 4 <= G::STAGES * G::BYTES, "rows on their way out");
     float *rows = (float *)lds + wave * 16 * PITCH;
@@ -849,7 +852,7 @@ __device__ __forceinline__ int owner_among(const LoraArgs &l, int first, int end
 
 // A wave has four columns, and four elements of low, which every workgroup computes for itself, by vector operations in 32
 // bits: at most as much is read of A as of W, and A comes from L2. Bound by two round trips, the lookup's and the operands'
-// (W's first ones are requested in front of the lookup): 5 us for 2048 over 1024, rank 8.
+// (W's first ones are requested in front of the lookup): 4.7 us for 2048 over 1024, rank 8.
 template <int ROWS>
 __global__ __launch_bounds__(256) void one_kernel(LoraArgs l) {
     constexpr int U = 2;
@@ -945,6 +948,11 @@ struct Pace {
     int tm, tn, at_once;
     double alone, full, fixed;
 };
+// What the large ones are for, us of a product without adapters (beside it the best of the other shapes): 256 by 192, 1152 rows of
+// 9728 over 2560 64 (71); 224 by 256, 2100 rows of 6144 over 2560 59 (70), 3200 rows of 4096 over 2560 60 (70), although it keeps
+// 22 registers in scratch memory, outside of the loop over whole steps; 192 by 256, 2500 rows of 4096 over 2560 51 (54); 128 by
+// 256, 700 rows of 19456 over 2560 82 (124). Of 24 drawn calls each that take 256 by 192, 224 by 256 or 128 by 128, the estimate's
+// next choice takes 7%, 11% and 4% longer on average.
 typedef Shape<256, 192, 64, 96, 64, 2> Wide;
 typedef Shape<224, 256, 112, 64, 64, 2> High;
 typedef Shape<192, 256, 96, 64, 64, 2> Square;
@@ -979,7 +987,9 @@ thread_local struct {
 
 // Few rows in all or of each sequence, on average: join_kernel has tiles of FEW rows. 60 rows of one sequence, 4096 over 2560
 // and rank 16, take 15 us so and 19 with tiles of 16; 64 sequences of two rows 18 and 21; 120 rows of one, 6144 over 2560 and
-// rank 128, 32 and 30; 128 sequences of four, 2560 over 9728 and rank 64, 95 and 89.
+// rank 128, 32 and 30; 128 sequences of four, 2560 over 9728 and rank 64, 95 and 89. Of 244 calls (4 to 512 rows, 1 to 256
+// sequences of equal length, ranks 8 to 128) 210 are within 3% of the shorter way; the others take up to 26% longer, of low
+// rank with tiles of 16 (16 sequences of 12 rows of 1024 over 1024, rank 8: 12.9 and 10.2), of high with tiles of FEW.
 bool few_each(int n_tokens, int n_seqs) { return n_tokens <= std::max(128, 2 * n_seqs); }
 
 // How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the

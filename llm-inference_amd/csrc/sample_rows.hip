@@ -241,7 +241,7 @@ __device__ __forceinline__ uint32_t sum_tokens(Row &row, int carries) {
 }
 
 // e^x for x <= 0: k = rint(x log2 e), r = x - k ln 2 with ln 2 in two parts, the series of e^r to r^13 (|r| <= 0.347:
-// the next term is below 2^-58), times 2^k.
+// the next term is below 2^-57), times 2^k.
 __device__ __forceinline__ double exp_d(double x) {
     x = fmax(x, -1100.0);
     const double k = rint(x * 0x1.71547652b82fep+0);
