@@ -994,9 +994,9 @@ bool few_each(int n_tokens, int n_seqs) { return n_tokens <= std::max(128, 2 * n
 
 // How a call is computed: tiles of one of the shapes, in splits; and whether the adapters' terms are steps of the
 // product, or join_kernel's. The least of an estimate fitted to 107 calls (1 to 4079 rows, 1 to 128 sequences, ranks of 8
-// to 128, 500 to 151936 columns), each in every shape and many splits. Of 1200 other calls (1 to 4096 rows, more than half
-// of the widths of models) what it chooses takes 4% longer on average than the best shape and splits, one in 20 takes 17% longer
-// or more, one 50%.
+// to 128, 500 to 151936 columns), each in every shape and many splits. Of 600 other calls (1 to 4096 rows, more than half
+// of the widths of models) what it chooses takes 5% longer on average than the best shape and splits, one in 20 takes 22% longer
+// or more, one 60%.
 struct Plan {
     int shape, splits, split_steps;
     bool join;
@@ -1028,8 +1028,9 @@ struct Plan {
         for (int i = 0; i < SHAPES; i++) {
             const Pace &s = PACES[i];
             const double m_tiles = ceil(rows / s.tm), tiles = m_tiles * ceil((double)n_out / s.tn);
-            // W past the caches, for each row of tiles: 1344 rows of 6144 over 2560 take 114 us in tiles of 64 by 64, 50 in large ones
-            const double again = s.tm <= 64 ? 0.8 * (m_tiles - 1) : 0;
+            // W past the caches, for more rows of tiles (those of 128 columns have up to 16 MB of it in part from there): 1344
+            // rows of 6144 over 2560 take 114 us in tiles of 64 by 64, 50 in large ones
+            const double again = s.tm > 64 ? 0 : s.tn == 64 ? 0.7 * (m_tiles - 1) : 0.63 * std::min(m_tiles - 1, n_out * (double)n_in > 1 << 23 ? m_tiles : 8.0);
             const double memory = product ? 2.0 * n_out * n_in * (1 + again) / 5770 : 0;
             for (int n = 1; n <= std::min(MOST_SPLITS, std::max(steps, 1)) && (n == 1 || n * one <= (double)MOST_PART); n++) {
                 const double groups = tiles * n, step = s.alone + (s.full - s.alone) * std::min(1.0, groups / CUS);
